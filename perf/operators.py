@@ -13,18 +13,20 @@ bits from the operators' definitions.
 
 Definitions.  A row x in 8 bits: s = max |x| / 127 and q = rint(x / s), each operation
 rounded to 32 bits.  The product: c[i, j] = a_scale[i] w_scale[j] sum_k a[i, k] w[j, k].
-A group of 64 channels x in 4 bits: lo = min(0, x), hi = max(0, x), t = (hi - lo) / 15 in
-32 bits, s = t rounded up to four significant bits, z = rint(-lo / s), n = rint(x / s) + z
-within 0..15; it stands for s (n - z), a number of eight significant bits.  Attention: the
-new rows of a sequence are its last ones; row r of position p sees the keys at positions
-max(0, p - window + 1)..p (0..p without a window).
+A group of 64 channels x in 4 bits: s = max |x| / 6, rounded to 32 bits and then up to six
+significant bits; a channel is held as the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their
+negatives to x / s (rounded to 32 bits; halfway to the even code), and stands for s times
+that, a number of eight significant bits at most.  Attention: the new rows of a sequence are
+its last ones; row r of position p sees the keys at positions max(0, p - window + 1)..p
+(0..p without a window).
 
 The cache is a pool of pages of 64 tokens.  A page holds, head after head, the keys' codes
 [64][D / 2], the values' codes [64][D / 2], the keys' parameters [D / 64][64] and the
-values'.  A code byte holds two channels, the lower one in its low half.  A value row lies
-in channel order; in a key row, in blocks of 128 channels (64 for D = 64), the 4-byte word
-of channels 32 s + 8 h .. + 7 lies at word S h + s, S = block / 32.  A parameter is 16 bits:
-the upper twelve of s as a 32-bit float, then the four of z.
+values'.  A code is a sign (8) and the place 0..7 of the magnitude in the list above; a byte
+holds two channels, the lower one in its low half.  A value row lies in channel order; in a
+key row, in blocks of 128 channels (64 for D = 64), the 4-byte word of channels 32 s + 8 h ..
++ 7 lies at word S h + s, S = block / 32.  A parameter is the upper 16 bits of s as a 32-bit
+float.
 """
 from __future__ import annotations
 
@@ -245,13 +247,17 @@ def _regions(s):
 def _quantise(x):
     """Codes [rows, heads, D] and parameters [rows, heads, D / 64] of the groups of x."""
     g = x.float().unflatten(-1, (-1, GROUP))
-    lo, hi = g.amin(-1).clamp(max=0.0), g.amax(-1).clamp(min=0.0)
-    step = (hi - lo) / torch.full_like(lo, 15.0)
-    step = ((step.view(torch.int32) + 0xFFFFF) & -0x100000).view(torch.float32)
-    zero = torch.round(-lo / step)
-    n = (torch.round(g / step[..., None]) + zero[..., None]).clamp(0.0, 15.0).nan_to_num_(0.0)
-    params = (step.view(torch.int32) >> 16) | zero.nan_to_num_(0.0).int()
-    return n.to(torch.uint8).flatten(-2), params.to(torch.int16)
+    step = g.abs().amax(-1)
+    step = step / torch.full_like(step, 6.0)
+    step = ((step.view(torch.int32) + 0x3FFFF) & -0x40000).view(torch.float32)
+    y = (g / step[..., None]).nan_to_num_(0.0)
+    # The borders between the magnitudes; a border itself goes to the even one of its neighbours.
+    up = torch.tensor([0.75, 1.75, 3.5], device="cuda")
+    down = torch.tensor([0.25, 1.25, 2.5, 5.0], device="cuda")
+    a = y.abs()
+    code = torch.bucketize(a, up, right=True).add_(torch.bucketize(a, down))
+    code = torch.where(y < 0.0, code + 8, code)
+    return code.to(torch.uint8).flatten(-2), (step.view(torch.int32) >> 16).to(torch.int16)
 
 
 def _key_order(n, dim: int, back: bool):
@@ -273,22 +279,20 @@ def _store(s, k, v, sequence, position):
     value_params[page, :, :, slot] = vp
 
 
-def _values(codes, params):
-    """What codes [..., D / 2] and parameters [..., D / 64] stand for, in stored order of the codes' groups."""
-    n = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)
-    p = params.int()
-    step, zero = ((p & 0xFFF0) << 16).view(torch.float32), (p & 15).float()
-    return n, step, zero
+def _values(codes):
+    """The numbers that codes [..., D / 2] name, in stored order."""
+    n = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).int()
+    names = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device="cuda")
+    return torch.cat((names, -names))[n]
 
 
 def _load(s, page, slot):
     """Keys and values [..., heads, D] in 32 bits of the tokens at `slot` of `page` (indices of one shape)."""
     dim = s["case"]["dim"]
     keys, values, key_params, value_params = _regions(s)
-    n, step, zero = _values(keys[page, :, slot], key_params[page, :, :, slot])
-    k = (_key_order(n, dim, True).unflatten(-1, (-1, GROUP)).float() - zero[..., None]) * step[..., None]
-    n, step, zero = _values(values[page, :, slot], value_params[page, :, :, slot])
-    v = (n.unflatten(-1, (-1, GROUP)).float() - zero[..., None]) * step[..., None]
+    step = lambda params: (params[page, :, :, slot].int() << 16).view(torch.float32)[..., None]  # noqa: E731
+    k = _key_order(_values(keys[page, :, slot]), dim, True).unflatten(-1, (-1, GROUP)) * step(key_params)
+    v = _values(values[page, :, slot]).unflatten(-1, (-1, GROUP)) * step(value_params)
     return k.flatten(-2), v.flatten(-2)
 
 
@@ -413,15 +417,13 @@ def _to32(x):
 def _exact_values(x):
     """What the groups of x are held as, value by value from the definition."""
     g = x.double().reshape(*x.shape[:-1], x.shape[-1] // GROUP, GROUP)
-    lo, hi = torch.minimum(g, torch.zeros_like(g)).min(-1)[0], torch.maximum(g, torch.zeros_like(g)).max(-1)[0]
-    t = _to32(_to32(hi - lo) / 15.0)
-    # mantissa in [1/2, 1): four significant bits are sixteenths of the power of two above
-    mantissa, exponent = torch.frexp(t)
-    step = torch.ldexp(torch.ceil(mantissa * 16.0) / 16.0, exponent)
-    zero = torch.round(_to32(-lo / step))
-    step, zero = step[..., None], zero[..., None]
-    n = torch.minimum(torch.maximum(torch.round(_to32(g / step)) + zero, torch.zeros_like(g)), torch.full_like(g, 15.0))
-    return (step * (n - zero)).reshape(x.shape)
+    # mantissa in [1/2, 1): six significant bits are 64ths of the power of two above
+    mantissa, exponent = torch.frexp(_to32(g.abs().max(-1)[0] / 6.0))
+    step = torch.ldexp(torch.ceil(mantissa * 64.0) / 64.0, exponent)[..., None]
+    y = torch.where(step > 0.0, _to32(g / step), 0.0)
+    # The distance between neighbours doubles at 2 and at 4, and an even multiple of it is an even code.
+    unit = torch.where(y.abs() < 2.0, 0.5, torch.where(y.abs() < 4.0, 1.0, 2.0))
+    return (step * (torch.round(y / unit) * unit)).reshape(x.shape)
 
 
 def _exact_attention(case, x):
