@@ -93,6 +93,7 @@ enum {
   PROM_DETAIL_PATH_HIP_GEMV_F32 = 6121,
   PROM_DETAIL_PATH_HIP_MFMA_BF16 = 6122,
   PROM_DETAIL_PATH_HIP_SIMT_F32 = 6123,
+  PROM_DETAIL_PATH_HIP_MFMA_INT8 = 6124,
   /* NEW failure detail codes. */
   PROM_DETAIL_HIP_ALLOC_FAILED = -6901,
   PROM_DETAIL_HIP_COPY_FAILED = -6902,
@@ -877,6 +878,130 @@ PROM_REACTOR_API int prometheus_reactor_runtime_dit_block_bf16(void* handle, con
 PROM_REACTOR_API int prometheus_reactor_runtime_dit_block_bf16_device(void* handle,
                                                                       const PrometheusDitBlockBf16Request* request,
                                                                       PrometheusBlockResult* out_result);
+
+/* ------------------------------------------------------------------------ */
+/* NEW: a quantised decode path.  Rows and weights in 8-bit integers, their    */
+/* product, a paged cache of keys and values held in 4 bits, attention over it. */
+/* No reference counterpart.  Device pointers throughout; every call is queued */
+/* on the runtime's single stream and returns without waiting, like the other  */
+/* _device entries.  Invalid arguments: PROM_ERROR, stage INIT,                */
+/* PROM_DETAIL_INVALID_ARGUMENT, before the device is looked at.               */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of rows. */
+enum { PROM_DTYPE_F32 = 0u, PROM_DTYPE_BF16 = 1u };
+
+/* q[r, c] = rint(x[r, c] / s[r]), s[r] = max_c |x[r, c]| / 127, each operation
+   rounded to fp32 (halves to even), so |q| <= 127.  input: dtype [rows, width]
+   with input_row_stride >= width elements between rows, any alignment of its
+   type; output int8 [rows, width] and scales fp32 [rows], contiguous.  A row of
+   zeros has scale 0 and zeros; a row with an infinity or a NaN has scale NaN and
+   zeros, so that what is computed from it is NaN.  rows * width and rows *
+   input_row_stride below 2^40. */
+PROM_REACTOR_API int prometheus_reactor_runtime_quantize_rows_int8_device(
+    void* handle, const void* input, int8_t* output, float* scales, uint32_t rows, uint32_t width,
+    uint32_t input_row_stride, uint32_t dtype, uint32_t* out_stage, int* out_detail_code);
+
+/* c[i, j] = a_scale[i] * w_scale[j] * sum_k a[i, k] * w[j, k]: a int8 [m, k] (a row
+   per token), w int8 [n, k] (a row per output channel), c of `dtype` [m, n], all
+   contiguous, any alignment; the sum is exact (k <= 131071, so that 128 * 128 * k
+   fits 32 bits), the scales are applied in fp32 and the result is rounded once.
+   Admission and statuses otherwise as ..._gemm_bf16_device (m * k, n * k, m * n
+   below 2^32); success detail PROM_DETAIL_PATH_HIP_MFMA_INT8. */
+#define PROM_GEMM_INT8_MAX_K 131071u
+PROM_REACTOR_API int prometheus_reactor_runtime_gemm_int8_device(void* handle, const int8_t* a, const int8_t* w,
+                                                                 const float* a_scale, const float* w_scale, void* c,
+                                                                 uint32_t m, uint32_t n, uint32_t k, uint32_t dtype,
+                                                                 uint32_t* out_stage, int* out_detail_code);
+
+/* A cache of keys and values in 4 bits, in pages of PROM_KV4_PAGE_TOKENS tokens.
+   A group of 64 channels x of one token's head is held with a step s = max |x| / 6,
+   rounded to fp32 and then up to six significant bits, and per channel the nearest
+   of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives to x / s (rounded to fp32;
+   halfway to the even code); it stands for s times that, which fp32 and bf16 hold
+   exactly (6 s of magnitudes above 2^128 * 32 / 33 may be infinite), at most s away
+   from x.  A group with an infinity or a NaN reads back as NaN.
+   A page is kv_heads blocks of head_dim * 64 + head_dim * 4 bytes: the keys' codes
+   [64][head_dim / 2], the values' codes, the keys' steps [head_dim / 64][64] and the
+   values'.  A code is a sign (8) and the place 0..7 of the magnitude above; a byte
+   holds two channels, the lower in its low half.  Value rows lie in channel order;
+   key rows, in blocks of 128 channels (64 for head_dim 64), with the 4-byte word of
+   channels 32 s + 8 h .. + 7 at word S h + s, S = block / 32 (the order in which the
+   matrix units take them).  A step is the upper 16 bits of an fp32.
+   Sequence i has lengths[i] tokens (those of the call among them; negative counts as
+   0), token t in page page_table[i * table_stride + t / 64].  What lies in a page
+   behind a sequence's last token is never used.  A token whose page number is not in
+   0..pages-1, or whose place lies past table_stride pages, is not written, reads back
+   as NaN, and makes the rows that see it NaN. */
+#define PROM_KV4_PAGE_TOKENS 64u
+#define PROM_KV4_GROUP 64u
+typedef struct PrometheusKv4Cache {
+  uint32_t struct_size;
+  uint32_t head_dim;     /* 64, 128 or 256 */
+  uint32_t kv_heads;     /* 1..1024 */
+  uint32_t pages;        /* of the pool, 1..2^31-1 */
+  uint32_t sequences;    /* 1..2^20; sequences * kv_heads at most 2^23 */
+  uint32_t table_stride; /* page numbers a sequence, 1..2^24 */
+  void* pool;            /* pages * prometheus_reactor_kv4_page_bytes, 16-byte aligned */
+  const int32_t* page_table; /* [sequences, table_stride] */
+  const int32_t* lengths;    /* [sequences] */
+} PrometheusKv4Cache;
+/* Bytes of one page (all heads); 0 for a head_dim or kv_heads outside the above. */
+PROM_REACTOR_API uint64_t prometheus_reactor_kv4_page_bytes(uint32_t head_dim, uint32_t kv_heads);
+
+/* Rows of the last tokens of each sequence: rows row_starts[i] .. row_starts[i+1] - 1
+   (row_starts [sequences + 1], not decreasing) are sequence i's last tokens, the last
+   row its token lengths[i] - 1.  k and v: dtype [rows, kv_heads, head_dim] with
+   row_stride >= kv_heads * head_dim elements between rows (so that they may be columns
+   of one projection's output), any alignment of their type.  Rows outside every
+   sequence, or before its token 0, are passed over: not stored by a write, left as they
+   were by a read.  Write quantises k and v into the cache; read gives what the cache
+   holds (k or v may be NULL in a read). */
+typedef struct PrometheusKv4RowsRequest {
+  uint32_t struct_size;
+  uint32_t dtype;
+  uint32_t rows;        /* 1..2^24 */
+  uint32_t row_stride;  /* below 2^24 */
+  void* k;
+  void* v;
+  const int32_t* row_starts;
+} PrometheusKv4RowsRequest;
+PROM_REACTOR_API int prometheus_reactor_runtime_kv4_write_device(void* handle, const PrometheusKv4Cache* cache,
+                                                                 const PrometheusKv4RowsRequest* request,
+                                                                 uint32_t* out_stage, int* out_detail_code);
+PROM_REACTOR_API int prometheus_reactor_runtime_kv4_read_device(void* handle, const PrometheusKv4Cache* cache,
+                                                                const PrometheusKv4RowsRequest* request,
+                                                                uint32_t* out_stage, int* out_detail_code);
+
+/* out[r, h] = sum_t softmax_t(scale * q[r, h] . k[t, h / g]) v[t, h / g] over the cache,
+   g = q_heads / kv_heads: a row of position p (row_starts as above) sees tokens
+   max(0, p - window + 1) .. p (window 0: 0 .. p).  q and out: dtype [rows, q_heads,
+   head_dim] with q_stride and out_stride elements between rows, any alignment of their
+   type.  One row a sequence (decoding), whole prompts and mixtures of both are served.
+   A row that sees no token (before token 0) is zeros; rows outside every sequence are
+   left as they were.  max_rows (the most rows of a sequence) and max_length (the
+   longest sequence) size the launch; results do not depend on them beyond rounding, and
+   longer sequences are still computed whole.  Scores, softmax and sums are fp32; fp32
+   rows enter the products unrounded, probabilities with 24 significant bits (bf16 rows:
+   8 to 16). */
+typedef struct PrometheusKv4AttentionRequest {
+  uint32_t struct_size;
+  uint32_t dtype;
+  uint32_t rows;        /* 1..2^24 */
+  uint32_t q_heads;     /* a multiple of kv_heads, at most 2^16 */
+  uint32_t q_stride;    /* >= q_heads * head_dim, below 2^24 */
+  uint32_t out_stride;  /* >= q_heads * head_dim, below 2^24 */
+  uint32_t max_rows;    /* 1..rows */
+  uint32_t max_length;  /* at least 1 */
+  uint32_t window;
+  float scale;          /* finite, above 0 */
+  const void* q;
+  void* out;
+  const int32_t* row_starts;
+} PrometheusKv4AttentionRequest;
+PROM_REACTOR_API int prometheus_reactor_runtime_attention_kv4_device(void* handle, const PrometheusKv4Cache* cache,
+                                                                     const PrometheusKv4AttentionRequest* request,
+                                                                     uint32_t* out_stage, int* out_detail_code);
 
 /* ------------------------------------------------------------------------ */
 /* Asynchronous and batched SGEMM (reference lifecycle, HIP execution)       */

@@ -1,0 +1,473 @@
+// Attention over the 4-bit paged cache (kv4_cache.hip):
+// o[r, h] = sum_t softmax_t(scale q[r, h] . k[t]) v[t], k[t] = s code, v[t] = s code
+// with a step s for 64 channels of a token's head.
+//
+// Rows are (row, query head of the group) pairs: a tile is 16 of them, so that the heads
+// that share a key head, and a few rows of a prompt, read the cache once.  A wave takes
+// a page (64 tokens) at a time:
+//   S^T = K Q^T on v_mfma_f32_16x16x32_bf16.  E2M1 codes are exact in bf16 (one
+//   instruction turns two codes into two numbers), so K goes into the products as codes,
+//   one accumulator a group of 64 channels, and the groups' steps are applied to the
+//   scores in fp32.  A lane owns one row and 16 of the page's scores: tile c, register i
+//   of lane (h, row) is token 16 h + 4 c + i, so a lane's tokens are neighbours and their
+//   steps four 16-byte loads.
+//   Softmax with a running maximum that follows only when it grew by more than 2^8, in
+//   base 2.
+//   O^T = V^T P^T.  V's step goes to the probability; P s is split into bf16 terms
+//   that carry it to 16 bits (24 for fp32 rows), the codes again are exact.  The V^T
+//   operand (16 channels, tokens in k) comes from ds_read_b64_tr_b4, which hands a lane
+//   the 16 tokens of its channel; S^T's register order is already P^T's operand order.
+//   fp32 queries are three bf16 terms (exact).
+// No rounding but P's and fp32's is made anywhere.
+//
+// Pages of a sequence are dealt to the waves of a workgroup and to gridDim splits; the
+// waves join through LDS, splits through fp32 partials and a second kernel, in a fixed
+// order.  Bound by reading the cache for long sequences (272 bytes of a 64-channel
+// group pair... per token and head D + D / 16 bytes).
+#include <algorithm>
+
+#include "reactor_internal.h"
+
+namespace prom {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+
+constexpr float kLazyLog2 = 8.0f;
+constexpr int kTileRows = 16;
+constexpr int kWaves = 4;
+constexpr uint64_t kMostPartialBytes = 1ull << 30;
+
+struct Kv4Kernel {
+  Kv4View c;
+  const void* q;
+  void* out;
+  const int32_t* starts;
+  float* part;  // [splits][rows][q_heads][D + 2]: sums, maximum, weight
+  int rows, q_stride, out_stride;
+  int q_heads, group, tiles, splits;
+  uint32_t window;
+  float scale_log2;
+};
+
+// max / sum of v over lanes l and l ^ 16.
+__device__ __forceinline__ float max_rows16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_rows16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The eight numbers of a word of codes.
+__device__ __forceinline__ bf16x8 numbers(uint32_t codes) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.0f, 0);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.0f, 1);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.0f, 2);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.0f, 3);
+  return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Steps 2 j and 2 j + 1 of a word of two.
+__device__ __forceinline__ float step_of(uint32_t w, int odd) {
+  return __uint_as_float(odd ? w & 0xFFFF0000u : w << 16);
+}
+
+// kN bf16 terms that add up to x: each but the last is cut off (toward zero), so that the
+// rest is exact; the last is rounded.
+template <int kN>
+__device__ __forceinline__ void terms(float x, __bf16 (&t)[kN]) {
+#pragma unroll
+  for (int i = 0; i + 1 < kN; ++i) {
+    const uint32_t top = __float_as_uint(x) & 0xFFFF0000u;
+    t[i] = __builtin_bit_cast(__bf16, (uint16_t)(top >> 16));
+    x -= __uint_as_float(top);
+  }
+  t[kN - 1] = (__bf16)x;
+}
+
+template <int D>
+struct Page {
+  static constexpr int kG = D / 64;
+  static constexpr int kK = D >= 128 ? D / 128 : 1;  // 16-byte loads (8 for D = 64) of a key row's quarter
+  u32x4 k[4][kK];
+  u32x4 v[D / 32];
+  u32x4 ks[kG][2], vs[kG][2];
+};
+
+// Every page is read whole: what lies behind a sequence's last token is masked by its use.
+template <int D>
+__device__ __forceinline__ void load_page(Page<D>& p, const uint8_t* block, int lane) {
+  const int r = lane & 15, h = lane >> 4;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint8_t* row = block + (16 * (r >> 2) + 4 * c + (r & 3)) * (D / 2);
+    if constexpr (D == 64) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(row + 8 * h);
+      p.k[c][0] = u32x4{w.x, w.y, 0u, 0u};
+    } else {
+#pragma unroll
+      for (int j = 0; j < Page<D>::kK; ++j) p.k[c][j] = *reinterpret_cast<const u32x4*>(row + 64 * j + 16 * h);
+    }
+  }
+  const uint8_t* v = block + kKv4Page * D / 2;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) p.v[i] = *reinterpret_cast<const u32x4*>(v + 1024 * i + 16 * lane);
+  const uint8_t* s = block + kKv4Page * D + 32 * h;
+#pragma unroll
+  for (int g = 0; g < Page<D>::kG; ++g)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      p.ks[g][j] = *reinterpret_cast<const u32x4*>(s + 128 * g + 16 * j);
+      p.vs[g][j] = *reinterpret_cast<const u32x4*>(s + 128 * (Page<D>::kG + g) + 16 * j);
+    }
+}
+
+// Position of 16-byte chunk c of token t's value row in LDS, so that 16 neighbouring
+// tokens' reads of one chunk fall into different banks.
+template <int D>
+__device__ __forceinline__ int value_swz(int t) {
+  return D == 64 ? (t >> 3) & 1 : D == 128 ? (t >> 2) & 3 : (t >> 1) & 7;
+}
+
+template <bool kF32, int D>
+__global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Kernel g) {
+  constexpr int kG = D / 64, kQT = kF32 ? 3 : 1, kPT = kF32 ? 3 : 2;
+  constexpr int kSteps = D / 32;  // MFMA steps of 32 channels
+  constexpr int kB = D / 16;      // blocks of 16 output channels
+  constexpr int kValueBytes = kKv4Page * D / 2;
+  constexpr int kJoinBytes = kTileRows * (D + 4) * 4;  // a wave's sums [16][D], maxima, weights
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * (kValueBytes > kJoinBytes ? kValueBytes : kJoinBytes)];
+
+  const int lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int r16 = lane & 15, h = lane >> 4;
+  // Splits fastest, then key heads, then tiles, then sequences.
+  uint32_t b = blockIdx.x;
+  const int split = (int)(b % (uint32_t)g.splits);
+  b /= (uint32_t)g.splits;
+  const int head = (int)(b % (uint32_t)g.c.kv_heads);
+  b /= (uint32_t)g.c.kv_heads;
+  const int tile0 = (int)(b % (uint32_t)g.tiles);
+  const int seq = (int)(b / (uint32_t)g.tiles);
+
+  const int first_row = min(max(g.starts[seq], 0), g.rows);
+  const int n = min(max(g.starts[seq + 1], 0), g.rows) - first_row;
+  if (n <= 0) return;
+  const long long room = (long long)g.c.table_stride * kKv4Page;
+  const int length = max(g.c.lengths[seq], 0);
+  const int32_t* table = g.c.table + (size_t)seq * g.c.table_stride;
+  const size_t block_bytes = kv4_block_bytes(D);
+  uint8_t* my_lds = lds + wave * kValueBytes;
+
+  const long long tiles = ((long long)n * g.group + kTileRows - 1) / kTileRows;
+  for (long long tile = tile0; tile < tiles; tile += g.tiles) {
+    // This lane's row: pair x = row * group + query head.
+    const long long x0 = tile * kTileRows, x = x0 + r16;
+    const long long pairs = (long long)n * g.group;
+    const bool mine = x < pairs;
+    const int row = mine ? (int)(x / g.group) : 0;
+    const int q_head = head * g.group + (mine ? (int)(x - (long long)row * g.group) : 0);
+    const long long pos = mine ? (long long)length - n + row : -1;  // its position
+    const long long pos0 = (long long)length - n + x0 / g.group;    // the tile's first and last
+    const long long pos1 = (long long)length - n + (min(x0 + kTileRows, pairs) - 1) / g.group;
+    const long long low = g.window ? pos - g.window : -1;  // it sees low < t <= pos
+    const int page0 = g.window && pos0 >= (long long)g.window ? (int)((pos0 - g.window + 1) / kKv4Page) : 0;
+    const int page1 = pos1 < 0 ? 0 : (int)(pos1 / kKv4Page) + 1;
+    // Past the table every token is bad: one page of them stands for all.
+    const int last = (int)min((long long)page1, room / kKv4Page + 1);
+
+    // Q^T operand: lane (h, row), step s: channels 32 s + 8 h .. + 7.
+    bf16x8 q[kSteps][kQT];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const size_t at = (size_t)(first_row + row) * g.q_stride + (size_t)q_head * D + 32 * s + 8 * h;
+      if constexpr (kF32) {
+        float v[8];
+        __builtin_memcpy(v, static_cast<const float*>(g.q) + at, 32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          __bf16 t[kQT];
+          terms(mine ? v[j] : 0.0f, t);
+#pragma unroll
+          for (int i = 0; i < kQT; ++i) q[s][i][j] = t[i];
+        }
+      } else {
+        u32x4 v;
+        __builtin_memcpy(&v, static_cast<const uint16_t*>(g.q) + at, 16);
+        if (!mine) v = u32x4{0u, 0u, 0u, 0u};
+        q[s][0] = __builtin_bit_cast(bf16x8, v);
+      }
+    }
+
+    floatx4 o[kB] = {};
+    float m_run = -INFINITY, m_log2 = 0.0f, l_run = 0.0f;
+
+    const int stride = g.splits * kWaves;
+    int pg = page0 + split * kWaves + wave;
+    auto page_number = [&](int p) -> uint32_t {
+      return p < last && p < g.c.table_stride ? (uint32_t)__builtin_amdgcn_readfirstlane(table[p]) : 0xFFFFFFFFu;
+    };
+    auto page_block = [&](uint32_t number) -> const uint8_t* {
+      const uint32_t ok = number < g.c.pages ? number : 0u;
+      return g.c.pool + ((size_t)ok * g.c.kv_heads + head) * block_bytes;
+    };
+    Page<D> cur;
+    uint32_t number = page_number(pg), next_number = page_number(pg + stride);
+    if (pg < last) load_page<D>(cur, page_block(number), lane);
+    for (; pg < last; pg += stride) {
+      Page<D> next;
+      const uint32_t after = page_number(pg + 2 * stride);
+      if (pg + stride < last) load_page<D>(next, page_block(next_number), lane);
+
+      // Values to LDS, chunk swizzled; a wave's own region, in order with its reads.
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const int at = 1024 * i + 16 * lane, t = at / (D / 2), c = (at % (D / 2)) / 16;
+        *reinterpret_cast<u32x4*>(my_lds + t * (D / 2) + 16 * (c ^ value_swz<D>(t))) = cur.v[i];
+      }
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
+
+      floatx4 s[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int gr = 0; gr < kG; ++gr) {
+          floatx4 acc = {};
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int st = 2 * gr + u;
+            const bf16x8 kf = numbers(D == 64 ? cur.k[c][0][st] : cur.k[c][st / 4][st % 4]);
+#pragma unroll
+            for (int i = 0; i < kQT; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[st][i], acc, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = 4 * c + i;
+            const float step = step_of(cur.ks[gr][j / 8][j / 2 % 4], j & 1);
+            s[c][i] = gr == 0 ? acc[i] * step : __builtin_fmaf(acc[i], step, s[c][i]);
+          }
+        }
+      }
+      // Masked where the page has tokens that some row does not see, or is bad.
+      const long long t0 = (long long)pg * kKv4Page;
+      const bool bad = number >= g.c.pages;
+      const bool edge = bad || t0 + kKv4Page - 1 > pos0 || (g.window && t0 <= pos1 - (long long)g.window) ||
+                        x0 + kTileRows > pairs;
+      if (edge) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const long long t = t0 + 16 * h + 4 * c + i;
+            const bool seen = t <= pos && t > low;
+            if (bad) s[c][i] = NAN;
+            if (!seen) s[c][i] = -INFINITY;
+          }
+      }
+      float m = s[0][0];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, s[c][i]);
+      m = max_halves(max_rows16(m));
+      // (-inf) - (-inf) is NaN, which is not above: such a row has seen nothing yet.
+      if (__any((m - m_run) * g.scale_log2 > kLazyLog2)) {
+        const float m_new = fmaxf(m, m_run);
+        const float alpha = m_new == m_run ? 1.0f : __builtin_amdgcn_exp2f((m_run - m_new) * g.scale_log2);
+        m_run = m_new;
+        m_log2 = m_new == -INFINITY ? 0.0f : m_new * g.scale_log2;
+        l_run *= alpha;
+#pragma unroll
+        for (int i = 0; i < kB; ++i) o[i] *= alpha;
+      }
+      float p[16];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][i], g.scale_log2, -m_log2));
+          p[4 * c + i] = e;
+          l_run += e;
+        }
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr) {
+        // P s in bf16 terms, tokens 16 h + 0..7 and 8..15.
+        bf16x8 pf[2][kPT];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float step = step_of(cur.vs[gr][j / 8][j / 2 % 4], j & 1);
+          if (edge && s[j / 4][j % 4] == -INFINITY) step = 0.0f;  // a token not seen may hold anything
+          __bf16 t[kPT];
+          terms(p[j] * step, t);
+#pragma unroll
+          for (int i = 0; i < kPT; ++i) pf[j / 8][i][j % 8] = t[i];
+        }
+#pragma unroll
+        for (int bl = 4 * gr; bl < 4 * gr + 4; ++bl) {
+          const int t = 16 * h + r16;
+          const int at = t * (D / 2) + 16 * ((bl >> 1) ^ value_swz<D>(t)) + 8 * (bl & 1);
+          const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(my_lds + at));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const bf16x8 vf = numbers((uint32_t)w[u]);
+#pragma unroll
+            for (int i = 0; i < kPT; ++i) o[bl] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[u][i], o[bl], 0, 0, 0);
+          }
+        }
+      }
+      cur = next;
+      number = next_number;
+      next_number = after;
+    }
+
+    // Join the waves: unnormalised sums, maxima and weights through LDS.
+    l_run = sum_halves(sum_rows16(l_run));
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(lds) + (size_t)wave * kTileRows * (D + 4);
+#pragma unroll
+    for (int bl = 0; bl < kB; ++bl) *reinterpret_cast<floatx4*>(sums + r16 * (D + 4) + 16 * bl + 4 * h) = o[bl];
+    if (h == 0) {
+      sums[r16 * (D + 4) + D] = m_run;
+      sums[r16 * (D + 4) + D + 1] = l_run;
+    }
+    __syncthreads();
+    for (int e = (int)threadIdx.x; e < kTileRows * D; e += 64 * kWaves) {
+      const int tr = e / D, d = e % D;
+      const long long xe = x0 + tr;
+      if (xe >= pairs) break;
+      const float* all = reinterpret_cast<const float*>(lds) + tr * (D + 4);
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, all[w * kTileRows * (D + 4) + D]);
+      float sum = 0.0f, weight = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float* a = all + w * kTileRows * (D + 4);
+        const float f = a[D] == top ? 1.0f : __builtin_amdgcn_exp2f((a[D] - top) * g.scale_log2);
+        sum = __builtin_fmaf(a[d], f, sum);
+        weight = __builtin_fmaf(a[D + 1], f, weight);
+      }
+      const int er = first_row + (int)(xe / g.group);
+      const int eh = head * g.group + (int)(xe % g.group);
+      if (g.splits > 1) {
+        float* part = g.part + (((size_t)split * g.rows + er) * g.q_heads + eh) * (D + 2);
+        part[d] = sum;
+        if (d == 0) {
+          part[D] = top;
+          part[D + 1] = weight;
+        }
+      } else {
+        const float v = weight == 0.0f ? 0.0f : sum / weight;
+        const size_t at = (size_t)er * g.out_stride + (size_t)eh * D + d;
+        if constexpr (kF32)
+          static_cast<float*>(g.out)[at] = v;
+        else
+          static_cast<__bf16*>(g.out)[at] = (__bf16)v;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// One wave a row and query head: joins the splits' sums in order.
+template <bool kF32, int D>
+__global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
+  const long long pairs = (long long)g.rows * g.q_heads;
+  const int lane = (int)threadIdx.x & 63;
+  for (long long x = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); x < pairs; x += (long long)gridDim.x * 4) {
+    const int row = (int)(x / g.q_heads);
+    if (find_sequence(g.starts, g.c.sequences, row) < 0) continue;
+    const float* part = g.part + (size_t)x * (D + 2);
+    const size_t slab = (size_t)pairs * (D + 2);
+    float top = -INFINITY;
+    for (int s = 0; s < g.splits; ++s) top = fmaxf(top, part[s * slab + D]);
+    float sum[D / 64] = {}, weight = 0.0f;
+    for (int s = 0; s < g.splits; ++s) {
+      const float* a = part + s * slab;
+      const float f = a[D] == top ? 1.0f : __builtin_amdgcn_exp2f((a[D] - top) * g.scale_log2);
+      weight = __builtin_fmaf(a[D + 1], f, weight);
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) sum[j] = __builtin_fmaf(a[lane + 64 * j], f, sum[j]);
+    }
+    const size_t at = (size_t)row * g.out_stride + (size_t)(x - (long long)row * g.q_heads) * D + lane;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      const float v = weight == 0.0f ? 0.0f : sum[j] / weight;
+      if constexpr (kF32)
+        static_cast<float*>(g.out)[at + 64 * j] = v;
+      else
+        static_cast<__bf16*>(g.out)[at + 64 * j] = (__bf16)v;
+    }
+  }
+}
+
+// Tiles of 16 pairs that the longest sequence has (a workgroup takes several where the grid
+// would be too large), and the splits of its pages: enough workgroups for the chip to be
+// full and uneven sequences to be dealt out.
+void plan(const Kv4AttentionArgs& a, int head_dim, int* tiles, int* splits) {
+  const uint64_t columns = (uint64_t)a.c.sequences * a.c.kv_heads;  // at most kKv4MaxColumns
+  const uint64_t t = ((uint64_t)a.max_rows * (uint64_t)a.group + kTileRows - 1) / kTileRows;
+  *tiles = (int)std::min<uint64_t>(t, kKv4MaxColumns / columns);
+  const uint64_t base = columns * (uint64_t)*tiles;
+  uint64_t length = a.max_length;
+  if (a.window) length = std::min<uint64_t>(length, (uint64_t)a.window + 2 * kKv4Page);
+  const uint64_t pages = (length + kKv4Page - 1) / kKv4Page;
+  const uint64_t want = (2048 + base - 1) / base, most = (pages + 2 * kWaves - 1) / (2 * kWaves);
+  *splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({want, most, 64}));
+  if ((uint64_t)*splits * a.rows * (uint64_t)a.q_heads * (uint64_t)(head_dim + 2) * 4 > kMostPartialBytes) *splits = 1;
+}
+
+template <bool kF32, int D>
+hipError_t launch(const Kv4Kernel& g, hipStream_t stream) {
+  const uint64_t grid = (uint64_t)g.c.sequences * g.c.kv_heads * (uint64_t)g.tiles * (uint64_t)g.splits;
+  hipLaunchKernelGGL((kv4_attention_kernel<kF32, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, stream, g);
+  if (g.splits > 1) {
+    const uint64_t pairs = (uint64_t)g.rows * (uint64_t)g.q_heads;
+    hipLaunchKernelGGL((kv4_join_kernel<kF32, D>), dim3((unsigned)std::min<uint64_t>((pairs + 3) / 4, 1u << 20)), dim3(256),
+                       0, stream, g);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t kv4_attention_partial_bytes(const Kv4AttentionArgs& a, int head_dim) {
+  int tiles, splits;
+  plan(a, head_dim, &tiles, &splits);
+  return splits > 1 ? (size_t)splits * a.rows * a.q_heads * (head_dim + 2) * sizeof(float) : 0;
+}
+
+hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf16, hipStream_t stream) {
+  Kv4Kernel g{};
+  g.c = a.c;
+  g.q = a.q;
+  g.out = a.out;
+  g.starts = a.row_starts;
+  g.part = a.part;
+  g.rows = (int)a.rows;
+  g.q_stride = (int)a.q_stride;
+  g.out_stride = (int)a.out_stride;
+  g.q_heads = a.q_heads;
+  g.group = a.group;
+  g.window = a.window;
+  g.scale_log2 = a.scale * 1.4426950408889634f;
+  plan(a, head_dim, &g.tiles, &g.splits);
+  switch (head_dim) {
+    case 64: return bf16 ? launch<false, 64>(g, stream) : launch<true, 64>(g, stream);
+    case 128: return bf16 ? launch<false, 128>(g, stream) : launch<true, 128>(g, stream);
+    case 256: return bf16 ? launch<false, 256>(g, stream) : launch<true, 256>(g, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace prom

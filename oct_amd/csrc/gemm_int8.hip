@@ -1,0 +1,553 @@
+// The product of 8-bit rows: c[i, j] = a_scale[i] * w_scale[j] * sum_k a[i, k] w[j, k],
+// a [m, k] and w [n, k] int8 with k contiguous in both, exact int32 sums.
+//
+// Two kernels.  Many rows: macro tiles on v_mfma_i32_32x32x32_i8.  A workgroup's
+// waves form a kWM x kWN grid, each owning kMI x kNI blocks of 32 x 32.  Tiles of
+// both operands (rows of 128 bytes of k, a whole line) travel HBM -> LDS by
+// buffer_load ... lds into a ring of kSt stages; 16-byte chunks are XOR-swizzled by
+// row, applied by each lane's source address, so that operand reads (16 bytes a
+// lane, as they lie) are free of bank conflicts.  Descriptors end at the operand's
+// end and a's chunks past k are sent out of range, so tails add zeros.  Rows that
+// are not whole 16-byte chunks are copied to padded ones first.  Where tiles are few,
+// K is cut into slices whose int32 sums a second kernel adds (exact in any order).
+//
+// Few rows (a decode step, a short prompt): every weight is read once, so w goes
+// from memory straight into the operand registers of v_mfma_i32_16x16x64_i8 (16
+// rows of w, 64 bytes of k), K dealt to the waves of a workgroup, which add their
+// sums through LDS.  Bound by reading w.
+#include <algorithm>
+#include <type_traits>
+
+#include "reactor_internal.h"
+
+namespace prom {
+namespace {
+
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef int intx16 __attribute__((ext_vector_type(16)));
+
+constexpr int kGroupM = 8;
+constexpr uint32_t kOutOfRange = 0x80000000u;  // past every descriptor range
+
+struct Int8Args {
+  const int8_t* a;
+  const int8_t* w;
+  const float* a_scale;
+  const float* w_scale;
+  void* c;
+  int32_t* slabs;  // K slices' sums, [slices][m][n] (null: one slice)
+  int m, n, k;     // k of the operands as multiplied
+  int lda, ldw;
+  int tiles_m, tiles_n;
+};
+
+__device__ __forceinline__ void store_scaled(float* p, int sum, float as, float ws) { *p = (float)sum * as * ws; }
+__device__ __forceinline__ void store_scaled(__bf16* p, int sum, float as, float ws) {
+  *p = (__bf16)((float)sum * as * ws);
+}
+
+template <int kMI_, int kNI_, int kWM_, int kWN_, int kSt_>
+struct Cfg {
+  static constexpr int kMI = kMI_, kNI = kNI_, kWM = kWM_, kWN = kWN_, kSt = kSt_, kBK = 128;
+  static constexpr int kWaves = kWM * kWN;
+  static constexpr int kBM = 32 * kMI * kWM, kBN = 32 * kNI * kWN;
+  static constexpr int kABytes = kBM * kBK, kBBytes = kBN * kBK;
+  static constexpr int kStage = kABytes + kBBytes;
+  static constexpr int kAX = kABytes / 1024 / kWaves, kBX = kBBytes / 1024 / kWaves;  // transfers per wave and tile
+  static constexpr int kX = kAX + kBX;
+  static_assert(kAX * 1024 * kWaves == kABytes && kBX * 1024 * kWaves == kBBytes, "whole transfers per wave");
+  static_assert(kSt >= 2 && kSt * kStage <= 163840 && (kSt - 2) * kX < 64, "ring");
+};
+
+// Position of chunk c of row r within the row's eight.
+__device__ __forceinline__ int swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
+
+template <int kN>
+__device__ __forceinline__ void wait_vmcnt() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kN) : "memory");
+}
+
+// At most min(kMost, n) tiles of kX transfers may stay in flight.
+template <int kX, int kMost>
+__device__ __forceinline__ void wait_tiles(int n) {
+  if constexpr (kMost > 0) {
+    if (n < kMost) {
+      wait_tiles<kX, kMost - 1>(n);
+      return;
+    }
+  }
+  wait_vmcnt<kX * kMost>();
+}
+
+template <class C, typename TOut>
+__global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_int8_tile_kernel(const Int8Args g) {
+  __shared__ __attribute__((aligned(1024))) char lds[C::kSt * C::kStage];
+  constexpr int kBK = C::kBK, kSteps = kBK / 32;
+  const int num_tiles = g.tiles_m * g.tiles_n;
+  int tm, tn;
+  {
+    const int pid = xcd_pid((int)blockIdx.x, num_tiles);
+    const int per_group = kGroupM * g.tiles_n;
+    const int group = pid / per_group;
+    const int first_m = group * kGroupM;
+    const int group_m = min(g.tiles_m - first_m, kGroupM);
+    const int in_group = pid - group * per_group;
+    tm = first_m + in_group % group_m;
+    tn = in_group / group_m;
+  }
+  const int row0 = tm * C::kBM, col0 = tn * C::kBN;
+  const int all_tiles = (g.k + kBK - 1) / kBK;
+  const int slices = (int)gridDim.y;
+  const int kt0 = (int)((long long)blockIdx.y * all_tiles / slices);
+  const int kn = (int)((long long)(blockIdx.y + 1) * all_tiles / slices) - kt0;
+
+  const int tid = (int)threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / C::kWN, wn = wave % C::kWN;
+
+  // This wave's transfers: 1 KiB (eight rows) each.  Offsets are relative to the tile's first byte.
+  uint32_t a_off[C::kAX], b_off[C::kBX];
+  const int tr = lane >> 3;  // row within a transfer
+#pragma unroll
+  for (int i = 0; i < C::kAX; ++i) {
+    const int r = 8 * (wave * C::kAX + i) + tr;
+    a_off[i] = (uint32_t)(r * g.lda + 16 * ((lane & 7) ^ swz(r)));
+  }
+#pragma unroll
+  for (int i = 0; i < C::kBX; ++i) {
+    const int r = 8 * (wave * C::kBX + i) + tr;
+    b_off[i] = (uint32_t)(r * g.ldw + 16 * ((lane & 7) ^ swz(r)));
+  }
+  const int k16 = (g.k + 15) & ~15;
+  const char* a_ptr = (const char*)(g.a + (size_t)row0 * g.lda + (size_t)kt0 * kBK);
+  long long a_left = (long long)(g.m - 1 - row0) * g.lda + k16 - (long long)kt0 * kBK;
+  const char* b_ptr = (const char*)(g.w + (size_t)col0 * g.ldw + (size_t)kt0 * kBK);
+  long long b_left = (long long)(g.n - 1 - col0) * g.ldw + k16 - (long long)kt0 * kBK;
+  int issued = 0;
+  auto desc = [](const char* p, long long left) {
+    const unsigned long long a = (unsigned long long)p;
+    const unsigned range = left < 0 ? 0u : (left > 0x7fffffffll ? 0x7fffffffu : (unsigned)left);
+    intx4 d;
+    d.x = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffu));
+    d.y = __builtin_amdgcn_readfirstlane((int)(a >> 32));
+    d.z = __builtin_amdgcn_readfirstlane((int)range);
+    d.w = 0x00020000;
+    return d;
+  };
+  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds;
+  intx4 da = desc(a_ptr, a_left), db = desc(b_ptr, b_left);
+  uint32_t fill = lds0;  // LDS address of the stage the next tile goes to
+  // Transfer j (0 .. kX-1) of the tile being issued; tail: a's last chunks lie past k.
+  auto issue_one = [&](int j, bool tail) __attribute__((always_inline)) {
+    if (j < C::kAX) {
+      uint32_t off = a_off[j];
+      if (tail) {
+        const int r = 8 * (wave * C::kAX + j) + tr;
+        if ((kt0 + issued) * kBK + 16 * ((lane & 7) ^ swz(r)) >= g.k) off = kOutOfRange;
+      }
+      const uint32_t to = __builtin_amdgcn_readfirstlane(fill + (wave * C::kAX + j) * 1024);
+      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(da)
+                   : "memory", "m0");
+    } else {
+      const uint32_t to =
+          __builtin_amdgcn_readfirstlane(fill + C::kABytes + (wave * C::kBX + (j - C::kAX)) * 1024);
+      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(b_off[j - C::kAX]),
+                   "s"(db)
+                   : "memory", "m0");
+    }
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
+    a_ptr += kBK;
+    a_left -= kBK;
+    b_ptr += kBK;
+    b_left -= kBK;
+    da = desc(a_ptr, a_left);
+    db = desc(b_ptr, b_left);
+    fill = fill + C::kStage == lds0 + C::kSt * C::kStage ? lds0 : fill + C::kStage;
+    ++issued;
+  };
+
+  const int lrow = lane & 31;
+  const int hk = lane >> 5;
+  // Byte offsets within a stage: rows 32 further share the swizzle, and chunk 2 s + hk of a
+  // row is chunk hk's position XOR 2 s, so mi and ni are immediate offsets of the reads.
+  const int ra = wm * C::kMI * 32 + lrow, rb = wn * C::kNI * 32 + lrow;
+  uint32_t a_base[kSteps], b_base[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    a_base[s] = (uint32_t)(ra * kBK + (((2 * s + hk) ^ swz(ra)) << 4));
+    b_base[s] = (uint32_t)(C::kABytes + rb * kBK + (((2 * s + hk) ^ swz(rb)) << 4));
+  }
+  struct Frags {
+    intx4 a[C::kMI], b[C::kNI];
+  };
+  auto read = [&](uint32_t st, int s) __attribute__((always_inline)) {
+    Frags f;
+    const char* pa = lds + (st + a_base[s]);
+    const char* pb = lds + (st + b_base[s]);
+#pragma unroll
+    for (int mi = 0; mi < C::kMI; ++mi) f.a[mi] = *reinterpret_cast<const intx4*>(pa + mi * 32 * kBK);
+#pragma unroll
+    for (int ni = 0; ni < C::kNI; ++ni) f.b[ni] = *reinterpret_cast<const intx4*>(pb + ni * 32 * kBK);
+    return f;
+  };
+
+  intx16 acc[C::kMI][C::kNI];
+#pragma unroll
+  for (int i = 0; i < C::kMI; ++i)
+#pragma unroll
+    for (int j = 0; j < C::kNI; ++j) acc[i][j] = intx16{};
+
+  // Tiles of this slice whose chunks of a all lie below k: all, or all but the last.
+  const int whole = kn - ((kt0 + kn) * kBK > g.k ? 1 : 0);
+#pragma unroll
+  for (int s = 0; s < C::kSt - 1; ++s)
+    if (s < kn) {
+#pragma unroll
+      for (int j = 0; j < C::kX; ++j) issue_one(j, s >= whole);
+      advance();
+    }
+  constexpr int kDepth = C::kSt - 2;
+  uint32_t cur = 0;
+  // Step t: tile t has landed for this wave, later ones may stay in flight; after the
+  // barrier it is complete for all waves and tile t-1's stage is free.  The transfers of
+  // tile t + kSt - 1 go out between the MFMAs, spread evenly.
+  auto step = [&](int t, auto more_c, auto tail_c) __attribute__((always_inline)) {
+    constexpr bool kMore = decltype(more_c)::value, kTail = decltype(tail_c)::value;
+    constexpr int kMfma = kSteps * C::kMI * C::kNI;
+    if constexpr (kMore && !kTail)
+      wait_vmcnt<C::kX * kDepth>();
+    else
+      wait_tiles<C::kX, kDepth>(kn - 1 - t);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    Frags f = read(cur, 0);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      Frags nf;
+      if (s + 1 < kSteps) nf = read(cur, s + 1);
+      __builtin_amdgcn_sched_barrier(0);  // the next step's reads go out before this one's MFMAs
+#pragma unroll
+      for (int mi = 0; mi < C::kMI; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < C::kNI; ++ni) {
+          const int at = (s * C::kMI + mi) * C::kNI + ni;
+          acc[mi][ni] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[mi], f.b[ni], acc[mi][ni], 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < C::kX; ++j)
+            if (kMore && j * kMfma / C::kX == at) issue_one(j, kTail);
+        }
+      if (s + 1 < kSteps) f = nf;
+    }
+    if constexpr (kMore) advance();
+    cur = cur + C::kStage == C::kSt * C::kStage ? 0 : cur + C::kStage;
+  };
+  const std::integral_constant<bool, true> yes{};
+  const std::integral_constant<bool, false> no{};
+  int t = 0;
+  for (; t + C::kSt - 1 < whole; ++t) step(t, yes, no);
+  if (t + C::kSt - 1 < kn) {
+    step(t, yes, yes);
+    ++t;
+  }
+  for (; t < kn; ++t) step(t, no, no);
+
+  // Accumulator layout: lane l, register r holds row 8 (r/4) + 4 (l/32) + r%4, column l%32.
+#pragma unroll
+  for (int ni = 0; ni < C::kNI; ++ni) {
+    const int col = col0 + (wn * C::kNI + ni) * 32 + lrow;
+    if (col >= g.n) continue;
+    const float ws = g.slabs == nullptr ? g.w_scale[col] : 0.0f;
+#pragma unroll
+    for (int mi = 0; mi < C::kMI; ++mi) {
+      const int r0 = row0 + (wm * C::kMI + mi) * 32 + 4 * hk;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = r0 + 8 * (r >> 2) + (r & 3);
+        if (row >= g.m) continue;
+        const size_t at = (size_t)row * g.n + col;
+        if (g.slabs != nullptr)
+          g.slabs[(size_t)blockIdx.y * g.m * g.n + at] = acc[mi][ni][r];
+        else
+          store_scaled(static_cast<TOut*>(g.c) + at, acc[mi][ni][r], g.a_scale[row], ws);
+      }
+    }
+  }
+}
+
+// c = a_scale w_scale (sum of the K slices); the sums are exact, whatever their order.
+template <typename TOut>
+__global__ __launch_bounds__(256) void int8_slices_kernel(const int32_t* __restrict__ slabs, int slices,
+                                                          const float* __restrict__ a_scale,
+                                                          const float* __restrict__ w_scale, TOut* __restrict__ c,
+                                                          int m, int n) {
+  const int col = (int)(blockIdx.x * 256 + threadIdx.x);
+  if (col >= n) return;
+  const size_t slab = (size_t)m * n;
+  const float ws = w_scale[col];
+  for (int row = (int)blockIdx.y; row < m; row += (int)gridDim.y) {
+    const int32_t* p = slabs + (size_t)row * n + col;
+    int sum = 0;
+    for (int s = 0; s < slices; ++s) sum += p[s * slab];
+    store_scaled(c + (size_t)row * n + col, sum, a_scale[row], ws);
+  }
+}
+
+// dst [rows][ld] = src [rows][cols], zero from column cols on (ld a multiple of 16):
+// sixteen bytes a thread, read at any alignment.
+__global__ __launch_bounds__(256) void pad_rows8_kernel(const int8_t* __restrict__ src, int8_t* __restrict__ dst,
+                                                        int rows, int cols, int ld) {
+  const int c = (int)(blockIdx.x * 64 + (threadIdx.x & 63)) * 16;
+  if (c >= ld) return;
+  for (int r = (int)(blockIdx.y * 4 + (threadIdx.x >> 6)); r < rows; r += (int)gridDim.y * 4) {
+    const int8_t* p = src + (size_t)r * cols + c;
+    int8_t v[16];
+    if (c + 16 <= cols) {
+      __builtin_memcpy(v, p, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = c + j < cols ? p[j] : (int8_t)0;
+    }
+    __builtin_memcpy(__builtin_assume_aligned(dst + (size_t)r * ld + c, 16), v, 16);
+  }
+}
+
+// Sixteen bytes from column k of a row, zeros from column `cols` on.
+__device__ __forceinline__ intx4 load16(const int8_t* row, int k, int cols) {
+  intx4 v = {0, 0, 0, 0};
+  if (k + 16 <= cols) {
+    __builtin_memcpy(&v, row + k, 16);
+  } else if (k < cols) {
+    int8_t b[16] = {};
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (k + j < cols) b[j] = row[k + j];
+    __builtin_memcpy(&v, b, 16);
+  }
+  return v;
+}
+
+// Few rows: a workgroup computes 16 kNT columns of c for 16 kMT rows; its waves take K in
+// turn, kUnroll steps of 64 at a time.
+template <int kMT, int kNT, int kWaves, typename TOut>
+__global__ __launch_bounds__(64 * kWaves) void gemm_int8_rows_kernel(const Int8Args g) {
+  constexpr int kUnroll = kNT * kMT >= 4 ? 2 : 4;
+  __shared__ intx4 part[kWaves > 1 ? kWaves - 1 : 1][kMT * kNT][64];
+  const int lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int r16 = lane & 15, h = lane >> 4;
+  const int n0 = (int)blockIdx.x * 16 * kNT, m0 = (int)blockIdx.y * 16 * kMT;
+  const int8_t* wp[kNT];
+  const int8_t* ap[kMT];
+#pragma unroll
+  for (int i = 0; i < kNT; ++i) wp[i] = g.w + (size_t)min(n0 + 16 * i + r16, g.n - 1) * g.k;
+#pragma unroll
+  for (int i = 0; i < kMT; ++i) ap[i] = g.a + (size_t)min(m0 + 16 * i + r16, g.m - 1) * g.k;
+  intx4 acc[kNT][kMT] = {};
+  constexpr int kStep = 64 * kUnroll;
+  const int whole = g.k / kStep;  // steps without a tail
+  for (int t = wave; t < whole; t += kWaves) {
+    const int k = t * kStep + 16 * h;
+    intx4 w[kUnroll][kNT], a[kUnroll][kMT];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) __builtin_memcpy(&w[u][i], wp[i] + k + 64 * u, 16);
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) __builtin_memcpy(&a[u][i], ap[i] + k + 64 * u, 16);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int j = 0; j < kMT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][i], a[u][j], acc[i][j], 0, 0, 0);
+  }
+  if (whole % kWaves == wave)
+    for (int k = whole * kStep + 16 * h; k - 16 * h < g.k; k += 64) {
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) {
+        const intx4 w = load16(wp[i], k, g.k);
+#pragma unroll
+        for (int j = 0; j < kMT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, load16(ap[j], k, g.k), acc[i][j], 0, 0, 0);
+      }
+    }
+  if constexpr (kWaves > 1) {
+    if (wave > 0) {
+#pragma unroll
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int j = 0; j < kMT; ++j) part[wave - 1][i * kMT + j][lane] = acc[i][j];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    for (int s = 0; s < kWaves - 1; ++s)
+#pragma unroll
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int j = 0; j < kMT; ++j) acc[i][j] += part[s][i * kMT + j][lane];
+  }
+  // Lane l, register r: column (of w) 4 (l/16) + r, row (of a) l%16.
+#pragma unroll
+  for (int j = 0; j < kMT; ++j) {
+    const int row = m0 + 16 * j + r16;
+    if (row >= g.m) continue;
+    const float as = g.a_scale[row];
+#pragma unroll
+    for (int i = 0; i < kNT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = n0 + 16 * i + 4 * h + r;
+        if (col < g.n) store_scaled(static_cast<TOut*>(g.c) + (size_t)row * g.n + col, acc[i][j][r], as, g.w_scale[col]);
+      }
+  }
+}
+
+#define INT8_TILES(X)            \
+  X(0, 1, 1, 2, 2, 4) /* 64x64 */   \
+  X(1, 1, 2, 4, 2, 4) /* 128x128 */ \
+  X(2, 2, 2, 2, 4, 3) /* 128x256 */ \
+  X(3, 4, 2, 2, 4, 2) /* 256x256 */
+
+struct TileInfo {
+  int bm, bn, threads;
+};
+#define X(i, ...) {Cfg<__VA_ARGS__>::kBM, Cfg<__VA_ARGS__>::kBN, 64 * Cfg<__VA_ARGS__>::kWaves},
+constexpr TileInfo kTiles[] = {INT8_TILES(X)};
+#undef X
+constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
+
+template <typename TOut>
+hipError_t launch_tile(int tile, int slices, const Int8Args& g, hipStream_t stream) {
+  const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), (unsigned)slices);
+  const dim3 block((unsigned)kTiles[tile].threads);
+  switch (tile) {
+#define X(i, ...)                                                                                    \
+  case i:                                                                                            \
+    hipLaunchKernelGGL((gemm_int8_tile_kernel<Cfg<__VA_ARGS__>, TOut>), grid, block, 0, stream, g);  \
+    break;
+    INT8_TILES(X)
+#undef X
+  }
+  return hipGetLastError();
+}
+
+// Estimated microseconds as in gemm_bf16_tiles.hip: rounds of 256 * occ workgroups.
+struct TileCost {
+  int occ;
+  double step[2], fill, idle;
+};
+constexpr TileCost kCost[kNumTiles] = {
+    {2, {0.190, 0.375}, 2.49, 0.77},  // 64x64
+    {1, {0.585, 0.585}, 3.49, 0.46},  // 128x128
+    {1, {0.945, 0.945}, 5.67, 0.42},  // 128x256
+    {1, {1.852, 1.852}, 8.60, 0.46},  // 256x256
+};
+
+struct Plan {
+  int tile, slices;
+};
+Plan plan_tiles(uint32_t m, uint32_t n, uint32_t k) {
+  static const int kSlices[] = {1, 2, 3, 4, 6, 8, 12, 16};
+  const int all = (int)((k + 127) / 128);
+  double best = 1e300;
+  Plan plan{0, 1};
+  for (int t = 0; t < kNumTiles; ++t) {
+    const TileCost& c = kCost[t];
+    const long long tiles = (long long)((m + kTiles[t].bm - 1) / kTiles[t].bm) * ((n + kTiles[t].bn - 1) / kTiles[t].bn);
+    for (int s : kSlices) {
+      if (s > 1 && all < 3 * s) break;
+      const int kt = (all + s - 1) / s;
+      const long long slots = 256ll * c.occ, total = tiles * s, full = total / slots, rest = total - full * slots;
+      double us = (double)full * (c.fill + kt * c.step[c.occ - 1]);
+      if (rest > 0) {
+        const int w = (int)((rest + 255) / 256);
+        us += c.fill + kt * c.step[w - 1] * (c.idle + (1.0 - c.idle) * (double)rest / (256.0 * w));
+      }
+      if (s > 1) us += 6.1 + (double)(s + 1) * m * n * 4.0 / 10.0e6;
+      if (us < best) {
+        best = us;
+        plan = Plan{t, s};
+      }
+    }
+  }
+  return plan;
+}
+
+template <typename TOut>
+hipError_t launch_rows(const Int8Args& g, hipStream_t stream) {
+  const int tiles_n = (g.n + 15) / 16;
+#define ROWS(MT, NT, W)                                                                                          \
+  hipLaunchKernelGGL((gemm_int8_rows_kernel<MT, NT, W, TOut>), dim3((unsigned)((tiles_n + NT - 1) / NT),         \
+                     (unsigned)((g.m + 16 * MT - 1) / (16 * MT))), dim3(64 * W), 0, stream, g)
+  if (g.m <= 16) {
+    if (tiles_n >= 1024)
+      ROWS(1, 1, 4);
+    else
+      ROWS(1, 1, 16);
+  } else {
+    if (tiles_n >= 1024)
+      ROWS(2, 1, 4);
+    else
+      ROWS(2, 1, 16);
+  }
+#undef ROWS
+  return hipGetLastError();
+}
+
+constexpr uint32_t kFewRows = 32;
+
+template <typename TOut>
+hipError_t launch(Int8Args g, hipStream_t stream) {
+  const uint32_t m = (uint32_t)g.m, n = (uint32_t)g.n, k = (uint32_t)g.k;
+  if (m <= kFewRows) return launch_rows<TOut>(g, stream);
+  g.lda = g.ldw = g.k;
+  const bool aligned = k % 16 == 0 && ((uintptr_t)g.a & 15u) == 0 && ((uintptr_t)g.w & 15u) == 0;
+  if (!aligned) {
+    const int ld = (int)((k + 15) & ~15u);
+    int8_t* pa = static_cast<int8_t*>(staging(8, (size_t)m * ld));
+    int8_t* pw = static_cast<int8_t*>(staging(9, (size_t)n * ld));
+    if (pa == nullptr || pw == nullptr) return hipErrorOutOfMemory;
+    const unsigned bx = (unsigned)((ld / 16 + 63) / 64);
+    auto rows = [&](uint32_t r) { return std::min<unsigned>((r + 3) / 4, std::max(1u, 8192u / bx)); };
+    hipLaunchKernelGGL(pad_rows8_kernel, dim3(bx, rows(m)), dim3(256), 0, stream, g.a, pa, g.m, g.k, ld);
+    hipLaunchKernelGGL(pad_rows8_kernel, dim3(bx, rows(n)), dim3(256), 0, stream, g.w, pw, g.n, g.k, ld);
+    g.a = pa;
+    g.w = pw;
+    g.lda = g.ldw = ld;
+  }
+  Plan p = plan_tiles(m, n, k);
+  if (p.slices > 1) {
+    g.slabs = static_cast<int32_t*>(staging(6, (size_t)p.slices * m * n * sizeof(int32_t)));
+    if (g.slabs == nullptr) p.slices = 1;
+  }
+  g.tiles_m = (int)((m + kTiles[p.tile].bm - 1) / kTiles[p.tile].bm);
+  g.tiles_n = (int)((n + kTiles[p.tile].bn - 1) / kTiles[p.tile].bn);
+  const hipError_t e = launch_tile<TOut>(p.tile, p.slices, g, stream);
+  if (e != hipSuccess || p.slices == 1) return e;
+  hipLaunchKernelGGL((int8_slices_kernel<TOut>), dim3((n + 255) / 256, std::min<unsigned>(m, 4096u)), dim3(256), 0,
+                     stream, g.slabs, p.slices, g.a_scale, g.w_scale, static_cast<TOut*>(g.c), g.m, g.n);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_gemm_int8(const int8_t* a, const int8_t* w, const float* a_scale, const float* w_scale, void* c,
+                            bool bf16, uint32_t m, uint32_t n, uint32_t k, hipStream_t stream) {
+  Int8Args g{};
+  g.a = a;
+  g.w = w;
+  g.a_scale = a_scale;
+  g.w_scale = w_scale;
+  g.c = c;
+  g.m = (int)m;
+  g.n = (int)n;
+  g.k = (int)k;
+  return bf16 ? launch<__bf16>(g, stream) : launch<float>(g, stream);
+}
+
+}  // namespace prom

@@ -306,6 +306,62 @@ hipError_t launch_row_reduction_check(const float* in, float* out, uint32_t rows
 hipError_t launch_rmsnorm(const float* in, const float* w, float* out, float* inv_rms, uint32_t tokens,
                           uint32_t width, uint32_t stride, float eps, hipStream_t stream);
 
+// ---- the quantised decode path (int8_rows.hip, gemm_int8.hip, kv4_cache.hip, attention_kv4.hip)
+hipError_t launch_quantize_rows_int8(const void* x, bool bf16, int8_t* q, float* scales, uint32_t rows, uint32_t width,
+                                     uint32_t stride, hipStream_t stream);
+// c[m, n] (bf16 or fp32) = a_scale[i] w_scale[j] a[m, k] . w[n, k]; caller holds ctx().mu (K-slice sums and
+// padded copies in staging).  hipErrorOutOfMemory when that cannot be had.
+hipError_t launch_gemm_int8(const int8_t* a, const int8_t* w, const float* a_scale, const float* w_scale, void* c,
+                            bool bf16, uint32_t m, uint32_t n, uint32_t k, hipStream_t stream);
+// The 4-bit cache on the device; block = bytes of one head's part of a page.
+struct Kv4View {
+  uint8_t* pool;
+  const int32_t* table;
+  const int32_t* lengths;
+  int kv_heads, sequences, table_stride;
+  uint32_t pages;
+};
+constexpr int kKv4Page = 64;
+__host__ __device__ constexpr int kv4_block_bytes(int head_dim) { return kKv4Page * head_dim + 4 * head_dim; }
+// k and v: [rows][kv_heads][head_dim] with `stride` elements between rows.
+hipError_t launch_kv4_write(const Kv4View& c, int head_dim, const void* k, const void* v, bool bf16,
+                            const int32_t* row_starts, uint32_t rows, uint32_t stride, hipStream_t stream);
+hipError_t launch_kv4_read(const Kv4View& c, int head_dim, void* k, void* v, bool bf16, const int32_t* row_starts,
+                           uint32_t rows, uint32_t stride, hipStream_t stream);
+// part: fp32 partial outputs of kv4_attention_partial_bytes (0: none).
+struct Kv4AttentionArgs {
+  Kv4View c;
+  const void* q;
+  void* out;
+  const int32_t* row_starts;
+  float* part;
+  uint32_t rows, q_stride, out_stride, window, max_rows, max_length;
+  int q_heads, group;
+  float scale;
+};
+// Sequences times key heads (a workgroup at least each).
+constexpr uint64_t kKv4MaxColumns = 1ull << 23;
+size_t kv4_attention_partial_bytes(const Kv4AttentionArgs& a, int head_dim);
+hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf16, hipStream_t stream);
+
+// Largest i with starts[i] <= r (starts not decreasing, n + 1 entries), or -1 where r lies before starts[0] or
+// at or behind starts[n].  Called by a whole wave with one r; 64 places are looked at in each step.
+__device__ __forceinline__ int find_sequence(const int32_t* starts, int n, int r) {
+  const int lane = (int)threadIdx.x & 63;
+  int lo = 0, span = n + 1;
+  while (span > 1) {
+    const int step = (span + 63) >> 6;
+    const int at = lo + lane * step;
+    const bool below = at < lo + span && starts[at] <= r;
+    const int c = __popcll(__ballot(below));
+    if (c == 0) return -1;
+    const int from = lo + (c - 1) * step;
+    span = min(step, lo + span - from);
+    lo = from;
+  }
+  return lo < n && starts[lo] <= r ? lo : -1;
+}
+
 // ---- fp32 flash attention (attention_f32.hip)
 // O[t][hq*d + c] = sum_s softmax_s(scale * Q[hq][t] . K[hkv][s]) V[hkv][s][c] with
 // hkv = hq / group, keys s <= t when causal.  Element strides: Q[hq][t][c] at

@@ -55,11 +55,15 @@ DETAIL_SIZE_OVERFLOW = -6004
 DETAIL_PATH_HIP_MFMA_F32 = 6120
 DETAIL_PATH_HIP_GEMV_F32 = 6121
 DETAIL_PATH_HIP_MFMA_BF16 = 6122
+DETAIL_PATH_HIP_MFMA_INT8 = 6124
 DETAIL_HIP_UNAVAILABLE = -6905
 DETAIL_INVALID_ARGUMENT = -6906
 DETAIL_SCRATCH_LIMIT = -6930
 DETAIL_SCRATCH_UNAVAILABLE = -6931
 SGEMM_NOALLOC_SCRATCH_BYTES = 64 << 20
+DTYPE_F32, DTYPE_BF16 = 0, 1  # rows of the quantised decode path
+GEMM_INT8_MAX_K = 131071
+KV4_PAGE_TOKENS, KV4_GROUP = 64, 64
 GEMM_BF16_SWIGLU, GEMM_BF16_BLOCKED_A = 1, 2  # flags of the bf16 plan and variant entries
 GEMM_BF16_FIVE_STAGE, GEMM_BF16_STAGED = 9, 10  # kernels after the macro tiles 0-8
 # async and batch (reactor_api.h:84-114, 250-260, 282-295, 1448-1545)
@@ -439,6 +443,20 @@ class PrometheusBlockResult(Structure):
         ("end_to_end_ns", c_uint64),
         ("workspace_bytes", c_uint64),
     ]
+
+
+class PrometheusKv4Cache(Structure):
+    _fields_ = _fields("u32 struct_size, u32 head_dim, u32 kv_heads, u32 pages, u32 sequences, u32 table_stride, "
+                       "p pool, p page_table, p lengths")
+
+
+class PrometheusKv4RowsRequest(Structure):
+    _fields_ = _fields("u32 struct_size, u32 dtype, u32 rows, u32 row_stride, p k, p v, p row_starts")
+
+
+class PrometheusKv4AttentionRequest(Structure):
+    _fields_ = _fields("u32 struct_size, u32 dtype, u32 rows, u32 q_heads, u32 q_stride, u32 out_stride, u32 max_rows, "
+                       "u32 max_length, u32 window, f32 scale, p q, p out, p row_starts")
 
 
 class PrometheusAsyncStatus(Structure):
@@ -895,6 +913,22 @@ _SIGNATURES = {
     "prometheus_reactor_runtime_attention_bf16_device": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, c_uint32,
                 POINTER(c_uint32), POINTER(c_int)]),
+    "prometheus_reactor_runtime_quantize_rows_int8_device": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, c_uint32, POINTER(c_uint32),
+                POINTER(c_int)]),
+    "prometheus_reactor_runtime_gemm_int8_device": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, c_uint32,
+                POINTER(c_uint32), POINTER(c_int)]),
+    "prometheus_reactor_kv4_page_bytes": (c_uint64, [c_uint32, c_uint32]),
+    "prometheus_reactor_runtime_kv4_write_device": (
+        c_int, [c_void_p, POINTER(PrometheusKv4Cache), POINTER(PrometheusKv4RowsRequest), POINTER(c_uint32),
+                POINTER(c_int)]),
+    "prometheus_reactor_runtime_kv4_read_device": (
+        c_int, [c_void_p, POINTER(PrometheusKv4Cache), POINTER(PrometheusKv4RowsRequest), POINTER(c_uint32),
+                POINTER(c_int)]),
+    "prometheus_reactor_runtime_attention_kv4_device": (
+        c_int, [c_void_p, POINTER(PrometheusKv4Cache), POINTER(PrometheusKv4AttentionRequest), POINTER(c_uint32),
+                POINTER(c_int)]),
     "prometheus_reactor_runtime_gemm_bf16": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, POINTER(c_uint32), POINTER(c_int)]),
     "prometheus_reactor_runtime_gemm_bf16_device": (
@@ -1504,6 +1538,52 @@ class NativeRuntime:
             tokens, width, stride, eps, byref(stage), byref(detail))
         return self._check(rc, stage, detail, "rmsnorm_device")
 
+    # -- quantised decode path (device pointers as integers; a refusal raises) --
+    def quantize_rows_int8_device(self, din: int, dq: int, dscales: int, rows: int, width: int, stride: int,
+                                  dtype: int) -> int:
+        """q[r] = rint(x[r] / s[r]), s[r] = max |x[r]| / 127, for rows of `dtype` `stride` elements apart."""
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_quantize_rows_int8_device(
+            self.handle, din, dq, dscales, rows, width, stride, dtype, byref(stage), byref(detail))
+        return self._check(rc, stage, detail, "quantize_rows_int8_device")
+
+    def gemm_int8_device(self, da: int, dw: int, da_scale: int, dw_scale: int, dc: int, m: int, n: int, k: int,
+                         dtype: int) -> int:
+        """c[i, j] = a_scale[i] w_scale[j] sum_k a[i, k] w[j, k]: int8 a [m, k] and w [n, k], c [m, n] of `dtype`."""
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_gemm_int8_device(
+            self.handle, da, dw, da_scale, dw_scale, dc, m, n, k, dtype, byref(stage), byref(detail))
+        return self._check(rc, stage, detail, "gemm_int8_device")
+
+    def kv4_write_device(self, cache: PrometheusKv4Cache, dk: int, dv: int, drow_starts: int, rows: int,
+                         row_stride: int, dtype: int) -> int:
+        """Quantise the last rows of each sequence, k and v [rows, kv_heads, head_dim], into the 4-bit cache."""
+        req = PrometheusKv4RowsRequest(_KV4_ROWS_SIZE, dtype, rows, row_stride, dk, dv, drow_starts)
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_kv4_write_device(self.handle, byref(cache), byref(req), byref(stage),
+                                                                  byref(detail))
+        return self._check(rc, stage, detail, "kv4_write_device")
+
+    def kv4_read_device(self, cache: PrometheusKv4Cache, dk: Optional[int], dv: Optional[int], drow_starts: int,
+                        rows: int, row_stride: int, dtype: int) -> int:
+        """What the cache holds for the last rows of each sequence (either output may be None)."""
+        req = PrometheusKv4RowsRequest(_KV4_ROWS_SIZE, dtype, rows, row_stride, dk, dv, drow_starts)
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_kv4_read_device(self.handle, byref(cache), byref(req), byref(stage),
+                                                                 byref(detail))
+        return self._check(rc, stage, detail, "kv4_read_device")
+
+    def attention_kv4_device(self, cache: PrometheusKv4Cache, dq: int, dout: int, drow_starts: int, rows: int,
+                             q_heads: int, q_stride: int, out_stride: int, max_rows: int, max_length: int, window: int,
+                             scale: float, dtype: int) -> int:
+        """Attention of the last rows of each sequence, q and out [rows, q_heads, head_dim], over the 4-bit cache."""
+        req = PrometheusKv4AttentionRequest(_KV4_ATTENTION_SIZE, dtype, rows, q_heads, q_stride, out_stride, max_rows,
+                                            max_length, window, scale, dq, dout, drow_starts)
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_attention_kv4_device(self.handle, byref(cache), byref(req),
+                                                                      byref(stage), byref(detail))
+        return self._check(rc, stage, detail, "attention_kv4_device")
+
     # -- asynchronous SGEMM (bridge.go:438-470) ------------------------------
     def submit_async(self, m: int, n: int, k: int, a, b) -> Tuple[int, int, CallStatus]:
         """Returns (rc, task_id, status); A and B may be reused as soon as this returns."""
@@ -1624,6 +1704,23 @@ class NativeRuntime:
         if rc != PROM_OK:
             raise ReactorIssue("diagnostics_failed", f"batch_diagnostics returned {rc}")
         return d
+
+
+_KV4_ROWS_SIZE = ctypes.sizeof(PrometheusKv4RowsRequest)
+_KV4_ATTENTION_SIZE = ctypes.sizeof(PrometheusKv4AttentionRequest)
+
+
+def kv4_cache(pool: int, page_table: int, lengths: int, head_dim: int, kv_heads: int, pages: int, sequences: int,
+              table_stride: int) -> PrometheusKv4Cache:
+    """The 4-bit cache that a program keeps in its own device memory: pool of pages * kv4_page_bytes bytes,
+    page_table int32 [sequences, table_stride], lengths int32 [sequences] (device pointers)."""
+    return PrometheusKv4Cache(ctypes.sizeof(PrometheusKv4Cache), head_dim, kv_heads, pages, sequences, table_stride, pool,
+                              page_table, lengths)
+
+
+def kv4_page_bytes(head_dim: int, kv_heads: int, lib: Optional[ctypes.CDLL] = None) -> int:
+    """Bytes of one page of the 4-bit cache; 0 for sizes it does not take."""
+    return int((lib or shared_library()).prometheus_reactor_kv4_page_bytes(head_dim, kv_heads))
 
 
 def sgemm_plan(m: int, n: int, k: int, lib: Optional[ctypes.CDLL] = None) -> Tuple[int, PrometheusSgemmPlanInfo]:

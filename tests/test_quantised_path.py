@@ -1,0 +1,229 @@
+"""The quantised decode path without a device: the oracle's definitions, and every refusal of
+the entry points.  Refusals are checked on a runtime that has no device, so that nothing is
+launched; valid arguments stop there at INIT with the runtime's own detail."""
+from __future__ import annotations
+
+import ctypes
+from ctypes import byref, c_int, c_uint32
+
+import numpy as np
+import pytest
+
+import oracle
+from oracle import quantised as oq
+from oct_amd import prometheus as p
+
+OK = 1 << 20  # an aligned address; nothing is dereferenced on these paths
+
+
+@pytest.fixture(scope="module")
+def rt():
+    runtime = p.NativeRuntime(test_flags=p.TESTCFG_SKIP_VULKAN_INIT)
+    yield runtime
+    runtime.close()
+
+
+# ------------------------------------------------------------------ definitions
+def test_cache_values_stay_within_a_step():
+    x = oracle.normal(3, (500, 128)) * np.exp2(oracle.uniform(4, (500, 1), -60.0, 60.0))
+    codes, steps = oq.kv4_quantise(x)
+    v = oq.kv4_values(codes, steps)
+    step = np.repeat((steps.astype(np.uint32) << 16).view(np.float32), 64, axis=-1)
+    assert np.all(np.abs(v - x) <= step * (1 + 1e-6))
+    # at most 1/32 above the largest magnitude / 6, and never below it
+    top = np.abs(x.reshape(500, 2, 64)).max(-1)
+    assert np.all(step[:, ::64] * 6 >= top * (1 - 1e-6)) and np.all(step[:, ::64] * 6 <= top * (1 + 1 / 16))
+    # eight significant bits: bf16 holds every value
+    assert np.array_equal(oracle.from_bf16(oracle.to_bf16(v.astype(np.float32))).astype(np.float64), v)
+
+
+def test_cache_ties_go_to_the_even_code():
+    x = np.zeros((1, 64), np.float32)
+    x[0, :9] = [6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -5.0]  # step 1
+    v = oq.kv4_values(*oq.kv4_quantise(x))[0, :9]
+    assert v.tolist() == [6.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, -4.0]
+
+
+def test_key_order_is_a_permutation_within_groups_of_64():
+    for dim in (64, 128, 256):
+        order = oq.key_order(dim)
+        assert sorted(order) == list(range(dim))
+        assert np.array_equal(order[8 * np.arange(dim // 8)] % 8, np.zeros(dim // 8))
+
+
+def test_page_bytes():
+    assert p.kv4_page_bytes(128, 8) == 8 * (64 * 128 + 4 * 128)
+    assert p.kv4_page_bytes(64, 1) == 64 * 64 + 256 and p.kv4_page_bytes(256, 1024) == 1024 * 17408
+    for dim, heads in ((0, 1), (32, 1), (96, 1), (512, 1), (128, 0), (128, 1025)):
+        assert p.kv4_page_bytes(dim, heads) == 0
+
+
+# ------------------------------------------------------------------ refusals
+def _call(rt, name, *args):
+    stage, detail = c_uint32(99), c_int(99)
+    rc = getattr(rt.lib, name)(rt.handle, *args, byref(stage), byref(detail))
+    return rc, stage.value, detail.value
+
+
+def _refused(result):
+    return result == (p.PROM_ERROR, p.STAGE_INIT, p.DETAIL_INVALID_ARGUMENT)
+
+
+def _no_device(result):
+    return result == (p.PROM_ERROR, p.STAGE_INIT, p.DETAIL_HIP_UNAVAILABLE)
+
+
+ROWS = dict(x=OK, q=OK, s=OK, rows=4, width=64, stride=64, dtype=p.DTYPE_BF16)
+
+
+def _rows(rt, **change):
+    a = dict(ROWS, **change)
+    return _call(rt, "prometheus_reactor_runtime_quantize_rows_int8_device", a["x"], a["q"], a["s"], a["rows"],
+                 a["width"], a["stride"], a["dtype"])
+
+
+@pytest.mark.parametrize("change", [dict(x=0), dict(q=0), dict(s=0), dict(rows=0), dict(width=0), dict(stride=63),
+                                    dict(dtype=2), dict(x=OK + 1), dict(x=OK + 2, dtype=p.DTYPE_F32), dict(s=OK + 2),
+                                    dict(rows=1 << 20, stride=1 << 20)])
+def test_quantize_rows_refuses(rt, change):
+    assert _refused(_rows(rt, **change)), change
+
+
+def test_quantize_rows_takes(rt):
+    for change in ({}, dict(x=OK + 2, q=OK + 1), dict(stride=65), dict(rows=(1 << 20) - 1, stride=1 << 20)):
+        assert _no_device(_rows(rt, **change)), change
+
+
+PRODUCT = dict(a=OK, w=OK, sa=OK, sw=OK, c=OK, m=3, n=5, k=7, dtype=p.DTYPE_F32)
+
+
+def _product(rt, **change):
+    a = dict(PRODUCT, **change)
+    return _call(rt, "prometheus_reactor_runtime_gemm_int8_device", a["a"], a["w"], a["sa"], a["sw"], a["c"], a["m"],
+                 a["n"], a["k"], a["dtype"])
+
+
+def test_int8_product_refuses_in_the_order_of_the_other_products(rt):
+    for name in ("a", "w", "sa", "sw", "c"):
+        assert _product(rt, **{name: 0, "m": 0}) == (p.PROM_ERROR, p.STAGE_TRANSFER_IN, p.PROM_ERROR)
+    for name in ("m", "n", "k"):
+        assert _product(rt, **{name: 0}) == (p.PROM_ERROR, p.STAGE_INIT, p.PROM_ERROR)
+    for change in (dict(m=1 << 16, n=1 << 16), dict(m=1 << 31), dict(n=1 << 20, k=1 << 12)):
+        assert _product(rt, **change) == (p.PROM_ERROR, p.STAGE_TRANSFER_IN, p.DETAIL_SIZE_OVERFLOW), change
+    for change in (dict(k=p.GEMM_INT8_MAX_K + 1), dict(dtype=2), dict(sa=OK + 2), dict(sw=OK + 1), dict(c=OK + 2),
+                   dict(c=OK + 1, dtype=p.DTYPE_BF16)):
+        assert _refused(_product(rt, **change)), change
+    for change in ({}, dict(k=p.GEMM_INT8_MAX_K), dict(a=OK + 1, w=OK + 3), dict(c=OK + 2, dtype=p.DTYPE_BF16)):
+        assert _no_device(_product(rt, **change)), change
+
+
+CACHE = dict(head_dim=128, kv_heads=2, pages=5, sequences=3, table_stride=4, pool=OK, page_table=OK, lengths=OK)
+BAD_CACHES = [dict(struct_size=8), dict(head_dim=96), dict(head_dim=0), dict(kv_heads=0), dict(kv_heads=1025),
+              dict(pages=0), dict(pages=1 << 31), dict(sequences=0), dict(sequences=(1 << 20) + 1),
+              dict(sequences=1 << 20, kv_heads=9), dict(table_stride=0), dict(table_stride=(1 << 24) + 1), dict(pool=0),
+              dict(pool=OK + 8), dict(page_table=0), dict(page_table=OK + 2), dict(lengths=0), dict(lengths=OK + 1)]
+
+
+def _struct(cls, values):
+    s = cls()
+    s.struct_size = ctypes.sizeof(cls)
+    for name, value in values.items():
+        setattr(s, name, value)
+    return s
+
+
+def _cache_call(rt, name, cls, cache, request):
+    c = None if cache is None else byref(_struct(p.PrometheusKv4Cache, cache))
+    r = None if request is None else byref(_struct(cls, request))
+    return _call(rt, name, c, r)
+
+
+CACHE_ROWS = dict(dtype=p.DTYPE_F32, rows=6, row_stride=256, k=OK, v=OK, row_starts=OK)
+
+
+def _cache_rows(rt, write, cache=CACHE, request=CACHE_ROWS):
+    name = "prometheus_reactor_runtime_kv4_%s_device" % ("write" if write else "read")
+    return _cache_call(rt, name, p.PrometheusKv4RowsRequest, cache, request)
+
+
+@pytest.mark.parametrize("write", (True, False))
+def test_cache_rows_refuse(rt, write):
+    assert _refused(_cache_rows(rt, write, cache=None)) and _refused(_cache_rows(rt, write, request=None))
+    for change in BAD_CACHES:
+        assert _refused(_cache_rows(rt, write, cache=dict(CACHE, **change))), change
+    for change in (dict(struct_size=4), dict(dtype=2), dict(rows=0), dict(rows=(1 << 24) + 1), dict(row_stride=255),
+                   dict(row_stride=1 << 24), dict(k=OK + 2), dict(v=OK + 1), dict(k=0, v=0), dict(row_starts=0),
+                   dict(row_starts=OK + 2)):
+        assert _refused(_cache_rows(rt, write, request=dict(CACHE_ROWS, **change))), change
+    for change in (dict(k=0), dict(v=0)):
+        result = _cache_rows(rt, write, request=dict(CACHE_ROWS, **change))
+        assert _refused(result) if write else _no_device(result), change
+    assert _no_device(_cache_rows(rt, write))
+    assert _no_device(_cache_rows(rt, write, request=dict(CACHE_ROWS, dtype=p.DTYPE_BF16, k=OK + 2, v=OK + 6)))
+
+
+ATTENTION = dict(dtype=p.DTYPE_BF16, rows=6, q_heads=8, q_stride=1024, out_stride=1024, max_rows=4, max_length=200,
+                 window=0, scale=0.1, q=OK, out=OK, row_starts=OK)
+
+
+def _attention(rt, cache=CACHE, request=ATTENTION):
+    return _cache_call(rt, "prometheus_reactor_runtime_attention_kv4_device", p.PrometheusKv4AttentionRequest, cache,
+                       request)
+
+
+def test_attention_refuses(rt):
+    assert _refused(_attention(rt, cache=None)) and _refused(_attention(rt, request=None))
+    for change in BAD_CACHES:
+        assert _refused(_attention(rt, cache=dict(CACHE, **change))), change
+    for change in (dict(struct_size=4), dict(dtype=2), dict(rows=0), dict(rows=(1 << 24) + 1), dict(q_heads=0),
+                   dict(q_heads=7), dict(q_heads=(1 << 16) + 2), dict(q_stride=1023), dict(q_stride=1 << 24),
+                   dict(out_stride=1023), dict(out_stride=1 << 24), dict(max_rows=0), dict(max_rows=7),
+                   dict(max_length=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
+                   dict(scale=float("nan")), dict(q=0), dict(q=OK + 1), dict(out=0), dict(out=OK + 1),
+                   dict(row_starts=0), dict(row_starts=OK + 2), dict(dtype=p.DTYPE_F32, q=OK + 2)):
+        assert _refused(_attention(rt, request=dict(ATTENTION, **change))), change
+    assert _no_device(_attention(rt))
+    assert _no_device(_attention(rt, request=dict(ATTENTION, window=1, max_length=0xFFFFFFFF, q=OK + 2, out=OK + 6)))
+
+
+def test_unknown_handles_are_refused(rt):
+    stage, detail = c_uint32(99), c_int(99)
+    lib = rt.lib
+    calls = [
+        lambda: lib.prometheus_reactor_runtime_quantize_rows_int8_device(OK, OK, OK, OK, 1, 1, 1, 0, byref(stage), byref(detail)),
+        lambda: lib.prometheus_reactor_runtime_gemm_int8_device(OK, OK, OK, OK, OK, OK, 1, 1, 1, 0, byref(stage), byref(detail)),
+        lambda: lib.prometheus_reactor_runtime_kv4_write_device(OK, None, None, byref(stage), byref(detail)),
+        lambda: lib.prometheus_reactor_runtime_kv4_read_device(None, None, None, byref(stage), byref(detail)),
+        lambda: lib.prometheus_reactor_runtime_attention_kv4_device(OK, None, None, None, None),
+    ]
+    for call in calls:
+        stage.value = detail.value = 99
+        assert call() == p.PROM_INVALID_HANDLE
+    # the wrappers raise what the library refuses
+    with pytest.raises(p.ReactorIssue):
+        rt.quantize_rows_int8_device(0, OK, OK, 1, 1, 1, p.DTYPE_F32)
+    with pytest.raises(p.ReactorIssue):
+        rt.attention_kv4_device(p.kv4_cache(0, OK, OK, 128, 1, 1, 1, 1), OK, OK, OK, 1, 1, 128, 128, 1, 1, 0, 1.0,
+                                p.DTYPE_F32)
+
+
+def test_struct_layouts_match_the_header(tmp_path):
+    import subprocess
+    from pathlib import Path
+
+    header = Path(p.PACKAGE_DIR).parent / "include" / "prometheus_reactor.h"
+    classes = (p.PrometheusKv4Cache, p.PrometheusKv4RowsRequest, p.PrometheusKv4AttentionRequest)
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{header}"', "int main(void){"]
+    expect = []
+    for cls in classes:
+        lines.append(f'printf("%zu\\n", sizeof({cls.__name__}));')
+        expect.append(ctypes.sizeof(cls))
+        for field, _ in cls._fields_:
+            lines.append(f'printf("%zu\\n", offsetof({cls.__name__}, {field}));')
+            expect.append(getattr(cls, field).offset)
+    lines.append(f'printf("%u %u %u %u\\n", PROM_GEMM_INT8_MAX_K, PROM_KV4_PAGE_TOKENS, PROM_DTYPE_BF16, PROM_DETAIL_PATH_HIP_MFMA_INT8);')
+    (tmp_path / "l.c").write_text("\n".join(lines + ["return 0;}"]))
+    subprocess.run(["gcc", "-std=c11", "-o", str(tmp_path / "l"), str(tmp_path / "l.c")], check=True)
+    out = subprocess.run([str(tmp_path / "l")], capture_output=True, text=True, check=True).stdout.split()
+    assert [int(v) for v in out] == expect + [p.GEMM_INT8_MAX_K, p.KV4_PAGE_TOKENS, p.DTYPE_BF16,
+                                              p.DETAIL_PATH_HIP_MFMA_INT8]
