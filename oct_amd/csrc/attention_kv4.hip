@@ -36,6 +36,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
@@ -93,58 +94,56 @@ __device__ __forceinline__ void terms(float x, __bf16 (&t)[kN]) {
   t[kN - 1] = (__bf16)x;
 }
 
+// One head's part of a page in LDS, as it lies in memory but for the order of the 16-byte
+// chunks within a token's row, which is chosen so that an operand read's 16 tokens fall into
+// different banks: chunk c of token t is at c ^ key_swz(t) (tokens 16 a + 4 c + b for one c are
+// read together) or c ^ value_swz(t) (16 neighbours).  Filled by whole transfers of 1 KiB.
 template <int D>
-struct Page {
-  static constexpr int kG = D / 64;
-  static constexpr int kK = D >= 128 ? D / 128 : 1;  // 16-byte loads (8 for D = 64) of a key row's quarter
-  u32x4 k[4][kK];
-  u32x4 v[D / 32];
-  u32x4 ks[kG][2], vs[kG][2];
-};
+struct Stage {
+  static constexpr int kRow = D / 2;
+  static constexpr int kCodes = kKv4Page * kRow;  // keys, then values
+  static constexpr int kSteps = 2 * kCodes;       // keys' steps [D / 64][64], then the values'
+  static constexpr int kMoves = (kv4_block_bytes(D) + 1023) / 1024;
+  static constexpr int kBytes = 1024 * kMoves;
+  static_assert(2 * kMoves < 64, "transfers in flight");
 
-// Every page is read whole: what lies behind a sequence's last token is masked by its use.
-template <int D>
-__device__ __forceinline__ void load_page(Page<D>& p, const uint8_t* block, int lane) {
-  const int r = lane & 15, h = lane >> 4;
+  __device__ static __forceinline__ int key_swz(int t) {
+    return D == 64 ? (t >> 4) & 1 : D == 128 ? (t >> 4) & 3 : ((t >> 4) & 3) | ((t << 1) & 4);
+  }
+  __device__ static __forceinline__ int value_swz(int t) {
+    return D == 64 ? (t >> 3) & 1 : D == 128 ? (t >> 2) & 3 : (t >> 1) & 7;
+  }
+  // Queues the transfers of a block to LDS address `to` (a wave's own stage).
+  __device__ static __forceinline__ void fill(const uint8_t* block, uint32_t to, int lane) {
+    const unsigned long long a = (unsigned long long)block;
+    intx4 d;
+    d.x = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffu));
+    d.y = __builtin_amdgcn_readfirstlane((int)(a >> 32));
+    d.z = kv4_block_bytes(D);
+    d.w = 0x00020000;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const uint8_t* row = block + (16 * (r >> 2) + 4 * c + (r & 3)) * (D / 2);
-    if constexpr (D == 64) {
-      const u32x2 w = *reinterpret_cast<const u32x2*>(row + 8 * h);
-      p.k[c][0] = u32x4{w.x, w.y, 0u, 0u};
-    } else {
-#pragma unroll
-      for (int j = 0; j < Page<D>::kK; ++j) p.k[c][j] = *reinterpret_cast<const u32x4*>(row + 64 * j + 16 * h);
+    for (int i = 0; i < kMoves; ++i) {
+      const int at = 1024 * i + 16 * lane;
+      uint32_t off = (uint32_t)at;
+      if (1024 * i < kSteps) {
+        const int t = at % kCodes / kRow;
+        off ^= (uint32_t)(16 * (1024 * i < kCodes ? key_swz(t) : value_swz(t)));
+      }
+      const uint32_t m0 = __builtin_amdgcn_readfirstlane(to + 1024 * i);
+      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(off), "s"(d)
+                   : "memory", "m0");
     }
   }
-  const uint8_t* v = block + kKv4Page * D / 2;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) p.v[i] = *reinterpret_cast<const u32x4*>(v + 1024 * i + 16 * lane);
-  const uint8_t* s = block + kKv4Page * D + 32 * h;
-#pragma unroll
-  for (int g = 0; g < Page<D>::kG; ++g)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      p.ks[g][j] = *reinterpret_cast<const u32x4*>(s + 128 * g + 16 * j);
-      p.vs[g][j] = *reinterpret_cast<const u32x4*>(s + 128 * (Page<D>::kG + g) + 16 * j);
-    }
-}
-
-// Position of 16-byte chunk c of token t's value row in LDS, so that 16 neighbouring
-// tokens' reads of one chunk fall into different banks.
-template <int D>
-__device__ __forceinline__ int value_swz(int t) {
-  return D == 64 ? (t >> 3) & 1 : D == 128 ? (t >> 2) & 3 : (t >> 1) & 7;
-}
+};
 
 template <bool kF32, int D>
-__global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Kernel g) {
+__global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4Kernel g) {
   constexpr int kG = D / 64, kQT = kF32 ? 3 : 1, kPT = kF32 ? 3 : 2;
   constexpr int kSteps = D / 32;  // MFMA steps of 32 channels
   constexpr int kB = D / 16;      // blocks of 16 output channels
-  constexpr int kValueBytes = kKv4Page * D / 2;
+  using St = Stage<D>;
   constexpr int kJoinBytes = kTileRows * (D + 4) * 4;  // a wave's sums [16][D], maxima, weights
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * (kValueBytes > kJoinBytes ? kValueBytes : kJoinBytes)];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kWaves * (2 * St::kBytes > kJoinBytes ? 2 * St::kBytes : kJoinBytes)];
 
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -164,8 +163,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Ker
   const long long room = (long long)g.c.table_stride * kKv4Page;
   const int length = max(g.c.lengths[seq], 0);
   const int32_t* table = g.c.table + (size_t)seq * g.c.table_stride;
-  const size_t block_bytes = kv4_block_bytes(D);
-  uint8_t* my_lds = lds + wave * kValueBytes;
+  const uint8_t* mine_lds = lds + wave * 2 * St::kBytes;
+  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) const uint8_t*)mine_lds;
 
   const long long tiles = ((long long)n * g.group + kTileRows - 1) / kTileRows;
   for (long long tile = tile0; tile < tiles; tile += g.tiles) {
@@ -217,43 +216,61 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Ker
     };
     auto page_block = [&](uint32_t number) -> const uint8_t* {
       const uint32_t ok = number < g.c.pages ? number : 0u;
-      return g.c.pool + ((size_t)ok * g.c.kv_heads + head) * block_bytes;
+      return g.c.pool + ((size_t)ok * g.c.kv_heads + head) * kv4_block_bytes(D);
     };
-    Page<D> cur;
+    // Two stages: the next page is on its way while this one is worked on.  The transfers
+    // are the loop's only vector memory operations, and a wave waits for its own alone.
     uint32_t number = page_number(pg), next_number = page_number(pg + stride);
-    if (pg < last) load_page<D>(cur, page_block(number), lane);
+    int now = 0;
+    if (pg < last) St::fill(page_block(number), lds0, lane);
     for (; pg < last; pg += stride) {
-      Page<D> next;
+      // The other stage's reads have returned before it is filled again.
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       const uint32_t after = page_number(pg + 2 * stride);
-      if (pg + stride < last) load_page<D>(next, page_block(next_number), lane);
-
-      // Values to LDS, chunk swizzled; a wave's own region, in order with its reads.
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const int at = 1024 * i + 16 * lane, t = at / (D / 2), c = (at % (D / 2)) / 16;
-        *reinterpret_cast<u32x4*>(my_lds + t * (D / 2) + 16 * (c ^ value_swz<D>(t))) = cur.v[i];
+      if (pg + stride < last) {
+        St::fill(page_block(next_number), lds0 + (now ^ 1) * St::kBytes, lane);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(St::kMoves) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       }
-      __builtin_amdgcn_wave_barrier();
-      asm volatile("" ::: "memory");
+      const uint8_t* stage = mine_lds + now * St::kBytes;
 
+      u32x4 ks[kG][2];
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          ks[gr][j] = *reinterpret_cast<const u32x4*>(stage + St::kSteps + 128 * gr + 32 * h + 16 * j);
       floatx4 s[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
+        // Row r of the operand is token 16 (r / 4) + 4 c + r % 4.
+        const int t = 16 * (r16 >> 2) + 4 * c + (r16 & 3);
+        uint32_t k[kSteps];
+        if constexpr (D == 64) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(stage + t * St::kRow + ((8 * h) ^ (16 * St::key_swz(t))));
+          k[0] = w.x, k[1] = w.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < kSteps / 4; ++j) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(stage + t * St::kRow + 16 * ((4 * j + h) ^ St::key_swz(t)));
+            k[4 * j] = w.x, k[4 * j + 1] = w.y, k[4 * j + 2] = w.z, k[4 * j + 3] = w.w;
+          }
+        }
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
           floatx4 acc = {};
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int st = 2 * gr + u;
-            const bf16x8 kf = numbers(D == 64 ? cur.k[c][0][st] : cur.k[c][st / 4][st % 4]);
+            const bf16x8 kf = numbers(k[st]);
 #pragma unroll
             for (int i = 0; i < kQT; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[st][i], acc, 0, 0, 0);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = 4 * c + i;
-            const float step = step_of(cur.ks[gr][j / 8][j / 2 % 4], j & 1);
+            const float step = step_of(ks[gr][j / 8][j / 2 % 4], j & 1);
             s[c][i] = gr == 0 ? acc[i] * step : __builtin_fmaf(acc[i], step, s[c][i]);
           }
         }
@@ -301,11 +318,15 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Ker
         }
 #pragma unroll
       for (int gr = 0; gr < kG; ++gr) {
+        u32x4 vs[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          vs[j] = *reinterpret_cast<const u32x4*>(stage + St::kSteps + 128 * (kG + gr) + 32 * h + 16 * j);
         // P s in bf16 terms, tokens 16 h + 0..7 and 8..15.
         bf16x8 pf[2][kPT];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          float step = step_of(cur.vs[gr][j / 8][j / 2 % 4], j & 1);
+          float step = step_of(vs[j / 8][j / 2 % 4], j & 1);
           if (edge && s[j / 4][j % 4] == -INFINITY) step = 0.0f;  // a token not seen may hold anything
           __bf16 t[kPT];
           terms(p[j] * step, t);
@@ -315,8 +336,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Ker
 #pragma unroll
         for (int bl = 4 * gr; bl < 4 * gr + 4; ++bl) {
           const int t = 16 * h + r16;
-          const int at = t * (D / 2) + 16 * ((bl >> 1) ^ value_swz<D>(t)) + 8 * (bl & 1);
-          const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(my_lds + at));
+          const int at = St::kCodes + t * St::kRow + 16 * ((bl >> 1) ^ St::value_swz(t)) + 8 * (bl & 1);
+          const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(stage + at));
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const bf16x8 vf = numbers((uint32_t)w[u]);
@@ -325,7 +346,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Ker
           }
         }
       }
-      cur = next;
+      now ^= 1;
       number = next_number;
       next_number = after;
     }
