@@ -43,6 +43,7 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 constexpr float kLazyLog2 = 8.0f;
 constexpr int kTileRows = 16;
 constexpr int kWaves = 4;
+constexpr int kMaxSplits = 64;  // a lane each when they are joined
 constexpr uint64_t kMostPartialBytes = 1ull << 30;
 
 struct Kv4Kernel {
@@ -50,12 +51,15 @@ struct Kv4Kernel {
   const void* q;
   void* out;
   const int32_t* starts;
-  float* part;  // [splits][rows][q_heads][D + 2]: sums, maximum, weight
+  float* part;  // sums [splits][rows][q_heads][D], then (maximum, weight) [splits][rows][q_heads]
+  size_t ends;  // where these begin
   int rows, q_stride, out_stride;
   int q_heads, group, tiles, splits;
   uint32_t window;
   float scale_log2;
 };
+
+__device__ __forceinline__ float* ends(const Kv4Kernel& g) { return g.part + g.ends; }
 
 // max / sum of v over lanes l and l ^ 16.
 __device__ __forceinline__ float max_rows16(float v) {
@@ -162,7 +166,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
   if (n <= 0) return;
   const long long room = (long long)g.c.table_stride * kKv4Page;
   const int length = max(g.c.lengths[seq], 0);
-  const int32_t* table = g.c.table + (size_t)seq * g.c.table_stride;
+  // Constant address space: page numbers come by scalar loads, which do not wait for the
+  // transfers of pages as vector loads would.
+  const auto* table = (const __attribute__((address_space(4))) int32_t*)(g.c.table + (size_t)seq * g.c.table_stride);
   const uint8_t* mine_lds = lds + wave * 2 * St::kBytes;
   const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) const uint8_t*)mine_lds;
 
@@ -212,7 +218,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
     const int stride = g.splits * kWaves;
     int pg = page0 + split * kWaves + wave;
     auto page_number = [&](int p) -> uint32_t {
-      return p < last && p < g.c.table_stride ? (uint32_t)__builtin_amdgcn_readfirstlane(table[p]) : 0xFFFFFFFFu;
+      return p < last && p < g.c.table_stride ? (uint32_t)table[p] : 0xFFFFFFFFu;
     };
     auto page_block = [&](uint32_t number) -> const uint8_t* {
       const uint32_t ok = number < g.c.pages ? number : 0u;
@@ -322,12 +328,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           vs[j] = *reinterpret_cast<const u32x4*>(stage + St::kSteps + 128 * (kG + gr) + 32 * h + 16 * j);
+        if (edge) {  // a token not seen may hold anything: its step counts as 0
+#pragma unroll
+          for (int j = 0; j < 16; j += 2)
+            vs[j / 8][j / 2 % 4] &= (s[j / 4][j % 4] == -INFINITY ? 0u : 0xFFFFu) |
+                                    (s[j / 4][j % 4 + 1] == -INFINITY ? 0u : 0xFFFF0000u);
+        }
         // P s in bf16 terms, tokens 16 h + 0..7 and 8..15.
         bf16x8 pf[2][kPT];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          float step = step_of(vs[j / 8][j / 2 % 4], j & 1);
-          if (edge && s[j / 4][j % 4] == -INFINITY) step = 0.0f;  // a token not seen may hold anything
+          const float step = step_of(vs[j / 8][j / 2 % 4], j & 1);
           __bf16 t[kPT];
           terms(p[j] * step, t);
 #pragma unroll
@@ -381,12 +392,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
       const int er = first_row + (int)(xe / g.group);
       const int eh = head * g.group + (int)(xe % g.group);
       if (g.splits > 1) {
-        float* part = g.part + (((size_t)split * g.rows + er) * g.q_heads + eh) * (D + 2);
-        part[d] = sum;
-        if (d == 0) {
-          part[D] = top;
-          part[D + 1] = weight;
-        }
+        const size_t at = ((size_t)split * g.rows + er) * g.q_heads + eh;
+        g.part[at * D + d] = sum;
+        if (d == 0) reinterpret_cast<float2*>(ends(g))[at] = make_float2(top, weight);
       } else {
         const float v = weight == 0.0f ? 0.0f : sum / weight;
         const size_t at = (size_t)er * g.out_stride + (size_t)eh * D + d;
@@ -400,35 +408,61 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
   }
 }
 
-// One wave a row and query head: joins the splits' sums in order.
+// One workgroup a row and query head joins the splits' sums.  Its threads are D / 4 columns of
+// four channels times kParts: part i adds splits i, i + kParts, ..., the parts are added in
+// order.  Bound by latency: maxima and weights come in one load a lane, sums four at a time.
 template <bool kF32, int D>
 __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
+  constexpr int kColumns = D / 4, kParts = 256 / kColumns;
+  __shared__ floatx4 parts[kParts][kColumns];
+  __shared__ float factors[kMaxSplits];
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int column = tid % kColumns, part = tid / kColumns;
   const long long pairs = (long long)g.rows * g.q_heads;
-  const int lane = (int)threadIdx.x & 63;
-  for (long long x = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); x < pairs; x += (long long)gridDim.x * 4) {
+  for (long long x = blockIdx.x; x < pairs; x += gridDim.x) {
     const int row = (int)(x / g.q_heads);
     if (find_sequence(g.starts, g.c.sequences, row) < 0) continue;
-    const float* part = g.part + (size_t)x * (D + 2);
-    const size_t slab = (size_t)pairs * (D + 2);
-    float top = -INFINITY;
-    for (int s = 0; s < g.splits; ++s) top = fmaxf(top, part[s * slab + D]);
-    float sum[D / 64] = {}, weight = 0.0f;
-    for (int s = 0; s < g.splits; ++s) {
-      const float* a = part + s * slab;
-      const float f = a[D] == top ? 1.0f : __builtin_amdgcn_exp2f((a[D] - top) * g.scale_log2);
-      weight = __builtin_fmaf(a[D + 1], f, weight);
-#pragma unroll
-      for (int j = 0; j < D / 64; ++j) sum[j] = __builtin_fmaf(a[lane + 64 * j], f, sum[j]);
+    float top = -INFINITY, weight = 0.0f;
+    if (lane < g.splits) {
+      const float2 e = reinterpret_cast<const float2*>(ends(g))[(size_t)lane * pairs + x];
+      top = e.x;
+      weight = e.y;
     }
-    const size_t at = (size_t)row * g.out_stride + (size_t)(x - (long long)row * g.q_heads) * D + lane;
+    const float mine = top;
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-      const float v = weight == 0.0f ? 0.0f : sum[j] / weight;
-      if constexpr (kF32)
-        static_cast<float*>(g.out)[at + 64 * j] = v;
-      else
-        static_cast<__bf16*>(g.out)[at + 64 * j] = (__bf16)v;
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float f = mine == top ? 1.0f : __builtin_amdgcn_exp2f((mine - top) * g.scale_log2);
+    weight = lane < g.splits ? weight * f : 0.0f;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) weight += __shfl_xor(weight, d);
+    if (tid < g.splits) factors[tid] = f;
+    __syncthreads();
+    floatx4 sum = {};
+    const floatx4* at = reinterpret_cast<const floatx4*>(g.part + (size_t)x * D) + column;
+    const size_t slab = (size_t)pairs * kColumns;
+#pragma unroll 4
+    for (int s = part; s < g.splits; s += kParts) {
+      const floatx4 v = at[s * slab];
+      const float fs = factors[s];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(v[i], fs, sum[i]);
     }
+    parts[part][column] = sum;
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int i = 1; i < kParts; ++i) sum += parts[i][column];
+      const size_t to = (size_t)row * g.out_stride + (size_t)(x - (long long)row * g.q_heads) * D + 4 * column;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float v = weight == 0.0f ? 0.0f : sum[i] / weight;
+        if constexpr (kF32)
+          static_cast<float*>(g.out)[to + i] = v;
+        else
+          static_cast<__bf16*>(g.out)[to + i] = (__bf16)v;
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -444,7 +478,7 @@ void plan(const Kv4AttentionArgs& a, int head_dim, int* tiles, int* splits) {
   if (a.window) length = std::min<uint64_t>(length, (uint64_t)a.window + 2 * kKv4Page);
   const uint64_t pages = (length + kKv4Page - 1) / kKv4Page;
   const uint64_t want = (2048 + base - 1) / base, most = (pages + 2 * kWaves - 1) / (2 * kWaves);
-  *splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({want, most, 64}));
+  *splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({want, most, kMaxSplits}));
   if ((uint64_t)*splits * a.rows * (uint64_t)a.q_heads * (uint64_t)(head_dim + 2) * 4 > kMostPartialBytes) *splits = 1;
 }
 
@@ -454,7 +488,7 @@ hipError_t launch(const Kv4Kernel& g, hipStream_t stream) {
   hipLaunchKernelGGL((kv4_attention_kernel<kF32, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, stream, g);
   if (g.splits > 1) {
     const uint64_t pairs = (uint64_t)g.rows * (uint64_t)g.q_heads;
-    hipLaunchKernelGGL((kv4_join_kernel<kF32, D>), dim3((unsigned)std::min<uint64_t>((pairs + 3) / 4, 1u << 20)), dim3(256),
+    hipLaunchKernelGGL((kv4_join_kernel<kF32, D>), dim3((unsigned)std::min<uint64_t>(pairs, 1u << 20)), dim3(256),
                        0, stream, g);
   }
   return hipGetLastError();
@@ -483,6 +517,7 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf
   g.window = a.window;
   g.scale_log2 = a.scale * 1.4426950408889634f;
   plan(a, head_dim, &g.tiles, &g.splits);
+  g.ends = (size_t)g.splits * a.rows * (size_t)a.q_heads * (size_t)head_dim;
   switch (head_dim) {
     case 64: return bf16 ? launch<false, 64>(g, stream) : launch<true, 64>(g, stream);
     case 128: return bf16 ? launch<false, 128>(g, stream) : launch<true, 128>(g, stream);
