@@ -988,7 +988,7 @@ typedef struct PrometheusKv4AttentionRequest {
   uint32_t struct_size;
   uint32_t dtype;
   uint32_t rows;        /* 1..2^24 */
-  uint32_t q_heads;     /* a multiple of kv_heads, at most 2^16 */
+  uint32_t q_heads;     /* a multiple of kv_heads, at most 2^16; rows * (q_heads / kv_heads) below 2^30 */
   uint32_t q_stride;    /* >= q_heads * head_dim, below 2^24 */
   uint32_t out_stride;  /* >= q_heads * head_dim, below 2^24 */
   uint32_t max_rows;    /* 1..rows */

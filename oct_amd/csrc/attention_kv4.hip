@@ -55,8 +55,45 @@ struct Kv4Kernel {
   size_t ends;  // where these begin
   int rows, q_stride, out_stride;
   int q_heads, group, tiles, splits;
-  uint32_t window;
+  int split_shift;  // a split has 2^split_shift pages or a share of more
+  int window;       // 0: none
   float scale_log2;
+  uint32_t group_shift;
+  uint64_t group_magic;
+
+  // x / group for 0 <= x < 2^31: with 2^l >= group, floor(2^(31 + l) / group) + 1 is over the
+  // quotient by at most 2^l / 2^(31 + l), which no such x carries past a whole number.
+  __device__ __forceinline__ int over_group(int x) const {
+    return (int)(((uint64_t)(uint32_t)x * group_magic) >> group_shift);
+  }
+};
+
+typedef const __attribute__((address_space(4))) int32_t Constant;
+
+// A sequence's rows (within the call's) and length.
+struct Sequence {
+  int first, n, length;
+  __device__ __forceinline__ Sequence(const Kv4Kernel& g, int seq) {
+    Constant* starts = (Constant*)g.starts;
+    first = min(max(starts[seq], 0), g.rows);
+    n = min(max(starts[seq + 1], 0), g.rows) - first;
+    length = max(((Constant*)g.c.lengths)[seq], 0);
+  }
+};
+
+// The positions of a tile's first and last row, the pages that they see between them, and into
+// how many splits these are dealt.  Past the table every token is bad: the page behind its last
+// stands for all of them.
+struct Tile {
+  int pos0, pos1, page0, last, splits;
+  __device__ __forceinline__ Tile(const Kv4Kernel& g, const Sequence& s, int tile) {
+    const int x0 = tile * kTileRows, from = s.length - s.n;
+    pos0 = from + g.over_group(x0);
+    pos1 = from + g.over_group(min(x0 + kTileRows, s.n * g.group) - 1);
+    page0 = g.window && pos0 >= g.window ? min((pos0 - g.window + 1) / kKv4Page, g.c.table_stride) : 0;
+    last = pos1 < 0 ? 0 : min(pos1 / kKv4Page, g.c.table_stride) + 1;
+    splits = min(g.splits, max(1, (last - page0 + (1 << g.split_shift) - 1) >> g.split_shift));
+  }
 };
 
 __device__ __forceinline__ float* ends(const Kv4Kernel& g) { return g.part + g.ends; }
@@ -161,39 +198,32 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
   const int tile0 = (int)(b % (uint32_t)g.tiles);
   const int seq = (int)(b / (uint32_t)g.tiles);
 
-  const int first_row = min(max(g.starts[seq], 0), g.rows);
-  const int n = min(max(g.starts[seq + 1], 0), g.rows) - first_row;
-  if (n <= 0) return;
-  const long long room = (long long)g.c.table_stride * kKv4Page;
-  const int length = max(g.c.lengths[seq], 0);
+  const Sequence sq(g, seq);
+  if (sq.n <= 0) return;
   // Constant address space: page numbers come by scalar loads, which do not wait for the
   // transfers of pages as vector loads would.
-  const auto* table = (const __attribute__((address_space(4))) int32_t*)(g.c.table + (size_t)seq * g.c.table_stride);
+  const auto* table = (const Constant*)(g.c.table + (size_t)seq * g.c.table_stride);
   const uint8_t* mine_lds = lds + wave * 2 * St::kBytes;
   const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) const uint8_t*)mine_lds;
 
-  const long long tiles = ((long long)n * g.group + kTileRows - 1) / kTileRows;
-  for (long long tile = tile0; tile < tiles; tile += g.tiles) {
-    // This lane's row: pair x = row * group + query head.
-    const long long x0 = tile * kTileRows, x = x0 + r16;
-    const long long pairs = (long long)n * g.group;
+  const int pairs = sq.n * g.group;
+  for (int tile = tile0; tile * kTileRows < pairs; tile += g.tiles) {
+    const Tile tl(g, sq, tile);
+    if (split >= tl.splits) continue;
+    // This lane's row: pair x = row * group + query head.  Lanes without one work on zeros.
+    const int x0 = tile * kTileRows, x = x0 + r16;
     const bool mine = x < pairs;
-    const int row = mine ? (int)(x / g.group) : 0;
-    const int q_head = head * g.group + (mine ? (int)(x - (long long)row * g.group) : 0);
-    const long long pos = mine ? (long long)length - n + row : -1;  // its position
-    const long long pos0 = (long long)length - n + x0 / g.group;    // the tile's first and last
-    const long long pos1 = (long long)length - n + (min(x0 + kTileRows, pairs) - 1) / g.group;
-    const long long low = g.window ? pos - g.window : -1;  // it sees low < t <= pos
-    const int page0 = g.window && pos0 >= (long long)g.window ? (int)((pos0 - g.window + 1) / kKv4Page) : 0;
-    const int page1 = pos1 < 0 ? 0 : (int)(pos1 / kKv4Page) + 1;
-    // Past the table every token is bad: one page of them stands for all.
-    const int last = (int)min((long long)page1, room / kKv4Page + 1);
+    const int row = mine ? g.over_group(x) : 0;
+    const int q_head = head * g.group + (mine ? x - row * g.group : 0);
+    const int pos = mine ? sq.length - sq.n + row : tl.pos1;             // its position
+    const int low = g.window && pos >= g.window ? pos - g.window : -1;  // it sees low < t <= pos
+    const int page0 = tl.page0, last = tl.last;
 
     // Q^T operand: lane (h, row), step s: channels 32 s + 8 h .. + 7.
     bf16x8 q[kSteps][kQT];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const size_t at = (size_t)(first_row + row) * g.q_stride + (size_t)q_head * D + 32 * s + 8 * h;
+      const size_t at = (size_t)(sq.first + row) * g.q_stride + (size_t)q_head * D + 32 * s + 8 * h;
       if constexpr (kF32) {
         float v[8];
         __builtin_memcpy(v, static_cast<const float*>(g.q) + at, 32);
@@ -215,7 +245,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
     floatx4 o[kB] = {};
     float m_run = -INFINITY, m_log2 = 0.0f, l_run = 0.0f;
 
-    const int stride = g.splits * kWaves;
+    const int stride = tl.splits * kWaves;
     int pg = page0 + split * kWaves + wave;
     auto page_number = [&](int p) -> uint32_t {
       return p < last && p < g.c.table_stride ? (uint32_t)table[p] : 0xFFFFFFFFu;
@@ -282,19 +312,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
         }
       }
       // Masked where the page has tokens that some row does not see, or is bad.
-      const long long t0 = (long long)pg * kKv4Page;
-      const bool bad = number >= g.c.pages;
-      const bool edge = bad || t0 + kKv4Page - 1 > pos0 || (g.window && t0 <= pos1 - (long long)g.window) ||
-                        x0 + kTileRows > pairs;
+      const bool bad = number >= g.c.pages, past = pg >= g.c.table_stride;
+      const int t0 = pg * kKv4Page;
+      const bool edge = bad || t0 + (kKv4Page - 1) > tl.pos0 || (g.window && t0 <= tl.pos1 - g.window);
+      uint32_t seen = 0;  // bit j: token 16 h + j
       if (edge) {
+        // A row that lies past its table sees its own token at least, which is bad.
+        const bool lost = past && pos / kKv4Page >= g.c.table_stride;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const long long t = t0 + 16 * h + 4 * c + i;
-            const bool seen = t <= pos && t > low;
+            const int t = t0 + 16 * h + 4 * c + i;
+            const bool sees = past ? lost : t <= pos && t > low;
             if (bad) s[c][i] = NAN;
-            if (!seen) s[c][i] = -INFINITY;
+            if (!sees) s[c][i] = -INFINITY;
+            seen |= (uint32_t)sees << (4 * c + i);
           }
       }
       float m = s[0][0];
@@ -328,11 +361,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           vs[j] = *reinterpret_cast<const u32x4*>(stage + St::kSteps + 128 * (kG + gr) + 32 * h + 16 * j);
-        if (edge) {  // a token not seen may hold anything: its step counts as 0
+        if (edge) {  // a token that is not seen may have any step: it counts as 0
 #pragma unroll
           for (int j = 0; j < 16; j += 2)
-            vs[j / 8][j / 2 % 4] &= (s[j / 4][j % 4] == -INFINITY ? 0u : 0xFFFFu) |
-                                    (s[j / 4][j % 4 + 1] == -INFINITY ? 0u : 0xFFFF0000u);
+            vs[j / 8][j / 2 % 4] &= ((uint32_t)__builtin_amdgcn_sbfe((int)seen, j, 1) & 0xFFFFu) |
+                                    ((uint32_t)__builtin_amdgcn_sbfe((int)seen, j + 1, 1) & 0xFFFF0000u);
         }
         // P s in bf16 terms, tokens 16 h + 0..7 and 8..15.
         bf16x8 pf[2][kPT];
@@ -375,7 +408,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
     __syncthreads();
     for (int e = (int)threadIdx.x; e < kTileRows * D; e += 64 * kWaves) {
       const int tr = e / D, d = e % D;
-      const long long xe = x0 + tr;
+      const int xe = x0 + tr;
       if (xe >= pairs) break;
       const float* all = reinterpret_cast<const float*>(lds) + tr * (D + 4);
       float top = -INFINITY;
@@ -389,9 +422,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
         sum = __builtin_fmaf(a[d], f, sum);
         weight = __builtin_fmaf(a[D + 1], f, weight);
       }
-      const int er = first_row + (int)(xe / g.group);
-      const int eh = head * g.group + (int)(xe % g.group);
-      if (g.splits > 1) {
+      const int in_seq = g.over_group(xe), er = sq.first + in_seq, eh = head * g.group + xe - in_seq * g.group;
+      if (tl.splits > 1) {
         const size_t at = ((size_t)split * g.rows + er) * g.q_heads + eh;
         g.part[at * D + d] = sum;
         if (d == 0) reinterpret_cast<float2*>(ends(g))[at] = make_float2(top, weight);
@@ -420,10 +452,14 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
   const int column = tid % kColumns, part = tid / kColumns;
   const long long pairs = (long long)g.rows * g.q_heads;
   for (long long x = blockIdx.x; x < pairs; x += gridDim.x) {
-    const int row = (int)(x / g.q_heads);
-    if (find_sequence(g.starts, g.c.sequences, row) < 0) continue;
+    const int row = (int)(x / g.q_heads), q_head = (int)(x - (long long)row * g.q_heads);
+    const int seq = find_sequence(g.starts, g.c.sequences, row);
+    if (seq < 0) continue;
+    const Sequence sq(g, seq);
+    const int splits = Tile(g, sq, ((row - sq.first) * g.group + q_head % g.group) / kTileRows).splits;
+    if (splits == 1) continue;
     float top = -INFINITY, weight = 0.0f;
-    if (lane < g.splits) {
+    if (lane < splits) {
       const float2 e = reinterpret_cast<const float2*>(ends(g))[(size_t)lane * pairs + x];
       top = e.x;
       weight = e.y;
@@ -432,16 +468,16 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     const float f = mine == top ? 1.0f : __builtin_amdgcn_exp2f((mine - top) * g.scale_log2);
-    weight = lane < g.splits ? weight * f : 0.0f;
+    weight = lane < splits ? weight * f : 0.0f;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) weight += __shfl_xor(weight, d);
-    if (tid < g.splits) factors[tid] = f;
+    if (tid < splits) factors[tid] = f;
     __syncthreads();
     floatx4 sum = {};
     const floatx4* at = reinterpret_cast<const floatx4*>(g.part + (size_t)x * D) + column;
     const size_t slab = (size_t)pairs * kColumns;
 #pragma unroll 4
-    for (int s = part; s < g.splits; s += kParts) {
+    for (int s = part; s < splits; s += kParts) {
       const floatx4 v = at[s * slab];
       const float fs = factors[s];
 #pragma unroll
@@ -452,7 +488,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
     if (part == 0) {
 #pragma unroll
       for (int i = 1; i < kParts; ++i) sum += parts[i][column];
-      const size_t to = (size_t)row * g.out_stride + (size_t)(x - (long long)row * g.q_heads) * D + 4 * column;
+      const size_t to = (size_t)row * g.out_stride + (size_t)q_head * D + 4 * column;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float v = weight == 0.0f ? 0.0f : sum[i] / weight;
@@ -466,20 +502,28 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
   }
 }
 
-// Tiles of 16 pairs that the longest sequence has (a workgroup takes several where the grid
-// would be too large), and the splits of its pages: enough workgroups for the chip to be
-// full and uneven sequences to be dealt out.
-void plan(const Kv4AttentionArgs& a, int head_dim, int* tiles, int* splits) {
+// The grid: tiles of 16 pairs that the longest sequence has (a workgroup takes several where it
+// would be too large), and splits for the pages of the longest.  A split has 4 to 32 pages (one to
+// eight a wave), fewer where that is what fills the chip; a shorter sequence has fewer splits, so
+// that workgroups are of one size whatever the lengths.
+struct Plan {
+  int tiles, splits, shift;
+};
+Plan plan(const Kv4AttentionArgs& a, int head_dim) {
+  Plan p;
   const uint64_t columns = (uint64_t)a.c.sequences * a.c.kv_heads;  // at most kKv4MaxColumns
   const uint64_t t = ((uint64_t)a.max_rows * (uint64_t)a.group + kTileRows - 1) / kTileRows;
-  *tiles = (int)std::min<uint64_t>(t, kKv4MaxColumns / columns);
-  const uint64_t base = columns * (uint64_t)*tiles;
+  p.tiles = (int)std::min<uint64_t>(t, kKv4MaxColumns / columns);
   uint64_t length = a.max_length;
   if (a.window) length = std::min<uint64_t>(length, (uint64_t)a.window + 2 * kKv4Page);
-  const uint64_t pages = (length + kKv4Page - 1) / kKv4Page;
-  const uint64_t want = (2048 + base - 1) / base, most = (pages + 2 * kWaves - 1) / (2 * kWaves);
-  *splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({want, most, kMaxSplits}));
-  if ((uint64_t)*splits * a.rows * (uint64_t)a.q_heads * (uint64_t)(head_dim + 2) * 4 > kMostPartialBytes) *splits = 1;
+  const uint64_t pages = (length + kKv4Page - 1) / kKv4Page, base = columns * (uint64_t)p.tiles;
+  p.shift = 2;
+  while (p.shift < 5 && base * (pages >> p.shift) > 1024) ++p.shift;
+  while (((pages + (1ull << p.shift) - 1) >> p.shift) > (uint64_t)kMaxSplits) ++p.shift;
+  p.splits = (int)((pages + (1ull << p.shift) - 1) >> p.shift);
+  if (base >= 4096 || (uint64_t)p.splits * a.rows * (uint64_t)a.q_heads * (uint64_t)(head_dim + 2) * 4 > kMostPartialBytes)
+    p.splits = 1;
+  return p;
 }
 
 template <bool kF32, int D>
@@ -497,9 +541,8 @@ hipError_t launch(const Kv4Kernel& g, hipStream_t stream) {
 }  // namespace
 
 size_t kv4_attention_partial_bytes(const Kv4AttentionArgs& a, int head_dim) {
-  int tiles, splits;
-  plan(a, head_dim, &tiles, &splits);
-  return splits > 1 ? (size_t)splits * a.rows * a.q_heads * (head_dim + 2) * sizeof(float) : 0;
+  const Plan p = plan(a, head_dim);
+  return p.splits > 1 ? (size_t)p.splits * a.rows * a.q_heads * (head_dim + 2) * sizeof(float) : 0;
 }
 
 hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf16, hipStream_t stream) {
@@ -514,10 +557,17 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf
   g.out_stride = (int)a.out_stride;
   g.q_heads = a.q_heads;
   g.group = a.group;
-  g.window = a.window;
+  g.window = a.window > 0x7fffffffu ? 0 : (int)a.window;  // longer than any sequence
   g.scale_log2 = a.scale * 1.4426950408889634f;
-  plan(a, head_dim, &g.tiles, &g.splits);
-  g.ends = (size_t)g.splits * a.rows * (size_t)a.q_heads * (size_t)head_dim;
+  uint32_t l = 0;
+  while ((1u << l) < (uint32_t)a.group) ++l;
+  g.group_shift = 31 + l;
+  g.group_magic = (1ull << g.group_shift) / (uint64_t)a.group + 1;
+  const Plan p = plan(a, head_dim);
+  g.tiles = p.tiles;
+  g.splits = p.splits;
+  g.split_shift = p.shift;
+  g.ends = (size_t)p.splits * a.rows * (size_t)a.q_heads * (size_t)head_dim;
   switch (head_dim) {
     case 64: return bf16 ? launch<false, 64>(g, stream) : launch<true, 64>(g, stream);
     case 128: return bf16 ? launch<false, 128>(g, stream) : launch<true, 128>(g, stream);

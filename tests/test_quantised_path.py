@@ -176,7 +176,8 @@ def test_attention_refuses(rt):
     for change in BAD_CACHES:
         assert _refused(_attention(rt, cache=dict(CACHE, **change))), change
     for change in (dict(struct_size=4), dict(dtype=2), dict(rows=0), dict(rows=(1 << 24) + 1), dict(q_heads=0),
-                   dict(q_heads=7), dict(q_heads=(1 << 16) + 2), dict(q_stride=1023), dict(q_stride=1 << 24),
+                   dict(q_heads=7), dict(q_heads=(1 << 16) + 2), dict(rows=1 << 17, q_heads=1 << 15, q_stride=1 << 22, out_stride=1 << 22),
+                   dict(q_stride=1023), dict(q_stride=1 << 24),
                    dict(out_stride=1023), dict(out_stride=1 << 24), dict(max_rows=0), dict(max_rows=7),
                    dict(max_length=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
                    dict(scale=float("nan")), dict(q=0), dict(q=OK + 1), dict(out=0), dict(out=OK + 1),
