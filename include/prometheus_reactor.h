@@ -940,7 +940,7 @@ typedef struct PrometheusKv4Cache {
   uint32_t head_dim;     /* 64, 128 or 256 */
   uint32_t kv_heads;     /* 1..1024 */
   uint32_t pages;        /* of the pool, 1..2^31-1 */
-  uint32_t sequences;    /* 1..2^20; sequences * kv_heads at most 2^23 */
+  uint32_t sequences;    /* 1..2^20; sequences * kv_heads at most 2^22 */
   uint32_t table_stride; /* page numbers a sequence, 1..2^24 */
   void* pool;            /* pages * prometheus_reactor_kv4_page_bytes, 16-byte aligned */
   const int32_t* page_table; /* [sequences, table_stride] */

@@ -33,6 +33,10 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -43,6 +47,7 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 constexpr float kLazyLog2 = 8.0f;
 constexpr int kTileRows = 16;
 constexpr int kWaves = 4;
+constexpr uint64_t kFewPairs = 64;
 constexpr int kMaxSplits = 64;  // a lane each when they are joined
 constexpr uint64_t kMostPartialBytes = 1ull << 30;
 
@@ -54,7 +59,7 @@ struct Kv4Kernel {
   float* part;  // sums [splits][rows][q_heads][D], then (maximum, weight) [splits][rows][q_heads]
   size_t ends;  // where these begin
   int rows, q_stride, out_stride;
-  int q_heads, group, tiles, splits;
+  int q_heads, group, tiles, tile_rows, splits;
   int split_shift;  // a split has 2^split_shift pages or a share of more
   int window;       // 0: none
   float scale_log2;
@@ -86,10 +91,10 @@ struct Sequence {
 // stands for all of them.
 struct Tile {
   int pos0, pos1, page0, last, splits;
-  __device__ __forceinline__ Tile(const Kv4Kernel& g, const Sequence& s, int tile) {
-    const int x0 = tile * kTileRows, from = s.length - s.n;
+  __device__ __forceinline__ Tile(const Kv4Kernel& g, const Sequence& s, int tile, int tile_rows) {
+    const int x0 = tile * tile_rows, from = s.length - s.n;
     pos0 = from + g.over_group(x0);
-    pos1 = from + g.over_group(min(x0 + kTileRows, s.n * g.group) - 1);
+    pos1 = from + g.over_group(min(x0 + tile_rows, s.n * g.group) - 1);
     page0 = g.window && pos0 >= g.window ? min((pos0 - g.window + 1) / kKv4Page, g.c.table_stride) : 0;
     last = pos1 < 0 ? 0 : min(pos1 / kKv4Page, g.c.table_stride) + 1;
     splits = min(g.splits, max(1, (last - page0 + (1 << g.split_shift) - 1) >> g.split_shift));
@@ -177,6 +182,20 @@ struct Stage {
   }
 };
 
+// Key heads fastest, then sequences, tiles, splits.  Workgroups go to the XCDs, and there to groups
+// of CUs, in turn; the sequence moves on by one with each tile and split, so that the same CUs do
+// not get every workgroup of a long sequence, or the splits that a short one does not have.
+__device__ __forceinline__ void coordinates(const Kv4Kernel& g, int* head, int* seq, int* tile, int* split) {
+  uint32_t b = blockIdx.x;
+  *head = (int)(b % (uint32_t)g.c.kv_heads);
+  b /= (uint32_t)g.c.kv_heads;
+  const uint32_t i = b % (uint32_t)g.c.sequences;
+  b /= (uint32_t)g.c.sequences;
+  *tile = (int)(b % (uint32_t)g.tiles);
+  *split = (int)(b / (uint32_t)g.tiles);
+  *seq = (int)((i + (uint32_t)*tile + (uint32_t)*split) % (uint32_t)g.c.sequences);
+}
+
 template <bool kF32, int D>
 __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4Kernel g) {
   constexpr int kG = D / 64, kQT = kF32 ? 3 : 1, kPT = kF32 ? 3 : 2;
@@ -189,15 +208,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int r16 = lane & 15, h = lane >> 4;
-  // Splits fastest, then key heads, then tiles, then sequences.
-  uint32_t b = blockIdx.x;
-  const int split = (int)(b % (uint32_t)g.splits);
-  b /= (uint32_t)g.splits;
-  const int head = (int)(b % (uint32_t)g.c.kv_heads);
-  b /= (uint32_t)g.c.kv_heads;
-  const int tile0 = (int)(b % (uint32_t)g.tiles);
-  const int seq = (int)(b / (uint32_t)g.tiles);
-
+  int head, seq, tile0, split;
+  coordinates(g, &head, &seq, &tile0, &split);
   const Sequence sq(g, seq);
   if (sq.n <= 0) return;
   // Constant address space: page numbers come by scalar loads, which do not wait for the
@@ -208,7 +220,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
 
   const int pairs = sq.n * g.group;
   for (int tile = tile0; tile * kTileRows < pairs; tile += g.tiles) {
-    const Tile tl(g, sq, tile);
+    const Tile tl(g, sq, tile, kTileRows);
     if (split >= tl.splits) continue;
     // This lane's row: pair x = row * group + query head.  Lanes without one work on zeros.
     const int x0 = tile * kTileRows, x = x0 + r16;
@@ -440,6 +452,295 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
   }
 }
 
+// Many rows (prompts).  A workgroup takes 32 pairs a wave; a page's keys and values are turned
+// into bf16 (exactly, steps applied) once for all of them and kept in LDS, and a wave computes
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_bf16, the V^T operand by transpose reads.
+// The next page's codes are loaded into registers before a page is worked on and turned into
+// the other half of LDS after it: one barrier a page.  P goes to bf16 (fp32 rows: three terms,
+// as for the queries).  Bound by the vector unit (softmax, the conversion) beside the MFMAs.
+template <bool kF32, int D>
+struct Prompt {
+  static constexpr int kWaves = D == 256 || (kF32 && D == 128) ? 4 : 8;  // one or two a SIMD, by registers
+  static constexpr int kThreads = 64 * kWaves, kRows = 32 * kWaves;
+  static constexpr int kUnits = 4 * D;                                // of 8 bytes (16 channels): keys, and values
+  static constexpr int kEach = 2 * kUnits / kThreads > 0 ? 2 * kUnits / kThreads : 1;
+  static constexpr int kTileBytes = kKv4Page * D * 2;                 // bf16 keys, then values
+  static_assert(kEach * kThreads == 2 * kUnits && kUnits % 64 == 0, "units");
+
+  // Position of 16-byte chunk c (8 channels) of token t: operand reads of 32 keys, and transpose
+  // reads of 4 neighbouring tokens' 32 channels, then fall into different banks.
+  __device__ static __forceinline__ int key_swz(int t) { return D == 64 ? t & 7 : t & 15; }
+  __device__ static __forceinline__ int value_swz(int t) { return D == 64 ? 2 * t & 4 : 4 * (t & 3); }
+
+  struct Codes {
+    u32x2 w[kEach];
+    uint32_t step[kEach];
+  };
+  __device__ static __forceinline__ void unit(int i, int tid, bool* keys, int* t, int* b) {
+    const int u = tid + kThreads * i;
+    *keys = u < kUnits;
+    const int at = 8 * (u % kUnits);
+    *t = at / (D / 2);
+    *b = at % (D / 2);  // byte of the token's row
+  }
+  // Group of a unit: words of a key row lie four (D = 64: two) to a quarter, 32 channels apart.
+  __device__ static __forceinline__ int group_of(bool keys, int b) {
+    if (!keys) return b / 32;
+    return D == 64 ? 0 : 2 * (b / 64) + b / 8 % 2;
+  }
+  __device__ static __forceinline__ void load(Codes& c, const uint8_t* block, int tid) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      bool keys;
+      int t, b;
+      unit(i, tid, &keys, &t, &b);
+      c.w[i] = *reinterpret_cast<const u32x2*>(block + (keys ? 0 : Stage<D>::kCodes) + t * (D / 2) + b);
+      c.step[i] = *reinterpret_cast<const uint16_t*>(block + Stage<D>::kSteps + 128 * (group_of(keys, b) + (keys ? 0 : D / 64)) + 2 * t);
+    }
+  }
+  // Codes to bf16 in LDS.  zero_from: values from this token of the page on, and on an edge page
+  // those that are not finite, count as 0 (some row does not see them).
+  __device__ static __forceinline__ void store(const Codes& c, uint8_t* lds, int tid, bool edge, int zero_from) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      bool keys;
+      int t, b;
+      unit(i, tid, &keys, &t, &b);
+      uint32_t step = c.step[i] << 16;
+      if (edge && !keys && (t >= zero_from || (step & 0x7F800000u) == 0x7F800000u)) step = 0;
+      const float s = __uint_as_float(step);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t w = c.w[i][j];
+        const floatx2 v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0);
+        const floatx2 v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+        const floatx2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2);
+        const floatx2 v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+        const bf16x8 x = {(__bf16)(v0.x * s), (__bf16)(v0.y * s), (__bf16)(v1.x * s), (__bf16)(v1.y * s),
+                          (__bf16)(v2.x * s), (__bf16)(v2.y * s), (__bf16)(v3.x * s), (__bf16)(v3.y * s)};
+        const int word = b / 4 + j;
+        int chunk = word;
+        if (keys) chunk = D == 64 ? 4 * (word & 1) + (word >> 1) : (word & ~15) + 4 * (word & 3) + (word >> 2 & 3);
+        const int at = (keys ? 0 : kTileBytes) + t * 2 * D + 16 * (chunk ^ (keys ? key_swz(t) : value_swz(t)));
+        *reinterpret_cast<bf16x8*>(lds + at) = x;
+      }
+    }
+  }
+};
+
+template <bool kF32, int D>
+__global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWaves / 4)) void kv4_prompt_kernel(const Kv4Kernel g) {
+  using Pr = Prompt<kF32, D>;
+  constexpr int kG = D / 64, kT = kF32 ? 3 : 1;
+  constexpr int kSteps = D / 16;  // MFMA steps of 16 channels
+  constexpr int kB = D / 32;      // blocks of 32 output channels
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2 * Pr::kTileBytes];
+
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lq = lane & 31, hi = lane >> 5;
+  int head, seq, tile0, split;
+  coordinates(g, &head, &seq, &tile0, &split);
+  const Sequence sq(g, seq);
+  if (sq.n <= 0) return;
+  const auto* table = (const Constant*)(g.c.table + (size_t)seq * g.c.table_stride);
+  const int pairs = sq.n * g.group;
+  for (int tile = tile0; tile * Pr::kRows < pairs; tile += g.tiles) {
+    const Tile tl(g, sq, tile, Pr::kRows);
+    if (split >= tl.splits) continue;
+    // This lane's row, and the first and last position of the wave's 32.
+    const int x0 = tile * Pr::kRows + 32 * wave, x = x0 + lq;
+    const bool mine = x < pairs;
+    const int row = mine ? g.over_group(x) : 0;
+    const int q_head = head * g.group + (mine ? x - row * g.group : 0);
+    const int from = sq.length - sq.n;
+    const int wave0 = from + g.over_group(min(x0, pairs - 1)), wave1 = from + g.over_group(min(x0 + 32, pairs) - 1);
+    const int pos = mine ? from + row : wave1;
+    const int low = g.window && pos >= g.window ? pos - g.window : -1;  // it sees low < t <= pos
+
+    bf16x8 q[kSteps][kT];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const size_t at = (size_t)(sq.first + row) * g.q_stride + (size_t)q_head * D + 16 * s + 8 * hi;
+      if constexpr (kF32) {
+        float v[8];
+        __builtin_memcpy(v, static_cast<const float*>(g.q) + at, 32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          __bf16 t[kT];
+          terms(mine ? v[j] : 0.0f, t);
+#pragma unroll
+          for (int i = 0; i < kT; ++i) q[s][i][j] = t[i];
+        }
+      } else {
+        u32x4 v;
+        __builtin_memcpy(&v, static_cast<const uint16_t*>(g.q) + at, 16);
+        if (!mine) v = u32x4{0u, 0u, 0u, 0u};
+        q[s][0] = __builtin_bit_cast(bf16x8, v);
+      }
+    }
+
+    floatx16 o[kB] = {};
+    float m_run = -INFINITY, m_log2 = 0.0f, l_run = 0.0f;
+    auto page_number = [&](int p) -> uint32_t {
+      return p < tl.last && p < g.c.table_stride ? (uint32_t)table[p] : 0xFFFFFFFFu;
+    };
+    auto page_block = [&](uint32_t number) -> const uint8_t* {
+      const uint32_t ok = number < g.c.pages ? number : 0u;
+      return g.c.pool + ((size_t)ok * g.c.kv_heads + head) * kv4_block_bytes(D);
+    };
+    // Some row of the tile does not see all of the page.
+    auto page_edge = [&](int p, uint32_t number) {
+      return number >= g.c.pages || p * kKv4Page + (kKv4Page - 1) > tl.pos0 ||
+             (g.window && p * kKv4Page <= tl.pos1 - g.window);
+    };
+    // A split's pages are neighbours here.
+    const int share = (tl.last - tl.page0 + tl.splits - 1) / tl.splits;
+    const int begin = tl.page0 + split * share, end = min(begin + share, tl.last);
+    typename Pr::Codes codes;
+    uint32_t number = page_number(begin), next_number = begin + 1 < end ? page_number(begin + 1) : 0;
+    if (begin < end) {
+      Pr::load(codes, page_block(number), tid);
+      Pr::store(codes, lds[0], tid, page_edge(begin, number), number >= g.c.pages ? 0 : tl.pos1 - begin * kKv4Page + 1);
+    }
+    int now = 0;
+    for (int pg = begin; pg < end; ++pg) {
+      __syncthreads();  // this page is complete, the other half of LDS no longer read
+      const bool more = pg + 1 < end;
+      if (more) Pr::load(codes, page_block(next_number), tid);
+      const uint32_t after = pg + 2 < end ? page_number(pg + 2) : 0;
+      const uint8_t* keys = lds[now];
+      const uint8_t* values = lds[now] + Pr::kTileBytes;
+      const int t0 = pg * kKv4Page;
+      const bool bad = number >= g.c.pages, past = pg >= g.c.table_stride;
+
+      // Pages that no row of the wave sees, and waves without rows, are passed over.
+      if (x0 < pairs && (past || (t0 <= wave1 && !(g.window && t0 + (kKv4Page - 1) <= wave0 - g.window)))) {
+        floatx16 s[2] = {};
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u)
+#pragma unroll
+          for (int tb = 0; tb < 2; ++tb) {
+            const int t = 32 * tb + lq;
+            const bf16x8 k = *reinterpret_cast<const bf16x8*>(keys + t * 2 * D + 16 * ((2 * u + hi) ^ Pr::key_swz(t)));
+#pragma unroll
+            for (int i = 0; i < kT; ++i) s[tb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[u][i], s[tb], 0, 0, 0);
+          }
+        // Register r of block tb is token 32 tb + 8 (r / 4) + 4 hi + r % 4.
+        if (bad || t0 + (kKv4Page - 1) > wave0 || (g.window && t0 <= wave1 - g.window)) {
+          const bool lost = past && pos / kKv4Page >= g.c.table_stride;
+#pragma unroll
+          for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int t = t0 + 32 * tb + 8 * (r >> 2) + 4 * hi + (r & 3);
+              const bool sees = past ? lost : t <= pos && t > low;
+              if (bad) s[tb][r] = NAN;
+              if (!sees) s[tb][r] = -INFINITY;
+            }
+        }
+        float m = s[0][0];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) m = fmaxf(m, s[tb][r]);
+        m = max_halves(m);
+        if (__any((m - m_run) * g.scale_log2 > kLazyLog2)) {
+          const float m_new = fmaxf(m, m_run);
+          const float alpha = m_new == m_run ? 1.0f : __builtin_amdgcn_exp2f((m_run - m_new) * g.scale_log2);
+          m_run = m_new;
+          m_log2 = m_new == -INFINITY ? 0.0f : m_new * g.scale_log2;
+          l_run *= alpha;
+#pragma unroll
+          for (int i = 0; i < kB; ++i) o[i] *= alpha;
+        }
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            bf16x8 p[kT];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tb][8 * half + j], g.scale_log2, -m_log2));
+              l_run += e;
+              __bf16 t[kT];
+              terms(e, t);
+#pragma unroll
+              for (int i = 0; i < kT; ++i) p[i][j] = t[i];
+            }
+            // Tokens 32 tb + 16 half + 4 hi + 0..3, and 8 further.
+            const int t = 32 * tb + 16 * half + 4 * hi + ((lane & 15) >> 2);
+#pragma unroll
+            for (int bl = 0; bl < kB; ++bl) {
+              const int d = 32 * bl + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+              const uint8_t* at = values + t * 2 * D + 16 * ((d >> 3) ^ Pr::value_swz(t)) + 2 * (d & 7);
+              const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+              const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * 2 * D));
+              const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+              for (int i = 0; i < kT; ++i) o[bl] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p[i], o[bl], 0, 0, 0);
+            }
+          }
+        // Values that are not finite were left out of an edge page: the rows that see them get NaN.
+        if (!bad && page_edge(pg, number)) {
+          const uint16_t* steps = reinterpret_cast<const uint16_t*>(page_block(number) + Stage<D>::kSteps + 2 * D) + lane;
+#pragma unroll
+          for (int gr = 0; gr < kG; ++gr) {
+            const uint64_t odd = __ballot((steps[64 * gr] & 0x7F80) == 0x7F80);
+            if (odd != 0) {
+              // The page's tokens low < t <= pos as bits.
+              const int to = min(pos - t0, 63), first = max(low + 1 - t0, 0);
+              const bool some = to >= first && first < 64 && to >= 0;
+              const uint64_t sees = some ? (~0ull >> (63 - to)) & (~0ull << first) : 0;
+              const float add = (odd & sees) != 0 ? NAN : 0.0f;
+#pragma unroll
+              for (int bl = 2 * gr; bl < 2 * gr + 2; ++bl) o[bl] += add;
+            }
+          }
+        }
+      }
+      if (more)
+        Pr::store(codes, lds[now ^ 1], tid, page_edge(pg + 1, next_number),
+                  next_number >= g.c.pages ? 0 : tl.pos1 - (t0 + kKv4Page) + 1);
+      now ^= 1;
+      number = next_number;
+      next_number = after;
+    }
+
+    l_run = sum_halves(l_run);
+    if (mine) {
+      const size_t pair = (size_t)(sq.first + row) * g.q_heads + q_head;
+      if (tl.splits > 1) {
+        const size_t at = (size_t)split * g.rows * g.q_heads + pair;
+#pragma unroll
+        for (int bl = 0; bl < kB; ++bl)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            *reinterpret_cast<floatx4*>(g.part + at * D + 32 * bl + 8 * r + 4 * hi) =
+                floatx4{o[bl][4 * r], o[bl][4 * r + 1], o[bl][4 * r + 2], o[bl][4 * r + 3]};
+        if (hi == 0) reinterpret_cast<float2*>(ends(g))[at] = make_float2(m_run, l_run);
+      } else {
+        const float f = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+        const size_t at = (size_t)(sq.first + row) * g.out_stride + (size_t)q_head * D + 4 * hi;
+#pragma unroll
+        for (int bl = 0; bl < kB; ++bl)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (kF32) {
+              const float v[4] = {o[bl][4 * r] * f, o[bl][4 * r + 1] * f, o[bl][4 * r + 2] * f, o[bl][4 * r + 3] * f};
+              __builtin_memcpy(static_cast<float*>(g.out) + at + 32 * bl + 8 * r, v, 16);
+            } else {
+              const __bf16 v[4] = {(__bf16)(o[bl][4 * r] * f), (__bf16)(o[bl][4 * r + 1] * f),
+                                   (__bf16)(o[bl][4 * r + 2] * f), (__bf16)(o[bl][4 * r + 3] * f)};
+              __builtin_memcpy(static_cast<__bf16*>(g.out) + at + 32 * bl + 8 * r, v, 8);
+            }
+          }
+      }
+    }
+    __syncthreads();  // the next tile fills LDS again
+  }
+}
+
 // One workgroup a row and query head joins the splits' sums.  Its threads are D / 4 columns of
 // four channels times kParts: part i adds splits i, i + kParts, ..., the parts are added in
 // order.  Bound by latency: maxima and weights come in one load a lane, sums four at a time.
@@ -453,17 +754,15 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
   const long long pairs = (long long)g.rows * g.q_heads;
   for (long long x = blockIdx.x; x < pairs; x += gridDim.x) {
     const int row = (int)(x / g.q_heads), q_head = (int)(x - (long long)row * g.q_heads);
+    // Splits that this row's tile does not have hold anything; they are left out below.
+    float2 e = make_float2(-INFINITY, 0.0f);
+    if (lane < g.splits) e = reinterpret_cast<const float2*>(ends(g))[(size_t)lane * pairs + x];
     const int seq = find_sequence(g.starts, g.c.sequences, row);
     if (seq < 0) continue;
     const Sequence sq(g, seq);
-    const int splits = Tile(g, sq, ((row - sq.first) * g.group + q_head % g.group) / kTileRows).splits;
+    const int splits = Tile(g, sq, ((row - sq.first) * g.group + q_head % g.group) / g.tile_rows, g.tile_rows).splits;
     if (splits == 1) continue;
-    float top = -INFINITY, weight = 0.0f;
-    if (lane < splits) {
-      const float2 e = reinterpret_cast<const float2*>(ends(g))[(size_t)lane * pairs + x];
-      top = e.x;
-      weight = e.y;
-    }
+    float top = lane < splits ? e.x : -INFINITY, weight = e.y;
     const float mine = top;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -507,21 +806,24 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
 // eight a wave), fewer where that is what fills the chip; a shorter sequence has fewer splits, so
 // that workgroups are of one size whatever the lengths.
 struct Plan {
-  int tiles, splits, shift;
+  int tile_rows, tiles, splits, shift;
 };
-Plan plan(const Kv4AttentionArgs& a, int head_dim) {
+Plan plan(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
   Plan p;
   const uint64_t columns = (uint64_t)a.c.sequences * a.c.kv_heads;  // at most kKv4MaxColumns
-  const uint64_t t = ((uint64_t)a.max_rows * (uint64_t)a.group + kTileRows - 1) / kTileRows;
-  p.tiles = (int)std::min<uint64_t>(t, kKv4MaxColumns / columns);
+  const uint64_t most = (uint64_t)a.max_rows * (uint64_t)a.group;
+  const int prompt_rows = 32 * (head_dim == 256 || (!bf16 && head_dim == 128) ? 4 : 8);
+  p.tile_rows = most > kFewPairs ? prompt_rows : kTileRows;
+  p.tiles = (int)std::min<uint64_t>((most + p.tile_rows - 1) / p.tile_rows, kKv4MaxColumns / columns);
   uint64_t length = a.max_length;
-  if (a.window) length = std::min<uint64_t>(length, (uint64_t)a.window + 2 * kKv4Page);
+  if (a.window) length = std::min<uint64_t>(length, (uint64_t)a.window + p.tile_rows / a.group + 2 * kKv4Page);
   const uint64_t pages = (length + kKv4Page - 1) / kKv4Page, base = columns * (uint64_t)p.tiles;
-  p.shift = 2;
-  while (p.shift < 5 && base * (pages >> p.shift) > 1024) ++p.shift;
+  const uint64_t full = p.tile_rows == kTileRows ? 1024 : 512;
+  p.shift = p.tile_rows == kTileRows ? 2 : 3;
+  while (p.shift < 5 && base * (pages >> p.shift) > full) ++p.shift;
   while (((pages + (1ull << p.shift) - 1) >> p.shift) > (uint64_t)kMaxSplits) ++p.shift;
   p.splits = (int)((pages + (1ull << p.shift) - 1) >> p.shift);
-  if (base >= 4096 || (uint64_t)p.splits * a.rows * (uint64_t)a.q_heads * (uint64_t)(head_dim + 2) * 4 > kMostPartialBytes)
+  if (base >= 4 * full || (uint64_t)p.splits * a.rows * (uint64_t)a.q_heads * (uint64_t)(head_dim + 2) * 4 > kMostPartialBytes)
     p.splits = 1;
   return p;
 }
@@ -529,7 +831,10 @@ Plan plan(const Kv4AttentionArgs& a, int head_dim) {
 template <bool kF32, int D>
 hipError_t launch(const Kv4Kernel& g, hipStream_t stream) {
   const uint64_t grid = (uint64_t)g.c.sequences * g.c.kv_heads * (uint64_t)g.tiles * (uint64_t)g.splits;
-  hipLaunchKernelGGL((kv4_attention_kernel<kF32, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, stream, g);
+  if (g.tile_rows == kTileRows)
+    hipLaunchKernelGGL((kv4_attention_kernel<kF32, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, stream, g);
+  else
+    hipLaunchKernelGGL((kv4_prompt_kernel<kF32, D>), dim3((unsigned)grid), dim3((Prompt<kF32, D>::kThreads)), 0, stream, g);
   if (g.splits > 1) {
     const uint64_t pairs = (uint64_t)g.rows * (uint64_t)g.q_heads;
     hipLaunchKernelGGL((kv4_join_kernel<kF32, D>), dim3((unsigned)std::min<uint64_t>(pairs, 1u << 20)), dim3(256),
@@ -540,8 +845,8 @@ hipError_t launch(const Kv4Kernel& g, hipStream_t stream) {
 
 }  // namespace
 
-size_t kv4_attention_partial_bytes(const Kv4AttentionArgs& a, int head_dim) {
-  const Plan p = plan(a, head_dim);
+size_t kv4_attention_partial_bytes(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
+  const Plan p = plan(a, head_dim, bf16);
   return p.splits > 1 ? (size_t)p.splits * a.rows * a.q_heads * (head_dim + 2) * sizeof(float) : 0;
 }
 
@@ -563,7 +868,8 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf
   while ((1u << l) < (uint32_t)a.group) ++l;
   g.group_shift = 31 + l;
   g.group_magic = (1ull << g.group_shift) / (uint64_t)a.group + 1;
-  const Plan p = plan(a, head_dim);
+  const Plan p = plan(a, head_dim, bf16);
+  g.tile_rows = p.tile_rows;
   g.tiles = p.tiles;
   g.splits = p.splits;
   g.split_shift = p.shift;

@@ -193,13 +193,14 @@ PROM_REACTOR_API int prometheus_reactor_runtime_attention_kv4_device(void* handl
   DeviceContext& cx = ctx();
   std::lock_guard<std::mutex> lock(cx.mu);
   CurrentDevice device(cx.device);
-  const size_t bytes = kv4_attention_partial_bytes(a, (int)cache->head_dim);
+  const bool bf16 = r->dtype == PROM_DTYPE_BF16;
+  const size_t bytes = kv4_attention_partial_bytes(a, (int)cache->head_dim, bf16);
   if (bytes > 0) {
     a.part = static_cast<float*>(staging(6, bytes));
     if (a.part == nullptr)
       return refuse(out_stage, out_detail_code, PROM_STAGE_TRANSFER_IN, PROM_DETAIL_HIP_ALLOC_FAILED);
   }
-  return queued(launch_kv4_attention(a, (int)cache->head_dim, r->dtype == PROM_DTYPE_BF16, cx.stream), out_stage,
+  return queued(launch_kv4_attention(a, (int)cache->head_dim, bf16, cx.stream), out_stage,
                 out_detail_code, 0);
 }
 

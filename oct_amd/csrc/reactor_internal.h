@@ -340,8 +340,8 @@ struct Kv4AttentionArgs {
   float scale;
 };
 // Sequences times key heads (a workgroup at least each).
-constexpr uint64_t kKv4MaxColumns = 1ull << 23;
-size_t kv4_attention_partial_bytes(const Kv4AttentionArgs& a, int head_dim);
+constexpr uint64_t kKv4MaxColumns = 1ull << 22;
+size_t kv4_attention_partial_bytes(const Kv4AttentionArgs& a, int head_dim, bool bf16);
 hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf16, hipStream_t stream);
 
 // Largest i with starts[i] <= r (starts not decreasing, n + 1 entries), or -1 where r lies before starts[0] or

@@ -120,7 +120,7 @@ def test_int8_product_refuses_in_the_order_of_the_other_products(rt):
 CACHE = dict(head_dim=128, kv_heads=2, pages=5, sequences=3, table_stride=4, pool=OK, page_table=OK, lengths=OK)
 BAD_CACHES = [dict(struct_size=8), dict(head_dim=96), dict(head_dim=0), dict(kv_heads=0), dict(kv_heads=1025),
               dict(pages=0), dict(pages=1 << 31), dict(sequences=0), dict(sequences=(1 << 20) + 1),
-              dict(sequences=1 << 20, kv_heads=9), dict(table_stride=0), dict(table_stride=(1 << 24) + 1), dict(pool=0),
+              dict(sequences=1 << 20, kv_heads=5), dict(table_stride=0), dict(table_stride=(1 << 24) + 1), dict(pool=0),
               dict(pool=OK + 8), dict(page_table=0), dict(page_table=OK + 2), dict(lengths=0), dict(lengths=OK + 1)]
 
 
