@@ -59,7 +59,11 @@ struct Kv4Kernel {
   float* part;  // sums [splits][rows][q_heads][D], then (maximum, weight) [splits][rows][q_heads]
   size_t ends;  // where these begin
   int rows, q_stride, out_stride;
-  int q_heads, group, tiles, tile_rows, splits;
+  int q_heads, group, tiles, splits;
+  int few_pairs;        // pairs (rows times group) up to which a sequence is not a prompt
+  uint64_t* units;      // prompts: page units before each sequence, [sequences + 1]
+  float* prompt_part;   // sums [2 workgroups][rows of a tile][D], then (maximum, weight) of each
+  size_t prompt_ends;   // where these begin
   int split_shift;  // a split has 2^split_shift pages or a share of more
   int window;       // 0: none
   float scale_log2;
@@ -91,7 +95,7 @@ struct Sequence {
 // stands for all of them.
 struct Tile {
   int pos0, pos1, page0, last, splits;
-  __device__ __forceinline__ Tile(const Kv4Kernel& g, const Sequence& s, int tile, int tile_rows) {
+  __device__ __forceinline__ Tile(const Kv4Kernel& g, const Sequence& s, int tile, int tile_rows = kTileRows) {
     const int x0 = tile * tile_rows, from = s.length - s.n;
     pos0 = from + g.over_group(x0);
     pos1 = from + g.over_group(min(x0 + tile_rows, s.n * g.group) - 1);
@@ -211,7 +215,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
   int head, seq, tile0, split;
   coordinates(g, &head, &seq, &tile0, &split);
   const Sequence sq(g, seq);
-  if (sq.n <= 0) return;
+  if (sq.n <= 0 || sq.n * g.group > g.few_pairs) return;
   // Constant address space: page numbers come by scalar loads, which do not wait for the
   // transfers of pages as vector loads would.
   const auto* table = (const Constant*)(g.c.table + (size_t)seq * g.c.table_stride);
@@ -220,7 +224,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
 
   const int pairs = sq.n * g.group;
   for (int tile = tile0; tile * kTileRows < pairs; tile += g.tiles) {
-    const Tile tl(g, sq, tile, kTileRows);
+    const Tile tl(g, sq, tile);
     if (split >= tl.splits) continue;
     // This lane's row: pair x = row * group + query head.  Lanes without one work on zeros.
     const int x0 = tile * kTileRows, x = x0 + r16;
@@ -331,14 +335,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
       if (edge) {
         // A row that lies past its table sees its own token at least, which is bad.
         const bool lost = past && pos / kKv4Page >= g.c.table_stride;
+        const float poison = bad ? NAN : 0.0f;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int t = t0 + 16 * h + 4 * c + i;
             const bool sees = past ? lost : t <= pos && t > low;
-            if (bad) s[c][i] = NAN;
-            if (!sees) s[c][i] = -INFINITY;
+            s[c][i] = sees ? s[c][i] + poison : -INFINITY;
             seen |= (uint32_t)sees << (4 * c + i);
           }
       }
@@ -528,6 +532,93 @@ struct Prompt {
   }
 };
 
+// A prompt's work in units: a page of a tile (of Prompt::kRows pairs) of a key head.  All tiles of
+// a sequence count the pages from its first tile's first to its last tile's last.
+struct PromptSpan {
+  int page0, pages, tiles;
+  __device__ __forceinline__ PromptSpan(const Kv4Kernel& g, const Sequence& s, int tile_rows) {
+    const int pairs = s.n * g.group;
+    tiles = s.n > 0 && pairs > g.few_pairs ? (pairs + tile_rows - 1) / tile_rows : 0;
+    page0 = pages = 0;
+    if (tiles > 0) {
+      page0 = Tile(g, s, 0, tile_rows).page0;
+      pages = max(1, Tile(g, s, tiles - 1, tile_rows).last - page0);
+    }
+  }
+};
+
+// units[i] = units before sequence i: one workgroup, 256 sequences at a time.
+template <int kRows>
+__global__ __launch_bounds__(256) void kv4_prompt_units_kernel(const Kv4Kernel g) {
+  __shared__ uint64_t waves[4];
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  uint64_t before = 0;
+  for (int from = 0; from < g.c.sequences; from += 256) {
+    const int seq = from + tid;
+    uint64_t own = 0;
+    if (seq < g.c.sequences) {
+      const PromptSpan span(g, Sequence(g, seq), kRows);
+      own = (uint64_t)span.tiles * (uint64_t)span.pages * (uint64_t)g.c.kv_heads;
+    }
+    uint64_t sum = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint64_t o = __shfl_up(sum, d);
+      if (lane >= d) sum += o;
+    }
+    if (lane == 63) waves[tid >> 6] = sum;
+    __syncthreads();
+    uint64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < tid >> 6) sum += waves[w];
+      all += waves[w];
+    }
+    if (seq < g.c.sequences) g.units[seq] = before + sum - own;
+    before += all;
+    __syncthreads();
+  }
+  if (tid == 0) g.units[g.c.sequences] = before;
+}
+
+// A stretch of units within one tile and head: pages from..to of the sequence's span (0: its first).
+struct PromptPiece {
+  int seq, tile, head, from, to, pages;
+  // The piece at unit u, cut at `end`.
+  __device__ __forceinline__ PromptPiece(const Kv4Kernel& g, uint64_t u, uint64_t end, int tile_rows) {
+    // The sequence: the last whose units begin at or before u (64 places a step); it has units,
+    // since those without any begin where their successor does.
+    const int lane = (int)threadIdx.x & 63;
+    int lo = 0, span = g.c.sequences + 1;
+    while (span > 1) {
+      const int step = (span + 63) >> 6, at = lo + lane * step;
+      const int c = __popcll(__ballot(at < lo + span && g.units[at] <= u));
+      const int next = lo + (c - 1) * step;
+      span = min(step, lo + span - next);
+      lo = next;
+    }
+    seq = __builtin_amdgcn_readfirstlane(lo);
+    const PromptSpan sp(g, Sequence(g, seq), tile_rows);
+    pages = sp.pages;
+    const uint64_t rel = u - g.units[seq];
+    const uint64_t item = rel / (uint32_t)pages;
+    from = __builtin_amdgcn_readfirstlane((int)(rel - item * (uint32_t)pages));
+    const uint64_t left = end - u;
+    to = left < (uint64_t)(pages - from) ? from + __builtin_amdgcn_readfirstlane((int)left) : pages;
+    head = __builtin_amdgcn_readfirstlane((int)(item % (uint32_t)g.c.kv_heads));
+    tile = __builtin_amdgcn_readfirstlane((int)(item / (uint32_t)g.c.kv_heads));
+  }
+};
+
+// The first unit of workgroup w of n: shares that differ by one at most.
+__device__ __forceinline__ uint64_t first_unit(uint64_t total, uint64_t w, uint64_t n) {
+  return total / n * w + min(w, total % n);
+}
+
+// Workgroup w does units first_unit(w) to first_unit(w + 1), whatever tiles these cut through:
+// every workgroup has the same number of pages.  A piece that is not a whole tile leaves its sums
+// in place 2 w + 1 where it begins the tile (it is then the workgroup's last), 2 w otherwise (its
+// first), for kv4_prompt_join_kernel.
 template <bool kF32, int D>
 __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWaves / 4)) void kv4_prompt_kernel(const Kv4Kernel g) {
   using Pr = Prompt<kF32, D>;
@@ -539,15 +630,18 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lq = lane & 31, hi = lane >> 5;
-  int head, seq, tile0, split;
-  coordinates(g, &head, &seq, &tile0, &split);
-  const Sequence sq(g, seq);
-  if (sq.n <= 0) return;
-  const auto* table = (const Constant*)(g.c.table + (size_t)seq * g.c.table_stride);
-  const int pairs = sq.n * g.group;
-  for (int tile = tile0; tile * Pr::kRows < pairs; tile += g.tiles) {
+  const uint64_t total = g.units[g.c.sequences];
+  uint64_t unit = first_unit(total, blockIdx.x, gridDim.x);
+  const uint64_t unit_end = first_unit(total, blockIdx.x + 1ull, gridDim.x);
+  while (unit < unit_end) {
+    const PromptPiece piece(g, unit, unit_end, Pr::kRows);
+    unit += (uint64_t)(piece.to - piece.from);
+    const int head = piece.head, tile = piece.tile;
+    const Sequence sq(g, piece.seq);
+    const auto* table = (const Constant*)(g.c.table + (size_t)piece.seq * g.c.table_stride);
+    const int pairs = sq.n * g.group;
     const Tile tl(g, sq, tile, Pr::kRows);
-    if (split >= tl.splits) continue;
+    const int span0 = PromptSpan(g, sq, Pr::kRows).page0;
     // This lane's row, and the first and last position of the wave's 32.
     const int x0 = tile * Pr::kRows + 32 * wave, x = x0 + lq;
     const bool mine = x < pairs;
@@ -594,9 +688,7 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
       return number >= g.c.pages || p * kKv4Page + (kKv4Page - 1) > tl.pos0 ||
              (g.window && p * kKv4Page <= tl.pos1 - g.window);
     };
-    // A split's pages are neighbours here.
-    const int share = (tl.last - tl.page0 + tl.splits - 1) / tl.splits;
-    const int begin = tl.page0 + split * share, end = min(begin + share, tl.last);
+    const int begin = max(tl.page0, span0 + piece.from), end = min(tl.last, span0 + piece.to);
     typename Pr::Codes codes;
     uint32_t number = page_number(begin), next_number = begin + 1 < end ? page_number(begin + 1) : 0;
     if (begin < end) {
@@ -629,14 +721,14 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
         // Register r of block tb is token 32 tb + 8 (r / 4) + 4 hi + r % 4.
         if (bad || t0 + (kKv4Page - 1) > wave0 || (g.window && t0 <= wave1 - g.window)) {
           const bool lost = past && pos / kKv4Page >= g.c.table_stride;
+          const float poison = bad ? NAN : 0.0f;
 #pragma unroll
           for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int t = t0 + 32 * tb + 8 * (r >> 2) + 4 * hi + (r & 3);
               const bool sees = past ? lost : t <= pos && t > low;
-              if (bad) s[tb][r] = NAN;
-              if (!sees) s[tb][r] = -INFINITY;
+              s[tb][r] = sees ? s[tb][r] + poison : -INFINITY;
             }
         }
         float m = s[0][0];
@@ -709,16 +801,15 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
 
     l_run = sum_halves(l_run);
     if (mine) {
-      const size_t pair = (size_t)(sq.first + row) * g.q_heads + q_head;
-      if (tl.splits > 1) {
-        const size_t at = (size_t)split * g.rows * g.q_heads + pair;
+      if (piece.from > 0 || piece.to < piece.pages) {
+        const size_t at = (2ull * blockIdx.x + (piece.from == 0)) * Pr::kRows + 32 * wave + lq;
 #pragma unroll
         for (int bl = 0; bl < kB; ++bl)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            *reinterpret_cast<floatx4*>(g.part + at * D + 32 * bl + 8 * r + 4 * hi) =
+            *reinterpret_cast<floatx4*>(g.prompt_part + at * D + 32 * bl + 8 * r + 4 * hi) =
                 floatx4{o[bl][4 * r], o[bl][4 * r + 1], o[bl][4 * r + 2], o[bl][4 * r + 3]};
-        if (hi == 0) reinterpret_cast<float2*>(ends(g))[at] = make_float2(m_run, l_run);
+        if (hi == 0) reinterpret_cast<float2*>(g.prompt_part + g.prompt_ends)[at] = make_float2(m_run, l_run);
       } else {
         const float f = l_run == 0.0f ? 0.0f : 1.0f / l_run;
         const size_t at = (size_t)(sq.first + row) * g.out_stride + (size_t)q_head * D + 4 * hi;
@@ -741,6 +832,49 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
   }
 }
 
+// Joins the pieces of a tile that workgroups of kv4_prompt_kernel cut it into, 16 rows a workgroup:
+// blockIdx.y's last piece if it begins a tile that the next workgroup goes on with, and the first
+// pieces of those that follow up to the tile's end, in order.
+template <bool kF32, int D>
+__global__ __launch_bounds__(256) void kv4_prompt_join_kernel(const Kv4Kernel g) {
+  constexpr int kRows = Prompt<kF32, D>::kRows, kChannels = D / 16;
+  const uint64_t total = g.units[g.c.sequences], n = gridDim.y, w = blockIdx.y;
+  const uint64_t begin = first_unit(total, w, n), end = first_unit(total, w + 1, n);
+  if (begin == end) return;
+  const PromptPiece last(g, end - 1, end, kRows);
+  const uint64_t tile_begin = end - 1 - (uint64_t)last.from, tile_end = tile_begin + (uint64_t)last.pages;
+  if (tile_begin < begin || tile_end == end) return;  // begun before, or whole
+  uint64_t stop = w + 1;  // the workgroup behind the last that has a piece
+  while (stop < n && first_unit(total, stop, n) < tile_end) ++stop;
+
+  const Sequence sq(g, last.seq);
+  const int r = 16 * (int)blockIdx.x + (int)threadIdx.x / 16, x = last.tile * kRows + r;
+  if (x >= sq.n * g.group) return;
+  const int row = g.over_group(x), q_head = last.head * g.group + x - row * g.group;
+  const float2* all = reinterpret_cast<const float2*>(g.prompt_part + g.prompt_ends);
+  auto place = [&](uint64_t i) { return (2 * i + (i == w)) * kRows + r; };
+  float top = -INFINITY;
+  for (uint64_t i = w; i < stop; ++i) top = fmaxf(top, all[place(i)].x);
+  float sum[kChannels] = {}, weight = 0.0f;
+  for (uint64_t i = w; i < stop; ++i) {
+    const float2 e = all[place(i)];
+    const float f = e.x == top ? 1.0f : __builtin_amdgcn_exp2f((e.x - top) * g.scale_log2);
+    weight = __builtin_fmaf(e.y, f, weight);
+    const float* from = g.prompt_part + place(i) * D + kChannels * (threadIdx.x % 16);
+#pragma unroll
+    for (int c = 0; c < kChannels; ++c) sum[c] = __builtin_fmaf(from[c], f, sum[c]);
+  }
+  const size_t to = (size_t)(sq.first + row) * g.out_stride + (size_t)q_head * D + kChannels * (threadIdx.x % 16);
+#pragma unroll
+  for (int c = 0; c < kChannels; ++c) {
+    const float v = weight == 0.0f ? 0.0f : sum[c] / weight;
+    if constexpr (kF32)
+      static_cast<float*>(g.out)[to + c] = v;
+    else
+      static_cast<__bf16*>(g.out)[to + c] = (__bf16)v;
+  }
+}
+
 // One workgroup a row and query head joins the splits' sums.  Its threads are D / 4 columns of
 // four channels times kParts: part i adds splits i, i + kParts, ..., the parts are added in
 // order.  Bound by latency: maxima and weights come in one load a lane, sums four at a time.
@@ -760,7 +894,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
     const int seq = find_sequence(g.starts, g.c.sequences, row);
     if (seq < 0) continue;
     const Sequence sq(g, seq);
-    const int splits = Tile(g, sq, ((row - sq.first) * g.group + q_head % g.group) / g.tile_rows, g.tile_rows).splits;
+    if (sq.n * g.group > g.few_pairs) continue;
+    const int splits = Tile(g, sq, ((row - sq.first) * g.group + q_head % g.group) / kTileRows).splits;
     if (splits == 1) continue;
     float top = lane < splits ? e.x : -INFINITY, weight = e.y;
     const float mine = top;
@@ -806,48 +941,75 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
 // eight a wave), fewer where that is what fills the chip; a shorter sequence has fewer splits, so
 // that workgroups are of one size whatever the lengths.
 struct Plan {
-  int tile_rows, tiles, splits, shift;
+  int tiles, splits, shift;  // of the sequences with few rows
+  int few_pairs;             // up to so many pairs are few
+  bool few;                  // there may be such sequences
+  int prompt_groups;         // workgroups for prompts (0: there are none)
+  int prompt_rows;
+  size_t prompt_ends;        // floats of the prompts' partial sums
+  size_t part_bytes, prompt_bytes, unit_bytes;
 };
 Plan plan(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
-  Plan p;
+  Plan p{};
   const uint64_t columns = (uint64_t)a.c.sequences * a.c.kv_heads;  // at most kKv4MaxColumns
   const uint64_t most = (uint64_t)a.max_rows * (uint64_t)a.group;
-  const int prompt_rows = 32 * (head_dim == 256 || (!bf16 && head_dim == 128) ? 4 : 8);
-  p.tile_rows = most > kFewPairs ? prompt_rows : kTileRows;
-  p.tiles = (int)std::min<uint64_t>((most + p.tile_rows - 1) / p.tile_rows, kKv4MaxColumns / columns);
   uint64_t length = a.max_length;
-  if (a.window) length = std::min<uint64_t>(length, (uint64_t)a.window + p.tile_rows / a.group + 2 * kKv4Page);
+  if (most > kFewPairs) {
+    p.prompt_rows = 32 * (head_dim == 256 || (!bf16 && head_dim == 128) ? 4 : 8);
+    const uint64_t tiles = ((uint64_t)a.rows * (uint64_t)a.group + p.prompt_rows - 1) / p.prompt_rows;
+    const uint64_t units = tiles * (uint64_t)a.c.kv_heads * ((length + kKv4Page - 1) / kKv4Page);
+    p.prompt_groups = (int)std::max<uint64_t>(1, std::min<uint64_t>(256, units / 4));
+    p.prompt_ends = 2ull * p.prompt_groups * p.prompt_rows * (size_t)head_dim;
+    p.prompt_bytes = (p.prompt_ends + 4ull * p.prompt_groups * p.prompt_rows) * sizeof(float);
+    p.unit_bytes = ((size_t)a.c.sequences + 1) * sizeof(uint64_t);
+  }
+  // A call of one sequence is either; otherwise sequences of few rows go their own way beside prompts.
+  p.few = p.prompt_groups == 0 || a.c.sequences > 1;
+  p.few_pairs = p.prompt_groups == 0 ? 0x7fffffff : p.few ? (int)kFewPairs : 0;
+  if (!p.few) return p;
+  p.tiles = (int)std::min<uint64_t>((std::min<uint64_t>(most, p.few_pairs) + kTileRows - 1) / kTileRows, kKv4MaxColumns / columns);
+  if (a.window) length = std::min<uint64_t>(length, (uint64_t)a.window + 2 * kKv4Page);
   const uint64_t pages = (length + kKv4Page - 1) / kKv4Page, base = columns * (uint64_t)p.tiles;
-  const uint64_t full = p.tile_rows == kTileRows ? 1024 : 512;
-  p.shift = p.tile_rows == kTileRows ? 2 : 3;
-  while (p.shift < 5 && base * (pages >> p.shift) > full) ++p.shift;
+  p.shift = 2;
+  while (p.shift < 5 && base * (pages >> p.shift) > 1024) ++p.shift;
   while (((pages + (1ull << p.shift) - 1) >> p.shift) > (uint64_t)kMaxSplits) ++p.shift;
   p.splits = (int)((pages + (1ull << p.shift) - 1) >> p.shift);
-  if (base >= 4 * full || (uint64_t)p.splits * a.rows * (uint64_t)a.q_heads * (uint64_t)(head_dim + 2) * 4 > kMostPartialBytes)
-    p.splits = 1;
+  p.part_bytes = (size_t)p.splits * a.rows * (size_t)a.q_heads * (size_t)(head_dim + 2) * sizeof(float);
+  if (base >= 4096 || p.part_bytes > kMostPartialBytes) p.splits = 1;
+  if (p.splits == 1) p.part_bytes = 0;
   return p;
 }
 
 template <bool kF32, int D>
-hipError_t launch(const Kv4Kernel& g, hipStream_t stream) {
-  const uint64_t grid = (uint64_t)g.c.sequences * g.c.kv_heads * (uint64_t)g.tiles * (uint64_t)g.splits;
-  if (g.tile_rows == kTileRows)
-    hipLaunchKernelGGL((kv4_attention_kernel<kF32, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, stream, g);
-  else
-    hipLaunchKernelGGL((kv4_prompt_kernel<kF32, D>), dim3((unsigned)grid), dim3((Prompt<kF32, D>::kThreads)), 0, stream, g);
-  if (g.splits > 1) {
-    const uint64_t pairs = (uint64_t)g.rows * (uint64_t)g.q_heads;
-    hipLaunchKernelGGL((kv4_join_kernel<kF32, D>), dim3((unsigned)std::min<uint64_t>(pairs, 1u << 20)), dim3(256),
-                       0, stream, g);
+hipError_t launch(const Kv4Kernel& g, const Plan& p, hipStream_t stream) {
+  if (p.prompt_groups > 0) {
+    constexpr int kRows = Prompt<kF32, D>::kRows;
+    hipLaunchKernelGGL(kv4_prompt_units_kernel<kRows>, dim3(1), dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((kv4_prompt_kernel<kF32, D>), dim3((unsigned)p.prompt_groups), dim3((Prompt<kF32, D>::kThreads)), 0,
+                       stream, g);
+    if (p.prompt_groups > 1)
+      hipLaunchKernelGGL((kv4_prompt_join_kernel<kF32, D>), dim3(kRows / 16, (unsigned)p.prompt_groups), dim3(256), 0,
+                         stream, g);
+  }
+  if (p.few) {
+    const unsigned grid = (unsigned)g.c.sequences * (unsigned)g.c.kv_heads * (unsigned)p.tiles * (unsigned)p.splits;
+    hipLaunchKernelGGL((kv4_attention_kernel<kF32, D>), dim3(grid), dim3(64 * kWaves), 0, stream, g);
+    if (p.splits > 1) {
+      const uint64_t pairs = (uint64_t)g.rows * (uint64_t)g.q_heads;
+      hipLaunchKernelGGL((kv4_join_kernel<kF32, D>), dim3((unsigned)std::min<uint64_t>(pairs, 1u << 20)), dim3(256), 0,
+                         stream, g);
+    }
   }
   return hipGetLastError();
 }
+
+size_t round_up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 }  // namespace
 
 size_t kv4_attention_partial_bytes(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
   const Plan p = plan(a, head_dim, bf16);
-  return p.splits > 1 ? (size_t)p.splits * a.rows * a.q_heads * (head_dim + 2) * sizeof(float) : 0;
+  return round_up(p.part_bytes) + round_up(p.prompt_bytes) + p.unit_bytes;
 }
 
 hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf16, hipStream_t stream) {
@@ -856,7 +1018,6 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf
   g.q = a.q;
   g.out = a.out;
   g.starts = a.row_starts;
-  g.part = a.part;
   g.rows = (int)a.rows;
   g.q_stride = (int)a.q_stride;
   g.out_stride = (int)a.out_stride;
@@ -869,15 +1030,19 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf
   g.group_shift = 31 + l;
   g.group_magic = (1ull << g.group_shift) / (uint64_t)a.group + 1;
   const Plan p = plan(a, head_dim, bf16);
-  g.tile_rows = p.tile_rows;
   g.tiles = p.tiles;
   g.splits = p.splits;
   g.split_shift = p.shift;
+  g.few_pairs = p.few_pairs;
+  g.part = a.part;
   g.ends = (size_t)p.splits * a.rows * (size_t)a.q_heads * (size_t)head_dim;
+  g.prompt_part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.part) + round_up(p.part_bytes));
+  g.prompt_ends = p.prompt_ends;
+  g.units = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(g.prompt_part) + round_up(p.prompt_bytes));
   switch (head_dim) {
-    case 64: return bf16 ? launch<false, 64>(g, stream) : launch<true, 64>(g, stream);
-    case 128: return bf16 ? launch<false, 128>(g, stream) : launch<true, 128>(g, stream);
-    case 256: return bf16 ? launch<false, 256>(g, stream) : launch<true, 256>(g, stream);
+    case 64: return bf16 ? launch<false, 64>(g, p, stream) : launch<true, 64>(g, p, stream);
+    case 128: return bf16 ? launch<false, 128>(g, p, stream) : launch<true, 128>(g, p, stream);
+    case 256: return bf16 ? launch<false, 256>(g, p, stream) : launch<true, 256>(g, p, stream);
   }
   return hipErrorInvalidValue;
 }
