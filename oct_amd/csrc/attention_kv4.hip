@@ -25,6 +25,7 @@
 // order.  Bound by reading the cache for long sequences (272 bytes of a 64-channel
 // group pair... per token and head D + D / 16 bytes).
 #include <algorithm>
+#include <type_traits>
 
 #include "reactor_internal.h"
 
@@ -88,6 +89,19 @@ struct Sequence {
     n = min(max(starts[seq + 1], 0), g.rows) - first;
     length = max(((Constant*)g.c.lengths)[seq], 0);
   }
+};
+
+// The tokens that a row sees, or is spoilt by: t with t - first < count (as unsigned numbers).
+// On the page that stands for all behind the table (`past`) a row sees every token or none: one
+// that lies there sees its own at least, which is bad.
+struct Sees {
+  uint32_t first, count;
+  __device__ __forceinline__ Sees(const Kv4Kernel& g, int pos, bool past) {
+    const int low = g.window && pos >= g.window ? pos - g.window + 1 : 0;
+    first = past ? 0u : (uint32_t)low;
+    count = past ? (pos / kKv4Page >= g.c.table_stride ? 0xFFFFFFFFu : 0u) : pos < low ? 0u : (uint32_t)(pos - low) + 1u;
+  }
+  __device__ __forceinline__ bool operator()(int t) const { return (uint32_t)t - first < count; }
 };
 
 // The positions of a tile's first and last row, the pages that they see between them, and into
@@ -231,8 +245,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
     const bool mine = x < pairs;
     const int row = mine ? g.over_group(x) : 0;
     const int q_head = head * g.group + (mine ? x - row * g.group : 0);
-    const int pos = mine ? sq.length - sq.n + row : tl.pos1;             // its position
-    const int low = g.window && pos >= g.window ? pos - g.window : -1;  // it sees low < t <= pos
+    const int pos = mine ? sq.length - sq.n + row : tl.pos1;  // its position
     const int page0 = tl.page0, last = tl.last;
 
     // Q^T operand: lane (h, row), step s: channels 32 s + 8 h .. + 7.
@@ -333,15 +346,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
       const bool edge = bad || t0 + (kKv4Page - 1) > tl.pos0 || (g.window && t0 <= tl.pos1 - g.window);
       uint32_t seen = 0;  // bit j: token 16 h + j
       if (edge) {
-        // A row that lies past its table sees its own token at least, which is bad.
-        const bool lost = past && pos / kKv4Page >= g.c.table_stride;
+        const Sees row_sees(g, pos, past);
         const float poison = bad ? NAN : 0.0f;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int t = t0 + 16 * h + 4 * c + i;
-            const bool sees = past ? lost : t <= pos && t > low;
+            const bool sees = row_sees(t0 + 16 * h + 4 * c + i);
             s[c][i] = sees ? s[c][i] + poison : -INFINITY;
             seen |= (uint32_t)sees << (4 * c + i);
           }
@@ -468,7 +479,7 @@ struct Prompt {
   static constexpr int kThreads = 64 * kWaves, kRows = 32 * kWaves;
   static constexpr int kUnits = 4 * D;                                // of 8 bytes (16 channels): keys, and values
   static constexpr int kEach = 2 * kUnits / kThreads > 0 ? 2 * kUnits / kThreads : 1;
-  static constexpr int kTileBytes = kKv4Page * D * 2;                 // bf16 keys, then values
+  static constexpr int kTileBytes = kKv4Page * D * 2;                 // bf16 keys, or values
   static_assert(kEach * kThreads == 2 * kUnits && kUnits % 64 == 0, "units");
 
   // Position of 16-byte chunk c (8 channels) of token t: operand reads of 32 keys, and transpose
@@ -492,19 +503,22 @@ struct Prompt {
     if (!keys) return b / 32;
     return D == 64 ? 0 : 2 * (b / 64) + b / 8 % 2;
   }
-  __device__ static __forceinline__ void load(Codes& c, const uint8_t* block, int tid) {
+  // The thread's units of a keys' and a values' page.
+  __device__ static __forceinline__ void load(Codes& c, const uint8_t* key_block, const uint8_t* value_block, int tid) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       bool keys;
       int t, b;
       unit(i, tid, &keys, &t, &b);
+      const uint8_t* block = keys ? key_block : value_block;
       c.w[i] = *reinterpret_cast<const u32x2*>(block + (keys ? 0 : Stage<D>::kCodes) + t * (D / 2) + b);
       c.step[i] = *reinterpret_cast<const uint16_t*>(block + Stage<D>::kSteps + 128 * (group_of(keys, b) + (keys ? 0 : D / 64)) + 2 * t);
     }
   }
-  // Codes to bf16 in LDS.  zero_from: values from this token of the page on, and on an edge page
+  // Codes to bf16 in LDS.  Values of an edge page: those from token zero_from of the page on, and
   // those that are not finite, count as 0 (some row does not see them).
-  __device__ static __forceinline__ void store(const Codes& c, uint8_t* lds, int tid, bool edge, int zero_from) {
+  __device__ static __forceinline__ void store(const Codes& c, uint8_t* key_lds, uint8_t* value_lds, int tid, bool edge,
+                                               int zero_from) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       bool keys;
@@ -525,8 +539,8 @@ struct Prompt {
         const int word = b / 4 + j;
         int chunk = word;
         if (keys) chunk = D == 64 ? 4 * (word & 1) + (word >> 1) : (word & ~15) + 4 * (word & 3) + (word >> 2 & 3);
-        const int at = (keys ? 0 : kTileBytes) + t * 2 * D + 16 * (chunk ^ (keys ? key_swz(t) : value_swz(t)));
-        *reinterpret_cast<bf16x8*>(lds + at) = x;
+        const int at = t * 2 * D + 16 * (chunk ^ (keys ? key_swz(t) : value_swz(t)));
+        *reinterpret_cast<bf16x8*>((keys ? key_lds : value_lds) + at) = x;
       }
     }
   }
@@ -625,11 +639,12 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
   constexpr int kG = D / 64, kT = kF32 ? 3 : 1;
   constexpr int kSteps = D / 16;  // MFMA steps of 16 channels
   constexpr int kB = D / 32;      // blocks of 32 output channels
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2 * Pr::kTileBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t key_lds[2][Pr::kTileBytes], value_lds[2][Pr::kTileBytes];
 
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lq = lane & 31, hi = lane >> 5;
+  const int behind = Pr::kWaves == 8 ? wave >> 2 : 0;  // half a page behind the other four waves
   const uint64_t total = g.units[g.c.sequences];
   uint64_t unit = first_unit(total, blockIdx.x, gridDim.x);
   const uint64_t unit_end = first_unit(total, blockIdx.x + 1ull, gridDim.x);
@@ -650,7 +665,6 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
     const int from = sq.length - sq.n;
     const int wave0 = from + g.over_group(min(x0, pairs - 1)), wave1 = from + g.over_group(min(x0 + 32, pairs) - 1);
     const int pos = mine ? from + row : wave1;
-    const int low = g.window && pos >= g.window ? pos - g.window : -1;  // it sees low < t <= pos
 
     bf16x8 q[kSteps][kT];
 #pragma unroll
@@ -689,114 +703,161 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
              (g.window && p * kKv4Page <= tl.pos1 - g.window);
     };
     const int begin = max(tl.page0, span0 + piece.from), end = min(tl.last, span0 + piece.to);
+    const int pages = end - begin;
+    // Behind the last page the last one stands again, unused.
+    auto number_of = [&](int n) { return page_number(begin + min(n, pages - 1)); };
+    auto barrier = [] {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
     typename Pr::Codes codes;
-    uint32_t number = page_number(begin), next_number = begin + 1 < end ? page_number(begin + 1) : 0;
-    if (begin < end) {
-      Pr::load(codes, page_block(number), tid);
-      Pr::store(codes, lds[0], tid, page_edge(begin, number), number >= g.c.pages ? 0 : tl.pos1 - begin * kKv4Page + 1);
-    }
-    int now = 0;
-    for (int pg = begin; pg < end; ++pg) {
-      __syncthreads();  // this page is complete, the other half of LDS no longer read
-      const bool more = pg + 1 < end;
-      if (more) Pr::load(codes, page_block(next_number), tid);
-      const uint32_t after = pg + 2 < end ? page_number(pg + 2) : 0;
-      const uint8_t* keys = lds[now];
-      const uint8_t* values = lds[now] + Pr::kTileBytes;
+    floatx16 s[2];
+    bf16x8 p[4][kT];
+    // The matrix phase: O += V P of the page before and S = K Q of this one, in quads of four
+    // operand reads and the instructions that use them; a quad is read while the one before it is
+    // multiplied.  Operand e of the output: block e % kB of tokens 16 (e / kB) + 4 hi + 0..3 and 8
+    // further; of the scores: step e / 2 of tokens 32 (e % 2) + lq.
+    auto read_quad = [&](bf16x8 (&f)[4], int quad, const uint8_t* values, const uint8_t* keys) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = 4 * (quad % kB) + i;
+        if (quad < kB) {
+          const int t = 16 * (e / kB) + 4 * hi + ((lane & 15) >> 2);
+          const int d = 32 * (e % kB) + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+          const uint8_t* at = values + t * 2 * D + 16 * ((d >> 3) ^ Pr::value_swz(t)) + 2 * (d & 7);
+          const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+          const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * 2 * D));
+          f[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+          const int t = 32 * (e % 2) + lq;
+          f[i] = *reinterpret_cast<const bf16x8*>(keys + t * 2 * D + 16 * ((2 * (e / 2) + hi) ^ Pr::key_swz(t)));
+        }
+      }
+    };
+    auto use_quad = [&](const bf16x8 (&f)[4], int quad) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = 4 * (quad % kB) + i;
+#pragma unroll
+        for (int j = 0; j < kT; ++j) {
+          if (quad < kB)
+            o[e % kB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], p[e / kB][j], o[e % kB], 0, 0, 0);
+          else
+            s[e % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], q[e / 2][j], s[e % 2], 0, 0, 0);
+        }
+      }
+    };
+    auto multiply = [&](const uint8_t* values, const uint8_t* keys, auto scores) __attribute__((always_inline)) {
+      constexpr int kQuads = decltype(scores)::value ? 2 * kB : kB;
+      if constexpr (decltype(scores)::value) s[0] = s[1] = floatx16{};
+      bf16x8 f[2][4];
+      read_quad(f[0], 0, values, keys);
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i) {
+        if (i + 1 < kQuads) read_quad(f[(i + 1) & 1], i + 1, values, keys);
+        __builtin_amdgcn_sched_barrier(0);
+        use_quad(f[i & 1], i);
+      }
+    };
+    // Register r of block tb is token 32 tb + 8 (r / 4) + 4 hi + r % 4.
+    auto weights = [&](int pg, uint32_t number) __attribute__((always_inline)) {
       const int t0 = pg * kKv4Page;
-      const bool bad = number >= g.c.pages, past = pg >= g.c.table_stride;
-
-      // Pages that no row of the wave sees, and waves without rows, are passed over.
-      if (x0 < pairs && (past || (t0 <= wave1 && !(g.window && t0 + (kKv4Page - 1) <= wave0 - g.window)))) {
-        floatx16 s[2] = {};
-#pragma unroll
-        for (int u = 0; u < kSteps; ++u)
-#pragma unroll
-          for (int tb = 0; tb < 2; ++tb) {
-            const int t = 32 * tb + lq;
-            const bf16x8 k = *reinterpret_cast<const bf16x8*>(keys + t * 2 * D + 16 * ((2 * u + hi) ^ Pr::key_swz(t)));
-#pragma unroll
-            for (int i = 0; i < kT; ++i) s[tb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[u][i], s[tb], 0, 0, 0);
-          }
-        // Register r of block tb is token 32 tb + 8 (r / 4) + 4 hi + r % 4.
-        if (bad || t0 + (kKv4Page - 1) > wave0 || (g.window && t0 <= wave1 - g.window)) {
-          const bool lost = past && pos / kKv4Page >= g.c.table_stride;
-          const float poison = bad ? NAN : 0.0f;
-#pragma unroll
-          for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int t = t0 + 32 * tb + 8 * (r >> 2) + 4 * hi + (r & 3);
-              const bool sees = past ? lost : t <= pos && t > low;
-              s[tb][r] = sees ? s[tb][r] + poison : -INFINITY;
-            }
-        }
-        float m = s[0][0];
+      const bool bad = number >= g.c.pages;
+      const Sees row_sees(g, pos, pg >= g.c.table_stride);
+      if (bad || t0 + (kKv4Page - 1) > wave0 || (g.window && t0 <= wave1 - g.window)) {
+        const float poison = bad ? NAN : 0.0f;
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) m = fmaxf(m, s[tb][r]);
-        m = max_halves(m);
-        if (__any((m - m_run) * g.scale_log2 > kLazyLog2)) {
-          const float m_new = fmaxf(m, m_run);
-          const float alpha = m_new == m_run ? 1.0f : __builtin_amdgcn_exp2f((m_run - m_new) * g.scale_log2);
-          m_run = m_new;
-          m_log2 = m_new == -INFINITY ? 0.0f : m_new * g.scale_log2;
-          l_run *= alpha;
-#pragma unroll
-          for (int i = 0; i < kB; ++i) o[i] *= alpha;
-        }
-#pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            bf16x8 p[kT];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tb][8 * half + j], g.scale_log2, -m_log2));
-              l_run += e;
-              __bf16 t[kT];
-              terms(e, t);
-#pragma unroll
-              for (int i = 0; i < kT; ++i) p[i][j] = t[i];
-            }
-            // Tokens 32 tb + 16 half + 4 hi + 0..3, and 8 further.
-            const int t = 32 * tb + 16 * half + 4 * hi + ((lane & 15) >> 2);
-#pragma unroll
-            for (int bl = 0; bl < kB; ++bl) {
-              const int d = 32 * bl + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-              const uint8_t* at = values + t * 2 * D + 16 * ((d >> 3) ^ Pr::value_swz(t)) + 2 * (d & 7);
-              const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-              const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * 2 * D));
-              const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-              for (int i = 0; i < kT; ++i) o[bl] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p[i], o[bl], 0, 0, 0);
-            }
+          for (int r = 0; r < 16; ++r) {
+            const bool sees = row_sees(t0 + 32 * tb + 8 * (r >> 2) + 4 * hi + (r & 3));
+            s[tb][r] = sees ? s[tb][r] + poison : -INFINITY;
           }
-        // Values that are not finite were left out of an edge page: the rows that see them get NaN.
-        if (!bad && page_edge(pg, number)) {
-          const uint16_t* steps = reinterpret_cast<const uint16_t*>(page_block(number) + Stage<D>::kSteps + 2 * D) + lane;
+      }
+      float m = s[0][0];
 #pragma unroll
-          for (int gr = 0; gr < kG; ++gr) {
-            const uint64_t odd = __ballot((steps[64 * gr] & 0x7F80) == 0x7F80);
-            if (odd != 0) {
-              // The page's tokens low < t <= pos as bits.
-              const int to = min(pos - t0, 63), first = max(low + 1 - t0, 0);
-              const bool some = to >= first && first < 64 && to >= 0;
-              const uint64_t sees = some ? (~0ull >> (63 - to)) & (~0ull << first) : 0;
-              const float add = (odd & sees) != 0 ? NAN : 0.0f;
+      for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-              for (int bl = 2 * gr; bl < 2 * gr + 2; ++bl) o[bl] += add;
-            }
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, s[tb][r]);
+      m = max_halves(m);
+      if (__any((m - m_run) * g.scale_log2 > kLazyLog2)) {
+        const float m_new = fmaxf(m, m_run);
+        const float alpha = m_new == m_run ? 1.0f : __builtin_amdgcn_exp2f((m_run - m_new) * g.scale_log2);
+        m_run = m_new;
+        m_log2 = m_new == -INFINITY ? 0.0f : m_new * g.scale_log2;
+        l_run *= alpha;
+#pragma unroll
+        for (int i = 0; i < kB; ++i) o[i] *= alpha;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c & 1) + j], g.scale_log2, -m_log2));
+          l_run += e;
+          __bf16 t[kT];
+          terms(e, t);
+#pragma unroll
+          for (int i = 0; i < kT; ++i) p[c][i][j] = t[i];
+        }
+      // Values that are not finite are left out of an edge page: the rows that see them get NaN.
+      if (!bad && page_edge(pg, number)) {
+        const uint16_t* steps = reinterpret_cast<const uint16_t*>(page_block(number) + Stage<D>::kSteps + 2 * D) + lane;
+#pragma unroll
+        for (int gr = 0; gr < kG; ++gr) {
+          const uint64_t odd = __ballot((steps[64 * gr] & 0x7F80) == 0x7F80);
+          if (odd != 0) {
+            // The page's tokens that the row sees as bits.
+            const uint32_t skip = row_sees.first > (uint32_t)t0 ? row_sees.first - t0 : 0u;
+            const uint64_t upto = row_sees.first + row_sees.count - t0;  // tokens of the page before the end
+            uint64_t sees = 0;
+            if (row_sees.count != 0 && row_sees.first + row_sees.count > (uint32_t)t0 && skip < 64)
+              sees = (upto >= 64 ? ~0ull : (1ull << upto) - 1) & (~0ull << skip);
+            const float add = (odd & sees) != 0 ? NAN : 0.0f;
+#pragma unroll
+            for (int bl = 2 * gr; bl < 2 * gr + 2; ++bl) o[bl] += add;
           }
         }
       }
-      if (more)
-        Pr::store(codes, lds[now ^ 1], tid, page_edge(pg + 1, next_number),
-                  next_number >= g.c.pages ? 0 : tl.pos1 - (t0 + kKv4Page) + 1);
-      now ^= 1;
-      number = next_number;
-      next_number = after;
+    };
+    // A thread's units of keys' page n + 1 + behind and values' page n + behind, so that both are
+    // whole before the first wave needs them and no half of LDS is written while it is read.
+    auto convert = [&](int n, uint32_t value_number) __attribute__((always_inline)) {
+      const int pg = begin + min(n + behind, pages - 1);
+      Pr::store(codes, key_lds[(n + 1 + behind) & 1], value_lds[(n + behind) & 1], tid, page_edge(pg, value_number),
+                value_number >= g.c.pages ? 0 : tl.pos1 - pg * kKv4Page + 1);
+    };
+    if (pages > 0) {
+      uint32_t n0 = number_of(0), n1 = number_of(1), n2 = number_of(2);
+      Pr::load(codes, page_block(n0), page_block(n0), tid);
+      Pr::store(codes, key_lds[0], value_lds[1], tid, true, 0);  // keys; values of 0
+      barrier();
+      if (behind) {
+        Pr::load(codes, page_block(n1), page_block(n0), tid);
+        convert(-1, n0);
+        barrier();
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < kT; ++i) p[c][i] = bf16x8{};  // before the first page, with values of 0
+      for (int n = 0; n < pages; ++n) {
+        const uint32_t value_number = behind ? n1 : n0;
+        Pr::load(codes, page_block(behind ? n2 : n1), page_block(value_number), tid);
+        multiply(value_lds[(n + 1) & 1], key_lds[n & 1], std::true_type{});
+        barrier();
+        const uint32_t n3 = number_of(n + 3);  // here: the matrix phase's waits would wait for it
+        weights(begin + n, n0);
+        convert(n, value_number);
+        barrier();
+        n0 = n1;
+        n1 = n2;
+        n2 = n3;
+      }
+      multiply(value_lds[(pages + 1) & 1], nullptr, std::false_type{});
+      barrier();
+      if (Pr::kWaves == 8 && !behind) barrier();
     }
 
     l_run = sum_halves(l_run);
@@ -828,7 +889,6 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
           }
       }
     }
-    __syncthreads();  // the next tile fills LDS again
   }
 }
 
@@ -875,7 +935,7 @@ __global__ __launch_bounds__(256) void kv4_prompt_join_kernel(const Kv4Kernel g)
   }
 }
 
-// One workgroup a row and query head joins the splits' sums.  Its threads are D / 4 columns of
+// Joins the splits' sums: a workgroup a row, for every gridDim.y-th query head.  Its threads are D / 4 columns of
 // four channels times kParts: part i adds splits i, i + kParts, ..., the parts are added in
 // order.  Bound by latency: maxima and weights come in one load a lane, sums four at a time.
 template <bool kF32, int D>
@@ -885,16 +945,22 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
   __shared__ float factors[kMaxSplits];
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int column = tid % kColumns, part = tid / kColumns;
-  const long long pairs = (long long)g.rows * g.q_heads;
-  for (long long x = blockIdx.x; x < pairs; x += gridDim.x) {
-    const int row = (int)(x / g.q_heads), q_head = (int)(x - (long long)row * g.q_heads);
-    // Splits that this row's tile does not have hold anything; they are left out below.
-    float2 e = make_float2(-INFINITY, 0.0f);
-    if (lane < g.splits) e = reinterpret_cast<const float2*>(ends(g))[(size_t)lane * pairs + x];
-    const int seq = find_sequence(g.starts, g.c.sequences, row);
-    if (seq < 0) continue;
-    const Sequence sq(g, seq);
-    if (sq.n * g.group > g.few_pairs) continue;
+  const int row = (int)blockIdx.x;
+  const size_t pairs = (size_t)g.rows * g.q_heads;
+  auto end_of = [&](int q_head) {  // of this lane's split, if there is one
+    return lane < g.splits ? reinterpret_cast<const float2*>(ends(g))[lane * pairs + (size_t)row * g.q_heads + q_head]
+                           : make_float2(-INFINITY, 0.0f);
+  };
+  float2 next = end_of((int)blockIdx.y);
+  const int seq = find_sequence(g.starts, g.c.sequences, row);
+  if (seq < 0) return;
+  const Sequence sq(g, seq);
+  if (sq.n * g.group > g.few_pairs) return;
+  for (int q_head = (int)blockIdx.y; q_head < g.q_heads; q_head += (int)gridDim.y) {
+    const size_t x = (size_t)row * g.q_heads + q_head;
+    const float2 e = next;
+    if (q_head + (int)gridDim.y < g.q_heads) next = end_of(q_head + (int)gridDim.y);
+    // Splits that this row's tile does not have hold anything; they are left out.
     const int splits = Tile(g, sq, ((row - sq.first) * g.group + q_head % g.group) / kTileRows).splits;
     if (splits == 1) continue;
     float top = lane < splits ? e.x : -INFINITY, weight = e.y;
@@ -909,7 +975,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
     __syncthreads();
     floatx4 sum = {};
     const floatx4* at = reinterpret_cast<const floatx4*>(g.part + (size_t)x * D) + column;
-    const size_t slab = (size_t)pairs * kColumns;
+    const size_t slab = pairs * kColumns;
 #pragma unroll 4
     for (int s = part; s < splits; s += kParts) {
       const floatx4 v = at[s * slab];
@@ -995,9 +1061,8 @@ hipError_t launch(const Kv4Kernel& g, const Plan& p, hipStream_t stream) {
     const unsigned grid = (unsigned)g.c.sequences * (unsigned)g.c.kv_heads * (unsigned)p.tiles * (unsigned)p.splits;
     hipLaunchKernelGGL((kv4_attention_kernel<kF32, D>), dim3(grid), dim3(64 * kWaves), 0, stream, g);
     if (p.splits > 1) {
-      const uint64_t pairs = (uint64_t)g.rows * (uint64_t)g.q_heads;
-      hipLaunchKernelGGL((kv4_join_kernel<kF32, D>), dim3((unsigned)std::min<uint64_t>(pairs, 1u << 20)), dim3(256), 0,
-                         stream, g);
+      const unsigned heads = std::min<unsigned>((unsigned)g.q_heads, std::max(1u, 4096u / (unsigned)g.rows));
+      hipLaunchKernelGGL((kv4_join_kernel<kF32, D>), dim3((unsigned)g.rows, heads), dim3(256), 0, stream, g);
     }
   }
   return hipGetLastError();
