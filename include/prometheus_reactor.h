@@ -960,7 +960,7 @@ PROM_REACTOR_API uint64_t prometheus_reactor_kv4_page_bytes(uint32_t head_dim, u
 typedef struct PrometheusKv4RowsRequest {
   uint32_t struct_size;
   uint32_t dtype;
-  uint32_t rows;        /* 1..2^24 */
+  uint32_t rows;        /* 1..2^22 */
   uint32_t row_stride;  /* below 2^24 */
   void* k;
   void* v;
@@ -987,7 +987,7 @@ PROM_REACTOR_API int prometheus_reactor_runtime_kv4_read_device(void* handle, co
 typedef struct PrometheusKv4AttentionRequest {
   uint32_t struct_size;
   uint32_t dtype;
-  uint32_t rows;        /* 1..2^24 */
+  uint32_t rows;        /* 1..2^22 */
   uint32_t q_heads;     /* a multiple of kv_heads, at most 2^16; rows * (q_heads / kv_heads) below 2^30 */
   uint32_t q_stride;    /* >= q_heads * head_dim, below 2^24 */
   uint32_t out_stride;  /* >= q_heads * head_dim, below 2^24 */

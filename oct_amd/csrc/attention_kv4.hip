@@ -48,7 +48,15 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 constexpr float kLazyLog2 = 8.0f;
 constexpr int kTileRows = 16;
 constexpr int kWaves = 4;
+// Sequences of up to kFewPairs pairs (rows times query heads of a group) stay on the kernel for few
+// rows, whatever the call: a prompt tile has 128 or 256.  The prompt kernel's three launches and
+// their joins cost 25 to 50 us, and it saves 0.5 (64 channels) to 2.3 ns (256) for a page of 16 pairs
+// (us, two prompts over 4096 tokens, 4 key heads, groups of 4, few rows' kernel against it; 512 new
+// rows each: bf16 64 channels 57 / 52, 128 98 / 68, 256 241 / 151, fp32 66 / 69, 123 / 110; 64 new
+// rows: 18 / 42, 27 / 52, 49 / 84, 20 / 49, 31 / 55), so it is taken from kPromptWork such pages on.
+// fp32 rows of 256 channels do not fit its registers (310 / 409).
 constexpr uint64_t kFewPairs = 64;
+constexpr uint64_t kPromptWork = 40000;
 constexpr int kMaxSplits = 64;  // a lane each when they are joined
 constexpr uint64_t kMostPartialBytes = 1ull << 30;
 
@@ -1010,7 +1018,7 @@ struct Plan {
   int tiles, splits, shift;  // of the sequences with few rows
   int few_pairs;             // up to so many pairs are few
   bool few;                  // there may be such sequences
-  int prompt_groups;         // workgroups for prompts (0: there are none)
+  int prompt_groups;         // workgroups for prompts (0: all rows go the way of few)
   int prompt_rows;
   size_t prompt_ends;        // floats of the prompts' partial sums
   size_t part_bytes, prompt_bytes, unit_bytes;
@@ -1020,11 +1028,12 @@ Plan plan(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
   const uint64_t columns = (uint64_t)a.c.sequences * a.c.kv_heads;  // at most kKv4MaxColumns
   const uint64_t most = (uint64_t)a.max_rows * (uint64_t)a.group;
   uint64_t length = a.max_length;
-  if (most > kFewPairs) {
+  if (a.window) length = std::min<uint64_t>(length, (uint64_t)a.window + a.max_rows + 2 * kKv4Page);
+  const uint64_t small_tiles = ((uint64_t)a.rows * (uint64_t)a.group + kTileRows - 1) / kTileRows;
+  const uint64_t work = small_tiles * (uint64_t)a.c.kv_heads * ((length + kKv4Page - 1) / kKv4Page);
+  if (most > kFewPairs && work > kPromptWork && (bf16 || head_dim != 256)) {
     p.prompt_rows = 32 * (head_dim == 256 || (!bf16 && head_dim == 128) ? 4 : 8);
-    const uint64_t tiles = ((uint64_t)a.rows * (uint64_t)a.group + p.prompt_rows - 1) / p.prompt_rows;
-    const uint64_t units = tiles * (uint64_t)a.c.kv_heads * ((length + kKv4Page - 1) / kKv4Page);
-    p.prompt_groups = (int)std::max<uint64_t>(1, std::min<uint64_t>(256, units / 4));
+    p.prompt_groups = 256;
     p.prompt_ends = 2ull * p.prompt_groups * p.prompt_rows * (size_t)head_dim;
     p.prompt_bytes = (p.prompt_ends + 4ull * p.prompt_groups * p.prompt_rows) * sizeof(float);
     p.unit_bytes = ((size_t)a.c.sequences + 1) * sizeof(uint64_t);
@@ -1034,7 +1043,6 @@ Plan plan(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
   p.few_pairs = p.prompt_groups == 0 ? 0x7fffffff : p.few ? (int)kFewPairs : 0;
   if (!p.few) return p;
   p.tiles = (int)std::min<uint64_t>((std::min<uint64_t>(most, p.few_pairs) + kTileRows - 1) / kTileRows, kKv4MaxColumns / columns);
-  if (a.window) length = std::min<uint64_t>(length, (uint64_t)a.window + 2 * kKv4Page);
   const uint64_t pages = (length + kKv4Page - 1) / kKv4Page, base = columns * (uint64_t)p.tiles;
   p.shift = 2;
   while (p.shift < 5 && base * (pages >> p.shift) > 1024) ++p.shift;
@@ -1048,14 +1056,15 @@ Plan plan(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
 
 template <bool kF32, int D>
 hipError_t launch(const Kv4Kernel& g, const Plan& p, hipStream_t stream) {
-  if (p.prompt_groups > 0) {
-    constexpr int kRows = Prompt<kF32, D>::kRows;
-    hipLaunchKernelGGL(kv4_prompt_units_kernel<kRows>, dim3(1), dim3(256), 0, stream, g);
-    hipLaunchKernelGGL((kv4_prompt_kernel<kF32, D>), dim3((unsigned)p.prompt_groups), dim3((Prompt<kF32, D>::kThreads)), 0,
-                       stream, g);
-    if (p.prompt_groups > 1)
+  if constexpr (!kF32 || D != 256) {
+    if (p.prompt_groups > 0) {
+      constexpr int kRows = Prompt<kF32, D>::kRows;
+      hipLaunchKernelGGL(kv4_prompt_units_kernel<kRows>, dim3(1), dim3(256), 0, stream, g);
+      hipLaunchKernelGGL((kv4_prompt_kernel<kF32, D>), dim3((unsigned)p.prompt_groups),
+                         dim3((Prompt<kF32, D>::kThreads)), 0, stream, g);
       hipLaunchKernelGGL((kv4_prompt_join_kernel<kF32, D>), dim3(kRows / 16, (unsigned)p.prompt_groups), dim3(256), 0,
                          stream, g);
+    }
   }
   if (p.few) {
     const unsigned grid = (unsigned)g.c.sequences * (unsigned)g.c.kv_heads * (unsigned)p.tiles * (unsigned)p.splits;

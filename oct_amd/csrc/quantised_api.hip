@@ -70,7 +70,7 @@ int kv4_rows(void* handle, const PrometheusKv4Cache* cache, const PrometheusKv4R
   if (rt == nullptr) return bad_handle(stage, detail);
   if (!cache_valid(cache) || r == nullptr || r->struct_size < sizeof(*r)) return invalid(stage, detail);
   const bool pointers = write ? r->k != nullptr && r->v != nullptr : r->k != nullptr || r->v != nullptr;
-  if (r->dtype > PROM_DTYPE_BF16 || r->rows == 0u || r->rows > 1u << 24 ||
+  if (r->dtype > PROM_DTYPE_BF16 || r->rows == 0u || r->rows > 1u << 22 ||
       (uint64_t)cache->kv_heads * cache->head_dim > r->row_stride || r->row_stride >= 1u << 24 || !pointers ||
       !aligned(r->k, dtype_size(r->dtype)) || !aligned(r->v, dtype_size(r->dtype)) || r->row_starts == nullptr ||
       !aligned(r->row_starts, 4))
@@ -167,7 +167,7 @@ PROM_REACTOR_API int prometheus_reactor_runtime_attention_kv4_device(void* handl
   const PrometheusKv4AttentionRequest* r = request;
   if (!cache_valid(cache) || r == nullptr || r->struct_size < sizeof(*r)) return invalid(out_stage, out_detail_code);
   const uintptr_t size = dtype_size(r->dtype);
-  if (r->dtype > PROM_DTYPE_BF16 || r->rows == 0u || r->rows > 1u << 24 || r->q_heads == 0u || r->q_heads > 1u << 16 ||
+  if (r->dtype > PROM_DTYPE_BF16 || r->rows == 0u || r->rows > 1u << 22 || r->q_heads == 0u || r->q_heads > 1u << 16 ||
       r->q_heads % cache->kv_heads != 0u || (uint64_t)r->rows * (r->q_heads / cache->kv_heads) >= 1ull << 30 ||
       (uint64_t)r->q_heads * cache->head_dim > r->q_stride ||
       (uint64_t)r->q_heads * cache->head_dim > r->out_stride || r->q_stride >= 1u << 24 || r->out_stride >= 1u << 24 ||

@@ -409,16 +409,27 @@ ATTENTION_CASES = [
     (64, 1, 40, [130], [2], 0),
     (128, 1, 2, [3000], [1], 0),
     (128, 1, 2, [700, 650], [600, 300], 0),
+    (64, 2, 4, [600, 70, 300], [500, 1, 120], 0),  # prompts of several tiles beside a single row
+    (256, 1, 3, [400, 260], [390, 30], 0),
+    (64, 1, 1, [700, 300], [650, 300], 90),
+    (128, 3, 8, [100, 20, 5], [90, 20, 30], 0),  # thirty rows of a sequence of five tokens
 ]
 
 
+# A max_length that is far too large makes the call look like work for the prompts' kernel, which
+# then takes every sequence of more than 64 pairs.
+LOOKS_LONG = 1 << 24
+
+
+@pytest.mark.parametrize("longest", (None, LOOKS_LONG))
 @pytest.mark.parametrize("dtype", (F32, BF16))
 @pytest.mark.parametrize("index", range(len(ATTENTION_CASES)))
-def test_attention_equals_the_definition(gpu_runtime, index, dtype):
+def test_attention_equals_the_definition(gpu_runtime, index, dtype, longest):
     dim, heads, group, lengths, new, window = ATTENTION_CASES[index]
     case = Case(dim, heads, lengths, new, dtype, seed=index, extra_rows=index % 3, empty=index % 2).history(index + 50)
     q = _rounded(oracle.normal(index + 7, (case.rows, heads * group, dim), 0.0, 1.5), dtype)
-    got = _attend(gpu_runtime, case, q, group, dtype, window, pad=index % 4 * 3, lead=(index % 2) * 4)
+    got = _attend(gpu_runtime, case, q, group, dtype, window, pad=index % 4 * 3, lead=(index % 2) * 4,
+                  max_length=longest)
     _check_attention(got, case, q, group, dtype, window)
 
 
@@ -443,24 +454,28 @@ def test_attention_does_not_depend_on_the_launch_hints(gpu_runtime):
     """Too small and too large max_rows and max_length: whole results all the same."""
     case = Case(128, 2, [2000, 90, 700], [50, 1, 3], BF16, seed=8, extra_rows=2).history(12)
     q = _rounded(oracle.normal(5, (case.rows, 8, 128)), BF16)
-    for most, longest in ((50, 2000), (1, 1), (56, 1 << 20), (3, 0xFFFFFFFF), (56, 64)):
+    for most, longest in ((50, 2000), (1, 1), (56, LOOKS_LONG), (3, 0xFFFFFFFF), (56, 64), (17, LOOKS_LONG)):
         got = _attend(gpu_runtime, case, q, 4, BF16, max_rows=most, max_length=longest)
         _check_attention(got, case, q, 4, BF16)
 
 
-def test_attention_ignores_what_is_behind_a_sequence(gpu_runtime):
+@pytest.mark.parametrize("dim", (64, 128, 256))
+@pytest.mark.parametrize("longest", (130, LOOKS_LONG))
+def test_attention_ignores_what_is_behind_a_sequence(gpu_runtime, longest, dim):
     """The pool behind the last token, and of pages that are not its own, may hold anything: bit for bit the same."""
     outs = []
     for seed in (1, 2):
-        case = Case(128, 2, [77, 130], [5, 1], BF16, seed=3)
+        case = Case(dim, 2, [77, 130], [70, 1], BF16, seed=3)
         case.cache.pool[:] = np.random.default_rng(seed).integers(0, 256, case.cache.pool.shape, dtype=np.uint8)
         case.history(30)
-        q = _rounded(oracle.normal(6, (case.rows, 4, 128)), BF16)
-        outs.append(_attend(gpu_runtime, case, q, 2, BF16))
+        q = _rounded(oracle.normal(6, (case.rows, 4, dim)), BF16)
+        outs.append(_attend(gpu_runtime, case, q, 2, BF16, max_length=longest))
     assert np.array_equal(outs[0], outs[1]) and np.isfinite(outs[0]).all()
 
 
-def test_attention_of_bad_pages_and_values(gpu_runtime):
+@pytest.mark.parametrize("longest", (200, LOOKS_LONG))
+@pytest.mark.parametrize("window", (0, 90))
+def test_attention_of_bad_pages_and_values(gpu_runtime, longest, window):
     """A bad page, a place past the table and a NaN key make the rows NaN that see them, and only those."""
     case = Case(64, 1, [200, 70, 66], [140, 70, 2], F32, seed=5).history(31)
     case.table[0, 2] = case.pages
@@ -469,23 +484,30 @@ def test_attention_of_bad_pages_and_values(gpu_runtime):
     case.table = np.ascontiguousarray(case.table[:, :3])
     case.stride = 3  # tokens 192.. of sequence 0 have no place
     q = oracle.normal(8, (case.rows, 2, 64))
-    got = _attend(gpu_runtime, case, q, 2, F32)
+    got = _attend(gpu_runtime, case, q, 2, F32, window, max_length=longest)
     for row, seq, pos in case.places():
-        bad = (seq == 0 and pos >= 128) or (seq == 1 and pos >= 40)
+        first = max(0, pos - window + 1) if window else 0
+        bad = (seq == 0 and pos >= 128) or (seq == 1 and first <= 40 <= pos)
         assert np.isnan(got[row]).all() if bad else np.isfinite(got[row]).all(), (row, seq, pos)
 
 
-def test_attention_to_values_that_are_not_finite(gpu_runtime):
+@pytest.mark.parametrize("longest", (200, LOOKS_LONG))
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("window", (0, 20))
+def test_attention_to_values_that_are_not_finite(gpu_runtime, longest, dtype, window):
     """A NaN or infinite value group reaches its own channels, and only rows that see it."""
-    case = Case(128, 1, [100], [100], F32, seed=6).history(32)
+    case = Case(128, 1, [200], [100], dtype, seed=6).history(32)
     v = np.ones((1, 128), np.float32)
     v[0, 70] = np.inf
-    case.cache.store(case.table[0, 50 // 64], 50, np.ones((1, 128), np.float32), v)
-    q = oracle.normal(9, (case.rows, 1, 128))
-    got = _attend(gpu_runtime, case, q, 1, F32)
+    for at in (20, 150):
+        case.cache.store(case.table[0, at // 64], at % 64, np.ones((1, 128), np.float32), v)
+    q = _rounded(oracle.normal(9, (case.rows, 1, 128)), dtype)
+    got = _attend(gpu_runtime, case, q, 1, dtype, window, max_length=longest)
     for row, seq, pos in case.places():
+        first = max(0, pos - window + 1) if window else 0
         assert np.isfinite(got[row, :, :64]).all()
-        assert np.isnan(got[row, :, 64:]).all() if pos >= 50 else np.isfinite(got[row, :, 64:]).all(), pos
+        spoilt = first <= 20 <= pos or first <= 150 <= pos
+        assert np.isnan(got[row, :, 64:]).all() if spoilt else np.isfinite(got[row, :, 64:]).all(), pos
 
 
 # ------------------------------------------------------------------ a step of the whole path

@@ -151,7 +151,7 @@ def test_cache_rows_refuse(rt, write):
     assert _refused(_cache_rows(rt, write, cache=None)) and _refused(_cache_rows(rt, write, request=None))
     for change in BAD_CACHES:
         assert _refused(_cache_rows(rt, write, cache=dict(CACHE, **change))), change
-    for change in (dict(struct_size=4), dict(dtype=2), dict(rows=0), dict(rows=(1 << 24) + 1), dict(row_stride=255),
+    for change in (dict(struct_size=4), dict(dtype=2), dict(rows=0), dict(rows=(1 << 22) + 1), dict(row_stride=255),
                    dict(row_stride=1 << 24), dict(k=OK + 2), dict(v=OK + 1), dict(k=0, v=0), dict(row_starts=0),
                    dict(row_starts=OK + 2)):
         assert _refused(_cache_rows(rt, write, request=dict(CACHE_ROWS, **change))), change
@@ -175,7 +175,7 @@ def test_attention_refuses(rt):
     assert _refused(_attention(rt, cache=None)) and _refused(_attention(rt, request=None))
     for change in BAD_CACHES:
         assert _refused(_attention(rt, cache=dict(CACHE, **change))), change
-    for change in (dict(struct_size=4), dict(dtype=2), dict(rows=0), dict(rows=(1 << 24) + 1), dict(q_heads=0),
+    for change in (dict(struct_size=4), dict(dtype=2), dict(rows=0), dict(rows=(1 << 22) + 1), dict(q_heads=0),
                    dict(q_heads=7), dict(q_heads=(1 << 16) + 2), dict(rows=1 << 17, q_heads=1 << 15, q_stride=1 << 22, out_stride=1 << 22),
                    dict(q_stride=1023), dict(q_stride=1 << 24),
                    dict(out_stride=1023), dict(out_stride=1 << 24), dict(max_rows=0), dict(max_rows=7),
