@@ -11,10 +11,8 @@
 // are not whole 16-byte chunks are copied to padded ones first.  Where tiles are few,
 // K is cut into slices whose int32 sums a second kernel adds (exact in any order).
 //
-// Few rows (a decode step, a short prompt): every weight is read once, so w goes
-// from memory straight into the operand registers of v_mfma_i32_16x16x64_i8 (16
-// rows of w, 64 bytes of k), K dealt to the waves of a workgroup, which add their
-// sums through LDS.  Bound by reading w.
+// Few rows (a decode step, a short prompt): every weight is read once and K is dealt
+// to the waves of a workgroup, which add their sums through LDS.  Bound by reading w.
 #include <algorithm>
 #include <type_traits>
 
@@ -25,6 +23,7 @@ namespace {
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kGroupM = 8;
 constexpr uint32_t kOutOfRange = 0x80000000u;  // past every descriptor range
@@ -238,6 +237,15 @@ __global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_int8_tile_kernel(const
 #pragma unroll
     for (int j = 0; j < C::kNI; ++j) acc[i][j] = intx16{};
 
+  // The scales are fetched ahead of the sums: a thread a row's, a lane its columns'.
+  float row_scale = 0.0f, ws[C::kNI];
+  if (g.slabs == nullptr) {
+    static_assert(C::kBM <= 64 * C::kWaves, "a thread a row");
+    row_scale = g.a_scale[min(row0 + tid, g.m - 1)];
+#pragma unroll
+    for (int ni = 0; ni < C::kNI; ++ni) ws[ni] = g.w_scale[min(col0 + (wn * C::kNI + ni) * 32 + lrow, g.n - 1)];
+  }
+
   // Tiles of this slice whose chunks of a all lie below k: all, or all but the last.
   const int whole = kn - ((kt0 + kn) * kBK > g.k ? 1 : 0);
 #pragma unroll
@@ -297,31 +305,34 @@ __global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_int8_tile_kernel(const
   // stores 16 bytes of a row and neighbouring lanes neighbouring ones (stored from the accumulators,
   // two bytes a lane, 4224x20480 bf16 took 120 us longer).
   constexpr int kCols = 32 * C::kNI, kPitch = kCols + 4;
-  static_assert(C::kWaves * 32 * kPitch * 4 <= C::kSt * C::kStage, "the wave's part of LDS");
+  static_assert((C::kWaves * 32 * kPitch + C::kBM) * 4 <= C::kSt * C::kStage, "the waves' parts and the scales");
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();  // the last tiles have been read
   asm volatile("" ::: "memory");
   int32_t* mine = reinterpret_cast<int32_t*>(lds) + wave * 32 * kPitch;
+  float* scales = reinterpret_cast<float*>(lds) + C::kWaves * 32 * kPitch;
+  if (g.slabs == nullptr) {
+    if (tid < C::kBM) scales[tid] = row_scale;
+    __syncthreads();
+  }
   const int wave_col = col0 + wn * kCols;
-  float ws[C::kNI];
-#pragma unroll
-  for (int ni = 0; ni < C::kNI; ++ni)
-    ws[ni] = g.slabs == nullptr ? g.w_scale[min(wave_col + 32 * ni + lrow, g.n - 1)] : 0.0f;
 #pragma unroll
   for (int mi = 0; mi < C::kMI; ++mi) {
     const int r0 = row0 + (wm * C::kMI + mi) * 32;
     if (r0 >= g.m) break;
     // Accumulator layout: lane l, register r holds row 8 (r/4) + 4 (l/32) + r%4, column l%32.
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int dr = 8 * (r >> 2) + 4 * hk + (r & 3);
-      const float as = g.slabs == nullptr ? g.a_scale[min(r0 + dr, g.m - 1)] : 0.0f;
+    for (int q = 0; q < 4; ++q) {
+      const int dr = 8 * q + 4 * hk;
+      const floatx4 as = *reinterpret_cast<const floatx4*>(scales + (wm * C::kMI + mi) * 32 + dr);
 #pragma unroll
-      for (int ni = 0; ni < C::kNI; ++ni) {
-        const int sum = acc[mi][ni][r];
-        mine[dr * kPitch + 32 * ni + lrow] =
-            g.slabs == nullptr ? __float_as_int((float)sum * as * ws[ni]) : sum;
-      }
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int ni = 0; ni < C::kNI; ++ni) {
+          const int sum = acc[mi][ni][4 * q + r];
+          mine[(dr + r) * kPitch + 32 * ni + lrow] =
+              g.slabs == nullptr ? __float_as_int((float)sum * as[r] * ws[ni]) : sum;
+        }
     }
     asm volatile("" ::: "memory");  // a wave's own part: its LDS operations stay in order
     if (g.slabs != nullptr)
@@ -350,31 +361,19 @@ __global__ __launch_bounds__(256) void int8_slices_kernel(const int32_t* __restr
   }
 }
 
-// dst [rows][ld] = src [rows][cols], zero from column cols on (ld a multiple of 16):
-// sixteen bytes a thread, read at any alignment.
-__global__ __launch_bounds__(256) void pad_rows8_kernel(const int8_t* __restrict__ src, int8_t* __restrict__ dst,
-                                                        int rows, int cols, int ld) {
-  const int c = (int)(blockIdx.x * 64 + (threadIdx.x & 63)) * 16;
-  if (c >= ld) return;
-  for (int r = (int)(blockIdx.y * 4 + (threadIdx.x >> 6)); r < rows; r += (int)gridDim.y * 4) {
-    const int8_t* p = src + (size_t)r * cols + c;
-    int8_t v[16];
-    if (c + 16 <= cols) {
-      __builtin_memcpy(v, p, 16);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = c + j < cols ? p[j] : (int8_t)0;
-    }
-    __builtin_memcpy(__builtin_assume_aligned(dst + (size_t)r * ld + c, 16), v, 16);
-  }
-}
-
-// Sixteen bytes from column k of a row, zeros from column `cols` on.
+// Sixteen bytes from column k of a row at any alignment, zeros from column `cols` on: the row's last
+// sixteen, shifted, where it ends within them.
 __device__ __forceinline__ intx4 load16(const int8_t* row, int k, int cols) {
   intx4 v = {0, 0, 0, 0};
-  if (k + 16 <= cols) {
+  const int past = k + 16 - cols;
+  if (past <= 0) {
     __builtin_memcpy(&v, row + k, 16);
-  } else if (k < cols) {
+  } else if (past < 16 && cols >= 16) {
+    unsigned __int128 b;
+    __builtin_memcpy(&b, row + cols - 16, 16);
+    b >>= 8 * past;
+    __builtin_memcpy(&v, &b, 16);
+  } else if (past < 16) {
     int8_t b[16] = {};
 #pragma unroll
     for (int j = 0; j < 16; ++j)
@@ -384,89 +383,151 @@ __device__ __forceinline__ intx4 load16(const int8_t* row, int k, int cols) {
   return v;
 }
 
-// Few rows: a workgroup computes 16 kNT columns of c for 16 kMT rows; its waves take K in
-// turn, kUnroll steps of 64 at a time.
-template <int kMT, int kNT, int kWaves, typename TOut>
-__global__ __launch_bounds__(64 * kWaves) void gemm_int8_rows_kernel(const Int8Args g) {
-  constexpr int kUnroll = kNT * kMT >= 4 ? 2 : 4;
-  __shared__ intx4 part[kWaves > 1 ? kWaves - 1 : 1][kMT * kNT][64];
-  const int lane = (int)threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int r16 = lane & 15, h = lane >> 4;
-  const int n0 = (int)blockIdx.x * 16 * kNT, m0 = (int)blockIdx.y * 16 * kMT;
-  const int8_t* wp[kNT];
-  const int8_t* ap[kMT];
-#pragma unroll
-  for (int i = 0; i < kNT; ++i) wp[i] = g.w + (size_t)min(n0 + 16 * i + r16, g.n - 1) * g.k;
-#pragma unroll
-  for (int i = 0; i < kMT; ++i) ap[i] = g.a + (size_t)min(m0 + 16 * i + r16, g.m - 1) * g.k;
-  intx4 acc[kNT][kMT] = {};
-  constexpr int kStep = 64 * kUnroll;
-  const int whole = g.k / kStep;  // steps without a tail
-  for (int t = wave; t < whole; t += kWaves) {
-    const int k = t * kStep + 16 * h;
-    intx4 w[kUnroll][kNT], a[kUnroll][kMT];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-#pragma unroll
-      for (int i = 0; i < kNT; ++i) __builtin_memcpy(&w[u][i], wp[i] + k + 64 * u, 16);
-#pragma unroll
-      for (int i = 0; i < kMT; ++i) __builtin_memcpy(&a[u][i], ap[i] + k + 64 * u, 16);
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-      for (int i = 0; i < kNT; ++i)
-#pragma unroll
-        for (int j = 0; j < kMT; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][i], a[u][j], acc[i][j], 0, 0, 0);
-  }
-  if (whole % kWaves == wave)
-    for (int k = whole * kStep + 16 * h; k - 16 * h < g.k; k += 64) {
-#pragma unroll
-      for (int i = 0; i < kNT; ++i) {
-        const intx4 w = load16(wp[i], k, g.k);
-#pragma unroll
-        for (int j = 0; j < kMT; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, load16(ap[j], k, g.k), acc[i][j], 0, 0, 0);
-      }
-    }
-  if constexpr (kWaves > 1) {
-    if (wave > 0) {
-#pragma unroll
-      for (int i = 0; i < kNT; ++i)
-#pragma unroll
-        for (int j = 0; j < kMT; ++j) part[wave - 1][i * kMT + j][lane] = acc[i][j];
-    }
-    __syncthreads();
-    if (wave > 0) return;
-    for (int s = 0; s < kWaves - 1; ++s)
-#pragma unroll
-      for (int i = 0; i < kNT; ++i)
-#pragma unroll
-        for (int j = 0; j < kMT; ++j) acc[i][j] += part[s][i * kMT + j][lane];
-  }
-  // Lane l, register r: column (of w) 4 (l/16) + r, row (of a) l%16.
-#pragma unroll
-  for (int j = 0; j < kMT; ++j) {
-    const int row = m0 + 16 * j + r16;
-    if (row >= g.m) continue;
-    const float as = g.a_scale[row];
-#pragma unroll
-    for (int i = 0; i < kNT; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int col = n0 + 16 * i + 4 * h + r;
-        if (col < g.n) store_scaled(static_cast<TOut*>(g.c) + (size_t)row * g.n + col, acc[i][j][r], as, g.w_scale[col]);
-      }
+// Both operands' rows, cols bytes each, to rows of ld (a multiple of 16), zero from column cols on:
+// sixteen bytes a thread, read at any alignment.
+__global__ __launch_bounds__(256) void pad_rows8_kernel(const int8_t* __restrict__ a, int8_t* __restrict__ to_a, int m,
+                                                        const int8_t* __restrict__ w, int8_t* __restrict__ to_w, int n,
+                                                        int cols, int ld) {
+  const int chunks = ld / 16;
+  const long long total = (long long)(m + n) * chunks;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const int row = (int)(i / chunks), c = (int)(i - (long long)row * chunks) * 16;
+    const bool first = row < m;
+    const size_t r = (size_t)(first ? row : row - m);
+    const intx4 v = load16((first ? a : w) + r * cols, c, cols);
+    *reinterpret_cast<intx4*>((first ? to_a : to_w) + r * ld + c) = v;
   }
 }
 
-#define INT8_TILES(X)            \
+// Few rows: a workgroup computes 16 columns of c for 16 kMT rows; its waves take K in turn, 256 bytes
+// of every row at a time, the next step's loads out while one is multiplied.  The matrix instruction
+// wants another row in each of 16 neighbouring lanes, a load neighbouring bytes there (loaded as they
+// are multiplied, a load keeps the cache four times as long: 15x2048x16384 16.4 us, now 8.6).  So a
+// load takes 256 bytes of four rows, and the wave's own part of LDS turns them, 16-byte chunks XORed
+// by row against bank conflicts.
+template <int kMT, int kWaves, typename TOut>
+__global__ __launch_bounds__(64 * kWaves) void gemm_int8_rows_kernel(const Int8Args g) {
+  constexpr int kSeg = 256, kWLoads = 4, kALoads = 4 * kMT, kBytes = 1024 * (kWLoads + kALoads);
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * kBytes];
+  const int lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int r16 = lane & 15, h = lane >> 4;
+  const int n0 = (int)blockIdx.x * 16, m0 = (int)blockIdx.y * 16 * kMT;
+  char* lw = lds + wave * kBytes;
+  char* la = lw + 1024 * kWLoads;
+  struct Step {
+    intx4 w[kWLoads], a[kALoads];
+  };
+  auto load = [&](Step& s, int t, auto tail_c) __attribute__((always_inline)) {
+    constexpr bool kTail = decltype(tail_c)::value;
+    const int k = t * kSeg + 16 * r16;
+#pragma unroll
+    for (int i = 0; i < kWLoads; ++i) {
+      const int8_t* p = g.w + (size_t)min(n0 + 4 * i + h, g.n - 1) * g.k;
+      if constexpr (kTail)
+        s.w[i] = load16(p, k, g.k);
+      else
+        __builtin_memcpy(&s.w[i], p + k, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < kALoads; ++i) {
+      const int row = m0 + 4 * i + h;
+      s.a[i] = intx4{0, 0, 0, 0};
+      if (row >= g.m) continue;
+      const int8_t* p = g.a + (size_t)row * g.k;
+      if constexpr (kTail)
+        s.a[i] = load16(p, k, g.k);
+      else
+        __builtin_memcpy(&s.a[i], p + k, 16);
+    }
+  };
+  auto put = [&](const Step& s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kWLoads; ++i) {
+      const int r = 4 * i + h;
+      *reinterpret_cast<intx4*>(lw + r * kSeg + ((r16 ^ (r & 15)) << 4)) = s.w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kALoads; ++i) {
+      const int r = 4 * i + h;
+      *reinterpret_cast<intx4*>(la + r * kSeg + ((r16 ^ (r & 15)) << 4)) = s.a[i];
+    }
+  };
+  intx4 acc[kMT] = {};
+  auto multiply = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int at = r16 * kSeg + (((4 * u + h) ^ r16) << 4);
+      const intx4 w = *reinterpret_cast<const intx4*>(lw + at);
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+        acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, *reinterpret_cast<const intx4*>(la + 16 * i * kSeg + at),
+                                                       acc[i], 0, 0, 0);
+    }
+  };
+  // The wave's own part: its LDS operations stay in order.
+  auto fence = [] {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+  };
+  const std::integral_constant<bool, true> yes{};
+  const std::integral_constant<bool, false> no{};
+  const int whole = g.k / kSeg;  // steps without a tail
+  int t = wave;
+  if (t < whole) {
+    Step s;
+    load(s, t, no);
+    for (; t + kWaves < whole; t += kWaves) {
+      put(s);
+      load(s, t + kWaves, no);
+      fence();
+      multiply();
+      fence();
+    }
+    put(s);
+    fence();
+    multiply();
+    fence();
+  }
+  if (whole * kSeg < g.k && whole % kWaves == wave) {
+    Step s;
+    load(s, whole, yes);
+    put(s);
+    fence();
+    multiply();
+  }
+  __syncthreads();  // the operands have been read
+  intx4* part = reinterpret_cast<intx4*>(lds) + lane;  // [wave - 1][kMT][64]
+  if (wave > 0) {
+#pragma unroll
+    for (int i = 0; i < kMT; ++i) part[((wave - 1) * kMT + i) * 64] = acc[i];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int s = 0; s < kWaves - 1; ++s)
+#pragma unroll
+    for (int i = 0; i < kMT; ++i) acc[i] += part[(s * kMT + i) * 64];
+  // Lane l, register r: column (of w) 4 (l/16) + r, row (of a) l%16.
+#pragma unroll
+  for (int i = 0; i < kMT; ++i) {
+    const int row = m0 + 16 * i + r16;
+    if (row >= g.m) continue;
+    const float as = g.a_scale[row];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int col = n0 + 4 * h + r;
+      if (col < g.n) store_scaled(static_cast<TOut*>(g.c) + (size_t)row * g.n + col, acc[i][r], as, g.w_scale[col]);
+    }
+  }
+}
+
+#define INT8_TILES(X)               \
   X(0, 1, 1, 2, 2, 4) /* 64x64 */   \
   X(1, 1, 2, 4, 2, 4) /* 128x128 */ \
-  X(2, 2, 2, 2, 4, 3) /* 128x256 */ \
-  X(3, 4, 2, 2, 4, 2) /* 256x256 */
+  X(2, 2, 2, 2, 2, 2) /* 128x128, two workgroups a CU */ \
+  X(3, 3, 2, 2, 4, 2) /* 192x256 */ \
+  X(4, 4, 2, 2, 4, 2) /* 256x256 */
 
 struct TileInfo {
   int bm, bn, threads;
@@ -491,16 +552,19 @@ hipError_t launch_tile(int tile, int slices, const Int8Args& g, hipStream_t stre
   return hipGetLastError();
 }
 
-// Estimated microseconds as in gemm_bf16_tiles.hip: rounds of 256 * occ workgroups.
+// Estimated microseconds of a tile's workgroup: `fill` plus step[w - 1] for each 128 of k where w of
+// them share a CU; on an otherwise idle chip a step takes `idle` of that.  From 16 x 16 tiles of
+// each with k 512, 2048 and 8192, and a single tile.
 struct TileCost {
   int occ;
   double step[2], fill, idle;
 };
 constexpr TileCost kCost[kNumTiles] = {
-    {2, {0.190, 0.375}, 2.49, 0.77},  // 64x64
-    {1, {0.585, 0.585}, 3.49, 0.46},  // 128x128
-    {1, {0.945, 0.945}, 5.67, 0.42},  // 128x256
-    {1, {1.852, 1.852}, 8.60, 0.46},  // 256x256
+    {2, {0.24, 0.46}, 2.6, 0.95},  // 64x64
+    {1, {0.615, 0.0}, 5.2, 0.70},  // 128x128
+    {2, {0.73, 1.19}, 4.5, 0.65},  // 128x128, two a CU
+    {1, {1.49, 0.0}, 11.5, 0.50},  // 192x256
+    {1, {1.85, 0.0}, 16.0, 0.52},  // 256x256
 };
 
 struct Plan {
@@ -535,20 +599,20 @@ Plan plan_tiles(uint32_t m, uint32_t n, uint32_t k) {
 
 template <typename TOut>
 hipError_t launch_rows(const Int8Args& g, hipStream_t stream) {
-  const int tiles_n = (g.n + 15) / 16;
-#define ROWS(MT, NT, W)                                                                                          \
-  hipLaunchKernelGGL((gemm_int8_rows_kernel<MT, NT, W, TOut>), dim3((unsigned)((tiles_n + NT - 1) / NT),         \
+#define ROWS(MT, W)                                                                          \
+  hipLaunchKernelGGL((gemm_int8_rows_kernel<MT, W, TOut>), dim3((unsigned)((g.n + 15) / 16), \
                      (unsigned)((g.m + 16 * MT - 1) / (16 * MT))), dim3(64 * W), 0, stream, g)
+  const bool many = g.n >= 16 * 1024;
   if (g.m <= 16) {
-    if (tiles_n >= 1024)
-      ROWS(1, 1, 4);
+    if (many)
+      ROWS(1, 4);
     else
-      ROWS(1, 1, 16);
+      ROWS(1, 8);
   } else {
-    if (tiles_n >= 1024)
-      ROWS(2, 1, 4);
+    if (many)
+      ROWS(2, 4);
     else
-      ROWS(2, 1, 16);
+      ROWS(2, 8);
   }
 #undef ROWS
   return hipGetLastError();
@@ -567,10 +631,9 @@ hipError_t launch(Int8Args g, hipStream_t stream) {
     int8_t* pa = static_cast<int8_t*>(staging(8, (size_t)m * ld));
     int8_t* pw = static_cast<int8_t*>(staging(9, (size_t)n * ld));
     if (pa == nullptr || pw == nullptr) return hipErrorOutOfMemory;
-    const unsigned bx = (unsigned)((ld / 16 + 63) / 64);
-    auto rows = [&](uint32_t r) { return std::min<unsigned>((r + 3) / 4, std::max(1u, 8192u / bx)); };
-    hipLaunchKernelGGL(pad_rows8_kernel, dim3(bx, rows(m)), dim3(256), 0, stream, g.a, pa, g.m, g.k, ld);
-    hipLaunchKernelGGL(pad_rows8_kernel, dim3(bx, rows(n)), dim3(256), 0, stream, g.w, pw, g.n, g.k, ld);
+    const unsigned long long chunks = (unsigned long long)(m + n) * (unsigned)(ld / 16);
+    hipLaunchKernelGGL(pad_rows8_kernel, dim3((unsigned)std::min<unsigned long long>((chunks + 255) / 256, 1u << 16)),
+                       dim3(256), 0, stream, g.a, pa, g.m, g.w, pw, g.n, g.k, ld);
     g.a = pa;
     g.w = pw;
     g.lda = g.ldw = ld;
