@@ -47,10 +47,15 @@ __device__ __forceinline__ uint32_t max_bits(const float (&v)[8], uint32_t m) {
   return m;
 }
 
-__device__ __forceinline__ void store8(int8_t* p, long long left, const float (&v)[8], float s) {
+__device__ __forceinline__ void store8(int8_t* p, long long left, const float (&v)[8], const Divisor& s) {
   int q[8];
+  if (s.usable()) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = s > 0.0f ? (int)__builtin_rintf(v[j] / s) : 0;
+    for (int j = 0; j < 8; ++j) q[j] = (int)__builtin_rintf(s(v[j]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = s.s > 0.0f ? (int)__builtin_rintf(v[j] / s.s) : 0;
+  }
   if (left >= 8) {
     u32x2 w;
 #pragma unroll
@@ -106,16 +111,17 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void quantize_rows
     // A row with an infinity or a NaN: scale NaN, and zeros (s > 0 fails).
     const float s = m >= kInfBits ? __uint_as_float(0x7FC00000u) : __uint_as_float(m) / 127.0f;
     if (lane == 0) scales[row] = s;
+    const Divisor d(s);
     if constexpr (kChunks > 0) {
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const long long at = 8ll * (lane + kLanes * i);
-        if (at < width) store8(dst + at, (long long)width - at, v[i], s);
+        if (at < width) store8(dst + at, (long long)width - at, v[i], d);
       }
     } else {
       for (long long at = 8ll * lane; at < width; at += 8ll * kLanes) {
         load8(src + at, (long long)width - at, v[0]);
-        store8(dst + at, (long long)width - at, v[0], s);
+        store8(dst + at, (long long)width - at, v[0], d);
       }
     }
   }

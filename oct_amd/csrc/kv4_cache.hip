@@ -65,8 +65,14 @@ __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], uint32_t* par
   const bool some = finite && s > 0.0f;
   uint32_t codes = 0;
   float y[8];
+  const Divisor by(some ? s : 1.0f);
+  if (__all(by.usable())) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = some ? v[j] / s : 0.0f;
+    for (int j = 0; j < 8; ++j) y[j] = some ? __builtin_copysignf(by(v[j]), v[j]) : 0.0f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = some ? v[j] / s : 0.0f;
+  }
   codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[0], y[1], 1.0f, 0);
   codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[2], y[3], 1.0f, 1);
   codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[4], y[5], 1.0f, 2);
