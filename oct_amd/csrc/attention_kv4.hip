@@ -256,31 +256,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
     const int pos = mine ? sq.length - sq.n + row : tl.pos1;  // its position
     const int page0 = tl.page0, last = tl.last;
 
-    // Q^T operand: lane (h, row), step s: channels 32 s + 8 h .. + 7.
-    bf16x8 q[kSteps][kQT];
+    // Q^T operand: lane (h, row), step s: channels 32 s + 8 h .. + 7.  Loaded here, used when the first
+    // page is on its way.
+    u32x4 q_raw[kSteps][kF32 ? 2 : 1];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const size_t at = (size_t)(sq.first + row) * g.q_stride + (size_t)q_head * D + 32 * s + 8 * h;
-      if constexpr (kF32) {
-        float v[8];
-        __builtin_memcpy(v, static_cast<const float*>(g.q) + at, 32);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          __bf16 t[kQT];
-          terms(mine ? v[j] : 0.0f, t);
-#pragma unroll
-          for (int i = 0; i < kQT; ++i) q[s][i][j] = t[i];
-        }
-      } else {
-        u32x4 v;
-        __builtin_memcpy(&v, static_cast<const uint16_t*>(g.q) + at, 16);
-        if (!mine) v = u32x4{0u, 0u, 0u, 0u};
-        q[s][0] = __builtin_bit_cast(bf16x8, v);
-      }
+      if constexpr (kF32)
+        __builtin_memcpy(q_raw[s], static_cast<const float*>(g.q) + at, 32);
+      else
+        __builtin_memcpy(q_raw[s], static_cast<const uint16_t*>(g.q) + at, 16);
     }
-
-    floatx4 o[kB] = {};
-    float m_run = -INFINITY, m_log2 = 0.0f, l_run = 0.0f;
+    __builtin_amdgcn_sched_barrier(0);
 
     const int stride = tl.splits * kWaves;
     int pg = page0 + split * kWaves + wave;
@@ -296,6 +283,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
     uint32_t number = page_number(pg), next_number = page_number(pg + stride);
     int now = 0;
     if (pg < last) St::fill(page_block(number), lds0, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    bf16x8 q[kSteps][kQT];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      if constexpr (kF32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          __bf16 t[kQT];
+          terms(mine ? __uint_as_float(q_raw[s][j / 4][j % 4]) : 0.0f, t);
+#pragma unroll
+          for (int i = 0; i < kQT; ++i) q[s][i][j] = t[i];
+        }
+      } else {
+        q[s][0] = __builtin_bit_cast(bf16x8, mine ? q_raw[s][0] : u32x4{0u, 0u, 0u, 0u});
+      }
+    }
+    floatx4 o[kB] = {};
+    float m_run = -INFINITY, m_log2 = 0.0f, l_run = 0.0f;
     for (; pg < last; pg += stride) {
       // The other stage's reads have returned before it is filled again.
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -441,34 +446,44 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
       sums[r16 * (D + 4) + D + 1] = l_run;
     }
     __syncthreads();
-    for (int e = (int)threadIdx.x; e < kTileRows * D; e += 64 * kWaves) {
-      const int tr = e / D, d = e % D;
+    // Four channels of a row a thread.
+    static_assert(64 * kWaves * kG * 4 == kTileRows * D, "the tile's sums");
+#pragma unroll
+    for (int i = 0; i < kG; ++i) {
+      const int e = (int)threadIdx.x + 64 * kWaves * i, tr = e / (D / 4), d = e % (D / 4) * 4;
       const int xe = x0 + tr;
-      if (xe >= pairs) break;
       const float* all = reinterpret_cast<const float*>(lds) + tr * (D + 4);
       float top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) top = fmaxf(top, all[w * kTileRows * (D + 4) + D]);
-      float sum = 0.0f, weight = 0.0f;
+      floatx4 sum = {};
+      float weight = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const float* a = all + w * kTileRows * (D + 4);
         const float f = a[D] == top ? 1.0f : __builtin_amdgcn_exp2f((a[D] - top) * g.scale_log2);
-        sum = __builtin_fmaf(a[d], f, sum);
+        const floatx4 v = *reinterpret_cast<const floatx4*>(a + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(v[j], f, sum[j]);
         weight = __builtin_fmaf(a[D + 1], f, weight);
       }
+      if (xe >= pairs) continue;
       const int in_seq = g.over_group(xe), er = sq.first + in_seq, eh = head * g.group + xe - in_seq * g.group;
       if (tl.splits > 1) {
         const size_t at = ((size_t)split * g.rows + er) * g.q_heads + eh;
-        g.part[at * D + d] = sum;
+        *reinterpret_cast<floatx4*>(g.part + at * D + d) = sum;
         if (d == 0) reinterpret_cast<float2*>(ends(g))[at] = make_float2(top, weight);
       } else {
-        const float v = weight == 0.0f ? 0.0f : sum / weight;
         const size_t at = (size_t)er * g.out_stride + (size_t)eh * D + d;
-        if constexpr (kF32)
-          static_cast<float*>(g.out)[at] = v;
-        else
-          static_cast<__bf16*>(g.out)[at] = (__bf16)v;
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = weight == 0.0f ? 0.0f : sum[j] / weight;
+        if constexpr (kF32) {
+          __builtin_memcpy(static_cast<float*>(g.out) + at, v, 16);
+        } else {
+          const __bf16 b[4] = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+          __builtin_memcpy(static_cast<__bf16*>(g.out) + at, b, 8);
+        }
       }
     }
     __syncthreads();
