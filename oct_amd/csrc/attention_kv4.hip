@@ -959,11 +959,15 @@ __global__ __launch_bounds__(256) void kv4_prompt_join_kernel(const Kv4Kernel g)
 }
 
 // Joins the splits' sums: a workgroup a row, for every gridDim.y-th query head.  Its threads are D / 4 columns of
-// four channels times kParts: part i adds splits i, i + kParts, ..., the parts are added in
-// order.  Bound by latency: maxima and weights come in one load a lane, sums four at a time.
-template <bool kF32, int D>
+// four channels times kJoinParts: part i adds splits i, i + kJoinParts, ..., the parts are added in order.  Bound
+// by latency: maxima and weights come in one load a lane, all sums at once beside them.  With no more splits than
+// parts, a kernel of one sum a thread keeps twice the waves on a CU (64 rows of 32 heads of 128 in 4 splits 6.0 us,
+// 8.2 with registers for 64; one row in 64 splits 4.9).
+template <int D>
+constexpr int kJoinParts = 256 / (D / 4);
+template <bool kF32, int D, int kEach>
 __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
-  constexpr int kColumns = D / 4, kParts = 256 / kColumns;
+  constexpr int kColumns = D / 4, kParts = kJoinParts<D>;
   __shared__ floatx4 parts[kParts][kColumns];
   __shared__ float factors[kMaxSplits];
   const int tid = (int)threadIdx.x, lane = tid & 63;
@@ -986,6 +990,13 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
     // Splits that this row's tile does not have hold anything; they are left out.
     const int splits = Tile(g, sq, ((row - sq.first) * g.group + q_head % g.group) / kTileRows).splits;
     if (splits == 1) continue;
+    // The sums, while the factors are worked out.
+    floatx4 v[kEach];
+    const floatx4* at = reinterpret_cast<const floatx4*>(g.part + (size_t)x * D) + column;
+    const size_t slab = pairs * kColumns;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (part + kParts * i < splits) v[i] = at[(part + kParts * i) * slab];
     float top = lane < splits ? e.x : -INFINITY, weight = e.y;
     const float mine = top;
 #pragma unroll
@@ -997,15 +1008,13 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
     if (tid < splits) factors[tid] = f;
     __syncthreads();
     floatx4 sum = {};
-    const floatx4* at = reinterpret_cast<const floatx4*>(g.part + (size_t)x * D) + column;
-    const size_t slab = pairs * kColumns;
-#pragma unroll 4
-    for (int s = part; s < splits; s += kParts) {
-      const floatx4 v = at[s * slab];
-      const float fs = factors[s];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(v[i], fs, sum[i]);
-    }
+    for (int i = 0; i < kEach; ++i)
+      if (part + kParts * i < splits) {
+        const float fs = factors[part + kParts * i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(v[i][j], fs, sum[j]);
+      }
     parts[part][column] = sum;
     __syncthreads();
     if (part == 0) {
@@ -1086,7 +1095,11 @@ hipError_t launch(const Kv4Kernel& g, const Plan& p, hipStream_t stream) {
     hipLaunchKernelGGL((kv4_attention_kernel<kF32, D>), dim3(grid), dim3(64 * kWaves), 0, stream, g);
     if (p.splits > 1) {
       const unsigned heads = std::min<unsigned>((unsigned)g.q_heads, std::max(1u, 4096u / (unsigned)g.rows));
-      hipLaunchKernelGGL((kv4_join_kernel<kF32, D>), dim3((unsigned)g.rows, heads), dim3(256), 0, stream, g);
+      const dim3 join((unsigned)g.rows, heads);
+      if (p.splits <= kJoinParts<D>)
+        hipLaunchKernelGGL((kv4_join_kernel<kF32, D, 1>), join, dim3(256), 0, stream, g);
+      else
+        hipLaunchKernelGGL((kv4_join_kernel<kF32, D, kMaxSplits / kJoinParts<D>>), join, dim3(256), 0, stream, g);
     }
   }
   return hipGetLastError();
