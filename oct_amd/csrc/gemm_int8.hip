@@ -158,24 +158,27 @@ __global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_int8_tile_kernel(const
     b_off[i] = (uint32_t)(r * g.ldw + 16 * ((lane & 7) ^ swz(r)));
   }
   const int k16 = (g.k + 15) & ~15;
-  const char* a_ptr = (const char*)(g.a + (size_t)row0 * g.lda + (size_t)kt0 * kBK);
-  long long a_left = (long long)(g.m - 1 - row0) * g.lda + k16 - (long long)kt0 * kBK;
-  const char* b_ptr = (const char*)(g.w + (size_t)col0 * g.ldw + (size_t)kt0 * kBK);
-  long long b_left = (long long)(g.n - 1 - col0) * g.ldw + k16 - (long long)kt0 * kBK;
   int issued = 0;
-  auto desc = [](const char* p, long long left) {
+  // What is left of the tile's rows of each operand from the next k on (at most 256 rows of 2^17 bytes).
+  const char* a_ptr = (const char*)(g.a + (size_t)row0 * g.lda + (size_t)kt0 * kBK);
+  const char* b_ptr = (const char*)(g.w + (size_t)col0 * g.ldw + (size_t)kt0 * kBK);
+  int a_left = (min(C::kBM, g.m - row0) - 1) * g.lda + k16 - kt0 * kBK;
+  int b_left = (min(C::kBN, g.n - col0) - 1) * g.ldw + k16 - kt0 * kBK;
+  auto desc = [](const char* p, int left) {
     const unsigned long long a = (unsigned long long)p;
-    const unsigned range = left < 0 ? 0u : (left > 0x7fffffffll ? 0x7fffffffu : (unsigned)left);
     intx4 d;
     d.x = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffu));
     d.y = __builtin_amdgcn_readfirstlane((int)(a >> 32));
-    d.z = __builtin_amdgcn_readfirstlane((int)range);
+    d.z = __builtin_amdgcn_readfirstlane(left);
     d.w = 0x00020000;
     return d;
   };
   const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds;
   intx4 da = desc(a_ptr, a_left), db = desc(b_ptr, b_left);
-  uint32_t fill = lds0;  // LDS address of the stage the next tile goes to
+  // LDS addresses of this wave's parts of the stage that the next tile goes to, and the stage's.
+  uint32_t fill_a = __builtin_amdgcn_readfirstlane(lds0 + wave * C::kAX * 1024);
+  uint32_t fill_b = __builtin_amdgcn_readfirstlane(lds0 + C::kABytes + wave * C::kBX * 1024);
+  uint32_t fill_stage = 0;
   // Transfer j (0 .. kX-1) of the tile being issued; tail: a's last chunks lie past k.
   auto issue_one = [&](int j, bool tail) __attribute__((always_inline)) {
     if (j < C::kAX) {
@@ -184,12 +187,11 @@ __global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_int8_tile_kernel(const
         const int r = 8 * (wave * C::kAX + j) + tr;
         if ((kt0 + issued) * kBK + 16 * ((lane & 7) ^ swz(r)) >= g.k) off = kOutOfRange;
       }
-      const uint32_t to = __builtin_amdgcn_readfirstlane(fill + (wave * C::kAX + j) * 1024);
+      const uint32_t to = __builtin_amdgcn_readfirstlane(fill_a + j * 1024);
       asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(da)
                    : "memory", "m0");
     } else {
-      const uint32_t to =
-          __builtin_amdgcn_readfirstlane(fill + C::kABytes + (wave * C::kBX + (j - C::kAX)) * 1024);
+      const uint32_t to = __builtin_amdgcn_readfirstlane(fill_b + (j - C::kAX) * 1024);
       asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(b_off[j - C::kAX]),
                    "s"(db)
                    : "memory", "m0");
@@ -202,7 +204,11 @@ __global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_int8_tile_kernel(const
     b_left -= kBK;
     da = desc(a_ptr, a_left);
     db = desc(b_ptr, b_left);
-    fill = fill + C::kStage == lds0 + C::kSt * C::kStage ? lds0 : fill + C::kStage;
+    const bool round = fill_stage == (C::kSt - 1) * C::kStage;
+    const uint32_t by = round ? 0u - (C::kSt - 1) * C::kStage : (uint32_t)C::kStage;
+    fill_stage = round ? 0u : fill_stage + C::kStage;
+    fill_a += by;
+    fill_b += by;
     ++issued;
   };
 
@@ -564,7 +570,7 @@ constexpr TileCost kCost[kNumTiles] = {
     {1, {0.615, 0.0}, 5.2, 0.70},  // 128x128
     {2, {0.73, 1.19}, 4.5, 0.65},  // 128x128, two a CU
     {1, {1.49, 0.0}, 11.5, 0.50},  // 192x256
-    {1, {1.85, 0.0}, 16.0, 0.52},  // 256x256
+    {1, {1.75, 0.0}, 14.0, 0.52},  // 256x256
 };
 
 struct Plan {
