@@ -608,17 +608,21 @@ hipError_t launch_rows(const Int8Args& g, hipStream_t stream) {
 #define ROWS(MT, W)                                                                          \
   hipLaunchKernelGGL((gemm_int8_rows_kernel<MT, W, TOut>), dim3((unsigned)((g.n + 15) / 16), \
                      (unsigned)((g.m + 16 * MT - 1) / (16 * MT))), dim3(64 * W), 0, stream, g)
-  const bool many = g.n >= 16 * 1024;
-  if (g.m <= 16) {
-    if (many)
-      ROWS(1, 4);
-    else
-      ROWS(1, 8);
-  } else {
-    if (many)
+  // More waves a workgroup where it has a long K to itself (us with 4, 8, 16 waves: 1x8192x2048 4.7, 5.3,
+  // 5.6; 1x12288x4096 9.4, 10.6, 12.1; 1x2048x8192 6.0, 5.3, 5.5; 15x2048x16384 -, 11.8, 10.7; 16x2048x65536
+  // 38, 28, 27; 16 do not fit LDS with 32 rows).
+  const int waves = g.n >= 16 * 1024 || g.k <= 4096 ? 4 : g.m > 16 || g.n > 4096 || g.k <= 8192 ? 8 : 16;
+  if (g.m > 16) {
+    if (waves == 4)
       ROWS(2, 4);
     else
       ROWS(2, 8);
+  } else if (waves == 4) {
+    ROWS(1, 4);
+  } else if (waves == 8) {
+    ROWS(1, 8);
+  } else {
+    ROWS(1, 16);
   }
 #undef ROWS
   return hipGetLastError();
