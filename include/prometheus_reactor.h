@@ -907,8 +907,9 @@ PROM_REACTOR_API int prometheus_reactor_runtime_quantize_rows_int8_device(
    contiguous, any alignment; the sum is exact (k <= 131071, so that 128 * 128 * k
    fits 32 bits), the scales are applied in fp32 and the result is rounded once.
    Admission and statuses otherwise as ..._gemm_bf16_device (m * k, n * k, m * n
-   below 2^32); success detail PROM_DETAIL_PATH_HIP_MFMA_INT8. */
+   below 2^32), with m and n at most 2^30; success detail PROM_DETAIL_PATH_HIP_MFMA_INT8. */
 #define PROM_GEMM_INT8_MAX_K 131071u
+#define PROM_GEMM_INT8_MAX_SIDE (1u << 30)
 PROM_REACTOR_API int prometheus_reactor_runtime_gemm_int8_device(void* handle, const int8_t* a, const int8_t* w,
                                                                  const float* a_scale, const float* w_scale, void* c,
                                                                  uint32_t m, uint32_t n, uint32_t k, uint32_t dtype,
@@ -956,7 +957,8 @@ PROM_REACTOR_API uint64_t prometheus_reactor_kv4_page_bytes(uint32_t head_dim, u
    of one projection's output), any alignment of their type.  Rows outside every
    sequence, or before its token 0, are passed over: not stored by a write, left as they
    were by a read.  Write quantises k and v into the cache; read gives what the cache
-   holds (k or v may be NULL in a read). */
+   holds (k or v may be NULL in a read).  No two tokens of a write may share a place
+   (sequences may share pages that a call only reads). */
 typedef struct PrometheusKv4RowsRequest {
   uint32_t struct_size;
   uint32_t dtype;

@@ -395,7 +395,7 @@ __global__ __launch_bounds__(256) void pad_rows8_kernel(const int8_t* __restrict
                                                         const int8_t* __restrict__ w, int8_t* __restrict__ to_w, int n,
                                                         int cols, int ld) {
   const int chunks = ld / 16;
-  const long long total = (long long)(m + n) * chunks;
+  const long long total = ((long long)m + n) * chunks;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     const int row = (int)(i / chunks), c = (int)(i - (long long)row * chunks) * 16;
     const bool first = row < m;
@@ -641,7 +641,7 @@ hipError_t launch(Int8Args g, hipStream_t stream) {
     int8_t* pa = static_cast<int8_t*>(staging(8, (size_t)m * ld));
     int8_t* pw = static_cast<int8_t*>(staging(9, (size_t)n * ld));
     if (pa == nullptr || pw == nullptr) return hipErrorOutOfMemory;
-    const unsigned long long chunks = (unsigned long long)(m + n) * (unsigned)(ld / 16);
+    const unsigned long long chunks = ((unsigned long long)m + n) * (unsigned)(ld / 16);
     hipLaunchKernelGGL(pad_rows8_kernel, dim3((unsigned)std::min<unsigned long long>((chunks + 255) / 256, 1u << 16)),
                        dim3(256), 0, stream, g.a, pa, g.m, g.w, pw, g.n, g.k, ld);
     g.a = pa;

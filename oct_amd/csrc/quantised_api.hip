@@ -128,7 +128,8 @@ PROM_REACTOR_API int prometheus_reactor_runtime_gemm_int8_device(void* handle, c
   if (a == nullptr || w == nullptr || a_scale == nullptr || w_scale == nullptr || c == nullptr)
     return refuse(out_stage, out_detail_code, PROM_STAGE_TRANSFER_IN, PROM_ERROR);
   if (m == 0u || n == 0u || k == 0u) return refuse(out_stage, out_detail_code, PROM_STAGE_INIT, PROM_ERROR);
-  if (!gemm_shape_fits(m, n, k))
+  // Rows and columns up to a tile behind the last are counted in 31 bits.
+  if (!gemm_shape_fits(m, n, k) || m > PROM_GEMM_INT8_MAX_SIDE || n > PROM_GEMM_INT8_MAX_SIDE)
     return refuse(out_stage, out_detail_code, PROM_STAGE_TRANSFER_IN, PROM_DETAIL_SIZE_OVERFLOW);
   if (k > PROM_GEMM_INT8_MAX_K || dtype > PROM_DTYPE_BF16 || !aligned(a_scale, 4) || !aligned(w_scale, 4) ||
       !aligned(c, dtype_size(dtype)))

@@ -63,6 +63,7 @@ DETAIL_SCRATCH_UNAVAILABLE = -6931
 SGEMM_NOALLOC_SCRATCH_BYTES = 64 << 20
 DTYPE_F32, DTYPE_BF16 = 0, 1  # rows of the quantised decode path
 GEMM_INT8_MAX_K = 131071
+GEMM_INT8_MAX_SIDE = 1 << 30
 KV4_PAGE_TOKENS, KV4_GROUP = 64, 64
 GEMM_BF16_SWIGLU, GEMM_BF16_BLOCKED_A = 1, 2  # flags of the bf16 plan and variant entries
 GEMM_BF16_FIVE_STAGE, GEMM_BF16_STAGED = 9, 10  # kernels after the macro tiles 0-8

@@ -117,6 +117,14 @@ def test_int8_product_refuses_in_the_order_of_the_other_products(rt):
         assert _no_device(_product(rt, **change)), change
 
 
+def test_int8_product_refuses_sides_past_its_counting(rt):
+    side = p.GEMM_INT8_MAX_SIDE
+    for change in (dict(m=side + 1, n=1, k=1), dict(m=1, n=side + 1, k=1), dict(m=1, n=0x7FFFFFFF, k=1)):
+        assert _product(rt, **change) == (p.PROM_ERROR, p.STAGE_TRANSFER_IN, p.DETAIL_SIZE_OVERFLOW), change
+    for change in (dict(m=side, n=1, k=1), dict(m=3, n=side, k=1)):
+        assert _no_device(_product(rt, **change)), change
+
+
 CACHE = dict(head_dim=128, kv_heads=2, pages=5, sequences=3, table_stride=4, pool=OK, page_table=OK, lengths=OK)
 BAD_CACHES = [dict(struct_size=8), dict(head_dim=96), dict(head_dim=0), dict(kv_heads=0), dict(kv_heads=1025),
               dict(pages=0), dict(pages=1 << 31), dict(sequences=0), dict(sequences=(1 << 20) + 1),
