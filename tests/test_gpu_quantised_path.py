@@ -115,6 +115,28 @@ def test_rows_at_borders_and_special_values(gpu_runtime):
     assert np.array_equal(q, eq)
 
 
+def _beside(x):
+    """x and its four nearest fp32 neighbours, on a last axis."""
+    bits = np.ascontiguousarray(x, np.float32).view(np.int32)
+    return np.stack([bits + d for d in (-2, -1, 0, 1, 2)], -1).view(np.float32)
+
+
+@pytest.mark.parametrize("power", (-120, -91, -60, 0, 60, 89, 110))
+def test_rows_next_to_where_rounding_changes(gpu_runtime, power):
+    """Values within two ulps of every half step, of scales of any significand."""
+    rng = np.random.default_rng(power + 200)
+    x = np.zeros((64, 640), np.float32)
+    top = (rng.uniform(1, 2, 64) * 2.0 ** power).astype(np.float32)
+    scale = (top / np.float32(127.0)).astype(np.float32)
+    halves = (np.arange(127) + 0.5).astype(np.float32)
+    x[:, :635] = _beside(scale[:, None] * halves).reshape(64, -1) * rng.choice([-1, 1], (64, 635))
+    x = np.where(np.abs(x) > top[:, None], np.float32(0.0), x)
+    x[:, 639] = top
+    q, s = _quantise_rows(gpu_runtime, x, F32)
+    eq, es = oq.quantize_rows(x)
+    assert np.array_equal(s, es) and np.array_equal(q, eq)
+
+
 # ------------------------------------------------------------------ the product
 def _product(rt, a, w, sa, sw, dtype, lead=0):
     (m, k), n = a.shape, w.shape[0]
@@ -175,6 +197,44 @@ def test_product_of_rows_that_were_not_finite_is_nan(gpu_runtime):
         sa[2] = np.nan
         got = _product(gpu_runtime, a, w, sa, sw, BF16)
         assert np.isnan(got[2]).all() and np.isfinite(np.delete(got, 2, 0)).all()
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("m,n,k", [
+    # few rows: 4, 8 and 16 waves a workgroup, one and two blocks of rows
+    (2, 17000, 4100), (16, 5000, 5000), (9, 4000, 8500), (15, 70, 20001), (31, 17000, 300), (20, 4100, 9000),
+    # K in slices; tiles of every size, in one round of workgroups and in several
+    (40, 100, 50000), (300, 300, 20000), (130, 9000, 256), (500, 1500, 1030), (1300, 5200, 144), (2300, 5000, 257),
+    (4100, 6200, 130)])
+def test_product_of_every_variant(gpu_runtime, m, n, k, dtype):
+    a, w = _whole(m + k, (m, k)), _whole(n + k, (n, k), -128)
+    sa, sw = oracle.uniform(1, (m,), 0.001, 0.03), oracle.uniform(2, (n,), -0.001, 0.001)
+    _check_product(_product(gpu_runtime, a, w, sa, sw, dtype), a, w, sa, sw, dtype)
+
+
+@pytest.mark.parametrize("m,n", [(70000, 40), (70000, 5), (5, 70000)])
+def test_product_of_operands_past_4_gib(gpu_runtime, m, n):
+    """The last rows of an operand of 4.27e9 bytes (what lies before them is not looked at)."""
+    k, last = 61000, 40
+    rt, big, small = gpu_runtime, max(m, n), min(m, n)
+    tail, other = _whole(1, (last, k)), _whole(2, (small, k))
+    scale = oracle.uniform(3, (big,), 0.001, 0.002)
+    one = oracle.uniform(4, (small,), 0.001, 0.002)
+    out = np.zeros((m, n), np.float32)
+    with Device(rt) as dev:
+        wide = rt.alloc(big * k)
+        dev.held.append(wide)
+        rt.upload(wide + (big - last) * k, tail)
+        do, narrow, sb, ss = dev.up(out), dev.up(other), dev.up(scale), dev.up(one)
+        if m > n:
+            rt.gemm_int8_device(wide, narrow, sb, ss, do, m, n, k, F32)
+        else:
+            rt.gemm_int8_device(narrow, wide, ss, sb, do, m, n, k, F32)
+        out = dev.down(out, do)
+    if m > n:
+        _check_product(out[-last:], tail, other, scale[-last:], one, F32)
+    else:
+        _check_product(out[:, -last:], other, tail, one, scale[-last:], F32)
 
 
 # ------------------------------------------------------------------ the cache
@@ -319,6 +379,77 @@ def test_cache_groups_of_special_values(gpu_runtime):
     assert np.isinf(expect).any()
     assert np.array_equal(np.isnan(k), np.isnan(expect)) and np.isnan(k).sum() == 3 * 64
     assert np.array_equal(k, expect, equal_nan=True) and np.array_equal(v, -expect, equal_nan=True)
+
+
+@pytest.mark.parametrize("power", (-125, -100, -81, 0, 79, 82, 120))
+def test_cache_groups_next_to_where_rounding_changes(gpu_runtime, power):
+    """Values within two ulps of the middle between two codes, tops within two of where the step changes, and
+    zeros of both signs: the page's bits."""
+    case = Case(dim=64, heads=2, lengths=[200], new=[200], dtype=F32)
+    rng = np.random.default_rng(power + 300)
+    x = np.zeros((400, 64), np.float32)
+    top = (rng.uniform(1, 2, 400) * 2.0 ** power).astype(np.float32)
+    # a step of six bits, six times over: the next top's step is the next
+    top[:200] = _beside((6.0 * (32 + np.arange(40) % 32) / 32 * 2.0 ** power).astype(np.float32)).reshape(-1)
+    t = (top / np.float32(6.0)).astype(np.float32)
+    step = ((t.view(np.uint32) + np.uint32(0x3FFFF)) & np.uint32(0xFFFC0000)).view(np.float32)
+    middles = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], np.float32)
+    x[:, :35] = _beside(step[:, None] * middles).reshape(400, -1) * rng.choice([-1, 1], (400, 35))
+    x = np.where(np.abs(x) > top[:, None], np.float32(0.0), x)
+    x[:, 40], x[:, 41], x[:, 63] = -0.0, 0.0, top
+    x = x.reshape(200, 128)
+    k, v = x.reshape(200, 2, 64), -x.reshape(200, 2, 64)
+    before = case.cache.pool.copy()
+    for row, seq, pos in case.places():
+        case.cache.store(case.table[seq, pos // oq.PAGE], pos % oq.PAGE, k[row], v[row])
+    with Device(gpu_runtime) as dev:
+        pool = dev.up(before)
+        handle, starts = case.handle(dev, pool), dev.up(case.starts)
+        gpu_runtime.kv4_write_device(handle, dev.up(x), dev.up(-x), starts, 200, 128, F32)
+        got = dev.down(before, pool)
+    assert np.array_equal(got, case.cache.pool)
+
+
+def test_cache_past_4_gib_of_pages_and_rows(gpu_runtime):
+    """Pages at the end of a pool of 4.6e9 bytes, rows 2^24 - 1 elements apart: written, read back, attended to."""
+    rt, dim, heads, group, pages, stride, rows = gpu_runtime, 256, 8, 2, 33000, (1 << 24) - 1, 260
+    case = Case(dim, heads, [260, 3], [258, 2], BF16, seed=2)
+    case.table[0], case.table[1, 0] = pages - 2 - np.arange(case.stride), pages - 1
+    case.pages = pages
+    k, v = (_rounded(oracle.normal(s, (rows, heads, dim)), BF16) for s in (1, 2))
+    q = _rounded(oracle.normal(3, (rows, heads * group, dim)), BF16)
+    block = heads * (oq.PAGE * dim + 4 * dim)
+    last = np.zeros((8, block), np.uint8)
+    with Device(rt) as dev:
+        pool = rt.alloc(pages * block)
+        dev.held.append(pool)
+        rt.upload(pool + (pages - 8) * block, last)
+        wide = rt.alloc(rows * stride * 2)
+        dev.held.append(wide)
+        q_at, k_at, v_at, o_at = 0, 8192, 16384, 24576  # elements of a row
+        for r in range(rows):
+            for at, x in ((q_at, q), (k_at, k), (v_at, v)):
+                rt.upload(wide + 2 * (r * stride + at), _bits(x[r], BF16))
+        handle, starts = case.handle(dev, pool), dev.up(case.starts)
+        rt.kv4_write_device(handle, wide + 2 * k_at, wide + 2 * v_at, starts, rows, stride, BF16)
+        back = k_at + heads * dim
+        rt.kv4_read_device(handle, wide + 2 * back, None, starts, rows, stride, BF16)
+        rt.attention_kv4_device(handle, wide, wide + 2 * o_at, starts, rows, heads * group, stride, stride, 258, 260, 0,
+                                dim ** -0.5, BF16)
+        rt.synchronize()
+        read, out = np.zeros_like(_bits(k, BF16)), np.zeros_like(_bits(q, BF16))
+        for r in range(rows):
+            rt.download(read[r], wide + 2 * (r * stride + back))
+            rt.download(out[r], wide + 2 * (r * stride + o_at))
+        last = rt.download(last, pool + (pages - 8) * block)
+    assert np.array_equal(_values(read, BF16), oq.kv4_values(*oq.kv4_quantise(k)))
+    # the two tokens before the call's in sequence 0 and the one in sequence 1: zeros in the pool
+    case.k, case.v = [], []
+    for i in range(2):
+        first, n, old = int(case.starts[i]), int(case.new[i]), int(case.lengths[i] - case.new[i])
+        for held, x in ((case.k, k), (case.v, v)):
+            held.append(np.concatenate([np.zeros((old, heads, dim)), oq.kv4_values(*oq.kv4_quantise(x[first:first + n]))]))
+    _check_attention(_values(out, BF16), case, q, group, BF16)
 
 
 def test_bad_pages_are_not_written_and_read_back_as_nan(gpu_runtime):
@@ -555,3 +686,47 @@ def test_decode_step(gpu_runtime, dtype):
     ea8, esa8 = oq.quantize_rows(attn)
     assert np.array_equal(a8, ea8) and np.array_equal(sa8, esa8)
     _check_product(back, a8, wo, sa8, so, dtype)
+
+
+def _calls(rt, dev, seed, sizes):
+    """Queues a product in slices of K, one of padded rows and an attention in splits, of the sizes given, without a
+    wait; what checks them."""
+    checks = []
+    for i, (m, n, k, length) in enumerate(sizes):
+        a, w = _whole(seed + i, (m, k)), _whole(seed + i + 9, (n, k))
+        sa, sw = oracle.uniform(1, (m,), 0.001, 0.03), oracle.uniform(2, (n,), -0.001, 0.001)
+        c = np.zeros((m, n), np.float32)
+        dc = dev.up(c)
+        rt.gemm_int8_device(dev.up(a), dev.up(w), dev.up(sa), dev.up(sw), dc, m, n, k, F32)
+        case = Case(64, 2, [length, 5], [1, 1], F32, seed=seed + i).history(seed + i)
+        q = oracle.normal(seed + i, (2, 4, 64))
+        out = np.zeros((2, 256), np.float32)
+        do = dev.up(out)
+        rt.attention_kv4_device(case.handle(dev, dev.up(case.cache.pool)), dev.up(q), do, dev.up(case.starts), 2, 4, 256, 256,
+                                1, length, 0, 0.125, F32)
+
+        def check(a=a, w=w, sa=sa, sw=sw, c=c, dc=dc, case=case, q=q, out=out, do=do):
+            _check_product(dev.down(c, dc), a, w, sa, sw, F32)
+            _check_attention(dev.down(out, do).reshape(2, 4, 64), case, q, 2, F32)
+        checks.append(check)
+    return checks
+
+
+def test_calls_that_share_and_grow_the_workspaces(gpu_runtime):
+    with Device(gpu_runtime) as dev:
+        for check in _calls(gpu_runtime, dev, 60, [(40, 60, 9000, 700), (40, 3000, 4095, 3000), (70, 50, 2001, 100),
+                                                   (600, 500, 4112, 1300), (40, 60, 9001, 900)]):
+            check()
+
+
+def test_calls_from_two_threads(gpu_runtime):
+    from concurrent.futures import ThreadPoolExecutor
+
+    def run(seed):
+        with Device(gpu_runtime) as dev:
+            for check in _calls(gpu_runtime, dev, seed, [(33 + seed, 90, 3000 + seed, 400 + seed)] * 6):
+                check()
+        return True
+
+    with ThreadPoolExecutor(2) as pool:
+        assert all(pool.map(run, (1, 2)))
