@@ -58,6 +58,7 @@ constexpr int kWaves = 4;
 constexpr uint64_t kFewPairs = 64;
 constexpr uint64_t kPromptWork = 40000;
 constexpr int kMaxSplits = 64;  // a lane each when they are joined
+constexpr int kPromptGroups = 256;  // workgroups that prompts are dealt to: one a CU
 constexpr uint64_t kMostPartialBytes = 1ull << 30;
 
 struct Kv4Kernel {
@@ -70,7 +71,8 @@ struct Kv4Kernel {
   int rows, q_stride, out_stride;
   int q_heads, group, tiles, splits;
   int few_pairs;        // pairs (rows times group) up to which a sequence is not a prompt
-  uint64_t* units;      // prompts: page units before each sequence, [sequences + 1]
+  int join_heads;       // query heads that are joined at a time
+  uint64_t* units;      // prompts: page units before each sequence, [sequences + 1]; null: no prompts
   float* prompt_part;   // sums [2 workgroups][rows of a tile][D], then (maximum, weight) of each
   size_t prompt_ends;   // where these begin
   int split_shift;  // a split has 2^split_shift pages or a share of more
@@ -222,6 +224,60 @@ __device__ __forceinline__ void coordinates(const Kv4Kernel& g, int* head, int* 
   *seq = (int)((i + (uint32_t)*tile + (uint32_t)*split) % (uint32_t)g.c.sequences);
 }
 
+// A prompt's work in units: a page of a tile (of Prompt::kRows pairs) of a key head.  All tiles of
+// a sequence count the pages from its first tile's first to its last tile's last.
+struct PromptSpan {
+  int page0, pages, tiles;
+  __device__ __forceinline__ PromptSpan(const Kv4Kernel& g, const Sequence& s, int tile_rows) {
+    const int pairs = s.n * g.group;
+    tiles = s.n > 0 && pairs > g.few_pairs ? (pairs + tile_rows - 1) / tile_rows : 0;
+    page0 = pages = 0;
+    if (tiles > 0) {
+      page0 = Tile(g, s, 0, tile_rows).page0;
+      pages = max(1, Tile(g, s, tiles - 1, tile_rows).last - page0);
+    }
+  }
+};
+
+// units[i] = units before sequence i: one workgroup of 256 threads, as many sequences at a time.
+// waves: LDS of four numbers.
+template <int kRows>
+__device__ void count_prompt_units(const Kv4Kernel& g, uint64_t* waves) {
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  uint64_t before = 0;
+  for (int from = 0; from < g.c.sequences; from += 256) {
+    const int seq = from + tid;
+    uint64_t own = 0;
+    if (seq < g.c.sequences) {
+      const PromptSpan span(g, Sequence(g, seq), kRows);
+      own = (uint64_t)span.tiles * (uint64_t)span.pages * (uint64_t)g.c.kv_heads;
+    }
+    uint64_t sum = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint64_t o = __shfl_up(sum, d);
+      if (lane >= d) sum += o;
+    }
+    if (lane == 63) waves[tid >> 6] = sum;
+    __syncthreads();
+    uint64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < tid >> 6) sum += waves[w];
+      all += waves[w];
+    }
+    if (seq < g.c.sequences) g.units[seq] = before + sum - own;
+    before += all;
+    __syncthreads();
+  }
+  if (tid == 0) g.units[g.c.sequences] = before;
+}
+
+// Waves of a prompt's workgroup, 32 pairs each: one or two a SIMD, by registers.
+template <bool kF32, int D>
+constexpr int kPromptWaves = D == 256 || (kF32 && D == 128) ? 4 : 8;
+
+// The few rows' tiles; with prompts in the call, the last workgroup counts their units instead.
 template <bool kF32, int D>
 __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4Kernel g) {
   constexpr int kG = D / 64, kQT = kF32 ? 3 : 1, kPT = kF32 ? 3 : 2;
@@ -234,6 +290,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int r16 = lane & 15, h = lane >> 4;
+  if (g.units != nullptr && blockIdx.x == gridDim.x - 1) {
+    static_assert(kWaves == 4, "units");
+    count_prompt_units<32 * kPromptWaves<kF32, D>>(g, reinterpret_cast<uint64_t*>(lds));
+    return;
+  }
   int head, seq, tile0, split;
   coordinates(g, &head, &seq, &tile0, &split);
   const Sequence sq(g, seq);
@@ -498,7 +559,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
 // as for the queries).  Bound by the vector unit (softmax, the conversion) beside the MFMAs.
 template <bool kF32, int D>
 struct Prompt {
-  static constexpr int kWaves = D == 256 || (kF32 && D == 128) ? 4 : 8;  // one or two a SIMD, by registers
+  static constexpr int kWaves = kPromptWaves<kF32, D>;
   static constexpr int kThreads = 64 * kWaves, kRows = 32 * kWaves;
   static constexpr int kUnits = 4 * D;                                // of 8 bytes (16 channels): keys, and values
   static constexpr int kEach = 2 * kUnits / kThreads > 0 ? 2 * kUnits / kThreads : 1;
@@ -568,55 +629,6 @@ struct Prompt {
     }
   }
 };
-
-// A prompt's work in units: a page of a tile (of Prompt::kRows pairs) of a key head.  All tiles of
-// a sequence count the pages from its first tile's first to its last tile's last.
-struct PromptSpan {
-  int page0, pages, tiles;
-  __device__ __forceinline__ PromptSpan(const Kv4Kernel& g, const Sequence& s, int tile_rows) {
-    const int pairs = s.n * g.group;
-    tiles = s.n > 0 && pairs > g.few_pairs ? (pairs + tile_rows - 1) / tile_rows : 0;
-    page0 = pages = 0;
-    if (tiles > 0) {
-      page0 = Tile(g, s, 0, tile_rows).page0;
-      pages = max(1, Tile(g, s, tiles - 1, tile_rows).last - page0);
-    }
-  }
-};
-
-// units[i] = units before sequence i: one workgroup, 256 sequences at a time.
-template <int kRows>
-__global__ __launch_bounds__(256) void kv4_prompt_units_kernel(const Kv4Kernel g) {
-  __shared__ uint64_t waves[4];
-  const int tid = (int)threadIdx.x, lane = tid & 63;
-  uint64_t before = 0;
-  for (int from = 0; from < g.c.sequences; from += 256) {
-    const int seq = from + tid;
-    uint64_t own = 0;
-    if (seq < g.c.sequences) {
-      const PromptSpan span(g, Sequence(g, seq), kRows);
-      own = (uint64_t)span.tiles * (uint64_t)span.pages * (uint64_t)g.c.kv_heads;
-    }
-    uint64_t sum = own;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint64_t o = __shfl_up(sum, d);
-      if (lane >= d) sum += o;
-    }
-    if (lane == 63) waves[tid >> 6] = sum;
-    __syncthreads();
-    uint64_t all = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (w < tid >> 6) sum += waves[w];
-      all += waves[w];
-    }
-    if (seq < g.c.sequences) g.units[seq] = before + sum - own;
-    before += all;
-    __syncthreads();
-  }
-  if (tid == 0) g.units[g.c.sequences] = before;
-}
 
 // A stretch of units within one tile and head: pages from..to of the sequence's span (0: its first).
 struct PromptPiece {
@@ -915,13 +927,14 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
   }
 }
 
-// Joins the pieces of a tile that workgroups of kv4_prompt_kernel cut it into, 16 rows a workgroup:
-// blockIdx.y's last piece if it begins a tile that the next workgroup goes on with, and the first
+// Joins the pieces of a tile that workgroups of kv4_prompt_kernel cut it into, 16 rows a workgroup: workgroup
+// `block` / (rows / 16)'s last piece if it begins a tile that the next workgroup goes on with, and the first
 // pieces of those that follow up to the tile's end, in order.
 template <bool kF32, int D>
-__global__ __launch_bounds__(256) void kv4_prompt_join_kernel(const Kv4Kernel g) {
+__device__ void join_prompts(const Kv4Kernel& g, uint32_t block) {
   constexpr int kRows = Prompt<kF32, D>::kRows, kChannels = D / 16;
-  const uint64_t total = g.units[g.c.sequences], n = gridDim.y, w = blockIdx.y;
+  const uint32_t part = block % (kRows / 16);
+  const uint64_t total = g.units[g.c.sequences], n = kPromptGroups, w = block / (kRows / 16);
   const uint64_t begin = first_unit(total, w, n), end = first_unit(total, w + 1, n);
   if (begin == end) return;
   const PromptPiece last(g, end - 1, end, kRows);
@@ -931,7 +944,7 @@ __global__ __launch_bounds__(256) void kv4_prompt_join_kernel(const Kv4Kernel g)
   while (stop < n && first_unit(total, stop, n) < tile_end) ++stop;
 
   const Sequence sq(g, last.seq);
-  const int r = 16 * (int)blockIdx.x + (int)threadIdx.x / 16, x = last.tile * kRows + r;
+  const int r = 16 * (int)part + (int)threadIdx.x / 16, x = last.tile * kRows + r;
   if (x >= sq.n * g.group) return;
   const int row = g.over_group(x), q_head = last.head * g.group + x - row * g.group;
   const float2* all = reinterpret_cast<const float2*>(g.prompt_part + g.prompt_ends);
@@ -958,35 +971,47 @@ __global__ __launch_bounds__(256) void kv4_prompt_join_kernel(const Kv4Kernel g)
   }
 }
 
-// Joins the splits' sums: a workgroup a row, for every gridDim.y-th query head.  Its threads are D / 4 columns of
+// Joins the splits' sums: a workgroup a row, for every join_heads-th query head.  Its threads are D / 4 columns of
 // four channels times kJoinParts: part i adds splits i, i + kJoinParts, ..., the parts are added in order.  Bound
 // by latency: maxima and weights come in one load a lane, all sums at once beside them.  With no more splits than
 // parts, a kernel of one sum a thread keeps twice the waves on a CU (64 rows of 32 heads of 128 in 4 splits 6.0 us,
 // 8.2 with registers for 64; one row in 64 splits 4.9).
 template <int D>
 constexpr int kJoinParts = 256 / (D / 4);
+// With prompts in the call, workgroups before those join their pieces: of one launch.
 template <bool kF32, int D, int kEach>
 __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Kernel g) {
+  uint32_t block = blockIdx.x;
+  if constexpr (!kF32 || D != 256) {
+    if (g.units != nullptr) {
+      constexpr uint32_t kPromptBlocks = kPromptGroups * Prompt<kF32, D>::kRows / 16;
+      if (block < kPromptBlocks) {
+        join_prompts<kF32, D>(g, block);
+        return;
+      }
+      block -= kPromptBlocks;
+    }
+  }
   constexpr int kColumns = D / 4, kParts = kJoinParts<D>;
   __shared__ floatx4 parts[kParts][kColumns];
   __shared__ float factors[kMaxSplits];
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int column = tid % kColumns, part = tid / kColumns;
-  const int row = (int)blockIdx.x;
+  const int row = (int)(block / (uint32_t)g.join_heads), head0 = (int)(block % (uint32_t)g.join_heads);
   const size_t pairs = (size_t)g.rows * g.q_heads;
   auto end_of = [&](int q_head) {  // of this lane's split, if there is one
     return lane < g.splits ? reinterpret_cast<const float2*>(ends(g))[lane * pairs + (size_t)row * g.q_heads + q_head]
                            : make_float2(-INFINITY, 0.0f);
   };
-  float2 next = end_of((int)blockIdx.y);
+  float2 next = end_of(head0);
   const int seq = find_sequence(g.starts, g.c.sequences, row);
   if (seq < 0) return;
   const Sequence sq(g, seq);
   if (sq.n * g.group > g.few_pairs) return;
-  for (int q_head = (int)blockIdx.y; q_head < g.q_heads; q_head += (int)gridDim.y) {
+  for (int q_head = head0; q_head < g.q_heads; q_head += g.join_heads) {
     const size_t x = (size_t)row * g.q_heads + q_head;
     const float2 e = next;
-    if (q_head + (int)gridDim.y < g.q_heads) next = end_of(q_head + (int)gridDim.y);
+    if (q_head + g.join_heads < g.q_heads) next = end_of(q_head + g.join_heads);
     // Splits that this row's tile does not have hold anything; they are left out.
     const int splits = Tile(g, sq, ((row - sq.first) * g.group + q_head % g.group) / kTileRows).splits;
     if (splits == 1) continue;
@@ -1042,7 +1067,7 @@ struct Plan {
   int tiles, splits, shift;  // of the sequences with few rows
   int few_pairs;             // up to so many pairs are few
   bool few;                  // there may be such sequences
-  int prompt_groups;         // workgroups for prompts (0: all rows go the way of few)
+  bool prompts;              // otherwise all rows go the way of few
   int prompt_rows;
   size_t prompt_ends;        // floats of the prompts' partial sums
   size_t part_bytes, prompt_bytes, unit_bytes;
@@ -1057,14 +1082,14 @@ Plan plan(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
   const uint64_t work = small_tiles * (uint64_t)a.c.kv_heads * ((length + kKv4Page - 1) / kKv4Page);
   if (most > kFewPairs && work > kPromptWork && (bf16 || head_dim != 256)) {
     p.prompt_rows = 32 * (head_dim == 256 || (!bf16 && head_dim == 128) ? 4 : 8);
-    p.prompt_groups = 256;
-    p.prompt_ends = 2ull * p.prompt_groups * p.prompt_rows * (size_t)head_dim;
-    p.prompt_bytes = (p.prompt_ends + 4ull * p.prompt_groups * p.prompt_rows) * sizeof(float);
+    p.prompts = true;
+    p.prompt_ends = 2ull * kPromptGroups * p.prompt_rows * (size_t)head_dim;
+    p.prompt_bytes = (p.prompt_ends + 4ull * kPromptGroups * p.prompt_rows) * sizeof(float);
     p.unit_bytes = ((size_t)a.c.sequences + 1) * sizeof(uint64_t);
   }
   // A call of one sequence is either; otherwise sequences of few rows go their own way beside prompts.
-  p.few = p.prompt_groups == 0 || a.c.sequences > 1;
-  p.few_pairs = p.prompt_groups == 0 ? 0x7fffffff : p.few ? (int)kFewPairs : 0;
+  p.few = !p.prompts || a.c.sequences > 1;
+  p.few_pairs = !p.prompts ? 0x7fffffff : p.few ? (int)kFewPairs : 0;
   if (!p.few) return p;
   p.tiles = (int)std::min<uint64_t>((std::min<uint64_t>(most, p.few_pairs) + kTileRows - 1) / kTileRows, kKv4MaxColumns / columns);
   const uint64_t pages = (length + kKv4Page - 1) / kKv4Page, base = columns * (uint64_t)p.tiles;
@@ -1079,28 +1104,25 @@ Plan plan(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
 }
 
 template <bool kF32, int D>
-hipError_t launch(const Kv4Kernel& g, const Plan& p, hipStream_t stream) {
+hipError_t launch(Kv4Kernel g, const Plan& p, hipStream_t stream) {
+  const unsigned tiles = p.few ? (unsigned)g.c.sequences * (unsigned)g.c.kv_heads * (unsigned)p.tiles * (unsigned)p.splits : 0u;
+  hipLaunchKernelGGL((kv4_attention_kernel<kF32, D>), dim3(tiles + (p.prompts ? 1u : 0u)), dim3(64 * kWaves), 0, stream, g);
+  unsigned joins = 0;
   if constexpr (!kF32 || D != 256) {
-    if (p.prompt_groups > 0) {
-      constexpr int kRows = Prompt<kF32, D>::kRows;
-      hipLaunchKernelGGL(kv4_prompt_units_kernel<kRows>, dim3(1), dim3(256), 0, stream, g);
-      hipLaunchKernelGGL((kv4_prompt_kernel<kF32, D>), dim3((unsigned)p.prompt_groups),
-                         dim3((Prompt<kF32, D>::kThreads)), 0, stream, g);
-      hipLaunchKernelGGL((kv4_prompt_join_kernel<kF32, D>), dim3(kRows / 16, (unsigned)p.prompt_groups), dim3(256), 0,
-                         stream, g);
+    if (p.prompts) {
+      hipLaunchKernelGGL((kv4_prompt_kernel<kF32, D>), dim3(kPromptGroups), dim3((Prompt<kF32, D>::kThreads)), 0, stream, g);
+      joins = kPromptGroups * Prompt<kF32, D>::kRows / 16;
     }
   }
-  if (p.few) {
-    const unsigned grid = (unsigned)g.c.sequences * (unsigned)g.c.kv_heads * (unsigned)p.tiles * (unsigned)p.splits;
-    hipLaunchKernelGGL((kv4_attention_kernel<kF32, D>), dim3(grid), dim3(64 * kWaves), 0, stream, g);
-    if (p.splits > 1) {
-      const unsigned heads = std::min<unsigned>((unsigned)g.q_heads, std::max(1u, 4096u / (unsigned)g.rows));
-      const dim3 join((unsigned)g.rows, heads);
-      if (p.splits <= kJoinParts<D>)
-        hipLaunchKernelGGL((kv4_join_kernel<kF32, D, 1>), join, dim3(256), 0, stream, g);
-      else
-        hipLaunchKernelGGL((kv4_join_kernel<kF32, D, kMaxSplits / kJoinParts<D>>), join, dim3(256), 0, stream, g);
-    }
+  if (p.few && p.splits > 1) {
+    g.join_heads = (int)std::min<unsigned>((unsigned)g.q_heads, std::max(1u, 4096u / (unsigned)g.rows));
+    joins += (unsigned)g.rows * (unsigned)g.join_heads;
+  }
+  if (joins > 0) {
+    if (p.splits <= kJoinParts<D>)
+      hipLaunchKernelGGL((kv4_join_kernel<kF32, D, 1>), dim3(joins), dim3(256), 0, stream, g);
+    else
+      hipLaunchKernelGGL((kv4_join_kernel<kF32, D, kMaxSplits / kJoinParts<D>>), dim3(joins), dim3(256), 0, stream, g);
   }
   return hipGetLastError();
 }
@@ -1140,7 +1162,7 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf
   g.ends = (size_t)p.splits * a.rows * (size_t)a.q_heads * (size_t)head_dim;
   g.prompt_part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.part) + round_up(p.part_bytes));
   g.prompt_ends = p.prompt_ends;
-  g.units = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(g.prompt_part) + round_up(p.prompt_bytes));
+  if (p.prompts) g.units = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(g.prompt_part) + round_up(p.prompt_bytes));
   switch (head_dim) {
     case 64: return bf16 ? launch<false, 64>(g, p, stream) : launch<true, 64>(g, p, stream);
     case 128: return bf16 ? launch<false, 128>(g, p, stream) : launch<true, 128>(g, p, stream);
