@@ -2,28 +2,30 @@
 // o[r, h] = sum_t softmax_t(scale q[r, h] . k[t]) v[t], k[t] = s code, v[t] = s code
 // with a step s for 64 channels of a token's head.
 //
-// Rows are (row, query head of the group) pairs: a tile is 16 of them, so that the heads
-// that share a key head, and a few rows of a prompt, read the cache once.  A wave takes
-// a page (64 tokens) at a time:
-//   S^T = K Q^T on v_mfma_f32_16x16x32_bf16.  E2M1 codes are exact in bf16 (one
-//   instruction turns two codes into two numbers), so K goes into the products as codes,
-//   one accumulator a group of 64 channels, and the groups' steps are applied to the
-//   scores in fp32.  A lane owns one row and 16 of the page's scores: tile c, register i
-//   of lane (h, row) is token 16 h + 4 c + i, so a lane's tokens are neighbours and their
-//   steps four 16-byte loads.
-//   Softmax with a running maximum that follows only when it grew by more than 2^8, in
-//   base 2.
-//   O^T = V^T P^T.  V's step goes to the probability; P s is split into bf16 terms
-//   that carry it to 16 bits (24 for fp32 rows), the codes again are exact.  The V^T
-//   operand (16 channels, tokens in k) comes from ds_read_b64_tr_b4, which hands a lane
-//   the 16 tokens of its channel; S^T's register order is already P^T's operand order.
-//   fp32 queries are three bf16 terms (exact).
-// No rounding but P's and fp32's is made anywhere.
+// Rows are (row, query head of the group) pairs, so that the heads that share a key head, and the
+// rows of a prompt, read the cache once.  Two kernels.
 //
-// Pages of a sequence are dealt to the waves of a workgroup and to gridDim splits; the
-// waves join through LDS, splits through fp32 partials and a second kernel, in a fixed
-// order.  Bound by reading the cache for long sequences (272 bytes of a 64-channel
-// group pair... per token and head D + D / 16 bytes).
+// Few rows (decoding): a tile is 16 pairs, a wave takes a page (64 tokens) at a time, which it moves to
+// its own part of LDS a page ahead (buffer_load ... lds, 16 bytes a lane; no wave waits for another).
+//   S^T = K Q^T on v_mfma_f32_16x16x32_bf16.  E2M1 codes are exact in bf16 (one instruction turns two
+//   codes into two numbers), so K goes into the products as codes, one accumulator a group of 64
+//   channels, and the groups' steps are applied to the scores in fp32.  A lane owns one row and 16 of the
+//   page's scores: tile c, register i of lane (h, row) is token 16 h + 4 c + i, so a lane's tokens are
+//   neighbours and their steps four 16-byte loads.
+//   Softmax in base 2 with a running maximum that follows only when it grew by more than 2^8.
+//   O^T = V^T P^T.  V's step goes to the probability; P s is split into bf16 terms that carry it to 16
+//   bits (24 for fp32 rows), the codes again are exact.  The V^T operand (16 channels, tokens in k) comes
+//   from ds_read_b64_tr_b4, which hands a lane the 16 tokens of its channel; S^T's register order is
+//   already P^T's operand order.  fp32 queries are three bf16 terms (exact).
+// No rounding but P's and fp32's is made.  Pages of a sequence are dealt to the waves of a workgroup and
+// to splits of the grid; the waves join through LDS, splits through fp32 partial sums and a second
+// kernel, in a fixed order.  Bound by reading the cache, D + D / 16 bytes a token and key head: 64 rows over
+// 64 sequences of up to 8192 tokens, 8 key heads of 128, groups of 4, bf16: 70 us, 4.6 TB/s, and 6 for the
+// join; one row over 131072 tokens: 29 us, 4.9 TB/s, and 5.  A short sequence is bound by latency: 777
+// tokens of one key head of 256, fp32, 9.5 us (a launch that does nothing 1.4, the way to the first page
+// 2.5, a page 4, joining 1) and 4.
+//
+// Prompts: see kv4_prompt_kernel.
 #include <algorithm>
 #include <type_traits>
 
@@ -49,14 +51,14 @@ constexpr float kLazyLog2 = 8.0f;
 constexpr int kTileRows = 16;
 constexpr int kWaves = 4;
 // Sequences of up to kFewPairs pairs (rows times query heads of a group) stay on the kernel for few
-// rows, whatever the call: a prompt tile has 128 or 256.  The prompt kernel's three launches and
-// their joins cost 25 to 50 us, and it saves 0.5 (64 channels) to 2.3 ns (256) for a page of 16 pairs
-// (us, two prompts over 4096 tokens, 4 key heads, groups of 4, few rows' kernel against it; 512 new
-// rows each: bf16 64 channels 57 / 52, 128 98 / 68, 256 241 / 151, fp32 66 / 69, 123 / 110; 64 new
-// rows: 18 / 42, 27 / 52, 49 / 84, 20 / 49, 31 / 55), so it is taken from kPromptWork such pages on.
-// fp32 rows of 256 channels do not fit its registers (310 / 409).
+// rows, whatever the call: a prompt tile has 128 or 256.  The prompts' kernel costs 40 to 80 us before
+// it does much and then takes half the time for a page of 16 pairs, so it is taken from so many of
+// them on (us with it / without, two prompts over 4096 tokens, 4 key heads, groups of 4; 256 new rows
+// each, 32768 pages of 16 pairs: bf16 64 channels 43 / 31, 128 54 / 51, 256 98 / 118, fp32 52 / 35,
+// 68 / 63; 512 new rows: 47 / 52, 62 / 92, 135 / 222, 62 / 61, 97 / 115).  fp32 rows of 256 channels do
+// not fit its registers (310 / 409).
 constexpr uint64_t kFewPairs = 64;
-constexpr uint64_t kPromptWork = 40000;
+constexpr uint64_t prompt_work(int head_dim) { return head_dim == 256 ? 24000 : 40000; }
 constexpr int kMaxSplits = 64;  // a lane each when they are joined
 constexpr int kPromptGroups = 256;  // workgroups that prompts are dealt to: one a CU
 constexpr uint64_t kMostPartialBytes = 1ull << 30;
@@ -554,9 +556,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
 // Many rows (prompts).  A workgroup takes 32 pairs a wave; a page's keys and values are turned
 // into bf16 (exactly, steps applied) once for all of them and kept in LDS, and a wave computes
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_bf16, the V^T operand by transpose reads.
-// The next page's codes are loaded into registers before a page is worked on and turned into
-// the other half of LDS after it: one barrier a page.  P goes to bf16 (fp32 rows: three terms,
-// as for the queries).  Bound by the vector unit (softmax, the conversion) beside the MFMAs.
+// The next page's codes are loaded into registers before a page is worked on and turned into the
+// other half of LDS after it.  Of eight waves, the second of each SIMD runs half a page behind the first:
+// one's products are beside the other's softmax.  P goes to bf16, 8 bits, as
+// many as the output has (fp32 rows: three terms, as for the queries).  Bound by the matrix and vector units together, which
+// two waves of a SIMD share less well than they could: four prompts of 1024 rows over up to 8000
+// tokens, 8 key heads of 128, groups of 4, bf16: 302 us for the call, 0.79 PFLOP/s (170 us at the rate of a
+// large product).  Another such call's 350 us, a part at a time: 65 without any of the four, 45 more with the
+// loads, and beside these 35 with turning the codes, 78 with softmax, 153 with the products.
 template <bool kF32, int D>
 struct Prompt {
   static constexpr int kWaves = kPromptWaves<kF32, D>;
@@ -1080,7 +1087,7 @@ Plan plan(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
   if (a.window) length = std::min<uint64_t>(length, (uint64_t)a.window + a.max_rows + 2 * kKv4Page);
   const uint64_t small_tiles = ((uint64_t)a.rows * (uint64_t)a.group + kTileRows - 1) / kTileRows;
   const uint64_t work = small_tiles * (uint64_t)a.c.kv_heads * ((length + kKv4Page - 1) / kKv4Page);
-  if (most > kFewPairs && work > kPromptWork && (bf16 || head_dim != 256)) {
+  if (most > kFewPairs && work > prompt_work(head_dim) && (bf16 || head_dim != 256)) {
     p.prompt_rows = 32 * (head_dim == 256 || (!bf16 && head_dim == 128) ? 4 : 8);
     p.prompts = true;
     p.prompt_ends = 2ull * kPromptGroups * p.prompt_rows * (size_t)head_dim;

