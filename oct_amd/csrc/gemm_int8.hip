@@ -10,11 +10,12 @@
 // end and a's chunks past k are sent out of range, so tails add zeros.  Rows that
 // are not whole 16-byte chunks are copied to padded ones first.  Where tiles are few,
 // K is cut into slices whose int32 sums a second kernel adds (exact in any order).
-// 4224x20480x3840 to bf16: 353 us, 1.88 POP/s (a library's product of the same shape to
-// int32 308 to 345); LDS is busy for as long as the matrix units (256x256 a workgroup:
-// 384 clocks of reads and 128 of transfers for 512 of products), and in the last of six
-// rounds of tiles 80 of 256 workgroups have one.  4097x3001x513 to fp32: 5.7 us to pad
-// and 22 for the tiles.
+// 4224x20480x3840 to bf16: 328 us, 2.03 POP/s (a library's product of the same shape to
+// int32 308 to 345): five whole rounds of 256x256 tiles and the columns left over as
+// 128x128 (as a sixth round 338).  Waves wait a third of their time, at the barrier of
+// each K tile and for the first operands behind it.  Loads through registers instead of
+// straight to LDS took 32 us longer, and at 4097x3001x513 to fp32 (5.7 us to pad and 22 for
+// the tiles) saved no more than the padding cost.
 //
 // Few rows (a decode step, a short prompt): every weight is read once and K is dealt
 // to the waves of a workgroup, which add their sums through LDS.  Bound by reading w:
@@ -42,7 +43,7 @@ struct Int8Args {
   void* c;
   int32_t* slabs;  // K slices' sums, [slices][m][n] (null: one slice)
   int m, n, k;     // k of the operands as multiplied
-  int lda, ldw;
+  int lda, ldw, ldc;
   int tiles_m, tiles_n;
 };
 
@@ -67,10 +68,10 @@ __device__ __forceinline__ void pack(const int32_t* from, __bf16 (&to)[8]) {
   }
 }
 
-// 32 rows of kCols words in LDS (rows kPitch apart) to rows r0.. and columns c0.. of out [m, n], 16
+// 32 rows of kCols words in LDS (rows kPitch apart) to rows r0.. and columns c0.. of out [m, n], rows ld apart, 16
 // bytes a lane at any alignment, the last columns of a row one by one.
 template <int kCols, int kPitch, typename T>
-__device__ __forceinline__ void store_rows(const int32_t* lds, T* out, int r0, int c0, int m, int n, int lane) {
+__device__ __forceinline__ void store_rows(const int32_t* lds, T* out, int r0, int c0, int m, int n, int ld, int lane) {
   constexpr int kEach = 16 / (int)sizeof(T), kLanes = kCols / kEach, kRows = 64 / kLanes;
   const int c = (lane % kLanes) * kEach, left = n - (c0 + c);
 #pragma unroll
@@ -79,7 +80,7 @@ __device__ __forceinline__ void store_rows(const int32_t* lds, T* out, int r0, i
     if (r0 + r >= m || left <= 0) continue;
     T v[kEach];
     pack(lds + r * kPitch + c, v);
-    T* to = out + (size_t)(r0 + r) * n + c0 + c;
+    T* to = out + (size_t)(r0 + r) * ld + c0 + c;
     if (left >= kEach) {
       __builtin_memcpy(to, v, 16);
     } else {
@@ -271,7 +272,8 @@ __global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_int8_tile_kernel(const
   uint32_t cur = 0;
   // Step t: tile t has landed for this wave, later ones may stay in flight; after the
   // barrier it is complete for all waves and tile t-1's stage is free.  The transfers of
-  // tile t + kSt - 1 go out between the MFMAs, spread evenly.
+  // tile t + kSt - 1 go out between the MFMAs of the first half (4224x20480x3840: 338 us; over
+  // all of them, where the last ones come late, 354, over a quarter 344).
   auto step = [&](int t, auto more_c, auto tail_c) __attribute__((always_inline)) {
     constexpr bool kMore = decltype(more_c)::value, kTail = decltype(tail_c)::value;
     constexpr int kMfma = kSteps * C::kMI * C::kNI;
@@ -296,7 +298,7 @@ __global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_int8_tile_kernel(const
           acc[mi][ni] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[mi], f.b[ni], acc[mi][ni], 0, 0, 0);
 #pragma unroll
           for (int j = 0; j < C::kX; ++j)
-            if (kMore && j * kMfma / C::kX == at) issue_one(j, kTail);
+            if (kMore && j * kMfma / C::kX / 2 == at) issue_one(j, kTail);
         }
       if (s + 1 < kSteps) f = nf;
     }
@@ -348,9 +350,9 @@ __global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_int8_tile_kernel(const
     }
     asm volatile("" ::: "memory");  // a wave's own part: its LDS operations stay in order
     if (g.slabs != nullptr)
-      store_rows<kCols, kPitch>(mine, g.slabs + (size_t)blockIdx.y * g.m * g.n, r0, wave_col, g.m, g.n, lane);
+      store_rows<kCols, kPitch>(mine, g.slabs + (size_t)blockIdx.y * g.m * g.n, r0, wave_col, g.m, g.n, g.n, lane);
     else
-      store_rows<kCols, kPitch>(mine, static_cast<TOut*>(g.c), r0, wave_col, g.m, g.n, lane);
+      store_rows<kCols, kPitch>(mine, static_cast<TOut*>(g.c), r0, wave_col, g.m, g.n, g.ldc, lane);
     asm volatile("" ::: "memory");
   }
 }
@@ -360,7 +362,7 @@ template <typename TOut>
 __global__ __launch_bounds__(256) void int8_slices_kernel(const int32_t* __restrict__ slabs, int slices,
                                                           const float* __restrict__ a_scale,
                                                           const float* __restrict__ w_scale, TOut* __restrict__ c,
-                                                          int m, int n) {
+                                                          int m, int n, int ldc) {
   const int col = (int)(blockIdx.x * 256 + threadIdx.x);
   if (col >= n) return;
   const size_t slab = (size_t)m * n;
@@ -369,7 +371,7 @@ __global__ __launch_bounds__(256) void int8_slices_kernel(const int32_t* __restr
     const int32_t* p = slabs + (size_t)row * n + col;
     int sum = 0;
     for (int s = 0; s < slices; ++s) sum += p[s * slab];
-    store_scaled(c + (size_t)row * n + col, sum, a_scale[row], ws);
+    store_scaled(c + (size_t)row * ldc + col, sum, a_scale[row], ws);
   }
 }
 
@@ -565,48 +567,76 @@ hipError_t launch_tile(int tile, int slices, const Int8Args& g, hipStream_t stre
 }
 
 // Estimated microseconds of a tile's workgroup: `fill` plus step[w - 1] for each 128 of k where w of
-// them share a CU; on an otherwise idle chip a step takes `idle` of that.  From 16 x 16 tiles of
-// each with k 512, 2048 and 8192, and a single tile.
+// them share a CU; on an otherwise idle chip a step takes `idle` of that.  From 15 x 17 tiles of
+// each with k 512, 2048 and 8192, two and three rounds of them, and a single tile.
 struct TileCost {
   int occ;
   double step[2], fill, idle;
 };
 constexpr TileCost kCost[kNumTiles] = {
-    {2, {0.24, 0.46}, 2.6, 0.95},  // 64x64
-    {1, {0.615, 0.0}, 5.2, 0.70},  // 128x128
-    {2, {0.73, 1.19}, 4.5, 0.65},  // 128x128, two a CU
-    {1, {1.49, 0.0}, 11.5, 0.50},  // 192x256
-    {1, {1.75, 0.0}, 14.0, 0.52},  // 256x256
+    {2, {0.215, 0.46}, 2.3, 0.95},  // 64x64
+    {1, {0.615, 0.0}, 4.3, 0.73},   // 128x128
+    {2, {0.72, 1.16}, 3.1, 0.54},   // 128x128, two a CU
+    {1, {1.45, 0.0}, 8.3, 0.54},    // 192x256
+    {1, {1.60, 0.0}, 12.5, 0.60},   // 256x256
 };
+constexpr double kLaunchUs = 3.0;  // of a further launch
+
+double rounds_us(int t, long long workgroups, int kt) {
+  const TileCost& c = kCost[t];
+  const long long slots = 256ll * c.occ, full = workgroups / slots, rest = workgroups - full * slots;
+  double us = (double)full * (c.fill + kt * c.step[c.occ - 1]);
+  if (rest > 0) {
+    const int w = (int)((rest + 255) / 256);
+    us += c.fill + kt * c.step[w - 1] * (c.idle + (1.0 - c.idle) * (double)rest / (256.0 * w));
+  }
+  return us;
+}
 
 struct Plan {
   int tile, slices;
+  uint32_t n;  // columns that it takes
 };
-Plan plan_tiles(uint32_t m, uint32_t n, uint32_t k) {
+long long tiles_of(int t, uint32_t m, uint32_t n) {
+  return (long long)((m + kTiles[t].bm - 1) / kTiles[t].bm) * ((n + kTiles[t].bn - 1) / kTiles[t].bn);
+}
+// The best tile and number of K slices for all of n columns.
+double plan_columns(uint32_t m, uint32_t n, uint32_t k, Plan* plan) {
   static const int kSlices[] = {1, 2, 3, 4, 6, 8, 12, 16};
   const int all = (int)((k + 127) / 128);
   double best = 1e300;
-  Plan plan{0, 1};
-  for (int t = 0; t < kNumTiles; ++t) {
-    const TileCost& c = kCost[t];
-    const long long tiles = (long long)((m + kTiles[t].bm - 1) / kTiles[t].bm) * ((n + kTiles[t].bn - 1) / kTiles[t].bn);
+  for (int t = 0; t < kNumTiles; ++t)
     for (int s : kSlices) {
       if (s > 1 && all < 3 * s) break;
-      const int kt = (all + s - 1) / s;
-      const long long slots = 256ll * c.occ, total = tiles * s, full = total / slots, rest = total - full * slots;
-      double us = (double)full * (c.fill + kt * c.step[c.occ - 1]);
-      if (rest > 0) {
-        const int w = (int)((rest + 255) / 256);
-        us += c.fill + kt * c.step[w - 1] * (c.idle + (1.0 - c.idle) * (double)rest / (256.0 * w));
-      }
+      double us = rounds_us(t, tiles_of(t, m, n) * s, (all + s - 1) / s);
       if (s > 1) us += 6.1 + (double)(s + 1) * m * n * 4.0 / 10.0e6;
       if (us < best) {
         best = us;
-        plan = Plan{t, s};
+        *plan = Plan{t, s, n};
       }
     }
+  return best;
+}
+// Or one tile for as many columns as are whole rounds of it, and another plan for the rest.
+int plan_tiles(uint32_t m, uint32_t n, uint32_t k, Plan (&plan)[2]) {
+  const int all = (int)((k + 127) / 128);
+  double best = plan_columns(m, n, k, &plan[0]);
+  int parts = 1;
+  for (int t = 1; t < kNumTiles; ++t) {
+    const long long high = tiles_of(t, m, 1), slots = 256ll * kCost[t].occ;
+    const long long columns = tiles_of(t, m, n) / slots * slots / high * kTiles[t].bn;
+    if (columns == 0 || columns >= n) continue;
+    Plan rest;
+    const double us = rounds_us(t, tiles_of(t, m, (uint32_t)columns), all) + kLaunchUs +
+                      plan_columns(m, n - (uint32_t)columns, k, &rest);
+    if (us < best) {
+      best = us;
+      parts = 2;
+      plan[0] = Plan{t, 1, (uint32_t)columns};
+      plan[1] = rest;
+    }
   }
-  return plan;
+  return parts;
 }
 
 template <typename TOut>
@@ -641,6 +671,7 @@ hipError_t launch(Int8Args g, hipStream_t stream) {
   const uint32_t m = (uint32_t)g.m, n = (uint32_t)g.n, k = (uint32_t)g.k;
   if (m <= kFewRows) return launch_rows<TOut>(g, stream);
   g.lda = g.ldw = g.k;
+  g.ldc = g.n;
   const bool aligned = k % 16 == 0 && ((uintptr_t)g.a & 15u) == 0 && ((uintptr_t)g.w & 15u) == 0;
   if (!aligned) {
     const int ld = (int)((k + 15) & ~15u);
@@ -654,17 +685,27 @@ hipError_t launch(Int8Args g, hipStream_t stream) {
     g.w = pw;
     g.lda = g.ldw = ld;
   }
-  Plan p = plan_tiles(m, n, k);
-  if (p.slices > 1) {
-    g.slabs = static_cast<int32_t*>(staging(6, (size_t)p.slices * m * n * sizeof(int32_t)));
-    if (g.slabs == nullptr) p.slices = 1;
+  Plan plans[2];
+  const int parts = plan_tiles(m, n, k, plans);
+  for (int i = 0; i < parts; ++i) {
+    Plan& p = plans[i];
+    g.n = (int)p.n;
+    g.slabs = nullptr;
+    if (p.slices > 1) {
+      g.slabs = static_cast<int32_t*>(staging(6, (size_t)p.slices * m * p.n * sizeof(int32_t)));
+      if (g.slabs == nullptr) p.slices = 1;
+    }
+    g.tiles_m = (int)((m + kTiles[p.tile].bm - 1) / kTiles[p.tile].bm);
+    g.tiles_n = (int)((p.n + kTiles[p.tile].bn - 1) / kTiles[p.tile].bn);
+    const hipError_t e = launch_tile<TOut>(p.tile, p.slices, g, stream);
+    if (e != hipSuccess) return e;
+    if (p.slices > 1)
+      hipLaunchKernelGGL((int8_slices_kernel<TOut>), dim3((p.n + 255) / 256, std::min<unsigned>(m, 4096u)), dim3(256),
+                         0, stream, g.slabs, p.slices, g.a_scale, g.w_scale, static_cast<TOut*>(g.c), g.m, g.n, g.ldc);
+    g.w += (size_t)p.n * g.ldw;
+    g.w_scale += p.n;
+    g.c = static_cast<TOut*>(g.c) + p.n;
   }
-  g.tiles_m = (int)((m + kTiles[p.tile].bm - 1) / kTiles[p.tile].bm);
-  g.tiles_n = (int)((n + kTiles[p.tile].bn - 1) / kTiles[p.tile].bn);
-  const hipError_t e = launch_tile<TOut>(p.tile, p.slices, g, stream);
-  if (e != hipSuccess || p.slices == 1) return e;
-  hipLaunchKernelGGL((int8_slices_kernel<TOut>), dim3((n + 255) / 256, std::min<unsigned>(m, 4096u)), dim3(256), 0,
-                     stream, g.slabs, p.slices, g.a_scale, g.w_scale, static_cast<TOut*>(g.c), g.m, g.n);
   return hipGetLastError();
 }
 
