@@ -582,13 +582,14 @@ constexpr TileCost kCost[kNumTiles] = {
 };
 constexpr double kLaunchUs = 3.0;  // of a further launch
 
-double rounds_us(int t, long long workgroups, int kt) {
+double rounds_us(int t, uint64_t workgroups, uint32_t kt) {
   const TileCost& c = kCost[t];
-  const long long slots = 256ll * c.occ, full = workgroups / slots, rest = workgroups - full * slots;
+  const uint64_t full = c.occ == 2 ? workgroups >> 9 : workgroups >> 8;
+  const uint32_t rest = (uint32_t)(workgroups - full * 256 * (uint64_t)c.occ);
   double us = (double)full * (c.fill + kt * c.step[c.occ - 1]);
   if (rest > 0) {
-    const int w = (int)((rest + 255) / 256);
-    us += c.fill + kt * c.step[w - 1] * (c.idle + (1.0 - c.idle) * (double)rest / (256.0 * w));
+    const uint32_t w = (rest + 255) >> 8;
+    us += c.fill + kt * c.step[w - 1] * (c.idle + (1.0 - c.idle) / 256.0 * rest / w);
   }
   return us;
 }
@@ -597,37 +598,41 @@ struct Plan {
   int tile, slices;
   uint32_t n;  // columns that it takes
 };
-long long tiles_of(int t, uint32_t m, uint32_t n) {
-  return (long long)((m + kTiles[t].bm - 1) / kTiles[t].bm) * ((n + kTiles[t].bn - 1) / kTiles[t].bn);
+uint64_t tiles_of(int t, uint32_t m, uint32_t n) {
+  const uint32_t bm = (uint32_t)kTiles[t].bm, bn = (uint32_t)kTiles[t].bn;
+  return (uint64_t)((m + bm - 1) / bm) * ((n + bn - 1) / bn);
 }
-// The best tile and number of K slices for all of n columns.
+// The best tile and number of K slices for all of n columns; slices where tiles are no two rounds.
 double plan_columns(uint32_t m, uint32_t n, uint32_t k, Plan* plan) {
-  static const int kSlices[] = {1, 2, 3, 4, 6, 8, 12, 16};
-  const int all = (int)((k + 127) / 128);
+  static const uint32_t kSlices[] = {1, 2, 3, 4, 6, 8, 12, 16};
+  const uint32_t all = (k + 127) / 128;
   double best = 1e300;
-  for (int t = 0; t < kNumTiles; ++t)
-    for (int s : kSlices) {
-      if (s > 1 && all < 3 * s) break;
-      double us = rounds_us(t, tiles_of(t, m, n) * s, (all + s - 1) / s);
+  for (int t = 0; t < kNumTiles; ++t) {
+    const uint64_t tiles = tiles_of(t, m, n);
+    for (uint32_t s : kSlices) {
+      if (s > 1 && (all < 3 * s || tiles >= 512u * (unsigned)kCost[t].occ)) break;
+      double us = rounds_us(t, tiles * s, (all + s - 1) / s);
       if (s > 1) us += 6.1 + (double)(s + 1) * m * n * 4.0 / 10.0e6;
       if (us < best) {
         best = us;
-        *plan = Plan{t, s, n};
+        *plan = Plan{t, (int)s, n};
       }
     }
+  }
   return best;
 }
-// Or one tile for as many columns as are whole rounds of it, and another plan for the rest.
+// Or one tile for as many columns as are whole rounds of it, and another plan for the rest, where that
+// promises 3 % (estimates are not that good).
 int plan_tiles(uint32_t m, uint32_t n, uint32_t k, Plan (&plan)[2]) {
-  const int all = (int)((k + 127) / 128);
-  double best = plan_columns(m, n, k, &plan[0]);
+  double best = 0.97 * plan_columns(m, n, k, &plan[0]);
   int parts = 1;
   for (int t = 1; t < kNumTiles; ++t) {
-    const long long high = tiles_of(t, m, 1), slots = 256ll * kCost[t].occ;
-    const long long columns = tiles_of(t, m, n) / slots * slots / high * kTiles[t].bn;
+    const uint64_t tiles = tiles_of(t, m, n), slots = 256u * (unsigned)kCost[t].occ;
+    if (tiles <= slots) continue;
+    const uint64_t columns = tiles / slots * slots / tiles_of(t, m, 1) * (unsigned)kTiles[t].bn;
     if (columns == 0 || columns >= n) continue;
     Plan rest;
-    const double us = rounds_us(t, tiles_of(t, m, (uint32_t)columns), all) + kLaunchUs +
+    const double us = rounds_us(t, tiles_of(t, m, (uint32_t)columns), (k + 127) / 128) + kLaunchUs +
                       plan_columns(m, n - (uint32_t)columns, k, &rest);
     if (us < best) {
       best = us;

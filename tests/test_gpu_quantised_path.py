@@ -205,7 +205,9 @@ def test_product_of_rows_that_were_not_finite_is_nan(gpu_runtime):
     (2, 17000, 4100), (16, 5000, 5000), (9, 4000, 8500), (15, 70, 20001), (31, 17000, 300), (20, 4100, 9000),
     # K in slices; tiles of every size, in one round of workgroups and in several
     (40, 100, 50000), (300, 300, 20000), (130, 9000, 256), (500, 1500, 1030), (1300, 5200, 144), (2300, 5000, 257),
-    (4100, 6200, 130), (2000, 1999, 4112), (2990, 4001, 2065), (3950, 3901, 2064), (5000, 4100, 1040)])
+    (4100, 6200, 130), (2000, 1999, 4112), (2990, 4001, 2065), (3950, 3901, 2064), (5000, 4100, 1040),
+    # whole rounds of one tile and the columns left over on another, in one piece and in slices of K
+    (1294, 11946, 1733), (2009, 8627, 1177), (358, 11183, 8230), (381, 11070, 7872)])
 def test_product_of_every_variant(gpu_runtime, m, n, k, dtype):
     a, w = _whole(m + k, (m, k)), _whole(n + k, (n, k), -128)
     sa, sw = oracle.uniform(1, (m,), 0.001, 0.03), oracle.uniform(2, (n,), -0.001, 0.001)
