@@ -203,6 +203,8 @@ def test_product_of_rows_that_were_not_finite_is_nan(gpu_runtime):
 @pytest.mark.parametrize("m,n,k", [
     # few rows: 4, 8 and 16 waves a workgroup, one and two blocks of rows
     (2, 17000, 4100), (16, 5000, 5000), (9, 4000, 8500), (15, 70, 20001), (31, 17000, 300), (20, 4100, 9000),
+    # rows shorter than a load and than a tile's part of K
+    (40, 50, 1), (70, 33, 15), (33, 40, 17), (3, 70, 1), (20, 5, 255), (32, 33, 257),
     # K in slices; tiles of every size, in one round of workgroups and in several
     (40, 100, 50000), (300, 300, 20000), (130, 9000, 256), (500, 1500, 1030), (1300, 5200, 144), (2300, 5000, 257),
     (4100, 6200, 130), (2000, 1999, 4112), (2990, 4001, 2065), (3950, 3901, 2064), (5000, 4100, 1040),
@@ -590,6 +592,25 @@ def test_attention_does_not_depend_on_the_launch_hints(gpu_runtime):
     for most, longest in ((50, 2000), (1, 1), (56, LOOKS_LONG), (3, 0xFFFFFFFF), (56, 64), (17, LOOKS_LONG)):
         got = _attend(gpu_runtime, case, q, 4, BF16, max_rows=most, max_length=longest)
         _check_attention(got, case, q, 4, BF16)
+
+
+@pytest.mark.parametrize("longest", (None, LOOKS_LONG))
+def test_attention_of_many_sequences(gpu_runtime, longest):
+    """More sequences than a search step, a workgroup's threads and a row of the grid hold, prompts among them."""
+    lengths = [1 + i * 7 % 90 for i in range(700)]
+    new = [n if i % 97 == 5 else i % 3 % (n + 1) for i, n in enumerate(lengths)]
+    case = Case(64, 1, lengths, new, BF16, seed=13, extra_rows=3, empty=2).history(77)
+    q = _rounded(oracle.normal(19, (case.rows, 2, 64)), BF16)
+    _check_attention(_attend(gpu_runtime, case, q, 2, BF16, max_length=longest), case, q, 2, BF16)
+
+
+@pytest.mark.parametrize("longest", (None, LOOKS_LONG))
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (256, F32)])
+def test_attention_gives_equal_bits_again(gpu_runtime, dim, dtype, longest):
+    case = Case(dim, 2, [900, 333], [300, 1], dtype, seed=14).history(78)
+    q = _rounded(oracle.normal(20, (case.rows, 8, dim)), dtype)
+    first, second = (_attend(gpu_runtime, case, q, 4, dtype, max_length=longest) for _ in range(2))
+    assert np.array_equal(first, second)
 
 
 @pytest.mark.parametrize("dim", (64, 128, 256))
