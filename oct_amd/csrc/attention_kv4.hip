@@ -561,7 +561,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
 // one's products are beside the other's softmax.  P goes to bf16, 8 bits, as
 // many as the output has (fp32 rows: three terms, as for the queries).  Bound by the matrix and vector units together, which
 // two waves of a SIMD share less well than they could: four prompts of 1024 rows over up to 8000
-// tokens, 8 key heads of 128, groups of 4, bf16: 302 us for the call, 0.79 PFLOP/s (170 us at the rate of a
+// tokens, 8 key heads of 128, groups of 4, bf16: 305 us for the call, 0.78 PFLOP/s (170 us at the rate of a
 // large product).  Another such call's 350 us, a part at a time: 65 without any of the four, 45 more with the
 // loads, and beside these 35 with turning the codes, 78 with softmax, 153 with the products.
 template <bool kF32, int D>
