@@ -985,8 +985,8 @@ PROM_REACTOR_API int prometheus_reactor_runtime_kv4_read_device(void* handle, co
    longest sequence) size the launch; results do not depend on them beyond rounding, and
    longer sequences are still computed whole.  Scores, softmax and sums are fp32; fp32
    rows enter the products unrounded, probabilities with 24 significant bits (bf16 rows:
-   8 to 16).  Sums are divided by the weights at the end: values whose magnitudes sum to
-   more than 2^119 over a row's tokens may give infinities.  Equal calls give equal bits. */
+   16).  Sums are divided by the weights at the end: values whose magnitudes sum to more
+   than 2^119 over a row's tokens may give infinities.  Equal calls give equal bits. */
 typedef struct PrometheusKv4AttentionRequest {
   uint32_t struct_size;
   uint32_t dtype;

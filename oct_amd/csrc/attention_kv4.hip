@@ -51,12 +51,12 @@ constexpr float kLazyLog2 = 8.0f;
 constexpr int kTileRows = 16;
 constexpr int kWaves = 4;
 // Sequences of up to kFewPairs pairs (rows times query heads of a group) stay on the kernel for few
-// rows, whatever the call: a prompt tile has 128 or 256.  The prompts' kernel costs 40 to 80 us before
+// rows, whatever the call: a prompt tile has 128 or 256.  The prompts' kernel costs 40 to 85 us before
 // it does much and then takes half the time for a page of 16 pairs, so it is taken from so many of
-// them on (us with it / without, two prompts over 4096 tokens, 4 key heads, groups of 4; 256 new rows
-// each, 32768 pages of 16 pairs: bf16 64 channels 43 / 31, 128 54 / 51, 256 98 / 118, fp32 52 / 35,
-// 68 / 63; 512 new rows: 47 / 52, 62 / 92, 135 / 222, 62 / 61, 97 / 115).  fp32 rows of 256 channels do
-// not fit its registers (310 / 409).
+// them on (us with it / without, two prompts over up to 4096 tokens, 4 key heads, groups of 4; 256 and 118
+// rows, 24064 pages of 16 pairs: bf16 64 channels 43 / 29, 128 56 / 49, 256 103 / 118, fp32 50 / 34,
+// 65 / 62; 512 and 236 rows, 47872 pages: 48 / 50, 65 / 90, 147 / 222, 59 / 58, 94 / 114).  fp32 rows of
+// 256 channels do not fit its registers (310 / 409).
 constexpr uint64_t kFewPairs = 64;
 constexpr uint64_t prompt_work(int head_dim) { return head_dim == 256 ? 24000 : 40000; }
 constexpr int kMaxSplits = 64;  // a lane each when they are joined
@@ -558,12 +558,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_bf16, the V^T operand by transpose reads.
 // The next page's codes are loaded into registers before a page is worked on and turned into the
 // other half of LDS after it.  Of eight waves, the second of each SIMD runs half a page behind the first:
-// one's products are beside the other's softmax.  P goes to bf16, 8 bits, as
-// many as the output has (fp32 rows: three terms, as for the queries).  Bound by the matrix and vector units together, which
-// two waves of a SIMD share less well than they could: four prompts of 1024 rows over up to 8000
-// tokens, 8 key heads of 128, groups of 4, bf16: 305 us for the call, 0.78 PFLOP/s (170 us at the rate of a
-// large product).  Another such call's 350 us, a part at a time: 65 without any of the four, 45 more with the
-// loads, and beside these 35 with turning the codes, 78 with softmax, 153 with the products.
+// one's products are beside the other's softmax.  P goes into the products as two bf16 terms (fp32 rows
+// and their queries: three), as in the kernel for few rows, so that a call's precision does not
+// depend on which of the two takes its sequences.  One term, 8 bits, was as far from 64 bits again as the
+// results' own rounding is (2.3e-3 of the values instead of 1.7e-3), and 308 us instead of the 381 below.
+// Bound by the matrix and vector units together, which two waves of a SIMD share less well than they
+// could: four prompts of 1024 rows over up to 8000 tokens, 8 key heads of 128, groups of 4, bf16: 381 us for the
+// call, 0.63 PFLOP/s of the definition's operations and half as many again for the second term (170 us at the rate of
+// a large product).  A call of 350 us with one term, a part at a time: 65 without any of the four, 45 more with
+// the loads, and beside these 35 with turning the codes, 78 with softmax, 153 with the products.
 template <bool kF32, int D>
 struct Prompt {
   static constexpr int kWaves = kPromptWaves<kF32, D>;
@@ -678,7 +681,7 @@ __device__ __forceinline__ uint64_t first_unit(uint64_t total, uint64_t w, uint6
 template <bool kF32, int D>
 __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWaves / 4)) void kv4_prompt_kernel(const Kv4Kernel g) {
   using Pr = Prompt<kF32, D>;
-  constexpr int kG = D / 64, kT = kF32 ? 3 : 1;
+  constexpr int kG = D / 64, kT = kF32 ? 3 : 1, kPT = kF32 ? 3 : 2;
   constexpr int kSteps = D / 16;  // MFMA steps of 16 channels
   constexpr int kB = D / 32;      // blocks of 32 output channels
   __shared__ __attribute__((aligned(1024))) uint8_t key_lds[2][Pr::kTileBytes], value_lds[2][Pr::kTileBytes];
@@ -755,7 +758,7 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
     };
     typename Pr::Codes codes;
     floatx16 s[2];
-    bf16x8 p[4][kT];
+    bf16x8 p[4][kPT];
     // The matrix phase: O += V P of the page before and S = K Q of this one, in quads of four
     // operand reads and the instructions that use them; a quad is read while the one before it is
     // multiplied.  Operand e of the output: block e % kB of tokens 16 (e / kB) + 4 hi + 0..3 and 8
@@ -781,12 +784,12 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int e = 4 * (quad % kB) + i;
+        if (quad < kB) {
 #pragma unroll
-        for (int j = 0; j < kT; ++j) {
-          if (quad < kB)
-            o[e % kB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], p[e / kB][j], o[e % kB], 0, 0, 0);
-          else
-            s[e % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], q[e / 2][j], s[e % 2], 0, 0, 0);
+          for (int j = 0; j < kPT; ++j) o[e % kB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], p[e / kB][j], o[e % kB], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kT; ++j) s[e % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], q[e / 2][j], s[e % 2], 0, 0, 0);
         }
       }
     };
@@ -838,10 +841,10 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
         for (int j = 0; j < 8; ++j) {
           const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c & 1) + j], g.scale_log2, -m_log2));
           l_run += e;
-          __bf16 t[kT];
+          __bf16 t[kPT];
           terms(e, t);
 #pragma unroll
-          for (int i = 0; i < kT; ++i) p[c][i][j] = t[i];
+          for (int i = 0; i < kPT; ++i) p[c][i][j] = t[i];
         }
       // Values that are not finite are left out of an edge page: the rows that see them get NaN.
       if (!bad && page_edge(pg, number)) {
@@ -883,7 +886,7 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int i = 0; i < kT; ++i) p[c][i] = bf16x8{};  // before the first page, with values of 0
+        for (int i = 0; i < kPT; ++i) p[c][i] = bf16x8{};  // before the first page, with values of 0
       for (int n = 0; n < pages; ++n) {
         const uint32_t value_number = behind ? n1 : n0;
         Pr::load(codes, page_block(behind ? n2 : n1), page_block(value_number), tid);

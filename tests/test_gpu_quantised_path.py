@@ -753,3 +753,25 @@ def test_calls_from_two_threads(gpu_runtime):
 
     with ThreadPoolExecutor(2) as pool:
         assert all(pool.map(run, (1, 2)))
+
+
+# ------------------------------------------------------------------ bits of the probabilities
+@pytest.mark.parametrize("longest", (None, LOOKS_LONG))
+@pytest.mark.parametrize("dim", (64, 128, 256))
+def test_attention_of_bf16_rows_carries_16_bits_of_the_probabilities(gpu_runtime, dim, longest):
+    """With either kernel, so that the launch hints do not choose the precision.  A probability is cut to eight bits and
+    the rest, below 2^-7 of it, rounded to eight: off by at most 2^-7 * 2^-8 = 2^-15.  Beside that and what fp32 sums
+    add (see above) a result is off by its own rounding alone, half the distance of its neighbours.  Small queries
+    keep the fp32 part below 2^-15 (eight-bit probabilities are off by up to 2^-8, about 1e-4 of W here)."""
+    case = Case(dim, 1, [260], [200], BF16, seed=21).history(79)
+    q = _rounded(oracle.normal(22, (case.rows, 1, dim), 0.0, 0.05), BF16)
+    got = _attend(gpu_runtime, case, q, 1, BF16, max_length=longest).astype(np.float64)
+    worst = 0.0
+    for row, seq, pos in case.places():
+        ref, size, reach = oq.attention(q[row].astype(np.float64), case.k[seq], case.v[seq], pos, float(np.float32(dim ** -0.5)))
+        rel = 2 * (dim + 16) * 2.0 ** -24 * (1 + reach[:, None]) + 2.0 ** -21 + ((pos + 1) / 16 + 64) * 2.0 ** -24
+        off = (rel + 2.0 ** -15) * size
+        half = 2.0 ** (np.floor(np.log2(np.abs(ref) + off)) - 8)
+        err = np.abs(got[row] - ref)
+        worst = max(worst, float((err / (half + off)).max()))
+    assert worst <= 1.0, worst
