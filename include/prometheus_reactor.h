@@ -892,7 +892,8 @@ PROM_REACTOR_API int prometheus_reactor_runtime_dit_block_bf16_device(void* hand
 enum { PROM_DTYPE_F32 = 0u, PROM_DTYPE_BF16 = 1u };
 
 /* q[r, c] = rint(x[r, c] / s[r]), s[r] = max_c |x[r, c]| / 127, each operation
-   rounded to fp32 (halves to even), so |q| <= 127.  input: dtype [rows, width]
+   rounded to fp32 (halves to even), and held within -127..127 (only a scale below
+   2^-142, whose rounding is coarse, gives quotients past that).  input: dtype [rows, width]
    with input_row_stride >= width elements between rows, any alignment of its
    type; output int8 [rows, width] and scales fp32 [rows], contiguous.  A row of
    zeros has scale 0 and zeros; a row with an infinity or a NaN has scale NaN and

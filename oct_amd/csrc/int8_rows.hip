@@ -1,4 +1,4 @@
-// Rows quantised to 8-bit integers: q = rint(x / s), s = max |x| / 127, a row's
+// Rows quantised to 8-bit integers: q = rint(x / s) within -127..127, s = max |x| / 127, a row's
 // own scale (the operand of the int8 product, gemm_int8.hip).
 //
 // Bound by memory: a row is read once into registers, reduced, and written as
@@ -54,8 +54,9 @@ __device__ __forceinline__ void store8(int8_t* p, long long left, const float (&
 #pragma unroll
     for (int j = 0; j < 8; ++j) q[j] = (int)__builtin_rintf(s(v[j]));
   } else {
+    // A scale of few units of 2^-149 may have been rounded down by up to a third: quotients past 127 are held there.
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = s.s > 0.0f ? (int)__builtin_rintf(v[j] / s.s) : 0;
+    for (int j = 0; j < 8; ++j) q[j] = s.s > 0.0f ? (int)fminf(fmaxf(__builtin_rintf(v[j] / s.s), -127.0f), 127.0f) : 0;
   }
   if (left >= 8) {
     u32x2 w;

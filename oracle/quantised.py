@@ -11,13 +11,14 @@ NAMES = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
 
 
 def quantize_rows(x: np.ndarray):
-    """int8 rows and fp32 scales of fp32 rows."""
+    """int8 rows and fp32 scales of fp32 rows.  A scale of few units of 2^-149 may have been rounded down by up to
+    a third: quotients past 127 are held there."""
     x = np.asarray(x, np.float32)
     finite = np.isfinite(x).all(-1)
     top = np.abs(np.where(finite[:, None], x, 0.0)).max(-1).astype(np.float32)
     scale = top / np.float32(127.0)
     with np.errstate(divide="ignore", invalid="ignore"):
-        q = np.rint(x / scale[:, None])
+        q = np.clip(np.rint(x / scale[:, None]), -127.0, 127.0)
     q = np.where(finite[:, None] & (scale[:, None] > 0.0), q, 0.0)
     return q.astype(np.int8), np.where(finite, scale, np.float32(np.nan)).astype(np.float32)
 

@@ -20,6 +20,7 @@ import pytest
 import oracle
 from oracle import quantised as oq
 from oct_amd import prometheus as p
+from tests.test_quantised_path import smallest_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -113,6 +114,13 @@ def test_rows_at_borders_and_special_values(gpu_runtime):
     eq, es = oq.quantize_rows(x)
     assert np.array_equal(s, es, equal_nan=True)
     assert np.array_equal(q, eq)
+
+
+def test_rows_of_the_smallest_numbers(gpu_runtime):
+    x, q, scale = smallest_rows()
+    got, got_scale = _quantise_rows(gpu_runtime, x, F32)
+    assert np.array_equal(got_scale, scale)
+    assert np.array_equal(got, q)
 
 
 def _beside(x):

@@ -37,6 +37,27 @@ def test_cache_values_stay_within_a_step():
     assert np.array_equal(oracle.from_bf16(oracle.to_bf16(v.astype(np.float32))).astype(np.float64), v)
 
 
+def smallest_rows():
+    """Rows of whole multiples of 2^-149, whose scales are such multiples too, and by whole numbers what they become:
+    the scale is m / 127 rounded to a multiple, x / scale is rounded to fp32 and then to a whole number, which is
+    held within 127.  m runs over all that a scale so small can make larger than that, and their neighbours."""
+    m = np.arange(1, 17000, dtype=np.int64)
+    units = np.stack([m, -m, m - 1, -(m * 2 // 3), m // 2, m * 0 + 1, m * 0, m // 64], -1)
+    scale = (2 * m + 127) // 254  # no ties: 127 is odd
+    quotient = (units / np.maximum(scale, 1)[:, None]).astype(np.float32).astype(np.float64)
+    q = np.where(scale[:, None] > 0, np.clip(np.rint(quotient), -127, 127), 0).astype(np.int64)
+    unit = 2.0 ** -149
+    return (units * unit).astype(np.float32), q, (scale * unit).astype(np.float32)
+
+
+def test_rows_of_the_smallest_numbers_keep_their_sign_and_range():
+    x, q, scale = smallest_rows()
+    got, got_scale = oq.quantize_rows(x)
+    assert np.array_equal(got_scale, scale)
+    assert np.all(got[x > 0] >= 0) and np.all(got[x < 0] <= 0) and got.min() == -127 and got.max() == 127
+    assert np.array_equal(got, q)
+
+
 def test_cache_ties_go_to_the_even_code():
     x = np.zeros((1, 64), np.float32)
     x[0, :9] = [6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -5.0]  # step 1
