@@ -921,8 +921,9 @@ PROM_REACTOR_API int prometheus_reactor_runtime_gemm_int8_device(void* handle, c
    rounded to fp32 and then up to six significant bits, and per channel the nearest
    of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives to x / s (rounded to fp32;
    halfway to the even code); it stands for s times that, which fp32 and bf16 hold
-   exactly (6 s of magnitudes above 2^128 * 32 / 33 may be infinite), at most s away
-   from x.  A group with an infinity or a NaN reads back as NaN.
+   exactly, at most s away from x (of magnitudes above 2^128 * 32 / 33, 6 s is past fp32's
+   range: reads give an infinity, attention may take 85 / 86 of s).  A group with an
+   infinity or a NaN reads back as NaN.
    A page is kv_heads blocks of head_dim * 64 + head_dim * 4 bytes: the keys' codes
    [64][head_dim / 2], the values' codes, the keys' steps [head_dim / 64][64] and the
    values'.  A code is a sign (8) and the place 0..7 of the magnitude above; a byte
@@ -987,7 +988,7 @@ PROM_REACTOR_API int prometheus_reactor_runtime_kv4_read_device(void* handle, co
    longer sequences are still computed whole.  Scores, softmax and sums are fp32; fp32
    rows enter the products unrounded, probabilities with 24 significant bits (bf16 rows:
    16).  Sums are divided by the weights at the end: values whose magnitudes sum to more
-   than 2^119 over a row's tokens may give infinities.  Equal calls give equal bits. */
+   than 2^119 over a row's tokens may give infinities or NaN.  Equal calls give equal bits. */
 typedef struct PrometheusKv4AttentionRequest {
   uint32_t struct_size;
   uint32_t dtype;

@@ -609,8 +609,10 @@ struct Prompt {
       c.step[i] = *reinterpret_cast<const uint16_t*>(block + Stage<D>::kSteps + 128 * (group_of(keys, b) + (keys ? 0 : D / 64)) + 2 * t);
     }
   }
-  // Codes to bf16 in LDS.  Values of an edge page: those from token zero_from of the page on, and
-  // those that are not finite, count as 0 (some row does not see them).
+  // Codes to bf16 in LDS.  Values of an edge page, whose tokens some row does not see: those from token
+  // zero_from of the page on, and those whose step is not finite, count as 0.  The one step that is larger than
+  // kMostStep, 86 / 85 of it, would give infinities, and these NaN with a probability of 0.
+  static constexpr int kMostStep = 0x7E2A0000;  // the largest that bf16 holds six of
   __device__ static __forceinline__ void store(const Codes& c, uint8_t* key_lds, uint8_t* value_lds, int tid, bool edge,
                                                int zero_from) {
 #pragma unroll
@@ -619,7 +621,8 @@ struct Prompt {
       int t, b;
       unit(i, tid, &keys, &t, &b);
       uint32_t step = c.step[i] << 16;
-      if (edge && !keys && (t >= zero_from || (step & 0x7F800000u) == 0x7F800000u)) step = 0;
+      if (edge && !keys)
+        step = t >= zero_from || (step & 0x7F800000u) == 0x7F800000u ? 0u : (uint32_t)min((int)step, kMostStep);
       const float s = __uint_as_float(step);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {

@@ -672,6 +672,36 @@ def test_attention_to_values_that_are_not_finite(gpu_runtime, longest, dtype, wi
         assert np.isnan(got[row, :, 64:]).all() if spoilt else np.isfinite(got[row, :, 64:]).all(), pos
 
 
+# With a window max_length alone does not: a call looks as long as max_rows and the window.  Rows that no sequence
+# has make it look like work for the prompts' kernel, if max_rows counts them.
+IDLE_ROWS = 8000
+
+
+@pytest.mark.parametrize("idle", (0, IDLE_ROWS))
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("window,at", [(0, 150), (0, 199), (20, 105), (20, 150)])
+def test_attention_to_values_at_the_end_of_the_range(gpu_runtime, idle, dtype, window, at):
+    """Six steps of a group of magnitudes above 2^128 * 32 / 33 are past fp32's range, though the step is not: rows
+    that do not see the token (before it, or with a window that has left it behind) are as without it."""
+    case = Case(128, 1, [200], [100], dtype, seed=6, extra_rows=idle).history(32)
+    v = np.ones((1, 128), np.float32)
+    v[0, 64:] = _rounded(np.linspace(-3.385e38, 3.385e38, 64).astype(np.float32), dtype)
+    case.cache.store(case.table[0, at // 64], at % 64, np.ones((1, 128), np.float32), v)
+    case.k[0][at], case.v[0][at] = 1.0, oq.kv4_values(*oq.kv4_quantise(v))
+    assert np.abs(case.v[0][at]).max() > np.finfo(np.float32).max
+    q = _rounded(oracle.normal(9, (case.rows, 1, 128)), dtype)
+    got = _attend(gpu_runtime, case, q, 1, dtype, window, max_rows=case.rows, max_length=LOOKS_LONG if idle else None)
+    sees = np.zeros(case.rows, bool)
+    for row, _, pos in case.places():
+        sees[row] = at <= pos and (not window or pos - window < at)
+    assert np.isfinite(got[:, :, :64]).all() and np.isfinite(got[~sees]).all() and sees.any() and not sees[:100].all()
+    case.v[0][at] = 0.0  # what the other rows are held to has it nowhere
+    got[sees] = 9.0
+    places = [x for x in case.places() if not sees[x[0]]]
+    case.places = lambda: iter(places)
+    _check_attention(got, case, q, 1, dtype, window)
+
+
 # ------------------------------------------------------------------ a step of the whole path
 @pytest.mark.parametrize("dtype", (F32, BF16))
 def test_decode_step(gpu_runtime, dtype):
