@@ -954,7 +954,8 @@ PROM_REACTOR_API uint64_t prometheus_reactor_kv4_page_bytes(uint32_t head_dim, u
 
 /* Rows of the last tokens of each sequence: rows row_starts[i] .. row_starts[i+1] - 1
    (row_starts [sequences + 1], not decreasing) are sequence i's last tokens, the last
-   row its token lengths[i] - 1.  k and v: dtype [rows, kv_heads, head_dim] with
+   row its token lengths[i] - 1.  Row starts may lie below 0 or past `rows`: a row that the
+   call has keeps its position, the others are passed over.  k and v: dtype [rows, kv_heads, head_dim] with
    row_stride >= kv_heads * head_dim elements between rows (so that they may be columns
    of one projection's output), any alignment of their type.  Rows outside every
    sequence, or before its token 0, are passed over: not stored by a write, left as they

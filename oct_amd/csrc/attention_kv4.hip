@@ -92,14 +92,16 @@ struct Kv4Kernel {
 
 typedef const __attribute__((address_space(4))) int32_t Constant;
 
-// A sequence's rows (within the call's) and length.
+// A sequence's rows (those of the call's) and the first one's position, counted back from its length
+// and the end of its rows, wherever that lies.
 struct Sequence {
-  int first, n, length;
+  int first, n, from;
   __device__ __forceinline__ Sequence(const Kv4Kernel& g, int seq) {
     Constant* starts = (Constant*)g.starts;
+    const int end = starts[seq + 1];
     first = min(max(starts[seq], 0), g.rows);
-    n = min(max(starts[seq + 1], 0), g.rows) - first;
-    length = max(((Constant*)g.c.lengths)[seq], 0);
+    n = min(max(end, 0), g.rows) - first;
+    from = max(((Constant*)g.c.lengths)[seq], 0) - (max(end, first) - first);
   }
 };
 
@@ -122,9 +124,9 @@ struct Sees {
 struct Tile {
   int pos0, pos1, page0, last, splits;
   __device__ __forceinline__ Tile(const Kv4Kernel& g, const Sequence& s, int tile, int tile_rows = kTileRows) {
-    const int x0 = tile * tile_rows, from = s.length - s.n;
-    pos0 = from + g.over_group(x0);
-    pos1 = from + g.over_group(min(x0 + tile_rows, s.n * g.group) - 1);
+    const int x0 = tile * tile_rows;
+    pos0 = s.from + g.over_group(x0);
+    pos1 = s.from + g.over_group(min(x0 + tile_rows, s.n * g.group) - 1);
     page0 = g.window && pos0 >= g.window ? min((pos0 - g.window + 1) / kKv4Page, g.c.table_stride) : 0;
     last = pos1 < 0 ? 0 : min(pos1 / kKv4Page, g.c.table_stride) + 1;
     splits = min(g.splits, max(1, (last - page0 + (1 << g.split_shift) - 1) >> g.split_shift));
@@ -316,7 +318,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
     const bool mine = x < pairs;
     const int row = mine ? g.over_group(x) : 0;
     const int q_head = head * g.group + (mine ? x - row * g.group : 0);
-    const int pos = mine ? sq.length - sq.n + row : tl.pos1;  // its position
+    const int pos = mine ? sq.from + row : tl.pos1;  // its position
     const int page0 = tl.page0, last = tl.last;
 
     // Q^T operand: lane (h, row), step s: channels 32 s + 8 h .. + 7.  Loaded here, used when the first
@@ -710,7 +712,7 @@ __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWav
     const bool mine = x < pairs;
     const int row = mine ? g.over_group(x) : 0;
     const int q_head = head * g.group + (mine ? x - row * g.group : 0);
-    const int from = sq.length - sq.n;
+    const int from = sq.from;
     const int wave0 = from + g.over_group(min(x0, pairs - 1)), wave1 = from + g.over_group(min(x0 + 32, pairs) - 1);
     const int pos = mine ? from + row : wave1;
 

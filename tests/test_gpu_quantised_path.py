@@ -576,6 +576,57 @@ def test_attention_equals_the_definition(gpu_runtime, index, dtype, longest):
     _check_attention(got, case, q, group, dtype, window)
 
 
+@pytest.mark.parametrize("longest", (None, LOOKS_LONG))
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("dim,lengths,new,first,rows,window", [
+    (128, [100, 70], [8, 15], 0, 12, 0),          # the last sequence's rows end behind the call's
+    (64, [400, 600], [10, 490], 3, 250, 0),       # and its first sequence's begin before them
+    (256, [90, 2000, 40], [2, 1, 9], 1, 4, 0),
+    (64, [300, 900], [130, 500], 90, 440, 50)])
+def test_rows_that_a_call_has_not_all_of(gpu_runtime, dim, lengths, new, first, rows, window, dtype, longest):
+    """Row starts below 0 and past `rows`: the positions of the rows that the call has do not depend on that, for
+    writing and reading as for attention."""
+    case = Case(dim, 2, lengths, new, dtype, seed=31).history(90)
+    case.starts, case.rows = case.starts - first, rows
+    assert case.starts[0] <= 0 and case.starts[-1] > rows
+    all_places = list(case.places())
+    places = [x for x in all_places if 0 <= x[0] < rows]
+    case.places = lambda: iter(places)
+    # the rows' keys and values are other ones than the cache holds there
+    k, v = _rows_of(case, 41), _rows_of(case, 42)
+    before = case.cache.pool.copy()
+    for row, seq, pos in places:
+        kk, vv = k[row].reshape(2, dim), v[row].reshape(2, dim)
+        case.cache.store(case.table[seq, pos // oq.PAGE], pos % oq.PAGE, kk, vv)
+        case.k[seq][pos], case.v[seq][pos] = (oq.kv4_values(*oq.kv4_quantise(x)) for x in (kk, vv))
+    with Device(gpu_runtime) as dev:
+        pool = dev.up(before)
+        handle, starts = case.handle(dev, pool), dev.up(case.starts)
+        gpu_runtime.kv4_write_device(handle, dev.up(_bits(k, dtype)), dev.up(_bits(v, dtype)), starts, rows, 2 * dim, dtype)
+        out = _bits(np.zeros_like(k), dtype)
+        do = dev.up(out)
+        gpu_runtime.kv4_read_device(handle, do, None, starts, rows, 2 * dim, dtype)
+        got_pool, read = dev.down(before, pool), _values(dev.down(out, do), dtype)
+    assert np.array_equal(got_pool, case.cache.pool)
+    for row, seq, pos in places:
+        assert np.array_equal(read[row], case.k[seq][pos].reshape(-1)), row
+    q = _rounded(oracle.normal(43, (rows, 8, dim)), dtype)
+    got = _attend(gpu_runtime, case, q, 4, dtype, window, max_rows=rows if longest else min(rows, max(new)), max_length=longest)
+    # As _check_attention, but for what underflows: scores are up to hundreds apart here, and where the token that
+    # wins holds a 0 the result is what the others leave.  Relative to a running maximum, which the largest may pass
+    # by 2^8, factors below 2^-126 count as 0 (a probability's, a step's times it, or the one that sums so far,
+    # of probabilities up to 2^8, are scaled with): less than 2^-117 |v| a token, divided by weights of 1 or more.
+    for row, seq, pos in places:
+        ref, size, reach = oq.attention(q[row].astype(np.float64), case.k[seq], case.v[seq], pos,
+                                        float(np.float32(dim ** -0.5)), window)
+        rel = 2 * (dim + 16) * 2.0 ** -24 * (1 + reach[:, None]) + 2.0 ** -21 + ((pos + 1) / 16 + 64) * 2.0 ** -24
+        tol = (rel + (2.0 ** -8 if dtype == BF16 else 0.0)) * size + (2.0 ** -8 if dtype == BF16 else 2.0 ** -24) * np.abs(ref)
+        tol += (pos + 1) * 2.0 ** -117 * max(6.0, np.abs(case.v[seq]).max())
+        assert np.all(np.abs(got[row] - ref) <= tol), (row, seq, pos)
+    mine = np.isin(np.arange(rows), [x[0] for x in places])
+    assert np.all(got[~mine] == 9.0)
+
+
 @pytest.mark.parametrize("dim", (64, 128, 256))
 def test_attention_peaked_and_large_scores(gpu_runtime, dim):
     """Scores of hundreds, which one token wins, and a maximum that keeps growing along the sequence."""
