@@ -532,7 +532,7 @@ __global__ __launch_bounds__(64 * kWaves) void gemm_int8_rows_kernel(const Int8A
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int col = n0 + 4 * h + r;
-      if (col < g.n) store_scaled(static_cast<TOut*>(g.c) + (size_t)row * g.n + col, acc[i][r], as, g.w_scale[col]);
+      if (col < g.n) store_scaled(static_cast<TOut*>(g.c) + (size_t)row * g.ldc + col, acc[i][r], as, g.w_scale[col]);
     }
   }
 }
@@ -646,7 +646,7 @@ int plan_tiles(uint32_t m, uint32_t n, uint32_t k, Plan (&plan)[2]) {
 }
 
 template <typename TOut>
-hipError_t launch_rows(const Int8Args& g, hipStream_t stream) {
+hipError_t launch_rows(Int8Args g, hipStream_t stream) {
 #define ROWS(MT, W)                                                                          \
   hipLaunchKernelGGL((gemm_int8_rows_kernel<MT, W, TOut>), dim3((unsigned)((g.n + 15) / 16), \
                      (unsigned)((g.m + 16 * MT - 1) / (16 * MT))), dim3(64 * W), 0, stream, g)
@@ -654,20 +654,29 @@ hipError_t launch_rows(const Int8Args& g, hipStream_t stream) {
   // 5.6; 1x12288x4096 9.4, 10.6, 12.1; 1x2048x8192 6.0, 5.3, 5.5; 15x2048x16384 -, 11.8, 10.7; 16x2048x65536
   // 38, 28, 27; 16 do not fit LDS with 32 rows).
   const int waves = g.n >= 16 * 1024 || g.k <= 4096 ? 4 : g.m > 16 || g.n > 4096 || g.k <= 8192 ? 8 : 16;
-  if (g.m > 16) {
-    if (waves == 4)
-      ROWS(2, 4);
-    else
-      ROWS(2, 8);
-  } else if (waves == 4) {
-    ROWS(1, 4);
-  } else if (waves == 8) {
-    ROWS(1, 8);
-  } else {
-    ROWS(1, 16);
+  // A launch has fewer than 2^32 threads: more than 2^27 columns (four waves take 16) go in blocks.
+  for (int left = g.n; left > 0; left -= g.n) {
+    g.n = std::min(left, 1 << 27);
+    if (g.m > 16) {
+      if (waves == 4)
+        ROWS(2, 4);
+      else
+        ROWS(2, 8);
+    } else if (waves == 4) {
+      ROWS(1, 4);
+    } else if (waves == 8) {
+      ROWS(1, 8);
+    } else {
+      ROWS(1, 16);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    g.w += (size_t)g.n * g.k;
+    g.w_scale += g.n;
+    g.c = static_cast<TOut*>(g.c) + g.n;
   }
 #undef ROWS
-  return hipGetLastError();
+  return hipSuccess;
 }
 
 constexpr uint32_t kFewRows = 32;
@@ -675,9 +684,9 @@ constexpr uint32_t kFewRows = 32;
 template <typename TOut>
 hipError_t launch(Int8Args g, hipStream_t stream) {
   const uint32_t m = (uint32_t)g.m, n = (uint32_t)g.n, k = (uint32_t)g.k;
+  g.ldc = g.n;
   if (m <= kFewRows) return launch_rows<TOut>(g, stream);
   g.lda = g.ldw = g.k;
-  g.ldc = g.n;
   const bool aligned = k % 16 == 0 && ((uintptr_t)g.a & 15u) == 0 && ((uintptr_t)g.w & 15u) == 0;
   if (!aligned) {
     const int ld = (int)((k + 15) & ~15u);

@@ -249,6 +249,35 @@ def test_product_of_operands_past_4_gib(gpu_runtime, m, n):
         _check_product(out[:, -last:], other, tail, one, scale[-last:], F32)
 
 
+@pytest.mark.parametrize("m,n,k", [(2, (1 << 28) + 37, 3), (1, 1 << 30, 1), (1 << 30, 1, 3)])
+def test_product_of_very_long_sides(gpu_runtime, m, n, k):
+    """More columns than one launch of the kernel for few rows takes, and the most columns and rows: the last ones, and
+    those where a launch ends (what lies elsewhere is not looked at)."""
+    rt, long, short, span = gpu_runtime, max(m, n), min(m, n), 64
+    edges = [at for at in (0, (1 << 27) - 32, (1 << 28) - 32) if at + 2 * span <= long] + [long - span]
+    tail, other = _whole(1, (span, k)), _whole(2, (short, k))
+    scale, one = oracle.uniform(3, (span,), 0.001, 0.002), oracle.uniform(4, (short,), 0.001, 0.002)
+    with Device(rt) as dev:
+        wide, scales, out = rt.alloc(long * k), rt.alloc(long * 4), rt.alloc(m * n * 2)
+        dev.held += [wide, scales, out]
+        for at in edges:
+            rt.upload(wide + at * k, tail)
+            rt.upload(scales + at * 4, scale)
+        narrow, ones = dev.up(other), dev.up(one)
+        if m > n:
+            rt.gemm_int8_device(wide, narrow, scales, ones, out, m, n, k, BF16)
+        else:
+            rt.gemm_int8_device(narrow, wide, ones, scales, out, m, n, k, BF16)
+        rt.synchronize()
+        for at in edges:
+            if m > n:
+                got = _values(rt.download(np.empty((span, n), np.uint16), out + at * n * 2), BF16)
+                _check_product(got, tail, other, scale, one, BF16)
+            else:
+                got = [rt.download(np.empty(span, np.uint16), out + (row * n + at) * 2) for row in range(m)]
+                _check_product(_values(np.stack(got), BF16), other, tail, one, scale, BF16)
+
+
 # ------------------------------------------------------------------ the cache
 class Case:
     """A paged cache on the host and on the device, with the rows that a call brings."""

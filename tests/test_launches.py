@@ -1,5 +1,6 @@
 """Launches that the host code chooses, recorded on the CPU (recorded_launches.h): the grids
-of the row kernels for very many rows, and the kernel of the decoder layer's GeGLU product."""
+of the row kernels for very many rows and of the int8 product for very many columns, and the kernel of
+the decoder layer's GeGLU product."""
 import subprocess
 from pathlib import Path
 
@@ -36,6 +37,22 @@ def geglu_check(tmp_path_factory):
                                         ((1 << 22) - 1, 8192), (1 << 22, 4100), (5 << 21, 5000), (1 << 26, 256)])
 def test_every_row_is_launched(rows_check, rows, width):
     proc = subprocess.run([str(rows_check), str(rows), str(width)], capture_output=True, text=True, timeout=60)
+    assert proc.returncode == 0, proc.stdout + proc.stderr
+
+
+@pytest.fixture(scope="module")
+def int8_check(tmp_path_factory):
+    return compiled(tmp_path_factory.mktemp("int8_launches") / "check", "int8_launch_check.cpp")
+
+
+# few rows: a workgroup of 256 threads takes 16 columns, 2^28 columns are 2^32 threads; many rows: 2^30 of
+# them in tiles of 64 would be as many
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 32768, 2048), (16, 2048, 65536), (32, 1 << 27, 31), (1, (1 << 27) + 1, 5),
+                                   (1, (1 << 28) - 16, 4), (1, (1 << 28) - 15, 4), (15, (1 << 28) + 5, 15),
+                                   (3, 1 << 30, 3), (7, 600000000, 7), (33, 130150523, 33), (1 << 30, 1, 1),
+                                   (1 << 30, 3, 3), ((1 << 30) - 64, 2, 1), (4224, 20480, 3840), (2009, 8627, 1177)])
+def test_every_column_of_an_int8_product_is_launched(int8_check, m, n, k):
+    proc = subprocess.run([str(int8_check), str(m), str(n), str(k)], capture_output=True, text=True, timeout=60)
     assert proc.returncode == 0, proc.stdout + proc.stderr
 
 
