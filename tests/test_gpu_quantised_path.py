@@ -20,7 +20,7 @@ import pytest
 import oracle
 from oracle import quantised as oq
 from oct_amd import prometheus as p
-from tests.test_quantised_path import smallest_rows
+from tests.test_quantised_path import PLANNED, smallest_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -654,6 +654,15 @@ def test_rows_that_a_call_has_not_all_of(gpu_runtime, dim, lengths, new, first, 
         assert np.all(np.abs(got[row] - ref) <= tol), (row, seq, pos)
     mine = np.isin(np.arange(rows), [x[0] for x in places])
     assert np.all(got[~mine] == 9.0)
+
+
+@pytest.mark.parametrize("name,dtype,dim,heads,group,lengths,new,window,plan", PLANNED, ids=[c[0] for c in PLANNED])
+def test_attention_as_planned(gpu_runtime, name, dtype, dim, heads, group, lengths, new, window, plan):
+    """Truthful hints: every split has pages, joins have all of them to add, beside pieces of prompts too."""
+    case = Case(dim, heads, lengths, new, dtype, seed=len(name)).history(len(name) + 60)
+    q = _rounded(oracle.normal(len(name) + 7, (case.rows, heads * group, dim), 0.0, 1.5), dtype)
+    got = _attend(gpu_runtime, case, q, group, dtype, window)
+    _check_attention(got, case, q, group, dtype, window)
 
 
 @pytest.mark.parametrize("dim", (64, 128, 256))

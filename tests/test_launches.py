@@ -7,6 +7,8 @@ from pathlib import Path
 import pytest
 
 from oct_amd import build
+from oct_amd import prometheus as p
+from tests.test_quantised_path import PLANNED
 
 HERE = Path(__file__).resolve().parent
 
@@ -54,6 +56,20 @@ def int8_check(tmp_path_factory):
 def test_every_column_of_an_int8_product_is_launched(int8_check, m, n, k):
     proc = subprocess.run([str(int8_check), str(m), str(n), str(k)], capture_output=True, text=True, timeout=60)
     assert proc.returncode == 0, proc.stdout + proc.stderr
+
+
+@pytest.fixture(scope="module")
+def kv4_check(tmp_path_factory):
+    return compiled(tmp_path_factory.mktemp("kv4_plans") / "check", "kv4_plan_check.cpp")
+
+
+@pytest.mark.parametrize("name,dtype,dim,heads,group,lengths,new,window,plan", PLANNED, ids=[c[0] for c in PLANNED])
+def test_plan_of_an_attention_call(kv4_check, name, dtype, dim, heads, group, lengths, new, window, plan):
+    """The plans that the same calls are tested with on the device."""
+    args = (int(dtype == p.DTYPE_BF16), dim, heads, group, len(lengths), sum(new), max(new), max(lengths), window)
+    proc = subprocess.run([str(kv4_check), *map(str, args)], capture_output=True, text=True, timeout=60)
+    splits, prompts, few, sums, pages = map(int, proc.stdout.split())
+    assert (splits, prompts, sums, pages) == plan and few == (not prompts or len(lengths) > 1)
 
 
 # up to 48 rows: the few-rows kernel, or the 64-row tile where it measured faster (a layer of

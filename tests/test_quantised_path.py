@@ -58,6 +58,26 @@ def test_rows_of_the_smallest_numbers_keep_their_sign_and_range():
     assert np.array_equal(got, q)
 
 
+# Calls whose sizes are what they say, so that what they are planned as happens: name, type, head width, key heads,
+# group, lengths, new rows, window; splits, whether the prompts' kernel runs, sums that a thread of the join adds,
+# pages of a split.
+PLANNED = [
+    ("more splits than parts, 64", p.DTYPE_F32, 64, 1, 2, [5000], [1], 0, (20, 0, 4, 4)),
+    ("more splits than parts, 64, bf16", p.DTYPE_BF16, 64, 1, 2, [5000, 1300, 70], [1, 2, 1], 0, (20, 0, 4, 4)),
+    ("more splits than parts, 128", p.DTYPE_BF16, 128, 1, 4, [3000], [1], 0, (12, 0, 8, 4)),
+    ("more splits than parts, 256", p.DTYPE_F32, 256, 1, 1, [2000], [1], 0, (8, 0, 16, 4)),
+    ("the most splits", p.DTYPE_BF16, 256, 1, 8, [16300, 100], [1, 1], 0, (64, 0, 16, 4)),
+    ("splits of 16 pages", p.DTYPE_BF16, 64, 8, 1, [2500, 1200] + [10 + 5 * i for i in range(62)], [1] * 64, 0, (3, 0, 1, 16)),
+    ("splits of 32 pages", p.DTYPE_BF16, 64, 8, 2, [4200, 3100, 2100] + [9 + 4 * i for i in range(61)], [1] * 64, 0, (3, 0, 1, 32)),
+    ("prompts beside splits, 64", p.DTYPE_BF16, 64, 2, 4, [400, 20000, 90], [300, 1, 20], 0, (40, 1, 4, 8)),
+    ("prompts beside splits, 128", p.DTYPE_F32, 128, 2, 4, [20000, 500, 3000, 70], [2, 280, 5, 70], 0, (20, 1, 8, 16)),
+    ("prompts beside splits, 256", p.DTYPE_BF16, 256, 1, 8, [350, 9600], [330, 1], 0, (38, 1, 16, 4)),
+    ("prompts in a window", p.DTYPE_BF16, 64, 3, 4, [2300, 900, 1500], [1500, 600, 1], 200, (8, 1, 1, 4)),
+    ("prompts in a narrow window, fp32", p.DTYPE_F32, 128, 3, 4, [1600, 1900], [1600, 500], 70, (8, 1, 1, 4)),
+    ("prompts in a wide window", p.DTYPE_BF16, 256, 2, 4, [2400], [1300], 1000, (0, 1, 1, 1)),
+]
+
+
 def test_cache_ties_go_to_the_even_code():
     x = np.zeros((1, 64), np.float32)
     x[0, :9] = [6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -5.0]  # step 1
