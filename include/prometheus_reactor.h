@@ -1000,7 +1000,7 @@ typedef struct PrometheusKv4AttentionRequest {
   uint32_t max_rows;    /* 1..rows */
   uint32_t max_length;  /* at least 1 */
   uint32_t window;
-  float scale;          /* finite, above 0 */
+  float scale;          /* above 0, scale * log2(e) finite */
   const void* q;
   void* out;
   const int32_t* row_starts;

@@ -1163,7 +1163,7 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf
   g.q_heads = a.q_heads;
   g.group = a.group;
   g.window = a.window > 0x7fffffffu ? 0 : (int)a.window;  // longer than any sequence
-  g.scale_log2 = a.scale * 1.4426950408889634f;
+  g.scale_log2 = a.scale * kLog2E;
   uint32_t l = 0;
   while ((1u << l) < (uint32_t)a.group) ++l;
   g.group_shift = 31 + l;

@@ -172,7 +172,7 @@ PROM_REACTOR_API int prometheus_reactor_runtime_attention_kv4_device(void* handl
       r->q_heads % cache->kv_heads != 0u || (uint64_t)r->rows * (r->q_heads / cache->kv_heads) >= 1ull << 30 ||
       (uint64_t)r->q_heads * cache->head_dim > r->q_stride ||
       (uint64_t)r->q_heads * cache->head_dim > r->out_stride || r->q_stride >= 1u << 24 || r->out_stride >= 1u << 24 ||
-      r->max_rows == 0u || r->max_rows > r->rows || r->max_length == 0u || !isfinite(r->scale) || r->scale <= 0.0f ||
+      r->max_rows == 0u || r->max_rows > r->rows || r->max_length == 0u || !isfinite(r->scale * kLog2E) || r->scale <= 0.0f ||
       r->q == nullptr || r->out == nullptr || r->row_starts == nullptr || !aligned(r->q, size) ||
       !aligned(r->out, size) || !aligned(r->row_starts, 4))
     return invalid(out_stage, out_detail_code);

@@ -337,8 +337,9 @@ struct Kv4AttentionArgs {
   float* part;
   uint32_t rows, q_stride, out_stride, window, max_rows, max_length;
   int q_heads, group;
-  float scale;
+  float scale;  // scale * kLog2E is finite
 };
+constexpr float kLog2E = 1.4426950408889634f;
 // Sequences times key heads (a workgroup at least each).
 constexpr uint64_t kKv4MaxColumns = 1ull << 22;
 size_t kv4_attention_partial_bytes(const Kv4AttentionArgs& a, int head_dim, bool bf16);

@@ -236,6 +236,15 @@ def test_attention_refuses(rt):
     assert _no_device(_attention(rt, request=dict(ATTENTION, window=1, max_length=0xFFFFFFFF, q=OK + 2, out=OK + 6)))
 
 
+def test_attention_refuses_scales_past_the_range_in_base_2(rt):
+    """The softmax is in base 2: scale * log2(e) has to be finite too, or equal scores would give NaN."""
+    most = np.float32(2.0 ** 128 / np.log2(np.e) * (1 - 2.0 ** -22))
+    for scale in (np.finfo(np.float32).max, np.float32(2.4e38), np.float32(2.0 ** 128 / np.log2(np.e) * (1 + 2.0 ** -22))):
+        assert np.isfinite(scale) and _refused(_attention(rt, request=dict(ATTENTION, scale=float(scale)))), scale
+    for scale in (most, np.float32(1e-45)):
+        assert _no_device(_attention(rt, request=dict(ATTENTION, scale=float(scale)))), scale
+
+
 def test_unknown_handles_are_refused(rt):
     stage, detail = c_uint32(99), c_int(99)
     lib = rt.lib
