@@ -906,7 +906,8 @@ PROM_REACTOR_API int prometheus_reactor_runtime_quantize_rows_int8_device(
 /* c[i, j] = a_scale[i] * w_scale[j] * sum_k a[i, k] * w[j, k]: a int8 [m, k] (a row
    per token), w int8 [n, k] (a row per output channel), c of `dtype` [m, n], all
    contiguous, any alignment; the sum is exact (k <= 131071, so that 128 * 128 * k
-   fits 32 bits), the scales are applied in fp32 and the result is rounded once.
+   fits 32 bits); the sum and its products with a_scale and then w_scale are each
+   rounded to fp32, a bf16 result once more.
    Admission and statuses otherwise as ..._gemm_bf16_device (m * k, n * k, m * n
    below 2^32), with m and n at most 2^30; success detail PROM_DETAIL_PATH_HIP_MFMA_INT8. */
 #define PROM_GEMM_INT8_MAX_K 131071u
@@ -921,7 +922,7 @@ PROM_REACTOR_API int prometheus_reactor_runtime_gemm_int8_device(void* handle, c
    rounded to fp32 and then up to six significant bits, and per channel the nearest
    of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives to x / s (rounded to fp32;
    halfway to the even code); it stands for s times that, which fp32 and bf16 hold
-   exactly, at most s away from x (of magnitudes above 2^128 * 32 / 33, 6 s is past fp32's
+   exactly, at most s away from x (of magnitudes above 2^128 * 63 / 64, 6 s is past fp32's
    range: reads give an infinity, attention may take 85 / 86 of s).  A group with an
    infinity or a NaN reads back as NaN.
    A page is kv_heads blocks of head_dim * 64 + head_dim * 4 bytes: the keys' codes

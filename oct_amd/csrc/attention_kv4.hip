@@ -56,7 +56,7 @@ constexpr int kWaves = 4;
 // them on (us with it / without, two prompts over up to 4096 tokens, 4 key heads, groups of 4; 256 and 118
 // rows, 24064 pages of 16 pairs: bf16 64 channels 43 / 29, 128 56 / 49, 256 103 / 118, fp32 50 / 34,
 // 65 / 62; 512 and 236 rows, 47872 pages: 48 / 50, 65 / 90, 147 / 222, 59 / 58, 94 / 114).  fp32 rows of
-// 256 channels do not fit its registers (310 / 409).
+// 256 channels do not fit its registers (409 / 310).
 constexpr uint64_t kFewPairs = 64;
 constexpr uint64_t prompt_work(int head_dim) { return head_dim == 256 ? 24000 : 40000; }
 constexpr int kMaxSplits = 64;  // a lane each when they are joined
@@ -562,10 +562,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attention_kernel(const Kv4
 // other half of LDS after it.  Of eight waves, the second of each SIMD runs half a page behind the first:
 // one's products are beside the other's softmax.  P goes into the products as two bf16 terms (fp32 rows
 // and their queries: three), as in the kernel for few rows, so that a call's precision does not
-// depend on which of the two takes its sequences.  One term, 8 bits, was as far from 64 bits again as the
-// results' own rounding is (2.3e-3 of the values instead of 1.7e-3), and 308 us instead of the 381 below.
+// depend on which of the two takes its sequences.  One term, 8 bits, added as much error as the results' own
+// rounding (2.3e-3 of the values instead of 1.7e-3), and took 308 us instead of the 380 below.
 // Bound by the matrix and vector units together, which two waves of a SIMD share less well than they
-// could: four prompts of 1024 rows over up to 8000 tokens, 8 key heads of 128, groups of 4, bf16: 381 us for the
+// could: four prompts of 1024 rows over up to 8000 tokens, 8 key heads of 128, groups of 4, bf16: 380 us for the
 // call, 0.63 PFLOP/s of the definition's operations and half as many again for the second term (170 us at the rate of
 // a large product).  A call of 350 us with one term, a part at a time: 65 without any of the four, 45 more with
 // the loads, and beside these 35 with turning the codes, 78 with softmax, 153 with the products.
@@ -679,10 +679,13 @@ __device__ __forceinline__ uint64_t first_unit(uint64_t total, uint64_t w, uint6
   return total / n * w + min(w, total % n);
 }
 
-// Workgroup w does units first_unit(w) to first_unit(w + 1), whatever tiles these cut through:
-// every workgroup has the same number of pages.  A piece that is not a whole tile leaves its sums
-// in place 2 w + 1 where it begins the tile (it is then the workgroup's last), 2 w otherwise (its
-// first), for kv4_prompt_join_kernel.
+// Workgroup w does units first_unit(w) to first_unit(w + 1), equal shares whatever tiles these cut through.
+// A unit need not be a page that its tile sees (all tiles count the sequence's whole span), so that the shares of
+// pages are even only where most of the span is seen: the busiest workgroup has 1.06 of the mean with four
+// prompts of 1024 rows over 8000 tokens, but 1.94 to 1.99 with one of 2048 to 32768 rows and nothing before
+// them (8 key heads, groups of 4; 4096 rows of 128 channels in bf16 320 us, 98 at the rate of a large product).  A
+// piece that is not a whole tile leaves its sums in place 2 w + 1 where it begins the tile (it is then the
+// workgroup's last), 2 w otherwise (its first), for join_prompts.
 template <bool kF32, int D>
 __global__ __launch_bounds__((Prompt<kF32, D>::kThreads), (Prompt<kF32, D>::kWaves / 4)) void kv4_prompt_kernel(const Kv4Kernel g) {
   using Pr = Prompt<kF32, D>;
@@ -1113,6 +1116,10 @@ Plan plan(const Kv4AttentionArgs& a, int head_dim, bool bf16) {
   while (((pages + (1ull << p.shift) - 1) >> p.shift) > (uint64_t)kMaxSplits) ++p.shift;
   p.splits = (int)((pages + (1ull << p.shift) - 1) >> p.shift);
   p.part_bytes = (size_t)p.splits * a.rows * (size_t)a.q_heads * (size_t)(head_dim + 2) * sizeof(float);
+  // With very many workgroups, or more than 1 GiB of partial sums (which count every row of the call), none is
+  // split: a few long sequences among many short ones, or beside a long prompt, are then a few workgroups' work
+  // (bf16, 8 key heads of 128, groups of 4: 1024 rows 42 us, eight rows over 131072 tokens 261, both in a call 869;
+  // 512 rows over 1000 tokens 117, with one of them over 131072 908).
   if (base >= 4096 || p.part_bytes > kMostPartialBytes) p.splits = 1;
   if (p.splits == 1) p.part_bytes = 0;
   return p;

@@ -10,7 +10,7 @@
 // end and a's chunks past k are sent out of range, so tails add zeros.  Rows that
 // are not whole 16-byte chunks are copied to padded ones first.  Where tiles are few,
 // K is cut into slices whose int32 sums a second kernel adds (exact in any order).
-// 4224x20480x3840 to bf16: 328 us, 2.03 POP/s (a library's product of the same shape to
+// 4224x20480x3840 to bf16: 328 to 343 us by the card, 2.03 to 1.94 POP/s (a library's product of the same shape to
 // int32 308 to 345): five whole rounds of 256x256 tiles and the columns left over as
 // 128x128 (as a sixth round 338).  Matrix units are busy 63 % of the time at a clock that
 // their load lowers, waves wait 26 % of theirs, at the barrier of each K tile and for the first

@@ -36,8 +36,7 @@ __device__ __forceinline__ void load8(const uint16_t* p, float (&v)[8]) {
   }
 }
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) { __builtin_memcpy(p, v, 32); }
-// Exact: what the cache holds has eight significant bits (a step near fp32's smallest
-// numbers, whose low bits bf16 drops, aside: these are rounded toward zero).
+// Exact: what the cache holds has eight significant bits, and is a multiple of 2^-132 (a step is one of 2^-131).
 __device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
   u32x4 w;
 #pragma unroll

@@ -770,7 +770,7 @@ IDLE_ROWS = 8000
 @pytest.mark.parametrize("dtype", (F32, BF16))
 @pytest.mark.parametrize("window,at", [(0, 150), (0, 199), (20, 105), (20, 150)])
 def test_attention_to_values_at_the_end_of_the_range(gpu_runtime, idle, dtype, window, at):
-    """Six steps of a group of magnitudes above 2^128 * 32 / 33 are past fp32's range, though the step is not: rows
+    """Six steps of a group of magnitudes above 2^128 * 63 / 64 are past fp32's range, though the step is not: rows
     that do not see the token (before it, or with a window that has left it behind) are as without it."""
     case = Case(128, 1, [200], [100], dtype, seed=6, extra_rows=idle).history(32)
     v = np.ones((1, 128), np.float32)
