@@ -893,8 +893,8 @@ enum { PROM_DTYPE_F32 = 0u, PROM_DTYPE_BF16 = 1u };
 
 /* q[r, c] = rint(x[r, c] / s[r]), s[r] = max_c |x[r, c]| / 127, each operation
    rounded to fp32 (halves to even), and held within -127..127 (only a scale below
-   2^-142, whose rounding is coarse, gives quotients past that).  input: dtype [rows, width]
-   with input_row_stride >= width elements between rows, any alignment of its
+   2^-142, whose rounding is coarse, gives quotients past that).  input: dtype [rows,
+   width] with input_row_stride >= width elements between rows, any alignment of its
    type; output int8 [rows, width] and scales fp32 [rows], contiguous.  A row of
    zeros has scale 0 and zeros; a row with an infinity or a NaN has scale NaN and
    zeros, so that what is computed from it is NaN.  rows * width and rows *
@@ -922,9 +922,9 @@ PROM_REACTOR_API int prometheus_reactor_runtime_gemm_int8_device(void* handle, c
    rounded to fp32 and then up to six significant bits, and per channel the nearest
    of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives to x / s (rounded to fp32;
    halfway to the even code); it stands for s times that, which fp32 and bf16 hold
-   exactly, at most s away from x (of magnitudes above 2^128 * 63 / 64, 6 s is past fp32's
-   range: reads give an infinity, attention may take 85 / 86 of s).  A group with an
-   infinity or a NaN reads back as NaN.
+   exactly, at most s away from x (of magnitudes above 2^128 * 63 / 64, 6 s is past
+   fp32's range: an infinity when it is read, in attention that or 85 / 86 of s).  A group
+   with an infinity or a NaN reads back as NaN.
    A page is kv_heads blocks of head_dim * 64 + head_dim * 4 bytes: the keys' codes
    [64][head_dim / 2], the values' codes, the keys' steps [head_dim / 64][64] and the
    values'.  A code is a sign (8) and the place 0..7 of the magnitude above; a byte
@@ -955,12 +955,12 @@ PROM_REACTOR_API uint64_t prometheus_reactor_kv4_page_bytes(uint32_t head_dim, u
 
 /* Rows of the last tokens of each sequence: rows row_starts[i] .. row_starts[i+1] - 1
    (row_starts [sequences + 1], not decreasing) are sequence i's last tokens, the last
-   row its token lengths[i] - 1.  Row starts may lie below 0 or past `rows`: a row that the
-   call has keeps its position, the others are passed over.  k and v: dtype [rows, kv_heads, head_dim] with
-   row_stride >= kv_heads * head_dim elements between rows (so that they may be columns
-   of one projection's output), any alignment of their type.  Rows outside every
-   sequence, or before its token 0, are passed over: not stored by a write, left as they
-   were by a read.  Write quantises k and v into the cache; read gives what the cache
+   row its token lengths[i] - 1.  Row starts may lie below 0 or past `rows`: a row that
+   the call has keeps its position, the others are passed over.  k and v: dtype [rows,
+   kv_heads, head_dim] with row_stride >= kv_heads * head_dim elements between rows (so
+   that they may be columns of one projection's output), any alignment of their type.
+   Rows outside every sequence, or before its token 0, are passed over: not stored by a
+   write, left as they were by a read.  Write quantises k and v into the cache; read gives what the cache
    holds (k or v may be NULL in a read).  No two tokens of a write may share a place
    (sequences may share pages that a call only reads). */
 typedef struct PrometheusKv4RowsRequest {
