@@ -1011,6 +1011,190 @@ PROM_REACTOR_API int prometheus_reactor_runtime_attention_kv4_device(void* handl
                                                                      uint32_t* out_stage, int* out_detail_code);
 
 /* ------------------------------------------------------------------------ */
+/* NEW: the rest of a decoder's step beside the quantised path: weights held   */
+/* in 4 bits and products with them, a mixture-of-experts layer on them,       */
+/* rotary positions, and the residual sum between two blocks with the norms    */
+/* before and after it.  No reference counterpart.  Device pointers, stream,   */
+/* statuses and refusals as in the quantised path above.  Outputs may not      */
+/* overlap operands except where it is said.  Equal calls give equal bits.     */
+/* ------------------------------------------------------------------------ */
+
+/* `count` weight matrices [n, k] (a row per output channel) in 4 bits.  A group is
+   `group` neighbouring weights of a row (fewer at the row's end), held with a step and
+   E2M1 codes as a group of the 4-bit cache is: s = max |w| / 6 rounded to fp32 and then
+   up to six significant bits, codes the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their
+   negatives to w / s (rounded to fp32; halfway to the even code).  A weight stands for s
+   times that, which fp32 and bf16 hold exactly, at most s away from w; a group with an
+   infinity or a NaN stands for NaN.
+   A matrix is prometheus_reactor_w4_bytes(n, k, group) bytes, matrices lie one behind the
+   other.  Tiles of 16 rows by 128 columns, in each row of tiles those of rising columns:
+   first all codes, 1024 bytes a tile, of which bytes 16 l .. + 15 are four words, word s the
+   codes of row l % 16, columns 32 s + 8 (l / 16) .. + 7, the lower column in the lower half
+   of a byte (the order in which the matrix units take them); behind them all steps, tile by
+   tile, [16][128 / group], each the upper 16 bits of an fp32.  Rows and columns behind the
+   last are zeros (w4_pack writes them), and no product depends on x there. */
+typedef struct PrometheusW4Matrix {
+  uint32_t struct_size;
+  uint32_t n;     /* 1..2^24 */
+  uint32_t k;     /* 1..2^20 */
+  uint32_t group; /* 32, 64 or 128 */
+  uint32_t count; /* 1..2^16; a product reads the first */
+  uint32_t reserved0; /* 0 */
+  void* data;     /* 16-byte aligned */
+} PrometheusW4Matrix;
+/* Bytes of one matrix; 0 for sizes outside the above. */
+PROM_REACTOR_API uint64_t prometheus_reactor_w4_bytes(uint32_t n, uint32_t k, uint32_t group);
+/* weights: dtype [count, n, k] with row_stride >= k elements between rows (below 2^24), any
+   alignment of their type.  Pack quantises them into `matrix`; unpack gives what it holds. */
+PROM_REACTOR_API int prometheus_reactor_runtime_w4_pack_device(void* handle, const PrometheusW4Matrix* matrix,
+                                                               const void* weights, uint32_t row_stride,
+                                                               uint32_t dtype, uint32_t* out_stage,
+                                                               int* out_detail_code);
+PROM_REACTOR_API int prometheus_reactor_runtime_w4_unpack_device(void* handle, const PrometheusW4Matrix* matrix,
+                                                                 void* weights, uint32_t row_stride, uint32_t dtype,
+                                                                 uint32_t* out_stage, int* out_detail_code);
+
+/* out[i, j] = sum_k x[i, k] w[j, k] for x of `dtype` [rows, k] and out [rows, n], x_stride and
+   out_stride elements between rows (below 2^24), any alignment of their type.  Operands
+   enter unrounded (bf16 rows times codes are exact, fp32 rows go in as three exact terms);
+   sums are fp32, a bf16 result is rounded once. */
+typedef struct PrometheusW4GemmRequest {
+  uint32_t struct_size;
+  uint32_t dtype;
+  uint32_t rows;       /* 1..2^20 */
+  uint32_t x_stride;   /* >= k */
+  uint32_t out_stride; /* >= n */
+  uint32_t reserved0;  /* 0 */
+  const void* x;
+  void* out;
+} PrometheusW4GemmRequest;
+PROM_REACTOR_API int prometheus_reactor_runtime_gemm_w4_device(void* handle, const PrometheusW4Matrix* matrix,
+                                                               const PrometheusW4GemmRequest* request,
+                                                               uint32_t* out_stage, int* out_detail_code);
+
+/* A mixture-of-experts layer of a few tokens.  Logits l = x router^T are sums in binary64; a
+   token's experts are the top_k largest (a NaN counts as less than every number; ties go to
+   the lower expert), their weights p = softmax(l) over all experts, divided by the sum over
+   the chosen ones where renormalise is set;
+     out[t] = sum over t's experts e, in their order, of p_e (act(x[t] gate_e^T) * (x[t] up_e^T)) down_e^T
+   in fp32, a bf16 result rounded once.  x of `dtype` [tokens, hidden] and out [tokens, hidden] as
+   in the product above, router fp32 [experts, hidden].  gate and up are [inner, hidden] of one group
+   size, down [hidden, inner]; each holds a matrix an expert (count = experts).  The hidden rows enter
+   the second product with 16 significant bits (fp32 rows: 24).  An expert's weights are read once for
+   up to 64 tokens that chose it. */
+enum { PROM_MOE_SILU = 0u, PROM_MOE_GELU_TANH = 1u };
+#define PROM_MOE_MAX_EXPERTS 1024u
+#define PROM_MOE_MAX_TOP_K 64u
+#define PROM_MOE_MAX_PAIRS 65536u
+typedef struct PrometheusMoeRequest {
+  uint32_t struct_size;
+  uint32_t dtype;
+  uint32_t tokens;      /* at least 1; tokens * top_k at most PROM_MOE_MAX_PAIRS */
+  uint32_t top_k;       /* 1..min(experts, PROM_MOE_MAX_TOP_K) */
+  uint32_t x_stride;    /* >= hidden, below 2^24 */
+  uint32_t out_stride;  /* >= hidden, below 2^24 */
+  uint32_t activation;  /* PROM_MOE_SILU or PROM_MOE_GELU_TANH */
+  uint32_t renormalise; /* 0 or 1 */
+  const float* router;
+  const void* x;
+  void* out;
+  int32_t* out_experts; /* [tokens, top_k], or NULL */
+  float* out_weights;   /* [tokens, top_k], or NULL */
+} PrometheusMoeRequest;
+PROM_REACTOR_API int prometheus_reactor_runtime_moe_w4_device(void* handle, const PrometheusW4Matrix* gate,
+                                                              const PrometheusW4Matrix* up,
+                                                              const PrometheusW4Matrix* down,
+                                                              const PrometheusMoeRequest* request,
+                                                              uint32_t* out_stage, int* out_detail_code);
+
+/* Rotary positions.  The first rotary_dim channels of each head of q and k are turned in pairs,
+   (i, i + rotary_dim / 2) (HALF) or (2 i, 2 i + 1) (PAIRS), by positions[row] * turns[i]
+   revolutions and scaled by magnitude; the others are copied.  q and k: dtype [rows, heads,
+   head_dim] with strides in elements between rows (below 2^24, at least heads * head_dim), any
+   alignment of their type; either may be NULL with its output.  An output may be its input
+   (with the same stride).  positions int32 [rows], any sign; turns binary64 [rotary_dim / 2].
+   Angles are binary64, the rotation fp32, a bf16 result rounded once. */
+enum { PROM_ROPE_HALF = 0u, PROM_ROPE_PAIRS = 1u };
+typedef struct PrometheusRopeRequest {
+  uint32_t struct_size;
+  uint32_t dtype;
+  uint32_t rows;       /* 1..2^22 */
+  uint32_t head_dim;   /* 2..1024 */
+  uint32_t rotary_dim; /* even, 2..head_dim */
+  uint32_t layout;     /* PROM_ROPE_HALF or PROM_ROPE_PAIRS */
+  uint32_t q_heads;    /* 1..2^16 where q is given */
+  uint32_t k_heads;    /* 1..2^16 where k is given */
+  uint32_t q_stride, k_stride, q_out_stride, k_out_stride;
+  float magnitude;     /* finite */
+  uint32_t reserved0;  /* 0 */
+  const int32_t* positions;
+  const double* turns; /* 8-byte aligned */
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+} PrometheusRopeRequest;
+PROM_REACTOR_API int prometheus_reactor_runtime_rope_device(void* handle, const PrometheusRopeRequest* request,
+                                                            uint32_t* out_stage, int* out_detail_code);
+/* On the host: the rotary_dim / 2 revolutions a token, base^(-2 i / rotary_dim) / (2 pi), and the
+   magnitude, scaled for contexts `factor` times as long as the trained one:
+   LINEAR divides all by factor; BASE takes base * factor^(rotary_dim / (rotary_dim - 2)) (rotary_dim
+   above 2); PARTS divides those that turn less than slow_turns times within `context` tokens, keeps
+   those that turn fast_turns times or more, goes linearly in i from the one border (rounded down) to
+   the other (rounded up), and has magnitude 1 + ln(factor) / 10.  PROM_ERROR for arguments outside
+   the comments below. */
+enum { PROM_ROPE_SCALE_NONE = 0u, PROM_ROPE_SCALE_LINEAR = 1u, PROM_ROPE_SCALE_BASE = 2u, PROM_ROPE_SCALE_PARTS = 3u };
+typedef struct PrometheusRopeScaling {
+  uint32_t struct_size;
+  uint32_t rotary_dim; /* even, 2..1024 */
+  uint32_t kind;       /* PROM_ROPE_SCALE_* */
+  uint32_t reserved0;  /* 0 */
+  double base;         /* finite, above 1 */
+  double factor;       /* finite, at least 1; not looked at by NONE */
+  double context;      /* PARTS: finite, at least 1 */
+  double fast_turns;   /* PARTS: finite, above slow_turns */
+  double slow_turns;   /* PARTS: above 0 */
+} PrometheusRopeScaling;
+PROM_REACTOR_API int prometheus_reactor_rope_turns(const PrometheusRopeScaling* scaling, double* out_turns,
+                                                   float* out_magnitude);
+
+/* The residual sum between two blocks with the norms before and after it:
+     h' = h + residual_scale * g * norm(y; post),  out = norm(h'; pre) * (1 + scale) + shift,
+   norm(x; w) = x / sqrt(mean(x^2) + eps) * (weight_offset + w).  y NULL: h' = h.  post NULL: y as it
+   is; pre NULL: weights 1; gate NULL: g = 1, otherwise gate or, with gate_tanh, its tanh; scale or
+   shift NULL: left out.  h_out (h') or out may be NULL, not both.  h, y, h_out, out: dtype [rows, width],
+   gate, scale, shift: dtype rows of `width` that rows_per_vector neighbouring rows share, vector_stride
+   elements apart; post and pre: fp32 [width]; any alignment of their type, strides below 2^24.  h_out may
+   be h or y and out h or y, with the same stride.  Squares are summed in binary64, the rest is fp32; out
+   is computed from h' before h' is rounded. */
+#define PROM_RESIDUAL_NORM_MAX_WIDTH 32768u
+typedef struct PrometheusResidualNormRequest {
+  uint32_t struct_size;
+  uint32_t dtype;
+  uint32_t rows;  /* 1..2^22 */
+  uint32_t width; /* 1..PROM_RESIDUAL_NORM_MAX_WIDTH */
+  uint32_t h_stride, y_stride, h_out_stride, out_stride; /* >= width where given */
+  uint32_t vector_stride;   /* >= width where gate, scale or shift is given */
+  uint32_t rows_per_vector; /* at least 1 where gate, scale or shift is given */
+  uint32_t gate_tanh;       /* 0 or 1 */
+  float residual_scale;     /* finite */
+  float weight_offset;      /* finite */
+  float eps;                /* finite, not below 0 */
+  const void* h;
+  const void* y;
+  const float* post;
+  const void* gate;
+  const float* pre;
+  const void* scale;
+  const void* shift;
+  void* h_out;
+  void* out;
+} PrometheusResidualNormRequest;
+PROM_REACTOR_API int prometheus_reactor_runtime_residual_norm_device(void* handle,
+                                                                     const PrometheusResidualNormRequest* request,
+                                                                     uint32_t* out_stage, int* out_detail_code);
+
+/* ------------------------------------------------------------------------ */
 /* Asynchronous and batched SGEMM (reference lifecycle, HIP execution)       */
 /* ------------------------------------------------------------------------ */
 

@@ -14,16 +14,13 @@
 // rows of 8 heads of 128, bf16: write 26.4 us, 4.4 TB/s; read 24.5 us, 4.7 TB/s)
 // and, for the few rows of a decode step, by the latency of the chain row ->
 // sequence -> page -> store (64 rows: 5 us a launch).
+#include "fp4_groups.h"
 #include "reactor_internal.h"
 
 namespace prom {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef float floatx2 __attribute__((ext_vector_type(2)));
-
-constexpr uint32_t kInfBits = 0x7F800000u;
-constexpr uint32_t kNanParam = 0x7FC0u;
 
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) { __builtin_memcpy(v, p, 32); }
 __device__ __forceinline__ void load8(const uint16_t* p, float (&v)[8]) {
@@ -51,62 +48,9 @@ __device__ __forceinline__ int key_word(int j) {
   return (j & ~15) + 4 * (j & 3) + ((j >> 2) & 3);
 }
 
-// The largest of eight neighbouring lanes.
-__device__ __forceinline__ uint32_t max_of_8(uint32_t m) {
-  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true));   // the other of a pair
-  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true));   // the other pair of four
-  return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, true));  // mirrored within eight
-}
-
-// The IEEE quotient x / d for d of at most six significant bits, r = 1 / d to within a few ulps: q = fl(x r)
-// is a few ulps off, the remainder q d - x has few enough bits to be exact, and x / d lies 2^-7 ulps or
-// more from where rounding changes, far more than the error of q - remainder r.  The sign of a zero is kept.
-__device__ __forceinline__ float quotient(float x, float d, float r) {
-  const float q = x * r;
-  return __builtin_fmaf(-__builtin_fmaf(q, d, -x), r, q);
-}
-
 // Step and codes of the eight channels v of a lane; the group's lanes are eight neighbours.
 __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], uint32_t* param) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-  m = max_of_8(m);
-  const float top = __uint_as_float(m);
-  // In this range nothing under- or overflows on the way to a quotient that is not rounded to zero.
-  const bool plain = (top >= 0x1p-80f && top <= 0x1p80f) || m == 0;
-  const bool all_plain = __all(plain);
-  const uint32_t t = __float_as_uint(all_plain ? quotient(top, 6.0f, 1.0f / 6.0f) : top / 6.0f);
-  const float s = __uint_as_float((t + 0x3FFFFu) & 0xFFFC0000u);
-  const bool finite = m < kInfBits;
-  *param = finite ? __float_as_uint(s) >> 16 : kNanParam;
-  const bool some = finite && s > 0.0f;
-  const float d = some ? s : 1.0f;
-  float y[8];
-  if (all_plain) {
-    const float r = __builtin_amdgcn_rcpf(d);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = quotient(v[j], d, r);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = v[j] / d;
-  }
-  uint32_t codes = 0;
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[0], y[1], 1.0f, 0);
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[2], y[3], 1.0f, 1);
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[4], y[5], 1.0f, 2);
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[6], y[7], 1.0f, 3);
-  return some ? codes : 0u;
-}
-
-__device__ __forceinline__ void values8(uint32_t codes, uint32_t param, float (&v)[8]) {
-  const float s = __uint_as_float(param << 16);
-  const floatx2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 0);
-  const floatx2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 1);
-  const floatx2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 2);
-  const floatx2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 3);
-  v[0] = a.x * s, v[1] = a.y * s, v[2] = b.x * s, v[3] = b.y * s;
-  v[4] = c.x * s, v[5] = c.y * s, v[6] = d.x * s, v[7] = d.y * s;
+  return fp4_codes(v, max_of_lanes<8>(max_bits(v)), param);
 }
 
 // The sequences of rows, asked by a whole wave with one row at a time.  Up to 63 sequences: their starts
@@ -191,11 +135,11 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(const Kv4View c, T* k, T*
         }
       } else if (live) {
         if (k != nullptr) {
-          values8(good ? *key : 0u, good ? params[0] : kNanParam, x);
+          fp4_values(good ? *key : 0u, good ? params[0] : kNanParam, x);
           store8(k + at, x);
         }
         if (v != nullptr) {
-          values8(good ? *value : 0u, good ? params[kValueParams] : kNanParam, x);
+          fp4_values(good ? *value : 0u, good ? params[kValueParams] : kNanParam, x);
           store8(v + at, x);
         }
       }

@@ -1,0 +1,41 @@
+// The mixture layer's arguments and workspace (moe_w4.hip; filled in by the entry points).
+#pragma once
+
+#include "w4_tiles.h"
+
+namespace prom {
+
+constexpr int kMoeMaxExperts = 1024, kMoeMaxTopK = 64;
+
+struct MoeExpert {
+  int expert, start, count, unused;  // its pairs: pairs[start] ..
+};
+
+struct W4MoeArgs {
+  W4View gate, up, down;  // [inner, hidden] twice, [hidden, inner]; a matrix an expert
+  const float* router;    // [experts, hidden]
+  const void* x;
+  void* out;
+  int32_t* out_chosen;  // may be null
+  float* out_weights;   // may be null
+  uint32_t x_stride, out_stride, activation;
+  int tokens, experts, top_k;
+  bool renormalise;
+  // workspace
+  double* logits;  // [tokens][experts]
+  int32_t* chosen;  // [pairs], pairs = tokens * top_k
+  float* weights;   // [pairs]
+  int32_t* pairs;   // by expert
+  MoeExpert* reached;
+  int32_t* reached_count;
+  uint16_t* hidden;  // terms of [pairs][hidden_stride], hidden_plane elements apart
+  size_t hidden_plane;
+  uint32_t hidden_stride;
+  float* part;  // [pairs][hidden width]
+};
+
+// Bytes of the workspace; sets the pointers into `base`.
+size_t moe_w4_workspace(W4MoeArgs& a, bool bf16, void* base);
+hipError_t launch_moe_w4(const W4MoeArgs& a, bool bf16, hipStream_t stream);
+
+}  // namespace prom

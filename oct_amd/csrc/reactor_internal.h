@@ -345,6 +345,40 @@ constexpr uint64_t kKv4MaxColumns = 1ull << 22;
 size_t kv4_attention_partial_bytes(const Kv4AttentionArgs& a, int head_dim, bool bf16);
 hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, int head_dim, bool bf16, hipStream_t stream);
 
+// ---- the rest of a decoder's step (w4_matrix.hip, gemm_w4.hip, moe_w4.hip, rope.hip, residual_norm.hip)
+struct W4View;  // w4_tiles.h
+// rows: [count][n][k] with `stride` elements between rows.
+hipError_t launch_w4_pack(const W4View& w, const void* rows, bool bf16, uint32_t stride, hipStream_t stream);
+hipError_t launch_w4_unpack(const W4View& w, void* rows, bool bf16, uint32_t stride, hipStream_t stream);
+// out[m, n] = x[m, k] w^T of the first matrix of w; caller holds ctx().mu (slices' sums in staging).
+// hipErrorOutOfMemory when that cannot be had.
+hipError_t launch_gemm_w4(const W4View& w, const void* x, uint32_t x_stride, void* out, uint32_t out_stride, bool bf16,
+                          uint32_t m, hipStream_t stream);
+struct RopeTensor {
+  const void* in;  // null: none
+  void* out;
+  uint32_t heads, in_stride, out_stride;
+};
+struct RopeArgs {
+  RopeTensor q, k;
+  const int32_t* positions;
+  const double* turns;
+  uint32_t rows, head_dim, rotary;
+  float magnitude;
+};
+constexpr uint32_t kRopeMaxDim = 1024;
+hipError_t launch_rope(const RopeArgs& a, bool bf16, bool pairs, hipStream_t stream);
+struct ResidualNormArgs {
+  const void *h, *y, *gate, *scale, *shift;
+  const float *post, *pre;
+  void *h_out, *out;
+  uint32_t rows, width, h_stride, y_stride, h_out_stride, out_stride, vector_stride, rows_per_vector;
+  float residual_scale, weight_offset, eps;
+  bool gate_tanh;
+};
+constexpr uint32_t kResidualNormMaxWidth = 32768;
+hipError_t launch_residual_norm(const ResidualNormArgs& a, bool bf16, hipStream_t stream);
+
 // IEEE quotients x / s of many x by one finite s > 0, four operations each instead of the fourteen of a
 // division.  hi is 1 / s correctly rounded, hi + lo is 1 / s to about 48 bits; q = fl(x hi + fl(x lo)) is then
 // within an ulp of x / s, x - q s has no more than 24 bits, and q plus that remainder times hi rounds to the

@@ -62,6 +62,11 @@ DETAIL_SCRATCH_LIMIT = -6930
 DETAIL_SCRATCH_UNAVAILABLE = -6931
 SGEMM_NOALLOC_SCRATCH_BYTES = 64 << 20
 DTYPE_F32, DTYPE_BF16 = 0, 1  # rows of the quantised decode path
+MOE_SILU, MOE_GELU_TANH = 0, 1
+MOE_MAX_EXPERTS, MOE_MAX_TOP_K, MOE_MAX_PAIRS = 1024, 64, 65536
+ROPE_HALF, ROPE_PAIRS = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_BASE, ROPE_SCALE_PARTS = 0, 1, 2, 3
+RESIDUAL_NORM_MAX_WIDTH = 32768
 GEMM_INT8_MAX_K = 131071
 GEMM_INT8_MAX_SIDE = 1 << 30
 KV4_PAGE_TOKENS, KV4_GROUP = 64, 64
@@ -100,8 +105,9 @@ DETAIL_M46_NONFINITE_INPUT = -7418
 
 # ---- ABI structs -----------------------------------------------------------
 def _fields(spec: str):
-    """'u32 a, u64 b, f32 c, p d, i32 e' -> ctypes field list."""
-    kinds = {"u32": c_uint32, "u64": c_uint64, "f32": c_float, "p": c_void_p, "i32": ctypes.c_int32}
+    """'u32 a, u64 b, f32 c, p d, i32 e, f64 g' -> ctypes field list."""
+    kinds = {"u32": c_uint32, "u64": c_uint64, "f32": c_float, "p": c_void_p, "i32": ctypes.c_int32,
+             "f64": ctypes.c_double}
     out = []
     for item in spec.split(","):
         kind, name = item.split()
@@ -458,6 +464,36 @@ class PrometheusKv4RowsRequest(Structure):
 class PrometheusKv4AttentionRequest(Structure):
     _fields_ = _fields("u32 struct_size, u32 dtype, u32 rows, u32 q_heads, u32 q_stride, u32 out_stride, u32 max_rows, "
                        "u32 max_length, u32 window, f32 scale, p q, p out, p row_starts")
+
+
+class PrometheusW4Matrix(Structure):
+    _fields_ = _fields("u32 struct_size, u32 n, u32 k, u32 group, u32 count, u32 reserved0, p data")
+
+
+class PrometheusW4GemmRequest(Structure):
+    _fields_ = _fields("u32 struct_size, u32 dtype, u32 rows, u32 x_stride, u32 out_stride, u32 reserved0, p x, p out")
+
+
+class PrometheusMoeRequest(Structure):
+    _fields_ = _fields("u32 struct_size, u32 dtype, u32 tokens, u32 top_k, u32 x_stride, u32 out_stride, u32 activation, "
+                       "u32 renormalise, p router, p x, p out, p out_experts, p out_weights")
+
+
+class PrometheusRopeRequest(Structure):
+    _fields_ = _fields("u32 struct_size, u32 dtype, u32 rows, u32 head_dim, u32 rotary_dim, u32 layout, u32 q_heads, "
+                       "u32 k_heads, u32 q_stride, u32 k_stride, u32 q_out_stride, u32 k_out_stride, f32 magnitude, "
+                       "u32 reserved0, p positions, p turns, p q, p k, p q_out, p k_out")
+
+
+class PrometheusRopeScaling(Structure):
+    _fields_ = _fields("u32 struct_size, u32 rotary_dim, u32 kind, u32 reserved0, f64 base, f64 factor, f64 context, "
+                       "f64 fast_turns, f64 slow_turns")
+
+
+class PrometheusResidualNormRequest(Structure):
+    _fields_ = _fields("u32 struct_size, u32 dtype, u32 rows, u32 width, u32 h_stride, u32 y_stride, u32 h_out_stride, "
+                       "u32 out_stride, u32 vector_stride, u32 rows_per_vector, u32 gate_tanh, f32 residual_scale, "
+                       "f32 weight_offset, f32 eps, p h, p y, p post, p gate, p pre, p scale, p shift, p h_out, p out")
 
 
 class PrometheusAsyncStatus(Structure):
@@ -930,6 +966,22 @@ _SIGNATURES = {
     "prometheus_reactor_runtime_attention_kv4_device": (
         c_int, [c_void_p, POINTER(PrometheusKv4Cache), POINTER(PrometheusKv4AttentionRequest), POINTER(c_uint32),
                 POINTER(c_int)]),
+    "prometheus_reactor_w4_bytes": (c_uint64, [c_uint32, c_uint32, c_uint32]),
+    "prometheus_reactor_runtime_w4_pack_device": (
+        c_int, [c_void_p, POINTER(PrometheusW4Matrix), c_void_p, c_uint32, c_uint32, POINTER(c_uint32), POINTER(c_int)]),
+    "prometheus_reactor_runtime_w4_unpack_device": (
+        c_int, [c_void_p, POINTER(PrometheusW4Matrix), c_void_p, c_uint32, c_uint32, POINTER(c_uint32), POINTER(c_int)]),
+    "prometheus_reactor_runtime_gemm_w4_device": (
+        c_int, [c_void_p, POINTER(PrometheusW4Matrix), POINTER(PrometheusW4GemmRequest), POINTER(c_uint32),
+                POINTER(c_int)]),
+    "prometheus_reactor_runtime_moe_w4_device": (
+        c_int, [c_void_p, POINTER(PrometheusW4Matrix), POINTER(PrometheusW4Matrix), POINTER(PrometheusW4Matrix),
+                POINTER(PrometheusMoeRequest), POINTER(c_uint32), POINTER(c_int)]),
+    "prometheus_reactor_runtime_rope_device": (
+        c_int, [c_void_p, POINTER(PrometheusRopeRequest), POINTER(c_uint32), POINTER(c_int)]),
+    "prometheus_reactor_rope_turns": (c_int, [POINTER(PrometheusRopeScaling), c_void_p, POINTER(c_float)]),
+    "prometheus_reactor_runtime_residual_norm_device": (
+        c_int, [c_void_p, POINTER(PrometheusResidualNormRequest), POINTER(c_uint32), POINTER(c_int)]),
     "prometheus_reactor_runtime_gemm_bf16": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, POINTER(c_uint32), POINTER(c_int)]),
     "prometheus_reactor_runtime_gemm_bf16_device": (
@@ -1585,6 +1637,71 @@ class NativeRuntime:
                                                                       byref(stage), byref(detail))
         return self._check(rc, stage, detail, "attention_kv4_device")
 
+    # -- the rest of a decoder's step (device pointers as integers; a refusal raises) --
+    def w4_pack_device(self, matrix: PrometheusW4Matrix, dweights: int, row_stride: int, dtype: int) -> int:
+        """Quantise weights [count, n, k] into 4 bits."""
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_w4_pack_device(self.handle, byref(matrix), dweights, row_stride, dtype,
+                                                                byref(stage), byref(detail))
+        return self._check(rc, stage, detail, "w4_pack_device")
+
+    def w4_unpack_device(self, matrix: PrometheusW4Matrix, dweights: int, row_stride: int, dtype: int) -> int:
+        """The weights [count, n, k] that 4-bit matrices stand for."""
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_w4_unpack_device(self.handle, byref(matrix), dweights, row_stride, dtype,
+                                                                  byref(stage), byref(detail))
+        return self._check(rc, stage, detail, "w4_unpack_device")
+
+    def gemm_w4_device(self, matrix: PrometheusW4Matrix, dx: int, dout: int, rows: int, x_stride: int, out_stride: int,
+                       dtype: int) -> int:
+        """out [rows, n] = x [rows, k] w^T with 4-bit weights."""
+        req = PrometheusW4GemmRequest(_W4_GEMM_SIZE, dtype, rows, x_stride, out_stride, 0, dx, dout)
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_gemm_w4_device(self.handle, byref(matrix), byref(req), byref(stage),
+                                                                byref(detail))
+        return self._check(rc, stage, detail, "gemm_w4_device")
+
+    def moe_w4_device(self, gate: PrometheusW4Matrix, up: PrometheusW4Matrix, down: PrometheusW4Matrix, drouter: int,
+                      dx: int, dout: int, tokens: int, top_k: int, x_stride: int, out_stride: int, dtype: int,
+                      activation: int = MOE_SILU, renormalise: bool = False, dexperts: Optional[int] = None,
+                      dweights: Optional[int] = None) -> int:
+        """A mixture-of-experts layer: router fp32 [experts, hidden], gate and up [inner, hidden] and down
+        [hidden, inner] an expert; the chosen experts int32 and their weights fp32 [tokens, top_k] where asked for."""
+        req = PrometheusMoeRequest(_MOE_SIZE, dtype, tokens, top_k, x_stride, out_stride, activation, int(renormalise),
+                                   drouter, dx, dout, dexperts, dweights)
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_moe_w4_device(self.handle, byref(gate), byref(up), byref(down),
+                                                               byref(req), byref(stage), byref(detail))
+        return self._check(rc, stage, detail, "moe_w4_device")
+
+    def rope_device(self, dpositions: int, dturns: int, rows: int, head_dim: int, rotary_dim: int, layout: int, dtype: int,
+                    magnitude: float = 1.0, q: Optional[tuple] = None, k: Optional[tuple] = None) -> int:
+        """Rotary positions of q and k, each (input, output, heads, input stride, output stride) or None, by
+        positions[row] * turns[i] revolutions (see rope_turns)."""
+        q, k = q or (None, None, 0, 0, 0), k or (None, None, 0, 0, 0)
+        req = PrometheusRopeRequest(_ROPE_SIZE, dtype, rows, head_dim, rotary_dim, layout, q[2], k[2], q[3], k[3], q[4],
+                                    k[4], magnitude, 0, dpositions, dturns, q[0], k[0], q[1], k[1])
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_rope_device(self.handle, byref(req), byref(stage), byref(detail))
+        return self._check(rc, stage, detail, "rope_device")
+
+    def residual_norm_device(self, dh: int, dh_out: Optional[int], dout: Optional[int], rows: int, width: int, dtype: int,
+                             dy: Optional[int] = None, dpost: Optional[int] = None, dgate: Optional[int] = None,
+                             gate_tanh: bool = False, dpre: Optional[int] = None, dscale: Optional[int] = None,
+                             dshift: Optional[int] = None, rows_per_vector: int = 1, residual_scale: float = 1.0,
+                             weight_offset: float = 0.0, eps: float = 1e-6, h_stride: int = 0, y_stride: int = 0,
+                             h_out_stride: int = 0, out_stride: int = 0, vector_stride: int = 0) -> int:
+        """h' = h + residual_scale * gate * norm(y; post), out = norm(h'; pre) * (1 + scale) + shift; what is None is
+        left out, strides of 0 are `width`."""
+        req = PrometheusResidualNormRequest(
+            _RESIDUAL_NORM_SIZE, dtype, rows, width, h_stride or width, y_stride or width, h_out_stride or width,
+            out_stride or width, vector_stride or width, rows_per_vector, int(gate_tanh), residual_scale, weight_offset,
+            eps, dh, dy, dpost, dgate, dpre, dscale, dshift, dh_out, dout)
+        stage, detail = c_uint32(0), c_int(0)
+        rc = self.lib.prometheus_reactor_runtime_residual_norm_device(self.handle, byref(req), byref(stage),
+                                                                      byref(detail))
+        return self._check(rc, stage, detail, "residual_norm_device")
+
     # -- asynchronous SGEMM (bridge.go:438-470) ------------------------------
     def submit_async(self, m: int, n: int, k: int, a, b) -> Tuple[int, int, CallStatus]:
         """Returns (rc, task_id, status); A and B may be reused as soon as this returns."""
@@ -1709,6 +1826,11 @@ class NativeRuntime:
 
 _KV4_ROWS_SIZE = ctypes.sizeof(PrometheusKv4RowsRequest)
 _KV4_ATTENTION_SIZE = ctypes.sizeof(PrometheusKv4AttentionRequest)
+_W4_MATRIX_SIZE = ctypes.sizeof(PrometheusW4Matrix)
+_W4_GEMM_SIZE = ctypes.sizeof(PrometheusW4GemmRequest)
+_MOE_SIZE = ctypes.sizeof(PrometheusMoeRequest)
+_ROPE_SIZE = ctypes.sizeof(PrometheusRopeRequest)
+_RESIDUAL_NORM_SIZE = ctypes.sizeof(PrometheusResidualNormRequest)
 
 
 def kv4_cache(pool: int, page_table: int, lengths: int, head_dim: int, kv_heads: int, pages: int, sequences: int,
@@ -1722,6 +1844,28 @@ def kv4_cache(pool: int, page_table: int, lengths: int, head_dim: int, kv_heads:
 def kv4_page_bytes(head_dim: int, kv_heads: int, lib: Optional[ctypes.CDLL] = None) -> int:
     """Bytes of one page of the 4-bit cache; 0 for sizes it does not take."""
     return int((lib or shared_library()).prometheus_reactor_kv4_page_bytes(head_dim, kv_heads))
+
+
+def w4_matrix(data: int, n: int, k: int, group: int, count: int = 1) -> PrometheusW4Matrix:
+    """`count` weight matrices [n, k] in 4 bits that a program keeps in its own device memory: count * w4_bytes bytes."""
+    return PrometheusW4Matrix(_W4_MATRIX_SIZE, n, k, group, count, 0, data)
+
+
+def w4_bytes(n: int, k: int, group: int, lib: Optional[ctypes.CDLL] = None) -> int:
+    """Bytes of a weight matrix in 4 bits; 0 for sizes it does not take."""
+    return int((lib or shared_library()).prometheus_reactor_w4_bytes(n, k, group))
+
+
+def rope_turns(rotary_dim: int, base: float = 10000.0, kind: int = ROPE_SCALE_NONE, factor: float = 1.0,
+               context: float = 0.0, fast_turns: float = 32.0, slow_turns: float = 1.0,
+               lib: Optional[ctypes.CDLL] = None) -> Tuple[np.ndarray, float]:
+    """Revolutions a token of each channel pair (binary64 [rotary_dim / 2]) and the magnitude, for rope_device."""
+    scaling = PrometheusRopeScaling(ctypes.sizeof(PrometheusRopeScaling), rotary_dim, kind, 0, base, factor, context,
+                                    fast_turns, slow_turns)
+    turns, magnitude = np.empty(max(0, rotary_dim) // 2, np.float64), c_float(0.0)
+    if (lib or shared_library()).prometheus_reactor_rope_turns(byref(scaling), turns.ctypes.data, byref(magnitude)) != PROM_OK:
+        raise ReactorIssue("invalid_argument", "rope_turns: arguments outside their ranges")
+    return turns, float(magnitude.value)
 
 
 def sgemm_plan(m: int, n: int, k: int, lib: Optional[ctypes.CDLL] = None) -> Tuple[int, PrometheusSgemmPlanInfo]:
