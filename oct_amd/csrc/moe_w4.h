@@ -5,7 +5,7 @@
 
 namespace prom {
 
-constexpr int kMoeMaxExperts = 1024, kMoeMaxTopK = 64;
+constexpr int kMoeMaxExperts = 1024, kMoeMaxTopK = 64, kMoeMaxPairs = 65536;
 
 struct MoeExpert {
   int expert, start, count, unused;  // its pairs: pairs[start] ..
@@ -22,16 +22,16 @@ struct W4MoeArgs {
   int tokens, experts, top_k;
   bool renormalise;
   // workspace
-  double* logits;  // [tokens][experts]
+  double* logits;   // [tokens][experts]
   int32_t* chosen;  // [pairs], pairs = tokens * top_k
   float* weights;   // [pairs]
   int32_t* pairs;   // by expert
-  MoeExpert* reached;
-  int32_t* reached_count;
-  uint16_t* hidden;  // terms of [pairs][hidden_stride], hidden_plane elements apart
+  MoeExpert* reached;  // min(experts, pairs), those behind the last with count 0
+  uint16_t* hidden;    // terms of [pairs][hidden_stride], hidden_plane elements apart
   size_t hidden_plane;
-  uint32_t hidden_stride;
-  float* part;  // [pairs][hidden width]
+  uint32_t hidden_stride;  // whole tiles of 128
+  float* part;             // [slices][tokens][hidden width] (few tokens) or [pairs][hidden width]
+  int slices, split;       // of the second product (few tokens)
 };
 
 // Bytes of the workspace; sets the pointers into `base`.
