@@ -6,6 +6,7 @@
 namespace prom {
 
 constexpr int kMoeMaxExperts = 1024, kMoeMaxTopK = 64, kMoeMaxPairs = 65536;
+constexpr int kMoeFewTokens = 64;  // a token a lane
 
 struct MoeExpert {
   int expert, start, count, unused;  // its pairs: pairs[start] ..
@@ -25,13 +26,14 @@ struct W4MoeArgs {
   double* logits;   // [tokens][experts]
   int32_t* chosen;  // [pairs], pairs = tokens * top_k
   float* weights;   // [pairs]
-  int32_t* pairs;   // by expert
-  MoeExpert* reached;  // min(experts, pairs), those behind the last with count 0
+  uint8_t* places;  // [tokens][experts]: 1 + an expert's place among the token's, 0 where it is none (few tokens)
+  int32_t* pairs;   // by expert (more tokens)
+  MoeExpert* reached;  // min(experts, pairs), those behind the last with count 0 (more tokens)
   uint16_t* hidden;    // terms of [pairs][hidden_stride], hidden_plane elements apart
   size_t hidden_plane;
   uint32_t hidden_stride;  // whole tiles of 128
   float* part;             // [slices][tokens][hidden width] (few tokens) or [pairs][hidden width]
-  int slices, split;       // of the second product (few tokens)
+  int out_tiles, slices, split;  // of the second product (few tokens)
 };
 
 // Bytes of the workspace; sets the pointers into `base`.
