@@ -256,6 +256,7 @@ PROM_REACTOR_API int prometheus_reactor_runtime_residual_norm_device(void* handl
   a.residual_scale = r->residual_scale;
   a.weight_offset = r->weight_offset;
   a.eps = r->eps;
+  a.over_width = 1.0 / r->width;
   a.gate_tanh = r->gate_tanh != 0u;
   DeviceContext& cx = ctx();
   std::lock_guard<std::mutex> lock(cx.mu);

@@ -374,6 +374,7 @@ struct ResidualNormArgs {
   void *h_out, *out;
   uint32_t rows, width, h_stride, y_stride, h_out_stride, out_stride, vector_stride, rows_per_vector;
   float residual_scale, weight_offset, eps;
+  double over_width;  // 1 / width
   bool gate_tanh;
 };
 constexpr uint32_t kResidualNormMaxWidth = 32768;

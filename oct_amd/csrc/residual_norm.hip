@@ -4,41 +4,69 @@
 //
 // A row is read once into registers and both norms are taken from there: bound by memory, and for the few rows of
 // a decode step by the chain of two sums over a workgroup.  Squares are summed in binary64, which holds those of every
-// fp32 number.  The second norm is that of h' before it is rounded to a bf16 row.
+// fp32 number.  The second norm is that of h' before it is rounded to a bf16 row.  A workgroup takes neighbouring rows and
+// keeps what they share, the weights and vectors joined to a factor of y, a factor of h' and a summand, in registers (read
+// again for each row, 4224 rows of 3840 in bf16 took 53 us); the next row is loaded meanwhile.  Those rows take 31 us, 130 MB at
+// 4.2 TB/s; a large copy runs at 5.1.
 #include <algorithm>
 
 #include "reactor_internal.h"
+#include "wave_ops.h"
 
 namespace prom {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Eight values from p (any alignment of T), zeros from the left-th on.
-__device__ __forceinline__ void load8(const float* p, int left, float (&v)[8]) {
-  if (left >= 8) {
-    __builtin_memcpy(v, p, 32);
-  } else {
+// Eight values of a row as they lie in memory.
+template <typename T>
+struct Raw;
+template <>
+struct Raw<float> {
+  float v[8];
+  __device__ __forceinline__ void get(float (&to)[8]) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.0f;
+    for (int j = 0; j < 8; ++j) to[j] = v[j];
   }
-}
-__device__ __forceinline__ void load8(const uint16_t* p, int left, float (&v)[8]) {
-  if (left >= 8) {
-    u32x4 w;
-    __builtin_memcpy(&w, p, 16);
+};
+template <>
+struct Raw<uint16_t> {
+  u32x4 w;
+  __device__ __forceinline__ void get(float (&to)[8]) const {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __uint_as_float(w[j] << 16);
-      v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      to[2 * j] = __uint_as_float(w[j] << 16);
+      to[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
     }
+  }
+};
+// From p (any alignment of T), zeros from the left-th on; kWhole: all eight are there.
+template <bool kWhole>
+__device__ __forceinline__ Raw<float> load8(const float* p, int left) {
+  Raw<float> r;
+  if (kWhole || left >= 8) {
+    __builtin_memcpy(r.v, p, 32);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < left ? __uint_as_float((uint32_t)p[j] << 16) : 0.0f;
+    for (int j = 0; j < 8; ++j) r.v[j] = j < left ? p[j] : 0.0f;
   }
+  return r;
 }
+template <bool kWhole>
+__device__ __forceinline__ Raw<uint16_t> load8(const uint16_t* p, int left) {
+  Raw<uint16_t> r;
+  if (kWhole || left >= 8) {
+    __builtin_memcpy(&r.w, p, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      r.w[j] = (2 * j < left ? (uint32_t)p[2 * j] : 0u) | (2 * j + 1 < left ? (uint32_t)p[2 * j + 1] << 16 : 0u);
+  }
+  return r;
+}
+template <bool kWhole>
 __device__ __forceinline__ void store8(float* p, int left, const float (&v)[8]) {
-  if (left >= 8) {
+  if (kWhole || left >= 8) {
     __builtin_memcpy(p, v, 32);
   } else {
 #pragma unroll
@@ -46,11 +74,12 @@ __device__ __forceinline__ void store8(float* p, int left, const float (&v)[8]) 
       if (j < left) p[j] = v[j];
   }
 }
+template <bool kWhole>
 __device__ __forceinline__ void store8(uint16_t* p, int left, const float (&v)[8]) {
   __bf16 w[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) w[j] = (__bf16)v[j];
-  if (left >= 8) {
+  if (kWhole || left >= 8) {
     __builtin_memcpy(p, w, 16);
   } else {
 #pragma unroll
@@ -62,8 +91,7 @@ __device__ __forceinline__ void store8(uint16_t* p, int left, const float (&v)[8
 // The sum over a row's lanes, in every lane.
 template <int kWaves>
 __device__ __forceinline__ double row_sum(double v, double (&part)[kWaves]) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  v = wave_sum(v);
   if constexpr (kWaves > 1) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -73,125 +101,159 @@ __device__ __forceinline__ double row_sum(double v, double (&part)[kWaves]) {
   }
   return v;
 }
-
-template <int kChunks>
-__device__ __forceinline__ double squares(const float (&v)[kChunks][8]) {
-  double s = 0.0;
-#pragma unroll
-  for (int i = 0; i < kChunks; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s = __builtin_fma((double)v[i][j], (double)v[i][j], s);
-  return s;
+// 1 / sqrt(mean + eps) of a sum of squares, over = 1 / width: the instruction's value is within 2^-23 or so, a step of
+// Newton's makes it 2^-45 (a division and a root in binary64 were a third of the kernel's time).  Where the step has no
+// value the root's is that of 0 or infinity, and stands.
+__device__ __forceinline__ float inverse_size(double sum, double over, float eps) {
+  const double x = __builtin_fma(sum, over, (double)eps), r = __builtin_amdgcn_rsq(x), e = __builtin_fma(-x * r, r, 1.0);
+  return (float)(e == e ? __builtin_fma(0.5 * r, e, r) : r);
 }
 
-// kWaves waves a row (with one, four rows a workgroup), kChunks groups of eight values a lane.
-template <typename T, int kWaves, int kChunks>
-__global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm_kernel(const ResidualNormArgs a) {
+// The squares' sum of eight values of which there are `left`, if any; what lies behind them is zero where it is not a repeat.
+__device__ __forceinline__ double squares(const float (&v)[8], int left) {
+  double sum = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum = __builtin_fma((double)v[j], (double)v[j], sum);
+  return left > 0 ? sum : 0.0;
+}
+
+// kWaves waves a row (with one, four rows a workgroup at once), kChunks groups of eight values a lane.  A workgroup takes rows
+// blockIdx.x * share ..  kWhole: the width is whole eights; the lanes behind it load the last eight and leave them out, so that
+// nothing branches between a load and its use (there the compiler waited for the row's stores too: 42 us instead of 31).
+template <typename T, int kWaves, int kChunks, bool kWhole>
+__global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm_kernel(const ResidualNormArgs a,
+                                                                                         uint32_t share) {
   constexpr int kRows = kWaves == 1 ? 4 : 1, kLanes = 64 * kWaves;
-  __shared__ double part[2][kWaves];
+  __shared__ double part[2][2][kWaves];
   const int lane = kWaves == 1 ? (int)threadIdx.x & 63 : (int)threadIdx.x;
   const int width = (int)a.width;
-  for (size_t row = (size_t)blockIdx.x * kRows + (kWaves == 1 ? threadIdx.x >> 6 : 0); row < a.rows;
-       row += (size_t)gridDim.x * kRows) {
-    const T* h_row = static_cast<const T*>(a.h) + row * a.h_stride;
+  int at[kChunks], left[kChunks];
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    at[i] = 8 * (lane + kLanes * i);
+    left[i] = max(width - at[i], 0);
+    at[i] = min(at[i], kWhole ? width - 8 : width);
+  }
+  uint32_t row = blockIdx.x * share + (kWaves == 1 ? threadIdx.x >> 6 : 0);
+  const uint32_t end = min(a.rows, (blockIdx.x + 1) * share);
+  if (row >= end) return;  // with several waves all agree
+  Raw<T> h_next[kChunks], y_next[kChunks];
+  const auto fetch = [&](uint32_t r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      h_next[i] = load8<kWhole>(static_cast<const T*>(a.h) + (size_t)r * a.h_stride + at[i], left[i]);
+      if (a.y != nullptr) y_next[i] = load8<kWhole>(static_cast<const T*>(a.y) + (size_t)r * a.y_stride + at[i], left[i]);
+    }
+  };
+  fetch(row);
+  float fy[kChunks][8], fh[kChunks][8], add[kChunks][8];
+  uint32_t vector = 0xFFFFFFFFu;  // the vectors that the factors are of
+  int turn = 0;
+  for (; row < end; row += kRows) {
+    if (row / a.rows_per_vector != vector) {
+      vector = row / a.rows_per_vector;
+      const size_t from = (size_t)vector * a.vector_stride;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) fy[i][j] = a.residual_scale, fh[i][j] = 1.0f, add[i][j] = 0.0f;
+        if (a.post != nullptr) {
+          load8<kWhole>(a.post + at[i], left[i]).get(v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) fy[i][j] *= a.weight_offset + v[j];
+        }
+        if (a.gate != nullptr) {
+          load8<kWhole>(static_cast<const T*>(a.gate) + from + at[i], left[i]).get(v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) fy[i][j] *= a.gate_tanh ? tanhf(v[j]) : v[j];
+        }
+        if (a.pre != nullptr) {
+          load8<kWhole>(a.pre + at[i], left[i]).get(v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) fh[i][j] = a.weight_offset + v[j];
+        }
+        if (a.scale != nullptr) {
+          load8<kWhole>(static_cast<const T*>(a.scale) + from + at[i], left[i]).get(v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) fh[i][j] *= 1.0f + v[j];
+        }
+        if (a.shift != nullptr) load8<kWhole>(static_cast<const T*>(a.shift) + from + at[i], left[i]).get(add[i]);
+      }
+    }
     float h[kChunks][8], y[kChunks][8];
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int at = 8 * (lane + kLanes * i);
-      load8(h_row + min(at, width), width - at, h[i]);
+      h_next[i].get(h[i]);
+      if (a.y != nullptr) y_next[i].get(y[i]);
     }
-    const size_t vector = (size_t)(row / a.rows_per_vector) * a.vector_stride;
+    if (row + kRows < end) fetch(row + kRows);
+    const uint32_t now = row;
     if (a.y != nullptr) {
-      const T* y_row = static_cast<const T*>(a.y) + row * a.y_stride;
+      float r = 1.0f;
+      if (a.post != nullptr) {
+        double sum = 0.0;
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int at = 8 * (lane + kLanes * i);
-        load8(y_row + min(at, width), width - at, y[i]);
+        for (int i = 0; i < kChunks; ++i) sum += squares(y[i], left[i]);
+        r = inverse_size(row_sum<kWaves>(sum, part[0][turn]), a.over_width, a.eps);
       }
-      float r = a.residual_scale;
-      if (a.post != nullptr) r *= (float)(1.0 / sqrt(row_sum<kWaves>(squares(y), part[0]) / width + (double)a.eps));
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int at = 8 * (lane + kLanes * i), left = width - at;
-        float f[8];
+      for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = r;
-        if (a.post != nullptr) {
-          float w[8];
-          load8(a.post + min(at, width), left, w);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] *= a.weight_offset + w[j];
-        }
-        if (a.gate != nullptr) {
-          float g[8];
-          load8(static_cast<const T*>(a.gate) + vector + min(at, width), left, g);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] *= a.gate_tanh ? tanhf(g[j]) : g[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[i][j] = __builtin_fmaf(y[i][j], f[j], h[i][j]);
-      }
+        for (int j = 0; j < 8; ++j) h[i][j] = __builtin_fmaf(y[i][j] * r, fy[i][j], h[i][j]);
     }
     if (a.h_out != nullptr) {
-      T* to = static_cast<T*>(a.h_out) + row * a.h_out_stride;
+      T* to = static_cast<T*>(a.h_out) + (size_t)now * a.h_out_stride;
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int at = 8 * (lane + kLanes * i);
-        if (at < width) store8(to + at, width - at, h[i]);
-      }
+      for (int i = 0; i < kChunks; ++i)
+        if (left[i] > 0) store8<kWhole>(to + at[i], left[i], h[i]);
     }
     if (a.out != nullptr) {
-      T* to = static_cast<T*>(a.out) + row * a.out_stride;
-      const float r = (float)(1.0 / sqrt(row_sum<kWaves>(squares(h), part[1]) / width + (double)a.eps));
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) sum += squares(h[i], left[i]);
+      const float r = inverse_size(row_sum<kWaves>(sum, part[1][turn]), a.over_width, a.eps);
+      T* to = static_cast<T*>(a.out) + (size_t)now * a.out_stride;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const int at = 8 * (lane + kLanes * i), left = width - at;
-        float f[8];
+        float o[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = h[i][j] * r;
-        if (a.pre != nullptr) {
-          float w[8];
-          load8(a.pre + min(at, width), left, w);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] *= a.weight_offset + w[j];
+        for (int j = 0; j < 8; ++j) {
+          o[j] = h[i][j] * r * fh[i][j];
+          if (a.shift != nullptr) o[j] += add[i][j];
         }
-        if (a.scale != nullptr) {
-          float s[8];
-          load8(static_cast<const T*>(a.scale) + vector + min(at, width), left, s);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] *= 1.0f + s[j];
-        }
-        if (a.shift != nullptr) {
-          float s[8];
-          load8(static_cast<const T*>(a.shift) + vector + min(at, width), left, s);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] += s[j];
-        }
-        if (left > 0) store8(to + at, left, f);
+        if (left[i] > 0) store8<kWhole>(to + at[i], left[i], o);
       }
     }
-    if constexpr (kWaves > 1) __syncthreads();  // the parts are read
+    // Parts are written again two rows on: a barrier of the next row lies between, if rows have any.
+    turn ^= 1;
   }
 }
 
-template <typename T>
+template <typename T, bool kWhole>
 hipError_t launch(const ResidualNormArgs& a, hipStream_t stream) {
-  const unsigned one = (unsigned)std::min<uint64_t>(a.rows, 1u << 20);
-  const unsigned four = (unsigned)std::min<uint64_t>((a.rows + 3ull) / 4, 1u << 20);
-#define ROWS(W, C, grid, block) \
-  hipLaunchKernelGGL((residual_norm_kernel<T, W, C>), dim3(grid), dim3(block), 0, stream, a)
+#define ROWS(W, C, WGS)                                                                                                 \
+  {                                                                                                                     \
+    const uint32_t at_once = W == 1 ? 4u : 1u, groups = (a.rows + at_once - 1) / at_once;                               \
+    const uint32_t share = (groups + WGS - 1) / WGS * at_once;                                                          \
+    hipLaunchKernelGGL((residual_norm_kernel<T, W, C, kWhole>), dim3((a.rows + share - 1) / share), dim3(W == 1 ? 256 : 64 * W), 0, \
+                       stream, a, share);                                                                               \
+  }
+  // Waves a row as few as hold it in 8 or 16 values a lane (4 waves of 16 values took 35 us where 8 of 8 took 31, at a width
+  // of 3840), and about as many workgroups as run at once: with twice as many their first rows' latency and the joining of
+  // the vectors came twice (34 us).
   if (a.width <= 512)
-    ROWS(1, 1, four, 256);
+    ROWS(1, 1, 1024)
   else if (a.width <= 2048)
-    ROWS(4, 1, one, 256);
+    ROWS(4, 1, 1024)
   else if (a.width <= 4096)
-    ROWS(8, 1, one, 512);
+    ROWS(8, 1, 512)
   else if (a.width <= 8192)
-    ROWS(8, 2, one, 512);
+    ROWS(8, 2, 512)
   else if (a.width <= 16384)
-    ROWS(16, 2, one, 1024);
+    ROWS(16, 2, 256)
   else
-    ROWS(16, 4, one, 1024);
+    ROWS(16, 4, 256)
 #undef ROWS
   return hipGetLastError();
 }
@@ -199,7 +261,8 @@ hipError_t launch(const ResidualNormArgs& a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_residual_norm(const ResidualNormArgs& a, bool bf16, hipStream_t stream) {
-  return bf16 ? launch<uint16_t>(a, stream) : launch<float>(a, stream);
+  if (a.width % 8 == 0) return bf16 ? launch<uint16_t, true>(a, stream) : launch<float, true>(a, stream);
+  return bf16 ? launch<uint16_t, false>(a, stream) : launch<float, false>(a, stream);
 }
 
 }  // namespace prom
