@@ -59,6 +59,9 @@ __device__ __forceinline__ void store8(uint16_t* p, int left, const float (&v)[8
 // Where word j (columns 8 j .. 8 j + 7) of row r of a tile lies, in words.
 __device__ __forceinline__ int tile_word(int r, int j) { return 4 * (16 * (j & 3) + r) + (j >> 2); }
 
+// Between a wave's LDS operations on words that only it uses: they are done in the program's order.
+__device__ __forceinline__ void own_lds() { asm volatile("" ::: "memory"); }
+
 template <typename T, int kGroup, bool kPack>
 __global__ __launch_bounds__(256) void w4_tiles_kernel(const W4View w, T* __restrict__ rows, uint32_t stride) {
   constexpr int kSteps = kW4TileK / kGroup, kLanes = kGroup / 8;
@@ -66,42 +69,52 @@ __global__ __launch_bounds__(256) void w4_tiles_kernel(const W4View w, T* __rest
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   const int j = lane & 15;  // eight columns of a row
   const unsigned long long per = (unsigned long long)w.tiles_n * w.tiles_k, tiles = per * w.count;
-  // Every wave of a workgroup makes the same number of rounds (barriers).
-  for (unsigned long long first = 4ull * blockIdx.x; first < tiles; first += 4ull * gridDim.x) {
-    const unsigned long long tile = first + wave;
-    const bool live = tile < tiles;
-    const int e = (int)((live ? tile : 0) / per);
-    const unsigned long long in = (live ? tile : 0) - e * per;
+  for (unsigned long long tile = 4ull * blockIdx.x + wave; tile < tiles; tile += 4ull * gridDim.x) {
+    const int e = (int)(tile / per);
+    const unsigned long long in = tile - e * per;
     const int tn = (int)(in / w.tiles_k), tk = (int)(in - (unsigned long long)tn * w.tiles_k);
     uint32_t* codes = reinterpret_cast<uint32_t*>(w.data + e * w.stride + in * kW4TileBytes);
     uint16_t* steps = reinterpret_cast<uint16_t*>(w.data + e * w.stride + per * kW4TileBytes) + in * (kW4TileN * kSteps);
-    const int k = tk * kW4TileK + 8 * j, left = w.k - k;
-    if constexpr (!kPack) {
-      u32x4 mine{};
-      if (live) mine = reinterpret_cast<const u32x4*>(codes)[lane];
-      *reinterpret_cast<u32x4*>(&words[wave][4 * lane]) = mine;
-      __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 4 * i + (lane >> 4), n = tn * kW4TileN + r;
-      const bool inside = live && n < w.n && left > 0;
-      T* at = rows + ((size_t)e * w.n + (inside ? n : 0)) * stride + (inside ? k : 0);
-      float v[8];
-      if constexpr (kPack) {
-        load8(at, inside ? left : 0, v);
-        uint32_t param;
-        words[wave][tile_word(r, j)] = fp4_codes(v, max_of_lanes<kLanes>(max_bits(v)), &param);
-        if (live && j % kLanes == 0) steps[r * kSteps + j / kLanes] = (uint16_t)param;
-      } else if (inside) {
-        fp4_values(words[wave][tile_word(r, j)], steps[r * kSteps + j / kLanes], v);
-        store8(at, left, v);
-      }
-    }
-    __syncthreads();
+    const int k = tk * kW4TileK + 8 * j, row = tn * kW4TileN + (lane >> 4);
+    const bool whole = tn * kW4TileN + kW4TileN <= w.n && tk * kW4TileK + kW4TileK <= w.k;
+    T* const at = rows + ((size_t)e * w.n + row) * stride + k;  // formed, not read, behind the last row or column
+    float v[4][8];
     if constexpr (kPack) {
-      if (live) reinterpret_cast<u32x4*>(codes)[lane] = *reinterpret_cast<const u32x4*>(&words[wave][4 * lane]);
-      __syncthreads();
+      // The four loads are on their way together where no row or column is missing.
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load8(at + (size_t)(4 * i) * stride, 8, v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load8(at + (size_t)(4 * i) * stride, row + 4 * i < w.n ? w.k - k : 0, v[i]);
+      }
+      own_lds();  // the words of the tile before are read
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * i + (lane >> 4);
+        uint32_t param;
+        words[wave][tile_word(r, j)] = fp4_codes(v[i], max_of_lanes<kLanes>(max_bits(v[i])), &param);
+        if (j % kLanes == 0) steps[r * kSteps + j / kLanes] = (uint16_t)param;
+      }
+      own_lds();
+      reinterpret_cast<u32x4*>(codes)[lane] = *reinterpret_cast<const u32x4*>(&words[wave][4 * lane]);
+    } else {
+      const u32x4 mine = reinterpret_cast<const u32x4*>(codes)[lane];
+      uint32_t step[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) step[i] = steps[(4 * i + (lane >> 4)) * kSteps + j / kLanes];
+      own_lds();
+      *reinterpret_cast<u32x4*>(&words[wave][4 * lane]) = mine;
+      own_lds();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fp4_values(words[wave][tile_word(4 * i + (lane >> 4), j)], step[i], v[i]);
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) store8(at + (size_t)(4 * i) * stride, 8, v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) store8(at + (size_t)(4 * i) * stride, row + 4 * i < w.n ? w.k - k : 0, v[i]);
+      }
     }
   }
 }
