@@ -32,8 +32,11 @@ struct W4MoeArgs {
   uint16_t* hidden;    // terms of [pairs][hidden_stride], hidden_plane elements apart
   size_t hidden_plane;
   uint32_t hidden_stride;  // whole tiles of 128
-  float* part;             // [slices][tokens][hidden width] (few tokens) or [pairs][hidden width]
-  int out_tiles, slices, split;  // of the second product (few tokens)
+  float* part;             // [column group][pairs][parts][columns of a group]
+  int out_tiles, split;    // of the second product
+  int parts;               // of K that leave sums of their own: split or 1
+  int blocks;              // of sixteen pairs of an expert, taken at once
+  bool joins;              // the second product's last workgroups join the sums
 };
 
 // Bytes of the workspace; sets the pointers into `base`.

@@ -2,17 +2,18 @@
 //   l = x router^T, a token's experts the top_k largest l (ties to the lower expert), p their softmax weights,
 //   out = sum_e p_e (act(x gate_e^T) * (x up_e^T)) down_e^T.
 //
-// Three launches.  The router: a wave makes an expert's logits of four tokens, in binary64 (a choice between two close
-// experts does not depend on the order of a sum); the last workgroup of four tokens' (tickets.h) chooses their experts, and
-// the last of those lists the pairs, a token with one of its experts, by expert.  The hidden columns: a workgroup takes 16
-// of one reached expert, its gate and up weights once for sixteen pairs at a time (w4_product.h), and leaves the hidden
-// rows as bf16 terms, in the form that the second product multiplies.  The output columns: a workgroup takes 16 of all
-// experts, its waves an expert (or a part of its K) each, weighs their sums and adds them by token in LDS.  Above 64 tokens
-// the products' sums by pair go to memory and are joined in a fourth launch.
+// Three launches.  The router: a wave makes an expert's logits of two tokens, in binary64 (a choice between two close
+// experts does not depend on the order of a sum); the last workgroup of two tokens' (tickets.h) chooses their experts.  The
+// hidden columns: a workgroup takes 32 of one reached expert, its gate and up weights once for sixteen pairs, a token with
+// one of its experts (w4_product.h), and leaves the hidden rows as bf16 terms, in the form that the second product
+// multiplies.  The output columns: a wave takes 32 or 64 of an expert (or of a part of its K) and leaves its sums by pair; the
+// last workgroup of those columns weighs and joins them in the order of a token's experts.  Up to 64 tokens each wave looks
+// up itself which of them chose its expert; above, the router's last workgroup lists the pairs by expert, and the sums are joined in
+// a fourth launch.
 //
 // Bound by the reached experts' weights, and for a token by the latency of three kernels that follow one another.  64
-// experts of 1024 with 2048 outer columns, 8 a token, in bf16: a token 6.4 + 6.0 + 6.6 us (28 MB at 2.2 TB/s in the last two), 64
-// tokens, which reach all experts, 10.2 + 33.5 + 28.5 us (214 MB at 3.5 TB/s; 64 rows of x and of the hidden columns come from L2
+// experts of 1024 with 2048 outer columns, 8 a token, in bf16: a token 6.4 + 5.4 + 6.6 us (28 MB at 2.4 TB/s in the last two), 64
+// tokens, which reach all experts, 9.8 + 33.2 + 24.1 us (214 MB at 3.7 TB/s; 64 rows of x and of the hidden columns come from L2
 // for each workgroup).
 #include <algorithm>
 
@@ -66,9 +67,9 @@ __device__ __forceinline__ float activation(float g, uint32_t kind) {
 }
 
 // ------------------------------------------------------------------ the router
-constexpr int kTokenBlock = 4;
+constexpr int kTokenBlock = 2;
 __device__ uint32_t moe_tickets[kMoeMaxPairs / kTokenBlock + 1];  // of blocks of tokens, and of the blocks
-constexpr int kColumnTickets = 256, kMaxSlices = 8;
+constexpr int kColumnTickets = 1024;
 constexpr int kHiddenTiles = 2, kHiddenWaves = 4, kOutWaves = 8;
 __device__ uint32_t moe_column_tickets[kColumnTickets];
 
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_hidden_kernel(const W4MoeArgs
   __shared__ int32_t lists[kFew ? kWaves : 1][kFew ? kMoeFewTokens : 1];
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const Reached ex = Reached::find<kFew>(a, (int)blockIdx.y, lists[kFew ? wave : 0]);
-  if (ex.count == 0) return;
+  if (16 * (int)blockIdx.z >= ex.count) return;
   const int tiles_k = a.gate.tiles_k;
   const u32x4* codes[2 * kTiles];
   const uint16_t* steps[2 * kTiles];
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_hidden_kernel(const W4MoeArgs
     steps[2 * i] = w4_steps<kSteps>(a.gate, ex.expert, tile);
     steps[2 * i + 1] = w4_steps<kSteps>(a.up, ex.expert, tile);
   }
-  for (int block = 0; block < ex.count; block += 16) {
+  for (int block = 16 * (int)blockIdx.z; block < ex.count; block += 16 * (int)gridDim.z) {
     W4Tile<kSteps, 2 * kTiles> first;
     first.fetch(codes, steps, min(wave, tiles_k - 1));
     const int rows = min(ex.count - block, 16);
@@ -318,7 +319,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_hidden_kernel(const W4MoeArgs
     x[0].p = static_cast<const T*>(a.x) + (size_t)((unsigned)mine / (unsigned)a.top_k) * a.x_stride;
     floatx4 acc[1][2 * kTiles] = {};
     w4_accumulate<kSteps, 2 * kTiles, 1, kEdge>(codes, steps, first, x, wave, tiles_k, kWaves, a.gate.k, acc);
-    if (block > 0) __syncthreads();  // the sums before are read
+    if (block >= 16 * (int)gridDim.z) __syncthreads();  // the sums before are read
 #pragma unroll
     for (int i = 0; i < 2 * kTiles; ++i)
 #pragma unroll
@@ -342,25 +343,85 @@ __global__ __launch_bounds__(64 * kWaves) void moe_hidden_kernel(const W4MoeArgs
   }
 }
 
-// Few tokens: output columns 16 kNT blockIdx.x .. .  A unit is a part of K of a slot; those of slice blockIdx.y are dealt to
-// the waves, which weigh their sums and add them by token in LDS, each in its own place.
-template <typename T, int kSteps, int kNT, int kWaves>
-__global__ __launch_bounds__(64 * kWaves) void moe_out_kernel(const W4MoeArgs a) {
+// The pairs' sums of a column group by token, weighed, in the order of the token's experts: items `first`, first + step .. of two
+// columns.  kItems times kSums loads are on their way together: they come from behind the L2 caches.
+template <typename T, int kColumns, int kItems, int kSums>
+__device__ __forceinline__ void join_some(const W4MoeArgs& a, const float* sums, int column0, int first, int step) {
+  constexpr int kTwos = kColumns / 2;
+  const int items = a.tokens * kTwos, parts = a.top_k * a.parts;
+  for (int at0 = first; at0 < items; at0 += kItems * step) {
+    float v[kItems] = {}, u[kItems] = {};
+    for (int q0 = 0; q0 < parts; q0 += kSums) {
+      unsigned long long both[kItems][kSums];
+      float w[kItems][kSums];
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int at = min(at0 + i * step, items - 1), token = at / kTwos;
+#pragma unroll
+        for (int q = 0; q < kSums; ++q) {
+          const int part = min(q0 + q, parts - 1);
+          both[i][q] = load_agent(reinterpret_cast<const unsigned long long*>(
+              sums + ((size_t)token * parts + part) * kColumns + 2 * (at - token * kTwos)));
+          w[i][q] = a.weights[token * a.top_k + part / a.parts];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kItems; ++i)
+#pragma unroll
+        for (int q = 0; q < kSums; ++q)
+          if (q0 + q < parts) {
+            v[i] = __builtin_fmaf(w[i][q], __uint_as_float((uint32_t)both[i][q]), v[i]);
+            u[i] = __builtin_fmaf(w[i][q], __uint_as_float((uint32_t)(both[i][q] >> 32)), u[i]);
+          }
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int at = at0 + i * step, token = at / kTwos, c = column0 + 2 * (at - token * kTwos);
+      if (at >= items) break;
+      T* to = static_cast<T*>(a.out) + (size_t)token * a.out_stride + c;
+      if (c < a.down.n) put(to, v[i]);
+      if (c + 1 < a.down.n) put(to + 1, u[i]);
+    }
+  }
+}
+template <typename T, int kColumns>
+__device__ __forceinline__ void join(const W4MoeArgs& a, const float* sums, int column0, int first, int step) {
+  if (a.top_k * a.parts <= 8)
+    join_some<T, kColumns, 4, 8>(a, sums, column0, first, step);
+  else
+    join_some<T, kColumns, 1, 32>(a, sums, column0, first, step);
+}
+
+// Output columns 16 kNT blockIdx.x .. .  A unit is a part of K of a slot, a wave's; it leaves its sums by pair.  Where parts of K
+// have a block of pairs at most (kParts), the slot's waves, neighbours in a workgroup, join their sums first.  Few tokens: the
+// last workgroup of a column group joins the pairs' sums.
+template <typename T, int kSteps, int kNT, bool kFew, bool kParts>
+__global__ __launch_bounds__(64 * kOutWaves) void moe_out_kernel(const W4MoeArgs a) {
   typedef W4RowsTerms<Kind<T>::kHiddenTerms> X;
-  constexpr int kColumns = 16 * kNT, kPart = kMoeFewTokens * kColumns;
-  extern __shared__ float sums[];  // [kWaves][tokens][kColumns]
-  __shared__ int32_t lists[kWaves][kMoeFewTokens];
+  constexpr int kColumns = 16 * kNT;
+  __shared__ int32_t lists[kFew ? kOutWaves : 1][kFew ? kMoeFewTokens : 1];
+  __shared__ float others[kParts ? kOutWaves : 1][kNT][4][64];
   __shared__ uint32_t ticket;
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int tiles_k = a.down.tiles_k, slots = min(a.experts, a.tokens * a.top_k);
-  const int count = a.tokens * kColumns;
-  float* own = sums + wave * count;
-  for (int at = lane; at < count; at += 64) own[at] = 0.0f;
-  for (int unit = (int)blockIdx.y * kWaves + wave; unit < slots * a.split; unit += kWaves * a.slices) {
-    const int slot = unit / a.split, part = unit - slot * a.split;
-    const Reached ex = Reached::find<true>(a, slot, lists[wave]);
+  const int tiles_k = a.down.tiles_k, pairs = a.tokens * a.top_k, units = min(a.experts, pairs) * a.split;
+  const int unit = (int)blockIdx.y * kOutWaves + wave, slot = unit / a.split, part = unit - slot * a.split;
+  float* const sums = a.part + (size_t)blockIdx.x * pairs * a.parts * kColumns;  // [pair][part][kColumns]
+  floatx4 acc[1][kNT];
+  int mine = 0, rows = 0;
+  const auto leave = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      // Row 4 (lane / 16) + r: its pair is with the lane of that number.
+      const int row = 4 * (lane >> 4) + r;
+      float* const to = sums + ((size_t)__shfl(mine, row) * a.parts + at) * kColumns + (lane & 15);
+      if (row < rows)
+#pragma unroll
+        for (int i = 0; i < kNT; ++i) store_agent(to + 16 * i, acc[0][i][r]);
+    }
+  };
+  if (unit < units) {
+    const Reached ex = Reached::find<kFew>(a, slot, lists[kFew ? wave : 0]);
     const int begin = tiles_k * part / a.split, end = tiles_k * (part + 1) / a.split;
-    if (ex.count == 0 || begin == end) continue;
     const u32x4* codes[kNT];
     const uint16_t* steps[kNT];
 #pragma unroll
@@ -369,106 +430,54 @@ __global__ __launch_bounds__(64 * kWaves) void moe_out_kernel(const W4MoeArgs a)
       codes[i] = w4_codes(a.down, ex.expert, tile);
       steps[i] = w4_steps<kSteps>(a.down, ex.expert, tile);
     }
-    for (int block = 0; block < ex.count; block += 16) {
+    for (int block = 16 * (int)blockIdx.z; block < ex.count; block += 16 * (int)gridDim.z) {
       W4Tile<kSteps, kNT> first;
       first.fetch(codes, steps, begin);
-      const int rows = min(ex.count - block, 16);
-      const int mine = ex.pairs[block + min(lane & 15, rows - 1)];
-      const float weight = a.weights[mine];
+      rows = min(ex.count - block, 16);
+      mine = ex.pairs[block + min(lane & 15, rows - 1)];
       X x[1];
       x[0].plane = a.hidden_plane;
       x[0].p = a.hidden + (size_t)mine * a.hidden_stride;
-      floatx4 acc[1][kNT] = {};
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) acc[0][i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
       w4_accumulate<kSteps, kNT, 1, kEdgeNone>(codes, steps, first, x, begin, end, 1, a.down.k, acc);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        // Row 4 (lane / 16) + r: its pair and weight are with the lane of that number.  An expert's rows are of different
-        // tokens.
-        const int row = 4 * (lane >> 4) + r;
-        const int token = (int)((unsigned)__shfl(mine, row) / (unsigned)a.top_k);
-        const float p = __shfl(weight, row);
-        if (row < rows)
-#pragma unroll
-          for (int i = 0; i < kNT; ++i) own[token * kColumns + 16 * i + (lane & 15)] += p * acc[0][i][r];
-      }
+      if constexpr (!kParts) leave(part);
     }
   }
-  __syncthreads();
-  const int column0 = (int)blockIdx.x * kColumns;
-  T* out = static_cast<T*>(a.out) + column0;
-  float* part = a.part + (size_t)blockIdx.x * a.slices * kPart;
-  for (int at = (int)threadIdx.x; at < count; at += 64 * kWaves) {
-    float v = sums[at];
+  if constexpr (kParts) {
+    if (part > 0 && rows > 0)
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) v += sums[w * count + at];
-    if (a.slices > 1)
-      store_agent(part + (size_t)blockIdx.y * kPart + at, v);
-    else if (column0 + at % kColumns < a.down.n)
-      put(out + (size_t)(at / kColumns) * a.out_stride + at % kColumns, v);
-  }
-  if (a.slices == 1 || !last_to_arrive(&moe_column_tickets[blockIdx.x], (uint32_t)a.slices, &ticket)) return;
-  for (int at = (int)threadIdx.x; at < count; at += 64 * kWaves) {
-    float p[kMaxSlices];
+      for (int i = 0; i < kNT; ++i)
 #pragma unroll
-    for (int s = 0; s < kMaxSlices; ++s) p[s] = s < a.slices ? load_agent(part + (size_t)s * kPart + at) : 0.0f;
-    float v = p[0];
-#pragma unroll
-    for (int s = 1; s < kMaxSlices; ++s) v += p[s];
-    if (column0 + at % kColumns < a.down.n) put(out + (size_t)(at / kColumns) * a.out_stride + at % kColumns, v);
-  }
-}
-
-// More tokens: output columns 16 blockIdx.x .. of reached expert blockIdx.y's pairs, and their sums by token.
-template <typename T, int kSteps>
-__global__ __launch_bounds__(256) void moe_down_kernel(const W4MoeArgs a) {
-  typedef W4RowsTerms<Kind<T>::kHiddenTerms> X;
-  __shared__ float sums[4][4][64];
-  const MoeExpert ex = a.reached[blockIdx.y];
-  if (ex.count == 0) return;
-  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int tile = (int)blockIdx.x, tiles_k = a.down.tiles_k;
-  const u32x4* const codes[1] = {w4_codes(a.down, ex.expert, tile)};
-  const uint16_t* const steps[1] = {w4_steps<kSteps>(a.down, ex.expert, tile)};
-  for (int block = 0; block < ex.count; block += 16) {
-    W4Tile<kSteps, 1> first;
-    first.fetch(codes, steps, min(wave, tiles_k - 1));
-    const int rows = min(ex.count - block, 16);
-    X x[1];
-    x[0].plane = a.hidden_plane;
-    x[0].p = a.hidden + (size_t)a.pairs[ex.start + block + min(lane & 15, rows - 1)] * a.hidden_stride;
-    floatx4 acc[1][1] = {};
-    w4_accumulate<kSteps, 1, 1, kEdgeNone>(codes, steps, first, x, wave, tiles_k, 4, a.down.k, acc);
-    if (block > 0) __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 4; ++r) sums[wave][r][lane] = acc[0][0][r];
+        for (int r = 0; r < 4; ++r) others[wave][i][r][lane] = acc[0][i][r];
     __syncthreads();
-    const int row = (int)threadIdx.x >> 4, n = tile * kW4TileN + ((int)threadIdx.x & 15);
-    const int r = row & 3, l = 16 * (row >> 2) + ((int)threadIdx.x & 15);
-    if (row < rows && n < a.down.n)
-      a.part[(size_t)a.pairs[ex.start + block + row] * a.down.n + n] =
-          sums[0][r][l] + sums[1][r][l] + sums[2][r][l] + sums[3][r][l];
+    if (part == 0 && rows > 0) {
+      for (int p = 1; p < a.split; ++p)
+#pragma unroll
+        for (int i = 0; i < kNT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[0][i][r] += others[wave + p][i][r][lane];
+      leave(0);
+    }
+  }
+  if constexpr (kFew) {
+    if (!a.joins || !last_to_arrive(&moe_column_tickets[blockIdx.x], gridDim.y, &ticket)) return;
+    join<T, kColumns>(a, sums, (int)blockIdx.x * kColumns, (int)threadIdx.x, 64 * kOutWaves);
   }
 }
 
-template <typename T>
+// Column groups blockIdx.x, and blockIdx.y's share of their tokens.
+template <typename T, int kNT>
 __global__ __launch_bounds__(256) void moe_join_kernel(const W4MoeArgs a) {
-  const unsigned long long count = (unsigned long long)a.tokens * (uint32_t)a.down.n;
-  for (unsigned long long at = blockIdx.x * 256ull + threadIdx.x; at < count; at += gridDim.x * 256ull) {
-    const unsigned long long t = at / (uint32_t)a.down.n;
-    const uint32_t n = (uint32_t)(at - t * (uint32_t)a.down.n);
-    float v = 0.0f;
-    for (int j = 0; j < a.top_k; ++j) {
-      const size_t pair = t * a.top_k + j;
-      v = __builtin_fmaf(a.weights[pair], a.part[pair * (uint32_t)a.down.n + n], v);
-    }
-    put(static_cast<T*>(a.out) + t * a.out_stride + n, v);
-  }
+  constexpr int kColumns = 16 * kNT;
+  join<T, kColumns>(a, a.part + (size_t)blockIdx.x * a.tokens * a.top_k * a.parts * kColumns, (int)blockIdx.x * kColumns,
+                    (int)(blockIdx.y * 256 + threadIdx.x), (int)gridDim.y * 256);
 }
 
 template <typename T, int kSteps, W4Edge kEdge>
 void launch_hidden(const W4MoeArgs& a, hipStream_t stream) {
   const dim3 grid((unsigned)(a.gate.tiles_n + kHiddenTiles - 1) / kHiddenTiles,
-                  (unsigned)std::min(a.experts, a.tokens * a.top_k));
+                  (unsigned)std::min(a.experts, a.tokens * a.top_k), (unsigned)a.blocks);
 #define HIDDEN(FEW)                                                                                                       \
   hipLaunchKernelGGL((moe_hidden_kernel<T, kSteps, kEdge, kHiddenTiles, kHiddenWaves, FEW>), grid, dim3(64 * kHiddenWaves), \
                      0, stream, a)
@@ -488,22 +497,31 @@ void launch_hidden(const W4MoeArgs& a, hipStream_t stream) {
     launch_hidden<T, kSteps, kEdgeShort>(a, stream);
 }
 
+template <typename T, int kSteps, int kNT, bool kFew, bool kParts>
+void launch_out(const W4MoeArgs& a, hipStream_t stream) {
+  const unsigned columns = (unsigned)(a.down.tiles_n + kNT - 1) / kNT;
+  const unsigned units = (unsigned)(std::min(a.experts, a.tokens * a.top_k) * a.split);
+  const dim3 grid(columns, (units + kOutWaves - 1) / kOutWaves, (unsigned)a.blocks);
+  hipLaunchKernelGGL((moe_out_kernel<T, kSteps, kNT, kFew, kParts>), grid, dim3(64 * kOutWaves), 0, stream, a);
+  if (a.joins) return;
+  const unsigned shares = (unsigned)std::min((a.tokens * 8 * kNT + 255) / 256, 64);
+  hipLaunchKernelGGL((moe_join_kernel<T, kNT>), dim3(columns, shares), dim3(256), 0, stream, a);
+}
 template <typename T, int kSteps>
 void launch_out(const W4MoeArgs& a, hipStream_t stream) {
   if (a.tokens <= kMoeFewTokens) {
-    const dim3 grid((unsigned)(a.down.tiles_n + a.out_tiles - 1) / (unsigned)a.out_tiles, (unsigned)a.slices);
-    const unsigned lds = kOutWaves * (unsigned)a.tokens * 16u * (unsigned)a.out_tiles * sizeof(float);
-    if (a.out_tiles == 2)
-      hipLaunchKernelGGL((moe_out_kernel<T, kSteps, 2, kOutWaves>), grid, dim3(64 * kOutWaves), lds, stream, a);
+    if (a.out_tiles == 4)
+      launch_out<T, kSteps, 4, true, false>(a, stream);
+    else if (a.split > a.parts)
+      launch_out<T, kSteps, 2, true, true>(a, stream);
     else
-      hipLaunchKernelGGL((moe_out_kernel<T, kSteps, 4, kOutWaves>), grid, dim3(64 * kOutWaves), lds, stream, a);
-    return;
+      launch_out<T, kSteps, 2, true, false>(a, stream);
+  } else {
+    if (a.out_tiles == 4)
+      launch_out<T, kSteps, 4, false, false>(a, stream);
+    else
+      launch_out<T, kSteps, 2, false, false>(a, stream);
   }
-  hipLaunchKernelGGL((moe_down_kernel<T, kSteps>),
-                     dim3((unsigned)a.down.tiles_n, (unsigned)std::min(a.experts, a.tokens * a.top_k)), dim3(256), 0, stream, a);
-  const uint64_t count = (uint64_t)a.tokens * (uint32_t)a.down.n;
-  hipLaunchKernelGGL((moe_join_kernel<T>), dim3((unsigned)std::min<uint64_t>((count + 255) / 256, 8192u)), dim3(256), 0,
-                     stream, a);
 }
 
 template <typename T>
@@ -546,15 +564,17 @@ size_t moe_w4_workspace(W4MoeArgs& a, bool bf16, void* base) {
     return p;
   };
   // Few slots: K is dealt out too.  Many: more columns a workgroup, which share the hidden rows (64 experts of 1024 hidden
-  // and 2048 output columns, 32 slots 11.9 us with 32 columns, 14.6 with 64; 64 slots of 8 tokens 18 to 21 and 15.7, of 64
-  // tokens 33 to 38 and 28.7).
+  // and 2048 outer columns: 32 slots 10.9 us with 32 columns, 12.4 with 64; 64 slots of 8 tokens 20 and 16, of 64 tokens 31.5
+  // and 24.5).
   const int slots = (int)std::min(experts, pairs);
   a.out_tiles = slots >= 64 ? 4 : 2;
   const int columns = (a.down.tiles_n + a.out_tiles - 1) / a.out_tiles;
   a.split = 1;
-  a.slices = 1;
   while (a.split < 4 && slots * a.split < 32 && a.down.tiles_k >= 4 * a.split) a.split *= 2;
-  while (a.slices < kMaxSlices && columns * a.slices < 256 && slots * a.split >= 2 * kOutWaves * a.slices) a.slices *= 2;
+  a.parts = a.tokens <= 16 ? 1 : a.split;
+  a.joins = a.tokens <= kMoeFewTokens && columns <= kColumnTickets;
+  // Blocks of sixteen pairs of an expert at once; those behind are taken in turn.
+  a.blocks = a.tokens <= kMoeFewTokens ? 1 : (int)std::min<size_t>((2 * pairs / experts + 15) / 16, 64);
   a.hidden_stride = (uint32_t)a.down.tiles_k * kW4TileK;
   a.hidden_plane = pairs * a.hidden_stride;
   a.logits = reinterpret_cast<double*>(take((size_t)a.tokens * experts * sizeof(double)));
@@ -564,8 +584,7 @@ size_t moe_w4_workspace(W4MoeArgs& a, bool bf16, void* base) {
   a.pairs = reinterpret_cast<int32_t*>(take(pairs * sizeof(int32_t)));
   a.reached = reinterpret_cast<MoeExpert*>(take((size_t)slots * sizeof(MoeExpert)));
   a.hidden = reinterpret_cast<uint16_t*>(take(a.hidden_plane * (bf16 ? 2 : 3) * sizeof(uint16_t)));
-  const size_t parts = a.tokens <= kMoeFewTokens ? (size_t)columns * a.slices * (kMoeFewTokens * 16u * (unsigned)a.out_tiles)
-                                                 : pairs * (size_t)a.down.n;
+  const size_t parts = pairs * a.parts * columns * 16u * a.out_tiles;
   a.part = reinterpret_cast<float*>(take(parts * sizeof(float)));
   return at;
 }

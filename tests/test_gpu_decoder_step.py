@@ -153,6 +153,23 @@ def test_product(gpu_runtime, dtype, group, rows, n, k, x_stride, out_stride, le
     _close(got, expect, _chain(k, group, dtype) * 2.0 ** -23 * size, dtype)
 
 
+# Sizes at which the kernels divide the work in other ways: more columns or fewer waves a workgroup, slices of K, larger
+# tiles.
+DIVISIONS = [
+    # rows, n, k, x stride, out stride, bytes in front
+    (1, 4500, 130, 130, 4500, 0), (3, 9000, 200, 204, 9001, 4), (2, 24600, 100, 100, 24600, 0), (40, 6000, 96, 96, 6000, 0),
+    (16, 700, 9000, 9000, 700, 0), (7, 2048, 8192, 8192, 2048, 0), (1, 40, 5, 5, 40, 0), (17, 4500, 6, 6, 4500, 0),
+    (20, 9000, 7, 9, 9000, 4), (50, 25000, 40, 40, 25000, 0), (300, 10000, 300, 300, 10000, 0), (1024, 4000, 256, 256, 4000, 0),
+    (1000, 10240, 130, 131, 10241, 4), (2049, 70, 520, 520, 70, 0), (700, 3000, 1030, 1032, 3000, 0), (1024, 520, 5, 5, 520, 0)]
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("group", (32, 64, 128))
+@pytest.mark.parametrize("rows,n,k,x_stride,out_stride,lead", DIVISIONS)
+def test_product_in_other_divisions(gpu_runtime, dtype, group, rows, n, k, x_stride, out_stride, lead):
+    test_product(gpu_runtime, dtype, group, rows, n, k, x_stride, out_stride, lead)
+
+
 @pytest.mark.parametrize("dtype", (F32, BF16))
 @pytest.mark.parametrize("rows", (3, 20, 70, 200))
 def test_product_of_single_ones(gpu_runtime, dtype, rows):
@@ -274,6 +291,38 @@ def test_mixture(gpu_runtime, index, dtype):
     _close(*_mixture(gpu_runtime, MIXTURES[index], dtype), dtype)
 
 
+# As above: parts of K with one block of pairs and with several, wide output columns, lists of pairs, blocks taken at once,
+# output columns joined in a launch of their own, rows shorter than eight.
+MIXTURE_DIVISIONS = [
+    dict(tokens=8, hidden=64, inner=600, experts=24, top_k=2, group=64),
+    dict(tokens=16, hidden=100, inner=2100, experts=5, top_k=3, gelu=True),
+    dict(tokens=20, hidden=96, inner=1030, experts=8, top_k=2, group=128, renormalise=True),
+    dict(tokens=64, hidden=48, inner=520, experts=4, top_k=4, group=64),
+    dict(tokens=64, hidden=256, inner=130, experts=64, top_k=8, renormalise=True, extra=3, lead=4),
+    dict(tokens=33, hidden=70, inner=48, experts=100, top_k=2, group=128),
+    dict(tokens=64, hidden=40, inner=20, experts=300, top_k=9, group=64, gelu=True),
+    dict(tokens=3, hidden=7, inner=5, experts=6, top_k=2),
+    dict(tokens=66, hidden=6, inner=200, experts=70, top_k=3, group=64, down_group=128),
+    dict(tokens=2, hidden=33000, inner=24, experts=2, top_k=1, gelu=True),
+    dict(tokens=100, hidden=130, inner=70, experts=80, top_k=4, group=64, extra=1),
+    dict(tokens=1000, hidden=64, inner=140, experts=4, top_k=2, group=128, gelu=True),
+    dict(tokens=520, hidden=33, inner=24, experts=200, top_k=1, renormalise=True),
+]
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("index", range(len(MIXTURE_DIVISIONS)))
+def test_mixture_in_other_divisions(gpu_runtime, index, dtype):
+    _close(*_mixture(gpu_runtime, MIXTURE_DIVISIONS[index], dtype), dtype)
+
+
+def test_mixtures_of_equal_calls_have_equal_bits(gpu_runtime):
+    for tokens in (1, 12, 64, 200):
+        case = dict(tokens=tokens, hidden=200, inner=600, experts=12, top_k=5)
+        first, again = (_mixture(gpu_runtime, case, F32)[0] for _ in range(2))
+        assert np.array_equal(first, again)
+
+
 @pytest.mark.parametrize("tokens", (1, 3, 30))
 def test_mixture_ties_go_to_the_lower_expert(gpu_runtime, tokens):
     """Equal logits (experts with equal router rows), and a token of zeros, whose logits are all equal."""
@@ -358,6 +407,16 @@ def test_rope(gpu_runtime, index, in_place, dtype):
             _close(got, expect, bound, dtype)
 
 
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("rows,dim,rotary,pairs,q_heads,k_heads", [
+    (4099, 64, 32, False, 5, 1), (4096, 64, 64, True, 3, 2), (5001, 10, 6, False, 3, 1), (4097, 6, 4, True, 1, 1),
+    (4102, 1024, 16, False, 1, 0)])
+def test_rope_of_many_rows(gpu_runtime, rows, dim, rotary, pairs, q_heads, k_heads, dtype, monkeypatch):
+    monkeypatch.setitem(globals(), "ROPES", [(rows, dim, rotary, pairs, q_heads, k_heads)])
+    for in_place in (False, True):
+        test_rope(gpu_runtime, 0, in_place, dtype)
+
+
 def test_rope_back_to_where_it_was(gpu_runtime):
     """The opposite position turns back: a rotation of far positions loses only roundings."""
     x = oracle.normal(1, (2, 128))
@@ -414,6 +473,20 @@ def test_residual_norm(gpu_runtime, index, parts, dtype):
                 got = _values(dev.down(blank, ptr), dtype)
                 assert np.all(got[:, width:] == -7.0)
                 _close(got[:, :width].astype(np.float64), value, limit, dtype)
+
+
+# Enough rows that a workgroup takes several, with vectors that change between them.
+MANY_NORMS = [dict(rows=9001, width=40, per=9), dict(rows=2500, width=600, per=7), dict(rows=1300, width=2056, per=500),
+              dict(rows=1201, width=4099, per=1, extra=1, lead=4), dict(rows=600, width=8200, per=77),
+              dict(rows=600, width=16400, per=600)]
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("parts", (0, 2, 3, 5, 6))
+@pytest.mark.parametrize("index", range(len(MANY_NORMS)))
+def test_residual_norm_of_many_rows(gpu_runtime, index, parts, dtype, monkeypatch):
+    monkeypatch.setitem(globals(), "NORMS", MANY_NORMS)
+    test_residual_norm(gpu_runtime, index, parts, dtype)
 
 
 def test_residual_norm_of_extreme_rows(gpu_runtime):
