@@ -1057,7 +1057,8 @@ PROM_REACTOR_API int prometheus_reactor_runtime_w4_unpack_device(void* handle, c
 /* out[i, j] = sum_k x[i, k] w[j, k] for x of `dtype` [rows, k] and out [rows, n], x_stride and
    out_stride elements between rows (below 2^24), any alignment of their type.  Operands
    enter unrounded (bf16 rows times codes are exact, fp32 rows go in as three exact terms);
-   sums are fp32, a bf16 result is rounded once. */
+   sums are fp32, a bf16 result is rounded once.  A group's sum may be taken before it is
+   multiplied by its step: with |x| above 2^118 it can overflow where the product would not. */
 typedef struct PrometheusW4GemmRequest {
   uint32_t struct_size;
   uint32_t dtype;
@@ -1081,7 +1082,7 @@ PROM_REACTOR_API int prometheus_reactor_runtime_gemm_w4_device(void* handle, con
    in the product above, router fp32 [experts, hidden].  gate and up are [inner, hidden] of one group
    size, down [hidden, inner]; each holds a matrix an expert (count = experts).  The hidden rows enter
    the second product with 16 significant bits (fp32 rows: 24).  An expert's weights are read once for
-   up to 64 tokens that chose it. */
+   every sixteen tokens that chose it, or fewer. */
 enum { PROM_MOE_SILU = 0u, PROM_MOE_GELU_TANH = 1u };
 #define PROM_MOE_MAX_EXPERTS 1024u
 #define PROM_MOE_MAX_TOP_K 64u

@@ -2,7 +2,8 @@
 //
 // A wave takes a tile of 16 rows by 128 columns (w4_tiles.h): it reads four rows at a time, eight columns a lane,
 // so that a group's largest magnitude is a maximum over 4, 8 or 16 neighbouring lanes, and turns the words into the
-// tile's order through LDS, so that codes leave as 16 bytes a lane.  Bound by memory.
+// tile's order through LDS, so that codes leave as 16 bytes a lane; unpacking goes the other way.  Bound by memory: 16384x2048
+// in bf16 packed in 19.4 us, 84 MB at 4.4 TB/s, unpacked in 13.5.
 #include "fp4_groups.h"
 #include "reactor_internal.h"
 #include "w4_tiles.h"

@@ -188,6 +188,8 @@ __device__ __forceinline__ void w4_add_tile(const W4Tile<kSteps, kNT>& w, const 
       for (int m = 0; m < kMT; ++m) {
         bf16x8 a[X::kTerms];
         X::terms(x.r[m][u], a);
+        // The terms are shifted, not the fp32 values before the split: of that the compiler made code in which a register
+        // was written while it was still needed.
         if (tail) {
           const int at = kt * kW4TileK + 32 * u + 8 * (((int)threadIdx.x & 63) >> 4);
           const int d = min(max(at + 8 - k, 0), 8);

@@ -160,7 +160,8 @@ DIVISIONS = [
     (1, 4500, 130, 130, 4500, 0), (3, 9000, 200, 204, 9001, 4), (2, 24600, 100, 100, 24600, 0), (40, 6000, 96, 96, 6000, 0),
     (16, 700, 9000, 9000, 700, 0), (7, 2048, 8192, 8192, 2048, 0), (1, 40, 5, 5, 40, 0), (17, 4500, 6, 6, 4500, 0),
     (20, 9000, 7, 9, 9000, 4), (50, 25000, 40, 40, 25000, 0), (300, 10000, 300, 300, 10000, 0), (1024, 4000, 256, 256, 4000, 0),
-    (1000, 10240, 130, 131, 10241, 4), (2049, 70, 520, 520, 70, 0), (700, 3000, 1030, 1032, 3000, 0), (1024, 520, 5, 5, 520, 0)]
+    (1000, 10240, 130, 131, 10241, 4), (2049, 70, 520, 520, 70, 0), (700, 3000, 1030, 1032, 3000, 0), (1024, 520, 5, 5, 520, 0),
+    (1, 24600, 128, 128, 24600, 0), (3, 9000, 256, 256, 9000, 0), (1024, 8000, 130, 130, 8000, 0), (1024, 5000, 256, 256, 5000, 0)]
 
 
 @pytest.mark.parametrize("dtype", (F32, BF16))
@@ -314,6 +315,15 @@ MIXTURE_DIVISIONS = [
 @pytest.mark.parametrize("index", range(len(MIXTURE_DIVISIONS)))
 def test_mixture_in_other_divisions(gpu_runtime, index, dtype):
     _close(*_mixture(gpu_runtime, MIXTURE_DIVISIONS[index], dtype), dtype)
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("group", (32, 64, 128))
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", [
+    (1, 5, 3, 70, 2), (70, 6, 130, 3, 2), (1, 128, 20, 300, 3), (4, 130, 1200, 6, 2), (1, 256, 128, 3, 1), (80, 384, 40, 2, 1)])
+def test_mixture_of_every_group(gpu_runtime, dtype, group, tokens, hidden, inner, experts, top_k):
+    case = dict(tokens=tokens, hidden=hidden, inner=inner, experts=experts, top_k=top_k, group=group)
+    _close(*_mixture(gpu_runtime, case, dtype), dtype)
 
 
 def test_mixtures_of_equal_calls_have_equal_bits(gpu_runtime):
@@ -478,6 +488,7 @@ def test_residual_norm(gpu_runtime, index, parts, dtype):
 # Enough rows that a workgroup takes several, with vectors that change between them.
 MANY_NORMS = [dict(rows=9001, width=40, per=9), dict(rows=2500, width=600, per=7), dict(rows=1300, width=2056, per=500),
               dict(rows=1201, width=4099, per=1, extra=1, lead=4), dict(rows=600, width=8200, per=77),
+              dict(rows=600, width=8201, per=77),
               dict(rows=600, width=16400, per=600)]
 
 
