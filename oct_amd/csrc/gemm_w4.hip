@@ -309,12 +309,13 @@ template <typename X>
 __global__ __launch_bounds__(256) void w4_terms_kernel(const void* __restrict__ x, uint32_t stride, uint16_t* __restrict__ to,
                                                        size_t plane, int m, int k, int ld) {
   typedef typename X::Element T;
+  constexpr W4Edge kTermsEdge = sizeof(T) == 2 ? kEdgeOdd : kEdgeNone;
   const int c = (int)(blockIdx.x * 64 + (threadIdx.x & 63)) * 8;
   if (c >= ld) return;
   for (int r = (int)(blockIdx.y * 4 + (threadIdx.x >> 6)); r < m; r += (int)gridDim.y * 4) {
     X row;
     row.p = static_cast<const T*>(x) + (size_t)r * stride;
-    typename X::Raw raw = c + 8 <= k ? row.template fetch<kEdgeNone>(c, k) : row.template fetch<kEdgeShort>(c, k);
+    typename X::Raw raw = c + 8 <= k ? row.template fetch<kTermsEdge>(c, k) : row.template fetch<kEdgeShort>(c, k);
     bf16x8 t[X::kTerms];
     X::terms(raw, t);
 #pragma unroll
@@ -368,8 +369,11 @@ hipError_t launch_rows(const RowsPlan& p, const W4Args& a, hipStream_t stream) {
 
 template <typename X, int kSteps>
 hipError_t launch_rows(const RowsPlan& p, const W4Args& a, hipStream_t stream) {
-  if (a.w.k % kW4TileK == 0) return launch_rows<X, kSteps, kEdgeNone>(p, a, stream);
-  if (a.w.k >= 8) return launch_rows<X, kSteps, kEdgeShift>(p, a, stream);
+  const W4Edge edge = w4_edge<typename X::Element>(a.x, a.x_stride, a.w.k);
+  if (edge == kEdgeNone) return launch_rows<X, kSteps, kEdgeNone>(p, a, stream);
+  if (edge == kEdgeShift) return launch_rows<X, kSteps, kEdgeShift>(p, a, stream);
+  if constexpr (sizeof(typename X::Element) == 2)
+    if (edge == kEdgeOdd) return launch_rows<X, kSteps, kEdgeOdd>(p, a, stream);
   hipLaunchKernelGGL((w4_rows_kernel<X, kSteps, 1, 8, kEdgeShort>),
                      dim3((unsigned)a.w.tiles_n * (unsigned)((a.m + 15) / 16)), dim3(512), 0, stream, a);
   return hipGetLastError();

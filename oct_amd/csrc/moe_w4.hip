@@ -489,12 +489,12 @@ void launch_hidden(const W4MoeArgs& a, hipStream_t stream) {
 }
 template <typename T, int kSteps>
 void launch_hidden(const W4MoeArgs& a, hipStream_t stream) {
-  if (a.gate.k % kW4TileK == 0)
-    launch_hidden<T, kSteps, kEdgeNone>(a, stream);
-  else if (a.gate.k >= 8)
-    launch_hidden<T, kSteps, kEdgeShift>(a, stream);
-  else
-    launch_hidden<T, kSteps, kEdgeShort>(a, stream);
+  const W4Edge edge = w4_edge<T>(a.x, a.x_stride, a.gate.k);
+  if (edge == kEdgeNone) return launch_hidden<T, kSteps, kEdgeNone>(a, stream);
+  if (edge == kEdgeShift) return launch_hidden<T, kSteps, kEdgeShift>(a, stream);
+  if constexpr (sizeof(T) == 2)
+    if (edge == kEdgeOdd) return launch_hidden<T, kSteps, kEdgeOdd>(a, stream);
+  launch_hidden<T, kSteps, kEdgeShort>(a, stream);
 }
 
 template <typename T, int kSteps, int kNT, bool kFew, bool kParts>

@@ -20,8 +20,17 @@ namespace prom {
 enum W4Edge {
   kEdgeNone,   // k is a multiple of 128
   kEdgeShift,  // the last tile's columns past k are cut off; k >= 8
+  kEdgeOdd,    // the same for bf16 rows that do not all lie on words' borders
   kEdgeShort,  // k < 8
 };
+
+// The edge of products with rows of x `stride` elements of T apart, the first at p.
+template <typename T>
+W4Edge w4_edge(const void* p, size_t stride, int k) {
+  if (k < 8) return kEdgeShort;
+  if (((uintptr_t)p | stride * sizeof(T)) % 4 != 0) return kEdgeOdd;
+  return k % kW4TileK == 0 ? kEdgeNone : kEdgeShift;
+}
 
 // Eight 16-bit values less the first d (0..8), zeros from behind.
 __device__ __forceinline__ u32x4 w4_drop(u32x4 v, int d) {
@@ -33,12 +42,13 @@ __device__ __forceinline__ u32x4 w4_drop(u32x4 v, int d) {
 }
 
 // Rows of x as one lane sees them: `p` is its row's first element.  fetch loads the eight columns from `at`, or where
-// they reach past k those that end there (kEdgeShift: their terms are shifted before they are used).
+// they reach past k those that end there (kEdgeShift, kEdgeOdd: their terms are shifted before they are used).
 struct W4RowsBf16 {
   static constexpr int kTerms = 1;
   typedef uint16_t Element;
   struct Raw {
     u32x4 v;
+    uint32_t behind, shift;  // kEdgeOdd: the word behind v, and where in v's first word the first column is
   };
   const uint16_t* p;
   template <W4Edge kEdge>
@@ -47,12 +57,24 @@ struct W4RowsBf16 {
     if constexpr (kEdge == kEdgeShort) {
       for (int j = 0; j < 8; ++j)
         if (at + j < k) r.v[j >> 1] |= (uint32_t)p[at + j] << (16 * (j & 1));
+    } else if constexpr (kEdge == kEdgeOdd) {
+      // Whole words, each of which holds one of the columns or two (33 rows of 3001x1999 7.7 us; with loads off words'
+      // borders 10.9; on them 6.1, but 7.7 this way).
+      const char* from = reinterpret_cast<const char*>(p + min(at, k - 8));
+      const uint32_t odd = (uint32_t)(uintptr_t)from & 2u;
+      __builtin_memcpy(&r.v, __builtin_assume_aligned(from - odd, 4), 16);
+      __builtin_memcpy(&r.behind, __builtin_assume_aligned(from + 12 + odd, 4), 4);
+      r.shift = 8 * odd;
     } else {
       __builtin_memcpy(&r.v, p + (kEdge == kEdgeShift ? min(at, k - 8) : at), 16);
     }
     return r;
   }
-  __device__ __forceinline__ static void terms(const Raw& r, bf16x8 (&x)[1]) { x[0] = __builtin_bit_cast(bf16x8, r.v); }
+  __device__ __forceinline__ static void terms(const Raw& r, bf16x8 (&x)[1]) {
+    const u32x4 v{__builtin_amdgcn_alignbit(r.v[1], r.v[0], r.shift), __builtin_amdgcn_alignbit(r.v[2], r.v[1], r.shift),
+                  __builtin_amdgcn_alignbit(r.v[3], r.v[2], r.shift), __builtin_amdgcn_alignbit(r.behind, r.v[3], r.shift)};
+    x[0] = __builtin_bit_cast(bf16x8, v);
+  }
 };
 
 // Eight fp32 values as three bf16 terms each, the upper half of what the ones before leave.  An infinity is its first
@@ -171,7 +193,7 @@ struct W4XTile {
 template <int kSteps, int kNT, int kMT, W4Edge kEdge, typename X>
 __device__ __forceinline__ void w4_add_tile(const W4Tile<kSteps, kNT>& w, const W4XTile<X, kMT>& x, int kt, int k,
                                             floatx4 (&acc)[kMT][kNT]) {
-  const bool tail = kEdge == kEdgeShift && kt == k / kW4TileK;
+  const bool tail = (kEdge == kEdgeShift || kEdge == kEdgeOdd) && kt == k / kW4TileK;
 #pragma unroll
   for (int g = 0; g < kSteps; ++g) {
     floatx4 sum[kMT][kNT];

@@ -161,7 +161,9 @@ DIVISIONS = [
     (16, 700, 9000, 9000, 700, 0), (7, 2048, 8192, 8192, 2048, 0), (1, 40, 5, 5, 40, 0), (17, 4500, 6, 6, 4500, 0),
     (20, 9000, 7, 9, 9000, 4), (50, 25000, 40, 40, 25000, 0), (300, 10000, 300, 300, 10000, 0), (1024, 4000, 256, 256, 4000, 0),
     (1000, 10240, 130, 131, 10241, 4), (2049, 70, 520, 520, 70, 0), (700, 3000, 1030, 1032, 3000, 0), (1024, 520, 5, 5, 520, 0),
-    (1, 24600, 128, 128, 24600, 0), (3, 9000, 256, 256, 9000, 0), (1024, 8000, 130, 130, 8000, 0), (1024, 5000, 256, 256, 5000, 0)]
+    (1, 24600, 128, 128, 24600, 0), (3, 9000, 256, 256, 9000, 0), (1024, 8000, 130, 130, 8000, 0), (1024, 5000, 256, 256, 5000, 0),
+    (9, 4500, 131, 131, 4500, 0), (40, 9000, 128, 129, 9000, 0), (2, 24600, 100, 101, 24600, 0), (5, 600, 9001, 9001, 600, 0),
+    (30, 9001, 256, 259, 9001, 0)]
 
 
 @pytest.mark.parametrize("dtype", (F32, BF16))
@@ -169,6 +171,13 @@ DIVISIONS = [
 @pytest.mark.parametrize("rows,n,k,x_stride,out_stride,lead", DIVISIONS)
 def test_product_in_other_divisions(gpu_runtime, dtype, group, rows, n, k, x_stride, out_stride, lead):
     test_product(gpu_runtime, dtype, group, rows, n, k, x_stride, out_stride, lead)
+
+
+@pytest.mark.parametrize("rows,k,x_stride", [(1, 8, 8), (1, 128, 128), (4, 300, 300), (20, 256, 258), (33, 1000, 1000),
+                                             (20, 9, 10), (300, 640, 640)])
+def test_product_of_bf16_rows_off_words(gpu_runtime, rows, k, x_stride):
+    """x and out two bytes behind a word's border, rows a whole number of words apart."""
+    test_product(gpu_runtime, BF16, 64, rows, 130, k, x_stride, 132, 2)
 
 
 @pytest.mark.parametrize("dtype", (F32, BF16))
@@ -308,6 +317,8 @@ MIXTURE_DIVISIONS = [
     dict(tokens=100, hidden=130, inner=70, experts=80, top_k=4, group=64, extra=1),
     dict(tokens=1000, hidden=64, inner=140, experts=4, top_k=2, group=128, gelu=True),
     dict(tokens=520, hidden=33, inner=24, experts=200, top_k=1, renormalise=True),
+    dict(tokens=3, hidden=131, inner=40, experts=3, top_k=1, group=128),
+    dict(tokens=70, hidden=129, inner=40, experts=3, top_k=1, group=128, gelu=True),
 ]
 
 
@@ -420,8 +431,10 @@ def test_rope(gpu_runtime, index, in_place, dtype):
 @pytest.mark.parametrize("dtype", (F32, BF16))
 @pytest.mark.parametrize("rows,dim,rotary,pairs,q_heads,k_heads", [
     (4099, 64, 32, False, 5, 1), (4096, 64, 64, True, 3, 2), (5001, 10, 6, False, 3, 1), (4097, 6, 4, True, 1, 1),
-    (4102, 1024, 16, False, 1, 0)])
-def test_rope_of_many_rows(gpu_runtime, rows, dim, rotary, pairs, q_heads, k_heads, dtype, monkeypatch):
+    (4102, 1024, 16, False, 1, 0), (4100, 80, 40, False, 3, 1), (4099, 80, 20, False, 2, 2), (4097, 80, 20, True, 2, 2),
+    (4098, 12, 2, True, 3, 1), (4097, 7, 4, False, 3, 1), (3, 80, 40, False, 3, 1), (5, 22, 20, False, 2, 1),
+    (3, 80, 20, True, 3, 1), (3, 20, 18, True, 2, 1), (2, 9, 4, True, 5, 1), (300, 9, 6, False, 5, 1)])
+def test_rope_in_other_divisions(gpu_runtime, rows, dim, rotary, pairs, q_heads, k_heads, dtype, monkeypatch):
     monkeypatch.setitem(globals(), "ROPES", [(rows, dim, rotary, pairs, q_heads, k_heads)])
     for in_place in (False, True):
         test_rope(gpu_runtime, 0, in_place, dtype)
