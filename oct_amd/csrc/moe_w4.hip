@@ -12,8 +12,8 @@
 // a fourth launch.
 //
 // Bound by the reached experts' weights, and for a token by the latency of three kernels that follow one another.  64
-// experts of 1024 with 2048 outer columns, 8 a token, in bf16: a token 6.4 + 5.4 + 6.6 us (28 MB at 2.4 TB/s in the last two), 64
-// tokens, which reach all experts, 9.8 + 33.2 + 24.1 us (214 MB at 3.7 TB/s; 64 rows of x and of the hidden columns come from L2
+// experts of 1024 with 2048 outer columns, 8 a token, in bf16: a token 5.6 + 6.5 + 7.0 us (28 MB at 2.1 TB/s in the last two), 64
+// tokens, which reach all experts, 9.6 + 33.0 + 24.0 us (214 MB at 3.8 TB/s; 64 rows of x and of the hidden columns come from L2
 // for each workgroup).
 #include <algorithm>
 
@@ -89,74 +89,125 @@ __device__ __forceinline__ unsigned long long order_of(double v) {
   return b >> 63 ? ~b : b | 1ull << 63;
 }
 
-// A wave chooses token t's experts, one after the other, and makes their weights; kMost logits a lane.
+__device__ __forceinline__ unsigned long long lane_value(unsigned long long v, int lane) {
+  const uint32_t low = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  const uint32_t high = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+  return (unsigned long long)high << 32 | low;
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  return __longlong_as_double((long long)lane_value((unsigned long long)__double_as_longlong(v), lane));
+}
+
+// A wave chooses a token's experts: the j-th is lane j's `expert`, with its logit; place[i] is what expert lane + 64 i is of
+// them, 1 + j, or 0.  kMost logits a lane.
 template <int kMost>
-__device__ __forceinline__ void choose(const W4MoeArgs& a, int t) {
-  const int lane = (int)threadIdx.x & 63;
-  const double* l = a.logits + (size_t)t * a.experts;
-  const int mine = (a.experts + 63) >> 6;
-  double logit[kMost];
-  unsigned long long key[kMost];
-  int place[kMost];
-#pragma unroll
-  for (int i = 0; i < kMost; ++i) {
-    key[i] = 0;
-    place[i] = 0;
-    logit[i] = 0.0;
-    if (i < mine && lane + 64 * i < a.experts) {
-      logit[i] = load_agent(l + lane + 64 * i);
-      key[i] = order_of(logit[i]);
-    }
-  }
-  double picked = 0.0, top = 0.0;  // lane j: the j-th expert's logit
-  int expert = 0;
-  for (int j = 0; j < a.top_k; ++j) {
-    unsigned long long best = 0;
-#pragma unroll
-    for (int i = 0; i < kMost; ++i)
-      if (i < mine) best = key[i] > best ? key[i] : best;
-    best = wave_max(best);
-    // The lowest expert that has it.
-    bool found = false;
+struct Choice {
+  int expert, place[kMost];
+  double logit[kMost], picked;
+  __device__ __forceinline__ Choice(const W4MoeArgs& a, int t, unsigned long long* keys) : expert(0), picked(0.0) {
+    const int lane = (int)threadIdx.x & 63, mine = (a.experts + 63) >> 6;
+    const double* l = a.logits + (size_t)t * a.experts;
+    uint32_t high[kMost], low[kMost];
 #pragma unroll
     for (int i = 0; i < kMost; ++i) {
-      if (i >= mine || found) continue;
-      const unsigned long long has = __ballot(key[i] == best);
-      if (has == 0) continue;
-      found = true;
-      const int at = __builtin_ctzll(has);
-      const unsigned long long bits = (unsigned long long)__double_as_longlong(logit[i]);
-      const uint32_t low = __builtin_amdgcn_readlane((int)(uint32_t)bits, at);
-      const uint32_t high = __builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), at);
-      const double v = __longlong_as_double((long long)((unsigned long long)high << 32 | low));
-      if (j == 0) top = v;
-      if (lane == j) picked = v, expert = at + 64 * i;
-      if (lane == at) key[i] = 0, place[i] = j + 1;
+      const bool some = i < mine && lane + 64 * i < a.experts;
+      logit[i] = some ? load_agent(l + lane + 64 * i) : 0.0;
+      const unsigned long long key = some ? order_of(logit[i]) : 0;
+      high[i] = (uint32_t)(key >> 32);
+      low[i] = (uint32_t)key;
+      place[i] = 0;
+    }
+    if constexpr (kMost == 1) {
+      rank(a, (unsigned long long)high[0] << 32 | low[0], keys);
+      return;
+    }
+#pragma unroll 1
+    for (int j = 0; j < a.top_k; ++j) {
+      uint32_t best = 0;
+#pragma unroll
+      for (int i = 0; i < kMost; ++i)
+        if (i < mine) best = max(best, high[i]);
+      best = wave_max(best);
+      // Upper halves mostly tell them apart; where they do not, the lower halves do, and then the lower expert wins.
+      int found = 0, at = 0, of = 0;
+      uint32_t below = 0;
+#pragma unroll
+      for (int i = kMost - 1; i >= 0; --i) {
+        if (i >= mine) continue;
+        const unsigned long long has = __ballot(high[i] == best && place[i] == 0);
+        found += __builtin_popcountll(has);
+        if (has != 0) at = __builtin_ctzll(has), of = i;
+        if (high[i] == best && place[i] == 0) below = max(below, low[i]);
+      }
+      if (found > 1) {
+        below = wave_max(below);
+#pragma unroll
+        for (int i = kMost - 1; i >= 0; --i) {
+          const unsigned long long has = __ballot(i < mine && high[i] == best && low[i] == below && place[i] == 0);
+          if (has != 0) at = __builtin_ctzll(has), of = i;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kMost; ++i) {
+        if (i != of) continue;
+        const double v = lane_value(logit[i], at);
+        if (lane == j) picked = v, expert = at + 64 * i;
+        if (lane == at) high[i] = low[i] = 0, place[i] = j + 1;
+      }
     }
   }
-  const double p = lane < a.top_k ? exp(picked - top) : 0.0;
-  double sum = p;
-  if (!a.renormalise) {
-    sum = 0.0;
+  // Up to 64 experts: a lane counts the larger logits, read from LDS (a token's 8 of 64 0.6 us sooner than one after the
+  // other).
+  __device__ __forceinline__ void rank(const W4MoeArgs& a, unsigned long long key, unsigned long long* keys) {
+    const int lane = (int)threadIdx.x & 63;
+    keys[lane] = key;
+    asm volatile("" ::: "memory");  // a wave's own words: its LDS operations stay in order
+    int r = 0;
+    for (int i = 0; i < a.experts; i += 16)
 #pragma unroll
-    for (int i = 0; i < kMost; ++i)
-      if (i < mine && lane + 64 * i < a.experts) sum += exp(logit[i] - top);
-  }
-  sum = wave_sum(sum);
-  if (lane < a.top_k) {
-    const size_t pair = (size_t)t * a.top_k + lane;
-    const float w = (float)(p / sum);
-    store_agent(a.chosen + pair, expert);
-    a.weights[pair] = w;
-    if (a.out_chosen != nullptr) a.out_chosen[pair] = expert;
-    if (a.out_weights != nullptr) a.out_weights[pair] = w;
-  }
-  if (a.tokens <= kMoeFewTokens)
+      for (int j = 0; j < 16; ++j) r += keys[i + j] > key ? 1 : 0;
+    if (lane >= a.experts) r = lane;
+    // Equal logits make equal ranks, whose sum is less than that of all: then the lower experts go first.
+    int all = r;
 #pragma unroll
-    for (int i = 0; i < kMost; ++i)
-      if (i < mine && lane + 64 * i < a.experts)
-        a.places[(size_t)t * a.experts + lane + 64 * i] = (uint8_t)place[i];
-}
+    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
+    if (all != 64 * 63 / 2)
+      for (int i = 0; i < a.experts; ++i)
+        if (keys[i] == key && i < lane && lane < a.experts) ++r;
+    place[0] = lane < a.experts && r < a.top_k ? r + 1 : 0;
+    expert = __builtin_amdgcn_ds_permute(4 * r, lane);
+    const unsigned long long bits = (unsigned long long)__double_as_longlong(logit[0]);
+    const uint32_t low = (uint32_t)__builtin_amdgcn_ds_permute(4 * r, (int)(uint32_t)bits);
+    const uint32_t high = (uint32_t)__builtin_amdgcn_ds_permute(4 * r, (int)(uint32_t)(bits >> 32));
+    picked = __longlong_as_double((long long)((unsigned long long)high << 32 | low));
+  }
+  // Leaves token t's experts and weights for the kernels that follow, and for the caller.
+  __device__ __forceinline__ void leave(const W4MoeArgs& a, int t) const {
+    const int lane = (int)threadIdx.x & 63, mine = (a.experts + 63) >> 6;
+    const double top = lane_value(picked, 0), p = lane < a.top_k ? exp(picked - top) : 0.0;
+    double sum = p;
+    if (!a.renormalise) {
+      sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < kMost; ++i)
+        if (i < mine && lane + 64 * i < a.experts) sum += exp(logit[i] - top);
+    }
+    sum = wave_sum(sum);
+    if (lane < a.top_k) {
+      const size_t pair = (size_t)t * a.top_k + lane;
+      const float w = (float)(p / sum);
+      store_agent(a.chosen + pair, expert);
+      a.weights[pair] = w;
+      if (a.out_chosen != nullptr) a.out_chosen[pair] = expert;
+      if (a.out_weights != nullptr) a.out_weights[pair] = w;
+    }
+    if (a.tokens <= kMoeFewTokens)
+#pragma unroll
+      for (int i = 0; i < kMost; ++i)
+        if (i < mine && lane + 64 * i < a.experts)
+          a.places[(size_t)t * a.experts + lane + 64 * i] = (uint8_t)place[i];
+  }
+};
 
 // A workgroup lists the pairs by expert.  Where a pair lies in its expert's list does not change what is computed from it.
 __device__ __forceinline__ void list_pairs(const W4MoeArgs& a, int (&count)[kMoeMaxExperts], int (&start)[kMoeMaxExperts],
@@ -215,6 +266,7 @@ __device__ __forceinline__ void load4(const uint16_t* p, float (&v)[4]) {
 template <typename T, int kMost, int kTokens>
 __global__ __launch_bounds__(256) void moe_router_kernel(const W4MoeArgs a) {
   __shared__ int count[kMoeMaxExperts], start[kMoeMaxExperts], wave_sums[2][4];
+  __shared__ unsigned long long keys[4][64];
   __shared__ uint32_t ticket;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   const int e = (int)blockIdx.x * 4 + wave, hidden = a.gate.k;
@@ -259,7 +311,7 @@ __global__ __launch_bounds__(256) void moe_router_kernel(const W4MoeArgs a) {
     }
   }
   if (!last_to_arrive(&moe_tickets[1 + blockIdx.y], gridDim.x, &ticket)) return;
-  if (wave < tokens) choose<kMost>(a, first + wave);
+  if (wave < tokens) Choice<kMost>(a, first + wave, keys[wave]).leave(a, first + wave);
   if (a.tokens <= kMoeFewTokens) return;
   if (!last_to_arrive(&moe_tickets[0], gridDim.y, &ticket)) return;
   list_pairs(a, count, start, wave_sums);

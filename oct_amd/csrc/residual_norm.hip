@@ -239,8 +239,8 @@ hipError_t launch(const ResidualNormArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((residual_norm_kernel<T, W, C, kWhole>), dim3((a.rows + share - 1) / share), dim3(W == 1 ? 256 : 64 * W), 0, \
                        stream, a, share);                                                                               \
   }
-  // Waves a row as few as hold it in 8 or 16 values a lane (4 waves of 16 values took 35 us where 8 of 8 took 31, at a width
-  // of 3840), and about as many workgroups as run at once: with twice as many their first rows' latency and the joining of
+  // As many waves a row as hold it in eight values a lane (with half the waves and 16 values: 4224 rows of 3840 35 us instead of
+  // 31, 1483 of 8192 36 instead of 26), and about as many workgroups as run at once: with twice as many their first rows' latency and the joining of
   // the vectors came twice (34 us).
   if (a.width <= 512)
     ROWS(1, 1, 1024)
@@ -249,7 +249,7 @@ hipError_t launch(const ResidualNormArgs& a, hipStream_t stream) {
   else if (a.width <= 4096)
     ROWS(8, 1, 512)
   else if (a.width <= 8192)
-    ROWS(8, 2, 512)
+    ROWS(16, 1, 256)
   else if (a.width <= 16384)
     ROWS(16, 2, 256)
   else

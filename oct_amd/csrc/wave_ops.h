@@ -1,4 +1,4 @@
-// Joins over the 64 lanes of a wave of 64-bit values, by DPP.
+// Joins over the 64 lanes of a wave, by DPP.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -32,8 +32,19 @@ __device__ __forceinline__ double wave_sum(double v) {
     return (unsigned long long)__double_as_longlong(__longlong_as_double((long long)a) + __longlong_as_double((long long)b));
   }));
 }
-__device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
-  return wave_join(v, [](auto a, auto b) { return a > b ? a : b; });
+// The wave's largest v.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t max_with_moved(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = max_with_moved<0x111, 0xF>(v);
+  v = max_with_moved<0x112, 0xF>(v);
+  v = max_with_moved<0x114, 0xF>(v);
+  v = max_with_moved<0x118, 0xF>(v);
+  v = max_with_moved<0x142, 0xA>(v);
+  v = max_with_moved<0x143, 0xC>(v);
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 #endif
 
