@@ -6,15 +6,15 @@
 // experts does not depend on the order of a sum); the last workgroup of two tokens' (tickets.h) chooses their experts.  The
 // hidden columns: a workgroup takes 32 of one reached expert, its gate and up weights once for sixteen pairs, a token with
 // one of its experts (w4_product.h), and leaves the hidden rows as bf16 terms, in the form that the second product
-// multiplies.  The output columns: a wave takes 32 or 64 of an expert (or of a part of its K) and leaves its sums by pair; the
-// last workgroup of those columns weighs and joins them in the order of a token's experts.  Up to 64 tokens each wave looks
-// up itself which of them chose its expert; above, the router's last workgroup lists the pairs by expert, and the sums are joined in
-// a fourth launch.
+// multiplies.  The output columns: a wave takes 32 or 64 of an expert (or of a part of its K) and leaves its sums by pair;
+// the last workgroup of those columns weighs and joins them in the order of a token's experts.  Up to 64 tokens each wave
+// looks up itself which of them chose its expert; above, the router's last workgroup lists the pairs by expert, and the
+// sums are joined in a fourth launch.
 //
 // Bound by the reached experts' weights, and for a token by the latency of three kernels that follow one another.  64
-// experts of 1024 with 2048 outer columns, 8 a token, in bf16: a token 5.6 + 6.5 + 7.0 us (28 MB at 2.1 TB/s in the last two), 64
-// tokens, which reach all experts, 9.6 + 33.0 + 24.0 us (214 MB at 3.8 TB/s; 64 rows of x and of the hidden columns come from L2
-// for each workgroup).
+// experts of 1024 with 2048 outer columns, 8 a token, in bf16: a token 5.6 + 6.5 + 7.0 us (28 MB at 2.1 TB/s in the last
+// two), 64 tokens, which reach all experts, 9.6 + 33.0 + 24.0 us (214 MB at 3.8 TB/s; 64 rows of x and of the hidden
+// columns come from L2 for each workgroup).
 #include <algorithm>
 
 #include "moe_w4.h"
@@ -318,9 +318,9 @@ __global__ __launch_bounds__(256) void moe_router_kernel(const W4MoeArgs a) {
 }
 
 // ------------------------------------------------------------------ the experts
-// A reached expert and its pairs as a wave sees them.  Few tokens: lane t looks up whether token t chose the expert, and the
-// rows' pairs go to the wave's own `list`; slot s is expert s, or where there are fewer pairs than experts that of pair s, unless
-// an earlier token has it too.  More tokens: slot s of the lists.
+// A reached expert and its pairs as a wave sees them.  Few tokens: lane t looks up whether token t chose the expert, and
+// the rows' pairs go to the wave's own `list`; slot s is expert s, or where there are fewer pairs than experts that of pair
+// s, unless an earlier token has it too.  More tokens: slot s of the lists.
 struct Reached {
   int expert, count;
   const int32_t* pairs;
@@ -395,8 +395,8 @@ __global__ __launch_bounds__(64 * kWaves) void moe_hidden_kernel(const W4MoeArgs
   }
 }
 
-// The pairs' sums of a column group by token, weighed, in the order of the token's experts: items `first`, first + step .. of two
-// columns.  kItems times kSums loads are on their way together: they come from behind the L2 caches.
+// The pairs' sums of a column group by token, weighed, in the order of the token's experts: items `first`, first + step ..
+// of two columns.  kItems times kSums loads are on their way together: they come from behind the L2 caches.
 template <typename T, int kColumns, int kItems, int kSums>
 __device__ __forceinline__ void join_some(const W4MoeArgs& a, const float* sums, int column0, int first, int step) {
   constexpr int kTwos = kColumns / 2;
@@ -444,9 +444,9 @@ __device__ __forceinline__ void join(const W4MoeArgs& a, const float* sums, int 
     join_some<T, kColumns, 1, 32>(a, sums, column0, first, step);
 }
 
-// Output columns 16 kNT blockIdx.x .. .  A unit is a part of K of a slot, a wave's; it leaves its sums by pair.  Where parts of K
-// have a block of pairs at most (kParts), the slot's waves, neighbours in a workgroup, join their sums first.  Few tokens: the
-// last workgroup of a column group joins the pairs' sums.
+// Output columns 16 kNT blockIdx.x .. .  A unit is a part of K of a slot, a wave's; it leaves its sums by pair.  Where
+// parts of K have a block of pairs at most (kParts), the slot's waves, neighbours in a workgroup, join their sums first.
+// Few tokens: the last workgroup of a column group joins the pairs' sums.
 template <typename T, int kSteps, int kNT, bool kFew, bool kParts>
 __global__ __launch_bounds__(64 * kOutWaves) void moe_out_kernel(const W4MoeArgs a) {
   typedef W4RowsTerms<Kind<T>::kHiddenTerms> X;

@@ -2,12 +2,12 @@
 //   h' = h + residual_scale * g * norm(y; post),  out = norm(h'; pre) * (1 + scale) + shift,
 // norm(x; w) = x / sqrt(mean(x^2) + eps) * w.
 //
-// A row is read once into registers and both norms are taken from there: bound by memory, and for the few rows of
-// a decode step by the chain of two sums over a workgroup.  Squares are summed in binary64, which holds those of every
-// fp32 number.  The second norm is that of h' before it is rounded to a bf16 row.  A workgroup takes neighbouring rows and
-// keeps what they share, the weights and vectors joined to a factor of y, a factor of h' and a summand, in registers (read
-// again for each row, 4224 rows of 3840 in bf16 took 53 us); the next row is loaded meanwhile.  Those rows take 31 us, 130 MB at
-// 4.2 TB/s; a large copy runs at 5.1.
+// A row is read once into registers and both norms are taken from there: bound by memory, and for the few rows of a decode
+// step by the chain of two sums over a workgroup.  Squares are summed in binary64, which holds those of every fp32 number.
+// The second norm is that of h' before it is rounded to a bf16 row.  A workgroup takes neighbouring rows and keeps what
+// they share, the weights and vectors joined to a factor of y, a factor of h' and a summand, in registers (read again for
+// each row, 4224 rows of 3840 in bf16 took 53 us); the next row is loaded meanwhile.  Those rows take 31 us, 130 MB at 4.2
+// TB/s; a large copy runs at 5.1.
 #include <algorithm>
 
 #include "reactor_internal.h"
@@ -232,16 +232,16 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm
 
 template <typename T, bool kWhole>
 hipError_t launch(const ResidualNormArgs& a, hipStream_t stream) {
-#define ROWS(W, C, WGS)                                                                                                 \
-  {                                                                                                                     \
-    const uint32_t at_once = W == 1 ? 4u : 1u, groups = (a.rows + at_once - 1) / at_once;                               \
-    const uint32_t share = (groups + WGS - 1) / WGS * at_once;                                                          \
-    hipLaunchKernelGGL((residual_norm_kernel<T, W, C, kWhole>), dim3((a.rows + share - 1) / share), dim3(W == 1 ? 256 : 64 * W), 0, \
-                       stream, a, share);                                                                               \
+#define ROWS(W, C, WGS)                                                                              \
+  {                                                                                                  \
+    const uint32_t at_once = W == 1 ? 4u : 1u, groups = (a.rows + at_once - 1) / at_once;            \
+    const uint32_t share = (groups + WGS - 1) / WGS * at_once;                                       \
+    hipLaunchKernelGGL((residual_norm_kernel<T, W, C, kWhole>), dim3((a.rows + share - 1) / share),  \
+                       dim3(W == 1 ? 256 : 64 * W), 0, stream, a, share);                            \
   }
-  // As many waves a row as hold it in eight values a lane (with half the waves and 16 values: 4224 rows of 3840 35 us instead of
-  // 31, 1483 of 8192 36 instead of 26), and about as many workgroups as run at once: with twice as many their first rows' latency and the joining of
-  // the vectors came twice (34 us).
+  // As many waves a row as hold it in eight values a lane (with half the waves and 16 values: 4224 rows of 3840 35 us
+  // instead of 31, 1483 of 8192 36 instead of 26), and about as many workgroups as run at once: with twice as many their
+  // first rows' latency and the joining of the vectors came twice (34 us).
   if (a.width <= 512)
     ROWS(1, 1, 1024)
   else if (a.width <= 2048)

@@ -3,7 +3,7 @@
 //   (a, b) -> m (a cos - b sin, b cos + a sin), the angle position * turns[i] revolutions,
 // pairs (i, i + rotary / 2) or (2 i, 2 i + 1) of the first `rotary` channels of each head; the others are copied.
 //
-// A workgroup takes a row: its threads make the row's cosines and sines once, in LDS, and go over the heads with eight
+// A workgroup takes a row, or four: its threads make the rows' cosines and sines once, in LDS, and go over the heads with eight
 // channels of each half (or eight neighbouring ones) a thread.  Angles are in binary64 and in revolutions, so that a
 // far position loses nothing but whole turns; what is left of a turn is within 2^-24 in fp32, and sincospi is good to
 // an ulp or two.  Bound by memory.
@@ -124,8 +124,8 @@ hipError_t launch(const RopeArgs& a, hipStream_t stream) {
 #define ROPE(R)                                                                                                   \
   hipLaunchKernelGGL((rope_kernel<T, kPairs, kN, R>), dim3(std::min<unsigned>((a.rows + R - 1) / R, 1u << 20)),   \
                      dim3(256), R * one, stream, a)
-  // Several rows a workgroup fill its last round of 256 items better (8191 rows of 32 + 8 heads of 128, half turned, bf16: 37 us with one,
-  // 34 with four, 43 with eight); few rows keep all CUs busy one by one.
+  // Several rows a workgroup fill its last round of 256 items better (8191 rows of 32 + 8 heads of 128, half turned, bf16:
+  // 37 us with one, 34 with four, 43 with eight); few rows keep all CUs busy one by one.
   if (a.rows < 4096)
     ROPE(1);
   else
