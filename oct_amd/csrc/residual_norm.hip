@@ -145,41 +145,57 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm
       if (a.y != nullptr) y_next[i] = load8<kWhole>(static_cast<const T*>(a.y) + (size_t)r * a.y_stride + at[i], left[i]);
     }
   };
-  fetch(row);
-  float fy[kChunks][8], fh[kChunks][8], add[kChunks][8];
+  // What h' takes of y / its size, and what out takes of h' / its size, for chunk i of a row with vector number `vector`.
+  const auto of_y = [&](uint32_t vector, int i, float (&f)[8]) __attribute__((always_inline)) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = a.residual_scale;
+    if (a.post != nullptr) {
+      load8<kWhole>(a.post + at[i], left[i]).get(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= a.weight_offset + v[j];
+    }
+    if (a.gate != nullptr) {
+      load8<kWhole>(static_cast<const T*>(a.gate) + (size_t)vector * a.vector_stride + at[i], left[i]).get(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= a.gate_tanh ? tanhf(v[j]) : v[j];
+    }
+  };
+  const auto of_h = [&](uint32_t vector, int i, float (&f)[8], float (&add)[8]) __attribute__((always_inline)) {
+    const size_t from = (size_t)vector * a.vector_stride + at[i];
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 1.0f, add[j] = 0.0f;
+    if (a.pre != nullptr) {
+      load8<kWhole>(a.pre + at[i], left[i]).get(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = a.weight_offset + v[j];
+    }
+    if (a.scale != nullptr) {
+      load8<kWhole>(static_cast<const T*>(a.scale) + from, left[i]).get(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= 1.0f + v[j];
+    }
+    if (a.shift != nullptr) load8<kWhole>(static_cast<const T*>(a.shift) + from, left[i]).get(add);
+  };
+  // Rows of several chunks a lane have no registers for the next row (900 rows of 16384 in bf16 28 us, with it 32), those of
+  // four none for these either (500 rows of 32768 70 us, with them 117).
+  constexpr bool kKeeps = kChunks <= 2, kAhead = kChunks == 1;
+  if constexpr (kAhead) fetch(row);
+  constexpr int kKept = kKeeps ? kChunks : 1, kStays = kKeeps ? 1 : 0;
+  float fy[kKept][8], fh[kKept][8], add[kKept][8];
   uint32_t vector = 0xFFFFFFFFu;  // the vectors that the factors are of
   int turn = 0;
   for (; row < end; row += kRows) {
+    if constexpr (!kAhead) fetch(row);
     if (row / a.rows_per_vector != vector) {
       vector = row / a.rows_per_vector;
-      const size_t from = (size_t)vector * a.vector_stride;
-      float v[8];
+      if constexpr (kKeeps)
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) fy[i][j] = a.residual_scale, fh[i][j] = 1.0f, add[i][j] = 0.0f;
-        if (a.post != nullptr) {
-          load8<kWhole>(a.post + at[i], left[i]).get(v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) fy[i][j] *= a.weight_offset + v[j];
+        for (int i = 0; i < kChunks; ++i) {
+          of_y(vector, i, fy[i]);
+          of_h(vector, i, fh[i], add[i]);
         }
-        if (a.gate != nullptr) {
-          load8<kWhole>(static_cast<const T*>(a.gate) + from + at[i], left[i]).get(v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) fy[i][j] *= a.gate_tanh ? tanhf(v[j]) : v[j];
-        }
-        if (a.pre != nullptr) {
-          load8<kWhole>(a.pre + at[i], left[i]).get(v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) fh[i][j] = a.weight_offset + v[j];
-        }
-        if (a.scale != nullptr) {
-          load8<kWhole>(static_cast<const T*>(a.scale) + from + at[i], left[i]).get(v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) fh[i][j] *= 1.0f + v[j];
-        }
-        if (a.shift != nullptr) load8<kWhole>(static_cast<const T*>(a.shift) + from + at[i], left[i]).get(add[i]);
-      }
     }
     float h[kChunks][8], y[kChunks][8];
 #pragma unroll
@@ -187,7 +203,8 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm
       h_next[i].get(h[i]);
       if (a.y != nullptr) y_next[i].get(y[i]);
     }
-    if (row + kRows < end) fetch(row + kRows);
+    if constexpr (kAhead)
+      if (row + kRows < end) fetch(row + kRows);
     const uint32_t now = row;
     if (a.y != nullptr) {
       float r = 1.0f;
@@ -198,9 +215,11 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm
         r = inverse_size(row_sum<kWaves>(sum, part[0][turn]), a.over_width, a.eps);
       }
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i)
+      for (int i = 0; i < kChunks; ++i) {
+        if constexpr (!kKeeps) of_y(vector, i, fy[0]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[i][j] = __builtin_fmaf(y[i][j] * r, fy[i][j], h[i][j]);
+        for (int j = 0; j < 8; ++j) h[i][j] = __builtin_fmaf(y[i][j] * r, fy[kStays * i][j], h[i][j]);
+      }
     }
     if (a.h_out != nullptr) {
       T* to = static_cast<T*>(a.h_out) + (size_t)now * a.h_out_stride;
@@ -216,11 +235,12 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm
       T* to = static_cast<T*>(a.out) + (size_t)now * a.out_stride;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
+        if constexpr (!kKeeps) of_h(vector, i, fh[0], add[0]);
         float o[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          o[j] = h[i][j] * r * fh[i][j];
-          if (a.shift != nullptr) o[j] += add[i][j];
+          o[j] = h[i][j] * r * fh[kStays * i][j];
+          if (a.shift != nullptr) o[j] += add[kStays * i][j];
         }
         if (left[i] > 0) store8<kWhole>(to + at[i], left[i], o);
       }
@@ -244,6 +264,8 @@ hipError_t launch(const ResidualNormArgs& a, hipStream_t stream) {
   // first rows' latency and the joining of the vectors came twice (34 us).
   if (a.width <= 512)
     ROWS(1, 1, 1024)
+  else if (a.width <= 1024)
+    ROWS(2, 1, 2048)
   else if (a.width <= 2048)
     ROWS(4, 1, 1024)
   else if (a.width <= 4096)

@@ -499,7 +499,9 @@ def test_residual_norm(gpu_runtime, index, parts, dtype):
 
 
 # Enough rows that a workgroup takes several, with vectors that change between them.
-MANY_NORMS = [dict(rows=9001, width=40, per=9), dict(rows=2500, width=600, per=7), dict(rows=1300, width=2056, per=500),
+MANY_NORMS = [dict(rows=9001, width=40, per=9), dict(rows=2500, width=600, per=7), dict(rows=4500, width=600, per=7),
+              dict(rows=4099, width=1001, per=2),
+              dict(rows=2500, width=1504, per=3), dict(rows=1300, width=2056, per=500),
               dict(rows=1201, width=4099, per=1, extra=1, lead=4), dict(rows=600, width=8200, per=77),
               dict(rows=600, width=8201, per=77),
               dict(rows=600, width=16400, per=600)]
