@@ -351,6 +351,8 @@ struct RowsPlan {
 // rows take three times the matrix instructions and have to be split into terms, so that more columns share that and
 // shorter K are cut: 15 rows of 2048x2048 7.4, 6.0 in four slices; 16 rows of 4096x4096 11.5 with 16 columns, 8.7 with 64 in
 // four slices.  Eight waves a workgroup where there are few of them: 12288x4096 7.3, with four 8.1; 32768x2048 9.0 and 8.6.
+// Two or one where there are many, whose sums are joined and stored while others multiply: 64 rows of 16384x2048 16.7 with
+// four waves, 14.1 with two, 16.0 with one; of 32768x2048 29, 30 and 24; fp32 rows the same, but 64 of 12288x4096 32.6 and 35.4.
 RowsPlan plan_rows(uint32_t m, const W4View& w, bool bf16) {
   constexpr int kMostCus = 140;
   const int blocks = (int)((m + 15) / 16);
@@ -361,7 +363,10 @@ RowsPlan plan_rows(uint32_t m, const W4View& w, bool bf16) {
     p.nt = 4;
   else if (groups(2) >= kMostCus || !bf16 || (cut && w.tiles_k >= 64))
     p.nt = 2;
-  if ((p.nt == 4 && groups(4) >= 384) || (p.nt == 2 && bf16)) p.waves = 4;
+  if (p.nt == 4)
+    p.waves = groups(4) >= 2000 ? 1 : groups(4) >= (bf16 ? 768 : 800) ? 2 : groups(4) >= 384 ? 4 : 8;
+  else if (p.nt == 2 && bf16)
+    p.waves = 4;
   if (cut && groups(p.nt) < kMostCus && w.tiles_k >= (bf16 ? 64 : 16))
     while (p.slices < kMaxSlices && groups(p.nt) * p.slices <= 128 && w.tiles_k >= 8 * p.slices) p.slices *= 2;
   return p;
@@ -378,7 +383,7 @@ hipError_t launch_rows(const RowsPlan& p, const W4Args& a, hipStream_t stream) {
   } else {
     ROWS(2, 8)
   }
-  ROWS(4, 4) ROWS(4, 8)
+  ROWS(4, 1) ROWS(4, 2) ROWS(4, 4) ROWS(4, 8)
 #undef ROWS
   return hipGetLastError();
 }
@@ -419,15 +424,19 @@ TilePlan plan_tiles(const TileCost (&costs)[kN], uint32_t m, const W4View& w) {
   }
   return best;
 }
-TilePlan plan_tiles(uint32_t m, const W4View& w, bool bf16) {
+// `terms`: x has to be brought into terms first, in a launch of its own.
+TilePlan plan_tiles(uint32_t m, const W4View& w, bool bf16, bool terms) {
   TilePlan p = bf16 ? plan_tiles(kTiles, m, w) : plan_tiles(kTilesF32, m, w);
-  if (!bf16) p.us += 3.0;  // the launch that makes the terms
+  p.us += 4.5e-7 * m * w.n + (terms ? 3.0 : 0.0);  // storing the result
   return p;
 }
-// Whether the few rows' kernel, which reads the weights again for each sixteen rows, is the shorter way (128 rows of
-// 4096x4096: 14 us, on tiles 18; 16384x2048 27 and 18).
+// Whether the few rows' kernel, which reads the weights again for each sixteen rows, is the shorter way: a launch, its
+// workgroups' ends and the products, from 180 to 400 rows of 2048 and 15008 by 128 to 8192 (bf16, 180 rows of 15008x128 7.8 us,
+// on tiles 6.2; 400 of 2048x1024 8.7 and 9.6).
 bool rows_are_few(uint32_t m, const W4View& w, bool bf16, const TilePlan& tiles) {
-  return m <= 64 || 3.0 + (bf16 ? 5.6e-9 : 10.5e-9) * m * (double)w.n * w.k <= tiles.us;
+  const double groups = (double)((w.tiles_n + 3) / 4) * ((m + 15) / 16), products = (double)m * w.n * w.tiles_k * kW4TileK;
+  return m <= 64 ||
+         (bf16 ? 3.2 + 1.15e-3 * groups + 5.2e-9 * products : 4.0 + 2.0e-3 * groups + 10.5e-9 * products) <= tiles.us;
 }
 
 template <int kSteps, int kTerms, typename T>
@@ -447,12 +456,18 @@ hipError_t launch_tiles(const TilePlan& p, W4TileArgs a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// Whether the tiles' DMA takes rows of x as they lie.
+template <typename X>
+bool takes_rows(const void* x, uint32_t x_stride, int k) {
+  return X::kTerms == 1 && k % 8 == 0 && x_stride % 8 == 0 && x_stride < kMaxTileStride && ((uintptr_t)x & 15u) == 0;
+}
+
 template <typename X>
 hipError_t launch_many(const TilePlan& p, W4TileArgs a, const void* x, uint32_t x_stride, hipStream_t stream) {
   typedef typename X::Element T;
   constexpr bool kBf16 = X::kTerms == 1;
   a.k = a.w.k;
-  if (kBf16 && a.w.k % 8 == 0 && x_stride % 8 == 0 && x_stride < kMaxTileStride && ((uintptr_t)x & 15u) == 0) {
+  if (takes_rows<X>(x, x_stride, a.w.k)) {
     a.x = static_cast<const uint16_t*>(x);
     a.ld = (int)x_stride;
   } else {
@@ -503,7 +518,7 @@ template <typename X>
 hipError_t launch(const W4View& w, const void* x, uint32_t x_stride, void* out, uint32_t out_stride, uint32_t m,
                   hipStream_t stream) {
   constexpr bool kBf16 = X::kTerms == 1;
-  const TilePlan p = plan_tiles(m, w, kBf16);
+  const TilePlan p = plan_tiles(m, w, kBf16, !takes_rows<X>(x, x_stride, w.k));
   if (rows_are_few(m, w, kBf16, p)) return launch_few<X>(W4Args{w, x, out, nullptr, x_stride, out_stride, (int)m, 1}, stream);
   W4TileArgs a{};
   a.w = w;

@@ -163,7 +163,8 @@ DIVISIONS = [
     (1000, 10240, 130, 131, 10241, 4), (2049, 70, 520, 520, 70, 0), (700, 3000, 1030, 1032, 3000, 0), (1024, 520, 5, 5, 520, 0),
     (1, 24600, 128, 128, 24600, 0), (3, 9000, 256, 256, 9000, 0), (1024, 8000, 130, 130, 8000, 0), (1024, 5000, 256, 256, 5000, 0),
     (9, 4500, 131, 131, 4500, 0), (40, 9000, 128, 129, 9000, 0), (2, 24600, 100, 101, 24600, 0), (5, 600, 9001, 9001, 600, 0),
-    (30, 9001, 256, 259, 9001, 0)]
+    (30, 9001, 256, 259, 9001, 0), (50, 14000, 256, 256, 14000, 0), (49, 14000, 70, 70, 14001, 0), (50, 13999, 200, 201, 13999, 0),
+    (49, 33000, 128, 128, 33000, 0), (64, 32999, 260, 260, 32999, 0), (50, 33000, 33, 33, 33000, 0), (200, 16000, 136, 136, 16000, 0)]
 
 
 @pytest.mark.parametrize("dtype", (F32, BF16))
@@ -433,7 +434,8 @@ def test_rope(gpu_runtime, index, in_place, dtype):
     (4099, 64, 32, False, 5, 1), (4096, 64, 64, True, 3, 2), (5001, 10, 6, False, 3, 1), (4097, 6, 4, True, 1, 1),
     (4102, 1024, 16, False, 1, 0), (4100, 80, 40, False, 3, 1), (4099, 80, 20, False, 2, 2), (4097, 80, 20, True, 2, 2),
     (4098, 12, 2, True, 3, 1), (4097, 7, 4, False, 3, 1), (3, 80, 40, False, 3, 1), (5, 22, 20, False, 2, 1),
-    (3, 80, 20, True, 3, 1), (3, 20, 18, True, 2, 1), (2, 9, 4, True, 5, 1), (300, 9, 6, False, 5, 1)])
+    (3, 80, 20, True, 3, 1), (3, 20, 18, True, 2, 1), (2, 9, 4, True, 5, 1), (300, 9, 6, False, 5, 1),
+    (4098, 9, 4, True, 3, 1)])
 def test_rope_in_other_divisions(gpu_runtime, rows, dim, rotary, pairs, q_heads, k_heads, dtype, monkeypatch):
     monkeypatch.setitem(globals(), "ROPES", [(rows, dim, rotary, pairs, q_heads, k_heads)])
     for in_place in (False, True):
@@ -501,7 +503,7 @@ def test_residual_norm(gpu_runtime, index, parts, dtype):
 # Enough rows that a workgroup takes several, with vectors that change between them.
 MANY_NORMS = [dict(rows=9001, width=40, per=9), dict(rows=2500, width=600, per=7), dict(rows=4500, width=600, per=7),
               dict(rows=4099, width=1001, per=2),
-              dict(rows=2500, width=1504, per=3), dict(rows=1300, width=2056, per=500),
+              dict(rows=2500, width=1504, per=3), dict(rows=2100, width=1501, per=4), dict(rows=1300, width=2056, per=500),
               dict(rows=1201, width=4099, per=1, extra=1, lead=4), dict(rows=600, width=8200, per=77),
               dict(rows=600, width=8201, per=77),
               dict(rows=600, width=16400, per=600)]
