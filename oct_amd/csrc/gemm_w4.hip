@@ -74,46 +74,30 @@ __global__ __launch_bounds__(64 * kWaves) void w4_rows_kernel(const W4Args a) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) sums[wave][i][r][lane] = acc[0][i][r];
   __syncthreads();
-  // Two columns of a row a thread.
-  const int column0 = group * kNT * kW4TileN, count = rows * kNT * 8;
+  const int column0 = group * kNT * kW4TileN, count = rows * kNT * 16;
   T* out = static_cast<T*>(a.out) + (size_t)row0 * a.out_stride + column0;
-  unsigned long long* part =
-      a.slices > 1 ? reinterpret_cast<unsigned long long*>(a.part + (size_t)id * a.slices * kPart) : nullptr;
-  const auto leave = [&](int at, floatx2 v) __attribute__((always_inline)) {
-    const int row = at / (8 * kNT), c = 2 * (at % (8 * kNT));
-    if (column0 + c < a.w.n) put(out + (size_t)row * a.out_stride + c, v.x);
-    if (column0 + c + 1 < a.w.n) put(out + (size_t)row * a.out_stride + c + 1, v.y);
-  };
+  float* part = a.slices > 1 ? a.part + (size_t)id * a.slices * kPart : nullptr;
   for (int at = (int)threadIdx.x; at < count; at += 64 * kWaves) {
-    const int row = at / (8 * kNT), c = 2 * (at % (8 * kNT)), r = row & 3, l = 16 * (row >> 2) + (c & 15);
-    floatx2 v = *reinterpret_cast<const floatx2*>(&sums[0][c >> 4][r][l]);
+    const int row = at / (16 * kNT), c = at % (16 * kNT), r = row & 3, l = 16 * (row >> 2) + (c & 15);
+    float v = sums[0][c >> 4][r][l];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-      const floatx2 u = *reinterpret_cast<const floatx2*>(&sums[w][c >> 4][r][l]);
-      v.x += u.x;
-      v.y += u.y;
-    }
+    for (int w = 1; w < kWaves; ++w) v += sums[w][c >> 4][r][l];
     if (part != nullptr)
-      __hip_atomic_store(part + (size_t)slice * (kPart / 2) + at, __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED,
-                         __HIP_MEMORY_SCOPE_AGENT);
-    else
-      leave(at, v);
+      __hip_atomic_store(part + (size_t)slice * kPart + at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else if (column0 + c < a.w.n)
+      put(out + (size_t)row * a.out_stride + c, v);
   }
   if (part == nullptr || !last_to_arrive(w4_tickets + id, (uint32_t)a.slices, &ticket)) return;
   for (int at = (int)threadIdx.x; at < count; at += 64 * kWaves) {
-    unsigned long long p[kMaxSlices];
+    const int row = at / (16 * kNT), c = at % (16 * kNT);
+    float p[kMaxSlices];
 #pragma unroll
     for (int s = 0; s < kMaxSlices; ++s)
-      p[s] = s < a.slices ? __hip_atomic_load(part + (size_t)s * (kPart / 2) + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-                          : 0;
-    floatx2 v = __builtin_bit_cast(floatx2, p[0]);
+      p[s] = s < a.slices ? __hip_atomic_load(part + (size_t)s * kPart + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0f;
+    float v = p[0];
 #pragma unroll
-    for (int s = 1; s < kMaxSlices; ++s) {
-      const floatx2 u = __builtin_bit_cast(floatx2, p[s]);
-      v.x += u.x;
-      v.y += u.y;
-    }
-    leave(at, v);
+    for (int s = 1; s < kMaxSlices; ++s) v += p[s];
+    if (column0 + c < a.w.n) put(out + (size_t)row * a.out_stride + c, v);
   }
 }
 
