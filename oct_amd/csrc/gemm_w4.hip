@@ -334,7 +334,8 @@ struct RowsPlan {
 // Where even 16 columns leave CUs idle and K is long it is cut: 2048x16384, one row 13.2 in one slice, 7.4 in four.  fp32
 // rows take three times the matrix instructions and have to be split into terms, so that more columns share that and
 // shorter K are cut: 15 rows of 2048x2048 7.4, 6.0 in four slices; 16 rows of 4096x4096 11.5 with 16 columns, 8.7 with 64 in
-// four slices.  Eight waves a workgroup where there are few of them: 12288x4096 7.3, with four 8.1; 32768x2048 9.0 and 8.6.
+// four slices.  Eight waves a workgroup where each has a CU: 12288x4096 7.3, with four 8.1; four where some would wait for
+// a second round: 20480x2048 8.1 with eight, 7.5; 16 fp32 rows of 17920x1024 12.1 and 9.1.
 // Two or one where there are many, whose sums are joined and stored while others multiply: 64 rows of 16384x2048 16.7 with
 // four waves, 14.1 with two, 16.0 with one; of 32768x2048 29, 30 and 24; fp32 rows the same, but 64 of 12288x4096 32.6 and 35.4.
 RowsPlan plan_rows(uint32_t m, const W4View& w, bool bf16) {
@@ -348,7 +349,7 @@ RowsPlan plan_rows(uint32_t m, const W4View& w, bool bf16) {
   else if (groups(2) >= kMostCus || !bf16 || (cut && w.tiles_k >= 64))
     p.nt = 2;
   if (p.nt == 4)
-    p.waves = groups(4) >= 2000 ? 1 : groups(4) >= (bf16 ? 768 : 800) ? 2 : groups(4) >= 384 ? 4 : 8;
+    p.waves = groups(4) >= 2000 ? 1 : groups(4) >= (bf16 ? 768 : 800) ? 2 : groups(4) > 256 ? 4 : 8;
   else if (p.nt == 2 && bf16)
     p.waves = 4;
   if (cut && groups(p.nt) < kMostCus && w.tiles_k >= (bf16 ? 64 : 16))

@@ -164,6 +164,7 @@ DIVISIONS = [
     (1, 24600, 128, 128, 24600, 0), (3, 9000, 256, 256, 9000, 0), (1024, 8000, 130, 130, 8000, 0), (1024, 5000, 256, 256, 5000, 0),
     (9, 4500, 131, 131, 4500, 0), (40, 9000, 128, 129, 9000, 0), (2, 24600, 100, 101, 24600, 0), (5, 600, 9001, 9001, 600, 0),
     (30, 9001, 256, 259, 9001, 0), (50, 14000, 256, 256, 14000, 0), (49, 14000, 70, 70, 14001, 0), (50, 13999, 200, 201, 13999, 0),
+    (33, 3001, 199, 199, 3001, 0), (1, 10000, 131, 131, 10000, 0),
     (49, 33000, 128, 128, 33000, 0), (64, 32999, 260, 260, 32999, 0), (50, 33000, 33, 33, 33000, 0), (200, 16000, 136, 136, 16000, 0)]
 
 
