@@ -1080,8 +1080,8 @@ PROM_REACTOR_API int prometheus_reactor_runtime_gemm_w4_device(void* handle, con
      out[t] = sum over t's experts e, in their order, of p_e (act(x[t] gate_e^T) * (x[t] up_e^T)) down_e^T
    in fp32, a bf16 result rounded once.  x of `dtype` [tokens, hidden] and out [tokens, hidden] as
    in the product above, router fp32 [experts, hidden].  gate and up are [inner, hidden] of one group
-   size, down [hidden, inner]; each holds a matrix an expert (count = experts).  The hidden rows enter
-   the second product with 16 significant bits (fp32 rows: 24).  An expert's weights are read once for
+   size, down [hidden, inner]; each holds a matrix an expert (count = experts).  The hidden rows are
+   fp32 and enter the second product as rows of that type do.  An expert's weights are read once for
    every sixteen tokens that chose it, or fewer. */
 enum { PROM_MOE_SILU = 0u, PROM_MOE_GELU_TANH = 1u };
 #define PROM_MOE_MAX_EXPERTS 1024u

@@ -135,10 +135,10 @@ PROM_REACTOR_API int prometheus_reactor_runtime_moe_w4_device(void* handle, cons
   DeviceContext& cx = ctx();
   std::lock_guard<std::mutex> lock(cx.mu);
   CurrentDevice device(cx.device);
-  void* base = staging(6, moe_w4_workspace(a, bf16, nullptr));
+  void* base = staging(6, moe_w4_workspace(a, nullptr));
   if (base == nullptr)
     return refuse(out_stage, out_detail_code, PROM_STAGE_TRANSFER_IN, PROM_DETAIL_HIP_ALLOC_FAILED);
-  moe_w4_workspace(a, bf16, base);
+  moe_w4_workspace(a, base);
   return queued(launch_moe_w4(a, bf16, cx.stream), out_stage, out_detail_code, 0);
 }
 

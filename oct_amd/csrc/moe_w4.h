@@ -40,7 +40,7 @@ struct W4MoeArgs {
 };
 
 // Bytes of the workspace; sets the pointers into `base`.
-size_t moe_w4_workspace(W4MoeArgs& a, bool bf16, void* base);
+size_t moe_w4_workspace(W4MoeArgs& a, void* base);
 hipError_t launch_moe_w4(const W4MoeArgs& a, bool bf16, hipStream_t stream);
 
 }  // namespace prom

@@ -31,26 +31,22 @@ struct Kind;
 template <>
 struct Kind<uint16_t> {
   typedef W4RowsBf16 Rows;
-  static constexpr int kHiddenTerms = 2;  // 16 significant bits
 };
 template <>
 struct Kind<float> {
   typedef W4RowsF32 Rows;
-  static constexpr int kHiddenTerms = 3;
 };
+// A hidden value's bf16 terms: all of fp32's bits (two terms, sixteen bits, moved a bf16 result by 1.1e-4 to 2.3e-4 of its
+// size, as its roundings fell another way).
+constexpr int kHiddenTerms = 3;
 
 __device__ __forceinline__ float value(const float* p) { return *p; }
 __device__ __forceinline__ float value(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(uint16_t* p, float v) { *p = __builtin_bit_cast(uint16_t, (__bf16)v); }
 
-__device__ __forceinline__ void put_terms(uint16_t* p, size_t plane, float v, uint16_t) {
-  const __bf16 high = (__bf16)v;
-  const float rest = __builtin_isfinite((float)high) ? v - (float)high : 0.0f;
-  p[0] = __builtin_bit_cast(uint16_t, high);
-  p[plane] = __builtin_bit_cast(uint16_t, (__bf16)rest);
-}
-__device__ __forceinline__ void put_terms(uint16_t* p, size_t plane, float v, float) {
+// The upper half of what the ones before leave, as w4_split; an infinity is its first term.
+__device__ __forceinline__ void put_terms(uint16_t* p, size_t plane, float v) {
   const uint32_t b = __float_as_uint(v);
   const float rest = __builtin_isinf(v) ? 0.0f : v - __uint_as_float(b & 0xFFFF0000u);
   const uint32_t c = __float_as_uint(rest);
@@ -387,10 +383,10 @@ __global__ __launch_bounds__(64 * kWaves) void moe_hidden_kernel(const W4MoeArgs
       uint16_t* to = a.hidden + (size_t)ex.pairs[block + row] * a.hidden_stride;
       // Columns behind the last are zeros: whole tiles are multiplied.
       const float h = f < (uint32_t)a.gate.n ? activation(g, a.activation) * u : 0.0f;
-      if (f < a.hidden_stride) put_terms(to + f, a.hidden_plane, h, T());
+      if (f < a.hidden_stride) put_terms(to + f, a.hidden_plane, h);
       if (blockIdx.x == gridDim.x - 1)
         for (uint32_t z = f + 16 * kTiles; z < a.hidden_stride; z += 16 * kTiles)
-          put_terms(to + z, a.hidden_plane, 0.0f, T());
+          put_terms(to + z, a.hidden_plane, 0.0f);
     }
   }
 }
@@ -449,7 +445,7 @@ __device__ __forceinline__ void join(const W4MoeArgs& a, const float* sums, int 
 // Few tokens: the last workgroup of a column group joins the pairs' sums.
 template <typename T, int kSteps, int kNT, bool kFew, bool kParts>
 __global__ __launch_bounds__(64 * kOutWaves) void moe_out_kernel(const W4MoeArgs a) {
-  typedef W4RowsTerms<Kind<T>::kHiddenTerms> X;
+  typedef W4RowsTerms<kHiddenTerms> X;
   constexpr int kColumns = 16 * kNT;
   __shared__ int32_t lists[kFew ? kOutWaves : 1][kFew ? kMoeFewTokens : 1];
   __shared__ float others[kParts ? kOutWaves : 1][kNT][4][64];
@@ -607,7 +603,7 @@ hipError_t launch(const W4MoeArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-size_t moe_w4_workspace(W4MoeArgs& a, bool bf16, void* base) {
+size_t moe_w4_workspace(W4MoeArgs& a, void* base) {
   const size_t pairs = (size_t)a.tokens * a.top_k, experts = (size_t)a.experts;
   size_t at = 0;
   const auto take = [&](size_t bytes) {
@@ -635,7 +631,7 @@ size_t moe_w4_workspace(W4MoeArgs& a, bool bf16, void* base) {
   a.places = reinterpret_cast<uint8_t*>(take((size_t)a.tokens * experts));
   a.pairs = reinterpret_cast<int32_t*>(take(pairs * sizeof(int32_t)));
   a.reached = reinterpret_cast<MoeExpert*>(take((size_t)slots * sizeof(MoeExpert)));
-  a.hidden = reinterpret_cast<uint16_t*>(take(a.hidden_plane * (bf16 ? 2 : 3) * sizeof(uint16_t)));
+  a.hidden = reinterpret_cast<uint16_t*>(take(a.hidden_plane * kHiddenTerms * sizeof(uint16_t)));
   const size_t parts = pairs * a.parts * columns * 16u * a.out_tiles;
   a.part = reinterpret_cast<float*>(take(parts * sizeof(float)));
   return at;

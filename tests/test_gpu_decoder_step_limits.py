@@ -1,0 +1,55 @@
+"""The rest of a decoder's step on the GPU where a looser test would not see a loss: values with all their bits.  Tolerances count roundings, each half a step (2^-24 of a value in fp32,
+2^-8 in bf16)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import oracle
+from tests.test_gpu_decoder_step import BF16, F32, HALF_STEP, _matrix
+from tests.test_gpu_quantised_path import Device, _bits, _rounded, _values
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+# ------------------------------------------------------------------ the mixture's hidden rows
+def _held(shape, at):
+    """Weights that groups of 32 hold exactly: `at` gives {(row, column): power of two}; the column behind each is six
+    times as large, so that the step is that power (and has to meet a zero)."""
+    w = np.zeros(shape, np.float32)
+    for (row, column), value in at.items():
+        w[row, column], w[row, column + 1] = value, 6.0 * abs(value)
+    return w
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("tokens", (1, 12, 40, 130))
+def test_hidden_rows_keep_all_their_bits(gpu_runtime, tokens, dtype):
+    """out = h1 - h2 for two hidden values of 24 bits that differ in the last eight: 32 (x0 + x32 / 2^8 + x64 / 2^16) and
+    the same without its last summand, from bf16 numbers in [1, 2).  The gate is 32, whose activation is 32 to 2^-46.
+    Every sum is exact but for a few roundings of what is left."""
+    hidden, inner = 128, 70
+    x = np.zeros((tokens, hidden), np.float32)
+    x[:, [0, 32, 64]] = _rounded(oracle.uniform(tokens, (tokens, 3), 1.0, 2.0), BF16)
+    x[:, 96] = 32.0
+    gate = np.zeros((inner, hidden), np.float32)
+    gate[[3, 40]] = _held((1, hidden), {(0, 96): 1.0})
+    up = np.zeros((inner, hidden), np.float32)
+    up[3] = _held((1, hidden), {(0, 0): 1.0, (0, 32): 2.0 ** -8, (0, 64): 2.0 ** -16})
+    up[40] = _held((1, hidden), {(0, 0): 1.0, (0, 32): 2.0 ** -8})
+    scales = np.exp2(np.arange(hidden) % 5).astype(np.float32)
+    down = np.zeros((hidden, inner), np.float32)
+    down[:, 3], down[:, 4], down[:, 40], down[:, 41] = scales, 6 * scales, -scales, 6 * scales
+    router = np.ones((1, hidden), np.float32)
+    with Device(gpu_runtime) as dev:
+        (gate, gv), (up, uv), (down, dv) = (_matrix(dev, w[None], 32) for w in (gate, up, down))
+        assert gv.max() == 6 and uv[0, 3, 64] == 2.0 ** -16 and np.array_equal(dv[0, :, 3], scales)
+        out = _bits(np.zeros((tokens, hidden), np.float32), dtype)
+        to = dev.up(out)
+        gpu_runtime.moe_w4_device(gate, up, down, dev.up(router), dev.up(_bits(x, dtype)), to, tokens, 1, hidden, hidden, dtype)
+        got = _values(dev.down(out, to), dtype).astype(np.float64)
+    expect = 32.0 * 2.0 ** -16 * x[:, 64:65].astype(np.float64) * scales
+    # activation and hidden values to 2^-46; two sums of terms that cancel exactly but for their last eight bits
+    assert np.all(np.abs(got - expect) <= (HALF_STEP[dtype] + 4 * U) * expect)
