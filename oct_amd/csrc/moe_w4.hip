@@ -621,8 +621,9 @@ size_t moe_w4_workspace(W4MoeArgs& a, void* base) {
   while (a.split < 4 && slots * a.split < 32 && a.down.tiles_k >= 4 * a.split) a.split *= 2;
   a.parts = a.tokens <= 16 ? 1 : a.split;
   a.joins = a.tokens <= kMoeFewTokens && columns <= kColumnTickets;
-  // Blocks of sixteen pairs of an expert at once; those behind are taken in turn.
-  a.blocks = a.tokens <= kMoeFewTokens ? 1 : (int)std::min<size_t>((2 * pairs / experts + 15) / 16, 64);
+  // Blocks of sixteen pairs of an expert at once, for twice as many pairs as experts have in the mean; those behind are taken
+  // in turn.
+  a.blocks = a.tokens <= kMoeFewTokens ? 1 : (int)std::min<size_t>(std::max<size_t>(2 * pairs / experts + 15, 16) / 16, 64);
   a.hidden_stride = (uint32_t)a.down.tiles_k * kW4TileK;
   a.hidden_plane = pairs * a.hidden_stride;
   a.logits = reinterpret_cast<double*>(take((size_t)a.tokens * experts * sizeof(double)));

@@ -1,12 +1,13 @@
-"""The rest of a decoder's step on the GPU where a looser test would not see a loss: values with all their bits.  Tolerances count roundings, each half a step (2^-24 of a value in fp32,
-2^-8 in bf16)."""
+"""The rest of a decoder's step on the GPU at the ends of its ranges: values with all their bits, few pairs among many
+experts.  Tolerances count roundings, each half a step (2^-24 of a value in fp32, 2^-8 in bf16), or are those of
+tests/test_gpu_decoder_step.py."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
 import oracle
-from tests.test_gpu_decoder_step import BF16, F32, HALF_STEP, _matrix
+from tests.test_gpu_decoder_step import BF16, F32, HALF_STEP, _close, _matrix, _mixture
 from tests.test_gpu_quantised_path import Device, _bits, _rounded, _values
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +54,13 @@ def test_hidden_rows_keep_all_their_bits(gpu_runtime, tokens, dtype):
     expect = 32.0 * 2.0 ** -16 * x[:, 64:65].astype(np.float64) * scales
     # activation and hidden values to 2^-46; two sums of terms that cancel exactly but for their last eight bits
     assert np.all(np.abs(got - expect) <= (HALF_STEP[dtype] + 4 * U) * expect)
+
+
+# ------------------------------------------------------------------ few pairs among many experts
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("tokens,experts,top_k,group,renormalise", [
+    (65, 131, 1, 32, False), (65, 132, 1, 64, True), (100, 256, 1, 32, True), (128, 1024, 2, 128, False),
+    (128, 1024, 3, 64, True), (70, 300, 2, 32, False)])
+def test_mixture_of_fewer_pairs_than_half_the_experts(gpu_runtime, tokens, experts, top_k, group, renormalise, dtype):
+    case = dict(tokens=tokens, hidden=64, inner=48, experts=experts, top_k=top_k, group=group, renormalise=renormalise)
+    _close(*_mixture(gpu_runtime, case, dtype), dtype)
