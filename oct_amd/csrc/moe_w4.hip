@@ -523,7 +523,7 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const W4MoeArgs a) {
 }
 
 template <typename T, int kSteps, W4Edge kEdge>
-void launch_hidden(const W4MoeArgs& a, hipStream_t stream) {
+hipError_t launch_hidden(const W4MoeArgs& a, hipStream_t stream) {
   const dim3 grid((unsigned)(a.gate.tiles_n + kHiddenTiles - 1) / kHiddenTiles,
                   (unsigned)std::min(a.experts, a.tokens * a.top_k), (unsigned)a.blocks);
 #define HIDDEN(FEW)                                                                                                       \
@@ -534,42 +534,39 @@ void launch_hidden(const W4MoeArgs& a, hipStream_t stream) {
   else
     HIDDEN(false);
 #undef HIDDEN
+  return hipGetLastError();
 }
 template <typename T, int kSteps>
-void launch_hidden(const W4MoeArgs& a, hipStream_t stream) {
+hipError_t launch_hidden(const W4MoeArgs& a, hipStream_t stream) {
   const W4Edge edge = w4_edge<T>(a.x, a.x_stride, a.gate.k);
   if (edge == kEdgeNone) return launch_hidden<T, kSteps, kEdgeNone>(a, stream);
   if (edge == kEdgeShift) return launch_hidden<T, kSteps, kEdgeShift>(a, stream);
   if constexpr (sizeof(T) == 2)
     if (edge == kEdgeOdd) return launch_hidden<T, kSteps, kEdgeOdd>(a, stream);
-  launch_hidden<T, kSteps, kEdgeShort>(a, stream);
+  return launch_hidden<T, kSteps, kEdgeShort>(a, stream);
 }
 
 template <typename T, int kSteps, int kNT, bool kFew, bool kParts>
-void launch_out(const W4MoeArgs& a, hipStream_t stream) {
+hipError_t launch_out(const W4MoeArgs& a, hipStream_t stream) {
   const unsigned columns = (unsigned)(a.down.tiles_n + kNT - 1) / kNT;
   const unsigned units = (unsigned)(std::min(a.experts, a.tokens * a.top_k) * a.split);
   const dim3 grid(columns, (units + kOutWaves - 1) / kOutWaves, (unsigned)a.blocks);
   hipLaunchKernelGGL((moe_out_kernel<T, kSteps, kNT, kFew, kParts>), grid, dim3(64 * kOutWaves), 0, stream, a);
-  if (a.joins) return;
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.joins) return e;
   const unsigned shares = (unsigned)std::min((a.tokens * 8 * kNT + 255) / 256, 64);
   hipLaunchKernelGGL((moe_join_kernel<T, kNT>), dim3(columns, shares), dim3(256), 0, stream, a);
+  return hipGetLastError();
 }
 template <typename T, int kSteps>
-void launch_out(const W4MoeArgs& a, hipStream_t stream) {
+hipError_t launch_out(const W4MoeArgs& a, hipStream_t stream) {
   if (a.tokens <= kMoeFewTokens) {
-    if (a.out_tiles == 4)
-      launch_out<T, kSteps, 4, true, false>(a, stream);
-    else if (a.split > a.parts)
-      launch_out<T, kSteps, 2, true, true>(a, stream);
-    else
-      launch_out<T, kSteps, 2, true, false>(a, stream);
-  } else {
-    if (a.out_tiles == 4)
-      launch_out<T, kSteps, 4, false, false>(a, stream);
-    else
-      launch_out<T, kSteps, 2, false, false>(a, stream);
+    if (a.out_tiles == 4) return launch_out<T, kSteps, 4, true, false>(a, stream);
+    if (a.split > a.parts) return launch_out<T, kSteps, 2, true, true>(a, stream);
+    return launch_out<T, kSteps, 2, true, false>(a, stream);
   }
+  if (a.out_tiles == 4) return launch_out<T, kSteps, 4, false, false>(a, stream);
+  return launch_out<T, kSteps, 2, false, false>(a, stream);
 }
 
 template <typename T>
@@ -588,17 +585,17 @@ hipError_t launch(const W4MoeArgs& a, hipStream_t stream) {
     ROUTER(16)
   }
 #undef ROUTER
-#define STEPS(what, group) \
-  if (group == 32)         \
-    what<T, 4>(a, stream); \
-  else if (group == 64)    \
-    what<T, 2>(a, stream); \
-  else                     \
-    what<T, 1>(a, stream);
+  // What reads a launch's results is queued only behind one that is.
+  hipError_t e = hipGetLastError();
+#define STEPS(what, group)                    \
+  if (e == hipSuccess)                        \
+    e = group == 32   ? what<T, 4>(a, stream) \
+        : group == 64 ? what<T, 2>(a, stream) \
+                      : what<T, 1>(a, stream);
   STEPS(launch_hidden, a.gate.group)
   STEPS(launch_out, a.down.group)
 #undef STEPS
-  return hipGetLastError();
+  return e;
 }
 
 }  // namespace

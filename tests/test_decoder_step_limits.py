@@ -23,3 +23,15 @@ def _run(check, *args):
 def test_every_mixture_is_launched(moe_check, bf16, hidden, inner, group):
     """No count of tokens, experts and chosen ones leaves a launch without workgroups."""
     _run(moe_check, bf16, -1, hidden, inner, group, 0, 0, 0)
+
+
+@pytest.mark.parametrize("bf16", (0, 1))
+@pytest.mark.parametrize("tokens,experts,top_k", [(1, 8, 2), (64, 64, 8), (100, 16, 2)])
+def test_a_failed_launch_of_a_mixture_is_its_last(moe_check, bf16, tokens, experts, top_k):
+    """What would read a failed launch's results is not queued, and the call returns its error."""
+    _run(moe_check, bf16, 0, 128, 64, 32, tokens, experts, top_k)
+
+
+def test_a_failed_launch_is_the_last_of_a_mixture_of_many_columns(moe_check):
+    """Few tokens whose sums are joined in a launch of their own."""
+    _run(moe_check, 1, 0, 70000, 24, 128, 2, 2, 1)
