@@ -36,6 +36,7 @@
 // cross-check of the parity tests.
 #include <type_traits>
 
+#include "lds_dma.h"
 #include "reactor_internal.h"
 
 namespace prom {
@@ -353,13 +354,9 @@ __global__ __launch_bounds__(256, 2) void flash_attn_bf16_dma_kernel(const uint1
     const uint32_t base = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)st;
     const uint32_t la = __builtin_amdgcn_readfirstlane(base + (4 * wave + i) * 1024);
     if (kx)
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(la), "v"(koff[i] + add),
-                   "s"(rs_k)
-                   : "memory", "m0");
+      lds_from_buffer(la, koff[i] + add, rs_k);
     else
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(la), "v"(voff[i] + add),
-                   "s"(rs_v)
-                   : "memory", "m0");
+      lds_from_buffer(la, voff[i] + add, rs_v);
   };
   auto issue_tile = [&](int j) {
 #pragma unroll

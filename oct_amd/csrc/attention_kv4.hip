@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "lds_dma.h"
 #include "reactor_internal.h"
 
 namespace prom {
@@ -208,8 +209,7 @@ struct Stage {
         off ^= (uint32_t)(16 * (1024 * i < kCodes ? key_swz(t) : value_swz(t)));
       }
       const uint32_t m0 = __builtin_amdgcn_readfirstlane(to + 1024 * i);
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(off), "s"(d)
-                   : "memory", "m0");
+      lds_from_buffer(m0, off, d);
     }
   }
 };

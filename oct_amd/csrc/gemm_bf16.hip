@@ -18,6 +18,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "lds_dma.h"
 #include "reactor_internal.h"
 
 namespace prom {
@@ -341,15 +342,11 @@ __device__ __forceinline__ void gemm_bf16_dl4_body(const uint16_t* __restrict__ 
     if ((j & 1) == 0) {
       const int sa = __builtin_amdgcn_readfirstlane(a_slice > 0 ? k0 * a_slice * 2 : k0 * 2);
       const uint32_t la = __builtin_amdgcn_readfirstlane(base + q * 1024);
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(la), "v"(a_off[i]), "s"(da),
-                   "s"(sa)
-                   : "memory", "m0");
+      lds_from_buffer(la, a_off[i], da, sa);
     } else {
       const int sb = __builtin_amdgcn_readfirstlane(k0 * ldb * 2);
       const uint32_t lb = __builtin_amdgcn_readfirstlane(base + 16384 + q * 1024);
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lb), "v"(b_off[i]), "s"(db),
-                   "s"(sb)
-                   : "memory", "m0");
+      lds_from_buffer(lb, b_off[i], db, sb);
     }
   };
   auto issue = [&](char* stage, int k0) {

@@ -22,6 +22,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "lds_dma.h"
 #include "reactor_internal.h"
 
 namespace prom {
@@ -185,14 +186,11 @@ __global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_bf16_tile_kernel(const
         if ((kt0 + issued) * kBK + 8 * c >= g.k) off = kOutOfRange;
       }
       const uint32_t to = __builtin_amdgcn_readfirstlane(fill + (wave * C::kAX + j) * 1024);
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(da)
-                   : "memory", "m0");
+      lds_from_buffer(to, off, da);
     } else {
       const uint32_t to =
           __builtin_amdgcn_readfirstlane(fill + C::kABytes + (wave * C::kBX + (j - C::kAX)) * 1024);
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(b_off[j - C::kAX]),
-                   "s"(db)
-                   : "memory", "m0");
+      lds_from_buffer(to, b_off[j - C::kAX], db);
     }
   };
   auto advance = [&]() __attribute__((always_inline)) {

@@ -24,6 +24,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "lds_dma.h"
 #include "reactor_internal.h"
 
 namespace prom {
@@ -196,13 +197,10 @@ __global__ __launch_bounds__(64 * C::kWaves, 2) void gemm_int8_tile_kernel(const
         if ((kt0 + issued) * kBK + 16 * ((lane & 7) ^ swz(r)) >= g.k) off = kOutOfRange;
       }
       const uint32_t to = __builtin_amdgcn_readfirstlane(fill_a + j * 1024);
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(da)
-                   : "memory", "m0");
+      lds_from_buffer(to, off, da);
     } else {
       const uint32_t to = __builtin_amdgcn_readfirstlane(fill_b + (j - C::kAX) * 1024);
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(b_off[j - C::kAX]),
-                   "s"(db)
-                   : "memory", "m0");
+      lds_from_buffer(to, b_off[j - C::kAX], db);
     }
   };
   auto advance = [&]() __attribute__((always_inline)) {

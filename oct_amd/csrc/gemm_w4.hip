@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "fp4_groups.h"
+#include "lds_dma.h"
 #include "reactor_internal.h"
 #include "tickets.h"
 #include "w4_product.h"
@@ -186,8 +187,7 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(const W4TileArgs a) {
       for (int m = 0; m < kMT; ++m) {
         const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + stage + (uint32_t)((t * kMT + m) * 4 + wave) * 1024u);
         const uint32_t off = at + (uint32_t)m * block;
-        asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(d)
-                     : "memory", "m0");
+        lds_from_buffer(to, off, d);
       }
     }
   };

@@ -28,6 +28,7 @@
 #include <cstring>
 #include <type_traits>
 
+#include "lds_dma.h"
 #include "reactor_internal.h"
 
 namespace prom {
@@ -722,12 +723,8 @@ __device__ __forceinline__ void sgemm_f32_dl64_body(const float* __restrict__ A,
       const int q = Cfg::kXfer * wave + i;
       const uint32_t la = __builtin_amdgcn_readfirstlane(base + q * 1024);
       const uint32_t lb = __builtin_amdgcn_readfirstlane(base + Cfg::kABytes + q * 1024);
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(la), "v"(a_off[i]), "s"(rsa),
-                   "s"(sa_k)
-                   : "memory", "m0");
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lb), "v"(b_off[i]), "s"(rsb),
-                   "s"(sb_k)
-                   : "memory", "m0");
+      lds_from_buffer(la, a_off[i], rsa, sa_k);
+      lds_from_buffer(lb, b_off[i], rsb, sb_k);
     }
   };
   // This wave's transfers of a tile: kPerTile; at most `in_flight` later
