@@ -1056,8 +1056,9 @@ PROM_REACTOR_API int prometheus_reactor_runtime_w4_unpack_device(void* handle, c
 
 /* out[i, j] = sum_k x[i, k] w[j, k] for x of `dtype` [rows, k] and out [rows, n], x_stride and
    out_stride elements between rows (below 2^24), any alignment of their type.  Operands
-   enter unrounded (bf16 rows times codes are exact, fp32 rows go in as three exact terms);
-   sums are fp32, a bf16 result is rounded once.  A group's sum may be taken before it is
+   enter unrounded (bf16 rows times codes are exact; fp32 rows go in as three bf16 terms, which
+   hold an element down to 2^-110 exactly and a smaller one down to 2^-133, bf16's smallest
+   number); sums are fp32, a bf16 result is rounded once.  A group's sum may be taken before it is
    multiplied by its step: with |x| above 2^118 it can overflow where the product would not. */
 typedef struct PrometheusW4GemmRequest {
   uint32_t struct_size;

@@ -5,7 +5,7 @@
 // then holds columns l % 16 and rows 4 (l / 16) .. + 3 of the sums, so that a column's step is one value a lane.  A
 // group's sum is multiplied by its step (one fused multiply-add for each of its four rows) rather than each weight:
 // 512 weights of a step are 8 a lane.  bf16 rows enter as they are; fp32 rows as three bf16 terms, exact (8 + 8 + 8
-// significant bits).
+// significant bits) but for what an element has below 2^-133, bf16's smallest number.
 //
 // A tile travels from memory to registers while the one before is used, x with it.  Loads are never skipped: lanes
 // without a row load the last row (its sums are not used), and behind the last tile that one is loaded again, so that

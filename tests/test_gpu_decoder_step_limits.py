@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import oracle
-from tests.test_gpu_decoder_step import BF16, F32, HALF_STEP, _close, _matrix, _mixture
+from tests.test_gpu_decoder_step import BF16, F32, HALF_STEP, _close, _matrix, _mixture, _product
 from tests.test_gpu_quantised_path import Device, _bits, _rounded, _values
 
 pytestmark = pytest.mark.gpu
@@ -64,3 +64,43 @@ def test_hidden_rows_keep_all_their_bits(gpu_runtime, tokens, dtype):
 def test_mixture_of_fewer_pairs_than_half_the_experts(gpu_runtime, tokens, experts, top_k, group, renormalise, dtype):
     case = dict(tokens=tokens, hidden=64, inner=48, experts=experts, top_k=top_k, group=group, renormalise=renormalise)
     _close(*_mixture(gpu_runtime, case, dtype), dtype)
+
+
+# ------------------------------------------------------------------ products of fp32 rows with all their bits
+def _single(rows, k, low, high, seed=3):
+    """Rows with one number each, of 24 significant bits, at columns that meet every part of a K tile."""
+    x = np.zeros((rows, k), np.float32)
+    columns = (np.arange(rows) * 53 + k - 1) % k
+    bits = np.random.default_rng(seed).integers(1 << 23, 1 << 24, rows).astype(np.float64)
+    x[np.arange(rows), columns] = np.ldexp(bits, np.random.default_rng(seed + 1).integers(low, high, rows) - 23)
+    x[::3] *= -1
+    return x, columns
+
+
+@pytest.mark.parametrize("group", (32, 64, 128))
+@pytest.mark.parametrize("rows,n,k", [(3, 47, 395), (16, 600, 256), (20, 40, 9001), (40, 4500, 131), (5, 40, 6),
+                                      (200, 47, 395), (300, 260, 256), (1024, 4000, 256), (1000, 4000, 395), (1024, 4000, 7),
+                                      (512, 2000, 1000)])  # the last four on tiles
+def test_fp32_rows_enter_with_all_their_bits(gpu_runtime, rows, n, k, group):
+    """x w from three terms.  The sums of the last two are exact to 2^-8 of a rounding; that with the first is within 2^-23,
+    as a matrix instruction may cut it off, and the product with the step within half of that.  Zeros' sums are exact."""
+    x, columns = _single(rows, k, -6, 7)
+    w = (oracle.normal(n, (n, k)) * np.exp2(oracle.uniform(2, (n, 1), -3.0, 3.0))).astype(np.float32)
+    got, values = _product(gpu_runtime, x, w, group, F32)
+    expect = x[np.arange(rows), columns].astype(np.float64)[:, None] * values[:, columns].T
+    assert np.all(np.abs(got - expect) <= 3.1 * U * np.abs(expect))
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("rows,n", ((20, 40), (1000, 4000)))
+def test_products_of_the_smallest_rows(gpu_runtime, rows, n, dtype):
+    """Elements down to fp32's smallest: what a term of eight bits holds ends at 2^-133, bf16's smallest number, so that
+    fp32 elements are exact down to 2^-110 and within 2^-133 below."""
+    k = 300
+    x, columns = _single(rows, k, -126, -100)
+    x = _rounded(x, dtype)
+    w = (oracle.normal(n, (n, k)) * 2.0 ** 60).astype(np.float32)
+    got, values = _product(gpu_runtime, x, w, 64, dtype)
+    expect = x[np.arange(rows), columns].astype(np.float64)[:, None] * values[:, columns].T
+    left_out = np.abs(values[:, columns].T) * (2.0 ** -133 if dtype == F32 else 0.0)
+    assert np.all(np.abs(got - expect) <= left_out + (3.1 * U + (HALF_STEP[BF16] if dtype == BF16 else 0.0)) * np.abs(expect))
