@@ -1076,8 +1076,8 @@ PROM_REACTOR_API int prometheus_reactor_runtime_gemm_w4_device(void* handle, con
 
 /* A mixture-of-experts layer of a few tokens.  Logits l = x router^T are sums in binary64; a
    token's experts are the top_k largest (a NaN counts as less than every number; ties go to
-   the lower expert), their weights p = softmax(l) over all experts, divided by the sum over
-   the chosen ones where renormalise is set;
+   the lower expert), their weights p = softmax(l) over all experts (NaN where an l is), divided
+   by the sum over the chosen ones where renormalise is set;
      out[t] = sum over t's experts e, in their order, of p_e (act(x[t] gate_e^T) * (x[t] up_e^T)) down_e^T
    in fp32, a bf16 result rounded once.  x of `dtype` [tokens, hidden] and out [tokens, hidden] as
    in the product above, router fp32 [experts, hidden].  gate and up are [inner, hidden] of one group

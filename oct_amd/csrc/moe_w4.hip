@@ -181,13 +181,15 @@ struct Choice {
   __device__ __forceinline__ void leave(const W4MoeArgs& a, int t) const {
     const int lane = (int)threadIdx.x & 63, mine = (a.experts + 63) >> 6;
     const double top = lane_value(picked, 0), p = lane < a.top_k ? exp(picked - top) : 0.0;
-    double sum = p;
-    if (!a.renormalise) {
-      sum = 0.0;
+    double sum = a.renormalise ? p : 0.0;
 #pragma unroll
-      for (int i = 0; i < kMost; ++i)
-        if (i < mine && lane + 64 * i < a.experts) sum += exp(logit[i] - top);
-    }
+    for (int i = 0; i < kMost; ++i)
+      if (i < mine && lane + 64 * i < a.experts) {
+        if (!a.renormalise)
+          sum += exp(logit[i] - top);
+        else if (logit[i] != logit[i])
+          sum = logit[i];  // the softmax over all experts has no value then
+      }
     sum = wave_sum(sum);
     if (lane < a.top_k) {
       const size_t pair = (size_t)t * a.top_k + lane;

@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 
 import oracle
+from oracle import decoder_step as od
 from tests.test_gpu_decoder_step import BF16, F32, HALF_STEP, _close, _matrix, _mixture, _product
 from tests.test_gpu_quantised_path import Device, _bits, _rounded, _values
 
@@ -104,3 +105,31 @@ def test_products_of_the_smallest_rows(gpu_runtime, rows, n, dtype):
     expect = x[np.arange(rows), columns].astype(np.float64)[:, None] * values[:, columns].T
     left_out = np.abs(values[:, columns].T) * (2.0 ** -133 if dtype == F32 else 0.0)
     assert np.all(np.abs(got - expect) <= left_out + (3.1 * U + (HALF_STEP[BF16] if dtype == BF16 else 0.0)) * np.abs(expect))
+
+
+# ------------------------------------------------------------------ logits without a value
+@pytest.mark.parametrize("renormalise", (False, True))
+@pytest.mark.parametrize("experts,tokens", ((6, 1), (6, 20), (70, 3), (300, 170)))
+def test_weights_are_nan_where_a_logit_is(gpu_runtime, experts, tokens, renormalise):
+    """A softmax over all experts has no value where one of its logits has none, chosen or not: the choice goes by the
+    others, the weights and the row of that token are NaN.  The other tokens' logit of that expert is below all numbers."""
+    hidden, inner, top_k = 64, 32, 2
+    x = oracle.normal(3, (tokens, hidden))
+    x[:, 5] = -1.0
+    x[0, 5] = 0.0
+    router = (oracle.normal(5, (experts, hidden)) * 0.2).astype(np.float32)
+    router[2, 5] = np.inf
+    shapes = ((inner, hidden), (inner, hidden), (hidden, inner))
+    with Device(gpu_runtime) as dev:
+        matrices = [_matrix(dev, oracle.normal(i, (experts, *shape)) * np.float32(0.1), 32)[0] for i, shape in enumerate(shapes)]
+        out, chosen = np.zeros((tokens, hidden), np.float32), np.zeros((tokens, top_k), np.int32)
+        weights = np.zeros((tokens, top_k), np.float32)
+        to, dc, dw = dev.up(out), dev.up(chosen), dev.up(weights)
+        gpu_runtime.moe_w4_device(*matrices, dev.up(router), dev.up(x), to, tokens, top_k, hidden, hidden, F32,
+                                  renormalise=renormalise, dexperts=dc, dweights=dw)
+        out, chosen, weights = dev.down(out, to), dev.down(chosen, dc), dev.down(weights, dw)
+    with np.errstate(invalid="ignore"):
+        expect_chosen, expect = od.route(x, router, top_k, renormalise)
+    assert np.array_equal(chosen, expect_chosen) and not (chosen == 2).any()
+    assert np.isnan(weights[0]).all() and np.isnan(out[0]).all() and np.isfinite(out[1:]).all()
+    assert np.allclose(weights, expect, rtol=2.0 ** -22, equal_nan=True)
