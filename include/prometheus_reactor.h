@@ -1115,7 +1115,7 @@ PROM_REACTOR_API int prometheus_reactor_runtime_moe_w4_device(void* handle, cons
    head_dim] with strides in elements between rows (below 2^24, at least heads * head_dim), any
    alignment of their type; either may be NULL with its output.  An output may be its input
    (with the same stride).  positions int32 [rows], any sign; turns binary64 [rotary_dim / 2].
-   Angles are binary64, the rotation fp32, a bf16 result rounded once. */
+   Angles, their cosines and sines are binary64, the rotation fp32, a bf16 result rounded once. */
 enum { PROM_ROPE_HALF = 0u, PROM_ROPE_PAIRS = 1u };
 typedef struct PrometheusRopeRequest {
   uint32_t struct_size;

@@ -4,9 +4,9 @@
 // pairs (i, i + rotary / 2) or (2 i, 2 i + 1) of the first `rotary` channels of each head; the others are copied.
 //
 // A workgroup takes a row, or four: its threads make the rows' cosines and sines once, in LDS, and go over the heads with eight
-// channels of each half (or eight neighbouring ones) a thread.  Angles are in binary64 and in revolutions, so that a
-// far position loses nothing but whole turns; what is left of a turn is within 2^-24 in fp32, and sincospi is good to
-// an ulp or two.  Bound by memory.
+// channels of each half (or eight neighbouring ones) a thread.  Angles, sines and cosines are in binary64 and in
+// revolutions, so that a far position loses nothing but whole turns; they are rounded once to fp32 (a fraction of a turn and
+// sincospif in fp32: 5.9e-8 of fp32 rows instead of 4.1e-8).  Bound by memory.
 #include <algorithm>
 
 #include "reactor_internal.h"
@@ -37,6 +37,23 @@ __device__ __forceinline__ void store(uint16_t* p, const float (&v)[kN]) {
 #pragma unroll
   for (int j = 0; j < kN; ++j) w[j] = (__bf16)v[j];
   __builtin_memcpy(p, w, 2 * kN);
+}
+
+// Cosine and sine of t revolutions, |t| <= 1/2, times m.  Within an eighth of the nearest quarter they are the power series of
+// x = 2 pi t, |x| <= pi / 4, whose first terms left out are x^15 / 15! and x^16 / 16!, below 2^-45 and 2^-49.
+__device__ __forceinline__ void turned(double t, double m, float* c, float* s) {
+  const double quarter = rint(4.0 * t), x = 6.283185307179586 * __builtin_fma(-0.25, quarter, t), z = x * x;
+  double sine = 1.0 / 6227020800.0, cosine = -1.0 / 87178291200.0;  // 1 / 13!, 1 / 14!
+  sine = __builtin_fma(sine, z, -1.0 / 39916800.0), cosine = __builtin_fma(cosine, z, 1.0 / 479001600.0);
+  sine = __builtin_fma(sine, z, 1.0 / 362880.0), cosine = __builtin_fma(cosine, z, -1.0 / 3628800.0);
+  sine = __builtin_fma(sine, z, -1.0 / 5040.0), cosine = __builtin_fma(cosine, z, 1.0 / 40320.0);
+  sine = __builtin_fma(sine, z, 1.0 / 120.0), cosine = __builtin_fma(cosine, z, -1.0 / 720.0);
+  sine = __builtin_fma(sine, z, -1.0 / 6.0), cosine = __builtin_fma(cosine, z, 1.0 / 24.0);
+  sine = x * __builtin_fma(sine, z, 1.0), cosine = __builtin_fma(__builtin_fma(cosine, z, -0.5), z, 1.0);
+  const int q = (int)quarter;
+  const double a = q & 1 ? -sine : cosine, b = q & 1 ? cosine : sine;  // a quarter turns (c, s) to (-s, c)
+  *c = (float)(q & 2 ? -m * a : m * a);
+  *s = (float)(q & 2 ? -m * b : m * b);
 }
 
 // kN channels of each of a pair's sides at once (kN = 1: any sizes), of row `r` of a workgroup's kRows, whose angles are
@@ -107,10 +124,7 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
       const uint32_t r = at / half, i = at - r * half;
       double t = (double)a.positions[row0 + r] * a.turns[i];
       t -= rint(t);
-      float s, c;
-      sincospif(2.0f * (float)t, &s, &c);
-      cs[2 * at] = c * a.magnitude;
-      cs[2 * at + 1] = s * a.magnitude;
+      turned(t, (double)a.magnitude, &cs[2 * at], &cs[2 * at + 1]);
     }
     __syncthreads();
     if (a.q.in != nullptr) turn_heads<T, kPairs, kN, kRows>(a, a.q, row0, rows, cs);

@@ -8,6 +8,7 @@ import pytest
 
 import oracle
 from oracle import decoder_step as od
+from oct_amd import prometheus as p
 from tests.test_gpu_decoder_step import BF16, F32, HALF_STEP, _close, _matrix, _mixture, _product
 from tests.test_gpu_quantised_path import Device, _bits, _rounded, _values
 
@@ -133,3 +134,39 @@ def test_weights_are_nan_where_a_logit_is(gpu_runtime, experts, tokens, renormal
     assert np.array_equal(chosen, expect_chosen) and not (chosen == 2).any()
     assert np.isnan(weights[0]).all() and np.isnan(out[0]).all() and np.isfinite(out[1:]).all()
     assert np.allclose(weights, expect, rtol=2.0 ** -22, equal_nan=True)
+
+
+# ------------------------------------------------------------------ rotary positions
+@pytest.mark.parametrize("pairs", (False, True))
+@pytest.mark.parametrize("magnitude", (1.0, 1.2079441541679836))
+@pytest.mark.parametrize("rows", (300, 4100))
+def test_rope_rounds_only_at_its_end(gpu_runtime, rows, magnitude, pairs):
+    """Angle, cosine, sine and magnitude in binary64, the last three's product rounded once to fp32, then a product, a fused
+    one and no other rounding: 2 |a c| + 3 |b s| halves of a step at most, in either order.  Such errors, spread evenly over
+    a step, have a mean square of at most a third of (a c)^2 + 2 (b s)^2 + out^2 halves of a step: 5/6 of x^2 over all."""
+    heads, dim = 2, 64
+    positions = np.random.default_rng(rows).integers(0, 1 << 20, rows).astype(np.int32)
+    turns, _ = p.rope_turns(dim)
+    x = _rounded(oracle.normal(rows, (rows, heads * dim)), F32)
+    with Device(gpu_runtime) as dev:
+        to = dev.up(x)
+        gpu_runtime.rope_device(dev.up(positions), dev.up(turns), rows, dim, dim, p.ROPE_PAIRS if pairs else p.ROPE_HALF, F32,
+                                magnitude, q=(to, to, heads, heads * dim, heads * dim))
+        got = dev.down(x, to).reshape(rows, heads, dim).astype(np.float64)
+    magnitude = float(np.float32(magnitude))
+    x = x.reshape(rows, heads, dim).astype(np.float64)
+    t = positions.astype(np.longdouble)[:, None] * turns.astype(np.longdouble)
+    angle = 2.0 * np.pi * (t - np.rint(t)).astype(np.float64)
+    c, s = (magnitude * f(angle)[:, None] for f in (np.cos, np.sin))
+    # positions * turns is rounded to 2^-53 of itself, 2^20 / (2 pi) at most: 2^-35 of a turn, far below U
+    off = 2 * np.pi * np.abs(t).astype(np.float64)[:, None] * 2.0 ** -53 * magnitude + magnitude * 2.0 ** -40
+    first = np.arange(dim // 2) * 2 if pairs else np.arange(dim // 2)
+    second = first + 1 if pairs else first + dim // 2
+    a, b = x[..., first], x[..., second]
+    square = 0.0
+    for out, u, v, f, g in ((first, a, b, c, -s), (second, b, a, c, s)):
+        expect = u * f + v * g
+        limit = U * (3 * np.abs(u * f) + 3 * np.abs(v * g)) * (1 + 2.0 ** -20) + (np.abs(u) + np.abs(v)) * off
+        assert np.all(np.abs(got[..., out] - expect) <= limit)
+        square += ((got[..., out] - expect) ** 2).sum()
+    assert square <= 5.0 / 6.0 * U ** 2 * magnitude ** 2 * (x * x).sum()
