@@ -101,12 +101,21 @@ __device__ __forceinline__ double row_sum(double v, double (&part)[kWaves]) {
   }
   return v;
 }
-// 1 / sqrt(mean + eps) of a sum of squares, over = 1 / width: the instruction's value is within 2^-23 or so, a step of
+// 1 / sqrt(mean + eps) as a product: past fp32's range, or where it would be among its subnormal numbers (rows below 2^-100,
+// above 2^100), `scale` is the power of two that keeps x scale and `rest` within it.
+struct Inverse {
+  float scale, rest;
+  __device__ __forceinline__ float of(float x) const { return x * scale * rest; }
+};
+// Of a sum of squares, over = 1 / width: the instruction's value is within 2^-23 or so, a step of
 // Newton's makes it 2^-45 (a division and a root in binary64 were a third of the kernel's time).  Where the step has no
 // value the root's is that of 0 or infinity, and stands.
-__device__ __forceinline__ float inverse_size(double sum, double over, float eps) {
-  const double x = __builtin_fma(sum, over, (double)eps), r = __builtin_amdgcn_rsq(x), e = __builtin_fma(-x * r, r, 1.0);
-  return (float)(e == e ? __builtin_fma(0.5 * r, e, r) : r);
+__device__ __forceinline__ Inverse inverse_size(double sum, double over, float eps) {
+  const double x = __builtin_fma(sum, over, (double)eps), q = __builtin_amdgcn_rsq(x), e = __builtin_fma(-x * q, q, 1.0);
+  const double r = e == e ? __builtin_fma(0.5 * q, e, q) : q;
+  if (r > 0x1p100) return Inverse{0x1p64f, (float)(r * 0x1p-64)};
+  if (r < 0x1p-100) return Inverse{0x1p-64f, (float)(r * 0x1p64)};
+  return Inverse{1.0f, (float)r};
 }
 
 // The squares' sum of eight values of which there are `left`, if any; what lies behind them is zero where it is not a repeat.
@@ -207,7 +216,7 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm
       if (row + kRows < end) fetch(row + kRows);
     const uint32_t now = row;
     if (a.y != nullptr) {
-      float r = 1.0f;
+      Inverse r{1.0f, 1.0f};
       if (a.post != nullptr) {
         double sum = 0.0;
 #pragma unroll
@@ -218,7 +227,7 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm
       for (int i = 0; i < kChunks; ++i) {
         if constexpr (!kKeeps) of_y(vector, i, fy[0]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[i][j] = __builtin_fmaf(y[i][j] * r, fy[kStays * i][j], h[i][j]);
+        for (int j = 0; j < 8; ++j) h[i][j] = __builtin_fmaf(r.of(y[i][j]), fy[kStays * i][j], h[i][j]);
       }
     }
     if (a.h_out != nullptr) {
@@ -231,7 +240,7 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm
       double sum = 0.0;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) sum += squares(h[i], left[i]);
-      const float r = inverse_size(row_sum<kWaves>(sum, part[1][turn]), a.over_width, a.eps);
+      const Inverse r = inverse_size(row_sum<kWaves>(sum, part[1][turn]), a.over_width, a.eps);
       T* to = static_cast<T*>(a.out) + (size_t)now * a.out_stride;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
@@ -239,7 +248,7 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void residual_norm
         float o[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          o[j] = h[i][j] * r * fh[kStays * i][j];
+          o[j] = r.of(h[i][j]) * fh[kStays * i][j];
           if (a.shift != nullptr) o[j] += add[kStays * i][j];
         }
         if (left[i] > 0) store8<kWhole>(to + at[i], left[i], o);

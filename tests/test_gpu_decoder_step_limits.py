@@ -170,3 +170,27 @@ def test_rope_rounds_only_at_its_end(gpu_runtime, rows, magnitude, pairs):
         assert np.all(np.abs(got[..., out] - expect) <= limit)
         square += ((got[..., out] - expect) ** 2).sum()
     assert square <= 5.0 / 6.0 * U ** 2 * magnitude ** 2 * (x * x).sum()
+
+
+# ------------------------------------------------------------------ residual norms
+@pytest.mark.parametrize("width", (8, 601, 1504, 16400))
+def test_residual_norm_at_the_ends_of_the_range(gpu_runtime, width):
+    """Rows of the smallest and largest numbers: 1 / sqrt of the mean may lie past fp32's range or among its subnormal
+    numbers, the quotient does not.  x / size: its scaling is exact, then a factor and a product: two roundings, and one
+    of the size."""
+    scales = [2.0 ** -146, 2.0 ** -140, 2.0 ** -129, 2.0 ** -127, 2.0 ** -126, 2.0 ** 120, 2.0 ** 126, 1.0]
+    x = np.clip(oracle.normal(1, (len(scales), width)), -1.9, 1.9).astype(np.float64)
+    x = (x * np.array(scales)[:, None]).astype(np.float32)
+    x[0, :2] = np.float32(2.0 ** -146)  # the smallest rows are not zeros
+    weight = (oracle.normal(2, (width,)) * 0.1 + 1.0).astype(np.float32)
+    h = np.zeros_like(x)
+    with Device(gpu_runtime) as dev:
+        dx, dw = dev.up(x), dev.up(weight)
+        norm, h_out = dev.up(x), dev.up(x)
+        gpu_runtime.residual_norm_device(dx, None, norm, len(x), width, F32, dpre=dw, eps=0.0)
+        gpu_runtime.residual_norm_device(dev.up(h), h_out, None, len(x), width, F32, dy=dx, dpost=dw, eps=0.0)
+        got = [dev.down(x, norm), dev.down(x, h_out)]
+    wide = x.astype(np.float64)
+    expect = wide / np.sqrt((wide ** 2).mean(1, keepdims=True)) * weight.astype(np.float64)
+    for v in got:
+        assert np.all(np.abs(v - expect) <= 4 * U * np.abs(expect) + 2.0 ** -140)
