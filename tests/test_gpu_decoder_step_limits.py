@@ -93,6 +93,58 @@ def test_fp32_rows_enter_with_all_their_bits(gpu_runtime, rows, n, k, group):
     assert np.all(np.abs(got - expect) <= 3.1 * U * np.abs(expect))
 
 
+@pytest.mark.parametrize("group", (32, 64, 128))
+@pytest.mark.parametrize("n", (100, 2400, 4800, 13600, 32800))
+@pytest.mark.parametrize("k", (7, 131, 256))
+def test_every_column_of_fp32_rows_enters_with_all_its_bits(gpu_runtime, n, k, group):
+    """As above, for each column of a K tile and of its rest, with one to eight waves a workgroup and 32 or 64 columns."""
+    w = (oracle.normal(n, (n, k)) * np.exp2(oracle.uniform(2, (n, 1), -3.0, 3.0))).astype(np.float32)
+    with Device(gpu_runtime) as dev:
+        matrix, values = _matrix(dev, w, group)
+        out = np.zeros((64, n), np.float32)
+        to = dev.up(out)
+        for first in range(0, k, 64):
+            columns = (first + np.arange(64)) % k
+            x = np.zeros((64, k), np.float32)
+            x[np.arange(64), columns] = np.random.default_rng(first).integers(1 << 23, 1 << 24, 64) * np.float32(2.0 ** -23)
+            gpu_runtime.gemm_w4_device(matrix, dev.up(x), to, 64, k, n, F32)
+            expect = x[np.arange(64), columns].astype(np.float64)[:, None] * values[:, columns].T
+            assert np.all(np.abs(dev.down(out, to) - expect) <= 3.1 * U * np.abs(expect)), first
+
+
+@pytest.mark.parametrize("group", (32, 64, 128))
+@pytest.mark.parametrize("hidden", (256, 260))
+@pytest.mark.parametrize("tokens,experts", ((64, 1), (255, 1), (64, 64), (255, 64)))
+def test_every_column_of_a_mixture_enters_with_all_its_bits(gpu_runtime, tokens, experts, hidden, group):
+    """A token has one number x besides its gate's, which makes one hidden value h = 48 (6 x), and out = h down[:, f]: x
+    and h are 24 bits each.  The sum 6 x and the last one are within 3.1 halves of a step, h, its activation, the weight 1
+    and the sum over experts are a rounding each."""
+    inner = 250
+    up = np.zeros((inner, hidden), np.float32)
+    up[np.arange(inner), np.arange(inner)] = 6.0
+    gate = np.zeros((inner, hidden), np.float32)
+    gate[:, hidden - 1] = 6.0
+    down = oracle.normal(4, (hidden, inner))
+    router = oracle.normal(5, (experts, hidden))
+    with Device(gpu_runtime) as dev:
+        matrices, values = [], None
+        for w in (gate, up, down):
+            codes, steps = od.w4_quantise(w, group)
+            values = od.w4_values(codes, steps, group)
+            matrices.append(p.w4_matrix(dev.up(np.tile(od.w4_pack(codes, steps, group), experts)), *w.shape, group, experts))
+        assert np.array_equal(od.w4_values(*od.w4_quantise(up, group), group), up)
+        out, drouter = np.zeros((tokens, hidden), np.float32), dev.up(router)
+        to = dev.up(out)
+        for first in range(0, inner, tokens):
+            f = (first + np.arange(tokens)) % inner
+            x = np.zeros((tokens, hidden), np.float32)
+            number = np.random.default_rng(first).integers(1 << 23, 1 << 24, tokens) * np.float32(2.0 ** -23)
+            x[np.arange(tokens), f], x[:, -1] = number, 8.0
+            gpu_runtime.moe_w4_device(*matrices, drouter, dev.up(x), to, tokens, 1, hidden, hidden, F32, renormalise=True)
+            expect = 288.0 * number.astype(np.float64)[:, None] * values[:, f].T
+            assert np.all(np.abs(dev.down(out, to) - expect) <= 11 * U * np.abs(expect)), first
+
+
 @pytest.mark.parametrize("dtype", (F32, BF16))
 @pytest.mark.parametrize("rows,n", ((20, 40), (1000, 4000)))
 def test_products_of_the_smallest_rows(gpu_runtime, rows, n, dtype):
