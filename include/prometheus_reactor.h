@@ -1025,7 +1025,9 @@ PROM_REACTOR_API int prometheus_reactor_runtime_attention_kv4_device(void* handl
    up to six significant bits, codes the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their
    negatives to w / s (rounded to fp32; halfway to the even code).  A weight stands for s
    times that, which fp32 and bf16 hold exactly, at most s away from w; a group with an
-   infinity or a NaN stands for NaN.
+   infinity or a NaN stands for NaN.  Weights up to 63 * 2^122 (3.35e38) stay finite; in a group with
+   a larger one 6 s lies past fp32's range: its largest weights are infinities, and a product
+   may be infinite, NaN or, where a sum is taken before it is multiplied by s, finite there.
    A matrix is prometheus_reactor_w4_bytes(n, k, group) bytes, matrices lie one behind the
    other.  Tiles of 16 rows by 128 columns, in each row of tiles those of rising columns:
    first all codes, 1024 bytes a tile, of which bytes 16 l .. + 15 are four words, word s the

@@ -211,8 +211,8 @@ __device__ __forceinline__ void w4_add_tile(const W4Tile<kSteps, kNT>& w, const 
         bf16x8 a[X::kTerms];
         X::terms(x.r[m][u], a);
         // The terms are shifted, not the fp32 values before the split: of that clang 22 made code that writes an element's
-        // rest over the element before its upper half, the first term, is taken (groups of 32 and 128; every odd column of
-        // a step lost its first term).  The tests hold each column of a tile with all its bits.
+        // rest over the element before its upper half, the first term, is taken (groups of 128: seven of eight columns of a
+        // tile's last step lost it).  The tests hold each column of a tile with all its bits.
         if (tail) {
           const int at = kt * kW4TileK + 32 * u + 8 * (((int)threadIdx.x & 63) >> 4);
           const int d = min(max(at + 8 - k, 0), 8);

@@ -3,9 +3,21 @@ from __future__ import annotations
 
 import subprocess
 
+import numpy as np
 import pytest
 
+from oracle import decoder_step as od
 from tests.test_launches import compiled
+
+
+def test_the_largest_weights_that_stay_finite():
+    """6 s is finite up to 63 * 2^122 and past fp32's range behind it."""
+    most = np.float32(63 * 2.0 ** 122)
+    w = np.zeros((2, 32), np.float32)
+    w[0, :3], w[1, 0] = (most, -most, most / 3), np.nextafter(most, np.float32(np.inf))
+    values = od.w4_values(*od.w4_quantise(w, 32), 32)
+    top = float(np.finfo(np.float32).max)
+    assert values[0].max() == 63 * 2.0 ** 122 <= top < values[1].max()
 
 
 @pytest.fixture(scope="module")

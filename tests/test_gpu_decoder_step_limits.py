@@ -112,6 +112,19 @@ def test_every_column_of_fp32_rows_enters_with_all_its_bits(gpu_runtime, n, k, g
             assert np.all(np.abs(dev.down(out, to) - expect) <= 3.1 * U * np.abs(expect)), first
 
 
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("rows,n", ((20, 40), (1024, 4000)))
+def test_products_with_the_largest_weights(gpu_runtime, rows, n, dtype):
+    """Weights up to the largest that stay finite, exactly, in both kernels; zeros beside them stay zeros."""
+    k, most = 256, 63 * 2.0 ** 122
+    w = np.clip(oracle.normal(n, (n, k)).astype(np.float64) * 2.0 ** 127, -most, most).astype(np.float32)
+    columns = (np.arange(rows) * 53) % k
+    x = np.zeros((rows, k), np.float32)
+    x[np.arange(rows), columns] = np.exp2(-(np.arange(rows) % 9))
+    got, values = _product(gpu_runtime, x, w, 64, dtype)
+    assert np.array_equal(got, x[np.arange(rows), columns].astype(np.float64)[:, None] * values[:, columns].T)
+
+
 @pytest.mark.parametrize("group", (32, 64, 128))
 @pytest.mark.parametrize("hidden", (256, 260))
 @pytest.mark.parametrize("tokens,experts", ((64, 1), (255, 1), (64, 64), (255, 64)))
