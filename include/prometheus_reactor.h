@@ -1144,9 +1144,10 @@ PROM_REACTOR_API int prometheus_reactor_runtime_rope_device(void* handle, const 
    magnitude, scaled for contexts `factor` times as long as the trained one:
    LINEAR divides all by factor; BASE takes base * factor^(rotary_dim / (rotary_dim - 2)) (rotary_dim
    above 2); PARTS divides those that turn less than slow_turns times within `context` tokens, keeps
-   those that turn fast_turns times or more, goes linearly in i from the one border (rounded down) to
-   the other (rounded up), and has magnitude 1 + ln(factor) / 10.  PROM_ERROR for arguments outside
-   the comments below. */
+   those that turn fast_turns times or more, goes linearly in i from the one border (rounded down, 0 at
+   least) to the other (rounded up, rotary_dim - 1 at most, and above the first), so that pair 0 is
+   always kept, and has magnitude 1 + ln(factor) / 10.  PROM_ERROR for arguments outside the comments
+   below. */
 enum { PROM_ROPE_SCALE_NONE = 0u, PROM_ROPE_SCALE_LINEAR = 1u, PROM_ROPE_SCALE_BASE = 2u, PROM_ROPE_SCALE_PARTS = 3u };
 typedef struct PrometheusRopeScaling {
   uint32_t struct_size;

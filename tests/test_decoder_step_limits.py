@@ -1,4 +1,5 @@
-"""The rest of a decoder's step without a device: what the host code launches, at the ends of its ranges."""
+"""The rest of a decoder's step without a device, at the ends of its ranges: what the host code launches, the largest weights,
+frequencies by parts."""
 from __future__ import annotations
 
 import subprocess
@@ -6,6 +7,7 @@ import subprocess
 import numpy as np
 import pytest
 
+from oct_amd import prometheus as p
 from oracle import decoder_step as od
 from tests.test_launches import compiled
 
@@ -47,3 +49,19 @@ def test_a_failed_launch_of_a_mixture_is_its_last(moe_check, bf16, tokens, exper
 def test_a_failed_launch_is_the_last_of_a_mixture_of_many_columns(moe_check):
     """Few tokens whose sums are joined in a launch of their own."""
     _run(moe_check, 1, 0, 70000, 24, 128, 2, 2, 1)
+
+
+@pytest.mark.parametrize("d,base,context,fast,slow", [
+    (128, 10000.0, 100.0, 32.0, 1.0), (128, 10000.0, 4.0, 32.0, 1.0), (64, 10000.0, 2048.0, 32.0, 1.0),
+    (8, 1.5, 1e4, 2000.0, 0.01), (8, 10.0, 1e9, 32.0, 1.0), (2, 10000.0, 4096.0, 32.0, 1.0), (1024, 5e5, 8192.0, 4.0, 1.0)])
+def test_rope_turns_by_parts_at_their_borders(d, base, context, fast, slow):
+    """Contexts so short that no pair turns often, and so long that all do: the borders stay within the pairs' numbers."""
+    factor, two_pi = 8.0, 2.0 * np.pi
+    got, _ = p.rope_turns(d, base, p.ROPE_SCALE_PARTS, factor, context, fast, slow)
+    plain = base ** (-2.0 * np.arange(d // 2) / d) / two_pi
+    # pair i turns context * plain_i times; the number i, not whole, that turns t times
+    number = lambda t: np.log(context / (two_pi * t)) / np.log(base) * d / 2.0  # noqa: E731
+    first, last = max(np.floor(number(fast)), 0.0), min(np.ceil(number(slow)), d - 1.0)
+    way = np.clip((np.arange(d // 2) - first) / max(last - first, 0.001), 0.0, 1.0)
+    assert np.allclose(got, plain * (1.0 - way + way / factor), rtol=1e-12)
+    assert got[0] == pytest.approx(plain[0], rel=1e-12)
