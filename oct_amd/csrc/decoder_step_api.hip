@@ -252,7 +252,7 @@ PROM_REACTOR_API int prometheus_reactor_runtime_residual_norm_device(void* handl
   a.h_out_stride = r->h_out_stride;
   a.out_stride = r->out_stride;
   a.vector_stride = r->vector_stride;
-  a.rows_per_vector = vectors ? r->rows_per_vector : 1u;
+  a.rows_per_vector = vectors ? r->rows_per_vector : r->rows;  // else the weights are joined once for all rows
   a.residual_scale = r->residual_scale;
   a.weight_offset = r->weight_offset;
   a.eps = r->eps;
