@@ -1085,7 +1085,11 @@ PROM_REACTOR_API int prometheus_reactor_runtime_gemm_w4_device(void* handle, con
    in the product above, router fp32 [experts, hidden].  gate and up are [inner, hidden] of one group
    size, down [hidden, inner]; each holds a matrix an expert (count = experts).  The hidden rows are
    fp32 and enter the second product as rows of that type do.  An expert's weights are read once for
-   every sixteen tokens that chose it, or fewer. */
+   every sixteen tokens that chose it, or fewer.  The runtime keeps a workspace for its largest
+   call: a pair (a token with one of its experts) takes 6 bytes an inner column, rounded up to
+   128, and 4 a hidden column (8 or 16 where above 16 tokens fewer than 32 experts are reached),
+   rounded up to 64; a token 9 an expert.  8192 tokens with 8 of 64 experts, 4096 hidden and 1024
+   inner columns: 1.5 GB. */
 enum { PROM_MOE_SILU = 0u, PROM_MOE_GELU_TANH = 1u };
 #define PROM_MOE_MAX_EXPERTS 1024u
 #define PROM_MOE_MAX_TOP_K 64u

@@ -10,8 +10,10 @@
 // Many rows: a workgroup's four waves take 16 kMT rows by 64 kNT columns.  x goes to LDS by DMA, in the order in which
 // the matrix units take it (1 KiB a transfer, each lane its own 16 bytes of source), a tile of K ahead; each wave holds its
 // columns' codes in registers and turns them into bf16 weights, code times step, between its matrix instructions (four
-// vector instructions for two weights, used for kMT blocks of rows).  Bound by the matrix units: bf16, 512 rows of 20480x3840
-// 86 us, 936 TFLOP/s, of which the matrix instructions alone take 69; a large bf16 product runs at 1256.
+// vector instructions for two weights, used for kMT blocks of rows).  Bound by the SIMDs, whose matrix instructions and
+// conversions take turns, and by the last round: bf16, 512 rows of 20480x3840 86 us, 936 TFLOP/s, of which the matrix
+// instructions alone take 69; its 428 workgroups leave 84 CUs with one for two places, done after 51 of 85 us of K tiles.  A large
+// bf16 product runs at 1256.
 #include <algorithm>
 
 #include "fp4_groups.h"
@@ -417,7 +419,8 @@ TilePlan plan_tiles(uint32_t m, const W4View& w, bool bf16, bool terms) {
 }
 // Whether the few rows' kernel, which reads the weights again for each sixteen rows, is the shorter way: a launch, its
 // workgroups' ends and the products, from 180 to 400 rows of 2048 and 15008 by 128 to 8192 (bf16, 180 rows of 15008x128 7.8 us,
-// on tiles 6.2; 400 of 2048x1024 8.7 and 9.6).
+// on tiles 6.2; 400 of 2048x1024 8.7 and 9.6).  Both ways were timed from 66 rows on; up to 64 it is taken without asking, also where
+// the estimates say otherwise (64 rows of 32768x2048: 27.9 us and 18.7; it takes 24).
 bool rows_are_few(uint32_t m, const W4View& w, bool bf16, const TilePlan& tiles) {
   const double groups = (double)((w.tiles_n + 3) / 4) * ((m + 15) / 16), products = (double)m * w.n * w.tiles_k * kW4TileK;
   return m <= 64 ||
@@ -450,7 +453,6 @@ bool takes_rows(const void* x, uint32_t x_stride, int k) {
 template <typename X>
 hipError_t launch_many(const TilePlan& p, W4TileArgs a, const void* x, uint32_t x_stride, hipStream_t stream) {
   typedef typename X::Element T;
-  constexpr bool kBf16 = X::kTerms == 1;
   a.k = a.w.k;
   if (takes_rows<X>(x, x_stride, a.w.k)) {
     a.x = static_cast<const uint16_t*>(x);

@@ -9,7 +9,8 @@ constexpr int kMoeMaxExperts = 1024, kMoeMaxTopK = 64, kMoeMaxPairs = 65536;
 constexpr int kMoeFewTokens = 64;  // a token a lane
 
 struct MoeExpert {
-  int expert, start, count, unused;  // its pairs: pairs[start] ..
+  int expert, start, count;  // its pairs: pairs[start] ..
+  int unused;                // sixteen bytes: one load
 };
 
 struct W4MoeArgs {

@@ -12,8 +12,8 @@
 // sums are joined in a fourth launch.
 //
 // Bound by the reached experts' weights, and for a token by the latency of three kernels that follow one another.  64
-// experts of 1024 with 2048 outer columns, 8 a token, in bf16: a token 5.6 + 6.5 + 7.0 us (28 MB at 2.1 TB/s in the last
-// two), 64 tokens, which reach all experts, 9.6 + 33.0 + 24.0 us (214 MB at 3.8 TB/s; 64 rows of x and of the hidden
+// experts of 1024 with 2048 outer columns, 8 a token, in bf16: a token 4.7 + 6.1 + 7.6 us (28 MB at 2.0 TB/s in the last
+// two), 64 tokens, which reach all experts, 9.9 + 33.2 + 29.7 us (214 MB at 3.4 TB/s; 64 rows of x and of the hidden
 // columns come from L2 for each workgroup).
 #include <algorithm>
 
@@ -611,8 +611,8 @@ size_t moe_w4_workspace(W4MoeArgs& a, void* base) {
     return p;
   };
   // Few slots: K is dealt out too.  Many: more columns a workgroup, which share the hidden rows (64 experts of 1024 hidden
-  // and 2048 outer columns: 32 slots 10.9 us with 32 columns, 12.4 with 64; 64 slots of 8 tokens 20 and 16, of 64 tokens 31.5
-  // and 24.5).
+  // and 2048 outer columns: 32 slots 13.7 us with 32 columns, 16.5 with 64; 64 slots of 8 tokens 21 and 18, of 64 tokens 42
+  // and 30).
   const int slots = (int)std::min(experts, pairs);
   a.out_tiles = slots >= 64 ? 4 : 2;
   const int columns = (a.down.tiles_n + a.out_tiles - 1) / a.out_tiles;
